@@ -242,6 +242,114 @@ int z2h_sample_feed(z2h_ctx * ctx, int n_active, const z2h_sampling * sp, const 
                     int hist_cap, const double * u, int32_t * codes);
 int z2h_step_resident(z2h_ctx * ctx, int n_active);
 
+/* ---------------------------------------------------------------------------------------------------------
+ * Operators on device tensors around a paged key / value cache (no reference counterpart: the reference keeps one
+ * contiguous band per slot, src/zonos2-graph.cpp:639-690, and its decode step, like z2h_step, reads a prompt that
+ * requests share once per request). For callers that keep their own buffers; z2h_step_paged below runs the
+ * model's layers over them. They take a context for its device and its error string only: no tensor, no weights and no
+ * z2h_finalize are needed, nothing is allocated, nothing synchronizes, and every call may be captured into a HIP graph.
+ * All tensors are on the context's device. Work is enqueued on `stream` (a hipStream_t, NULL = the null stream); the
+ * caller's current device is the same on return. Strides are in elements.
+ *
+ * Tables of lengths, positions and pages are read on the device and are not checked on the host: an entry out of range
+ * never leads outside the buffers described to the call (each function says what it does then). */
+enum { Z2H_BF16 = 30 };
+
+/* Rotary positions. Of each head's first n_dims dims, pair i of n_dims / 2 is (2i, 2i + 1), or with `halves`
+ * (i, i + n_dims / 2); at position p it turns by p theta'_i and is scaled by mscale. The dims behind n_dims stay as they are.
+ *   theta_i = base^(-2i / n_dims),  theta'_i = theta_i (g_i + (1 - g_i) / factor)
+ * orig_ctx = 0: g_i = 0 (every pair slowed by `factor`; 1 = plain). orig_ctx > 0, for contexts `factor` times as long
+ * as the orig_ctx positions of training: with r_i = orig_ctx theta_i / (2 pi) turns within these,
+ * g_i = clamp((r_i - low_turns) / (high_turns - low_turns), 0, 1): fast pairs keep their speed, slow ones are stretched.
+ * Angles are formed in 64 bits, so far positions keep their phase. */
+typedef struct z2h_rope {
+    float   base;
+    int32_t n_dims;           /* even, 0 .. head_dim */
+    int32_t halves;
+    float   factor;
+    float   low_turns, high_turns;
+    int32_t orig_ctx;
+    float   mscale;
+} z2h_rope;
+
+/* A paged cache of one layer: k and v are [n_pages][n_head_kv][page_rows][head_dim] of Z2H_F16 or Z2H_BF16, page_stride
+ * apart (at least n_head_kv * page_rows * head_dim; a multiple of 8; k and v 16-byte aligned). page_rows is a power of two
+ * from 16 to 4096, head_dim 32, 64 or 128. Row r of sequence s is row r % page_rows of page
+ * table[s * table_len + r / page_rows]; `table` is [n_seq][table_len] on the device. Sequences may name the same pages. */
+typedef struct z2h_pages {
+    void *  k, * v;
+    int64_t page_stride;
+    int32_t type, n_pages, page_rows, n_head_kv, head_dim;
+    int32_t n_seq, table_len;
+    const int32_t * table;
+} z2h_pages;
+
+/* Rotate n_rows rows of n_head heads at positions d_pos [n_rows]: out = rope(x), both [n_rows][n_head][head_dim] of `type`
+ * (Z2H_F32, Z2H_F16 or Z2H_BF16), rows x_stride / out_stride apart. head_dim is even, at most 128. d_out may be d_x
+ * (with the same stride). Products and sums in fp32, rounded once. */
+int z2h_rope_rows(z2h_ctx * ctx, const z2h_rope * rope, int n_rows, int n_head, int head_dim, int type, const void * d_x,
+                  int64_t x_stride, void * d_out, int64_t out_stride, const int32_t * d_pos, void * stream);
+
+/* Append n_rows rows to a paged cache: row t's keys, rotated at d_pos[t], and its values become row d_pos[t] of sequence
+ * d_seq[t]; its n_head query heads, rotated likewise, go to d_q_out. d_k, d_v [n_rows][n_head_kv][head_dim] and d_q,
+ * d_q_out [n_rows][n_head][head_dim] are of `type` (Z2H_F32, Z2H_F16 or Z2H_BF16), rows *_stride apart, so that they may
+ * be columns of one fused projection; d_q NULL: keys and values only. d_q_out may be d_q. Rounded once to the cache's type.
+ * No two rows may share (sequence, position). A row with d_seq[t] outside [0, n_seq) is padding: nothing of it is
+ * read or written. A row whose position lies outside the table, or whose page is outside [0, n_pages), leaves the cache
+ * as it was; its queries are rotated. */
+int z2h_paged_append(z2h_ctx * ctx, const z2h_pages * pages, const z2h_rope * rope, int n_rows, const int32_t * d_seq,
+                     const int32_t * d_pos, int type, const void * d_k, int64_t k_stride, const void * d_v, int64_t v_stride,
+                     int n_head, const void * d_q, int64_t q_stride, void * d_q_out, int64_t q_out_stride, void * stream);
+
+/* Attention of a batch of sequences over a paged cache, where groups of sequences may share a prefix (a voice prompt)
+ * that is read and multiplied once for the whole group.
+ *
+ * z2h_paged_plan lays out the work from the lengths, which it reads on the device, into the workspace; z2h_paged_attn
+ * may then be called any number of times (every layer of a step) with the same shapes and workspace. Sequence s has
+ * query rows [d_row_start[s], d_row_start[s + 1]) of the batch (d_row_start [n_seq + 1] ascending from 0 to n_rows; no
+ * rows: the sequence sits this call out) and d_kv_len[s] cache rows, its query rows' own among them: row j of m sees
+ * rows [0, d_kv_len[s] - m + j]. A row that sees nothing gives zeros. Group g is sequences
+ * [d_group_start[g], d_group_start[g + 1]) (d_group_start [n_group + 1] ascending), whose first d_prefix_len[g] cache rows
+ * hold the same values: they are read through the group's first sequence, and only as many as it has. Sequences outside every
+ * group share nothing; n_group may be 0. A page entry outside [0, n_pages) reads as page 0; lengths are clamped to the table.
+ *
+ * z2h_paged_attn: d_out = softmax(scale q k^T) v for d_q [n_rows][n_head][head_dim], rows q_stride / out_stride apart, n_head a
+ * multiple of n_head_kv, at most 64 query heads per key head; query head h reads key head h / (n_head / n_head_kv). `type` is Z2H_F32 or
+ * Z2H_F16 over Z2H_F16 pages, or Z2H_BF16 over Z2H_BF16 pages. d_out may be d_q (with the same stride). Softmax and sums in fp32;
+ * results do not depend on timing (no atomics).
+ *
+ * The workspace (z2h_paged_ws_bytes; 0 = the shapes are refused, see z2h_last_error; 256-byte aligned) holds the plan and the partial results of one call at a time: calls and graphs
+ * that may overlap need one each. z2h_paged_attn with another shape than the plan's leaves d_out as it was. */
+int64_t z2h_paged_ws_bytes(z2h_ctx * ctx, const z2h_pages * pages, int n_head, int n_rows, int n_group);
+int z2h_paged_plan(z2h_ctx * ctx, const z2h_pages * pages, int n_head, int n_rows, const int32_t * d_row_start,
+                   const int32_t * d_kv_len, int n_group, const int32_t * d_group_start, const int32_t * d_prefix_len,
+                   void * d_ws, int64_t ws_bytes, void * stream);
+int z2h_paged_attn(z2h_ctx * ctx, const z2h_pages * pages, int n_head, int n_rows, int n_group, float scale, int type,
+                   const void * d_q, int64_t q_stride, void * d_out, int64_t out_stride, void * d_ws, int64_t ws_bytes,
+                   void * stream);
+
+/* Verification of drafted frames against the target's probabilities, with the random numbers given (the device
+ * counterpart of z2h_sample for speculative decoding). Sequence s has d_n_draft[s] drafted frames (clamped to 0 .. n_draft_max; NULL:
+ * n_draft_max each) of n_codebooks codes, d_draft [n_seq][n_draft_max][n_codebooks]. d_target [n_seq][n_draft_max + 1]
+ * [n_codebooks][vocab] is what the target model says at each drafted frame and behind the last: probabilities, or with
+ * d_temperature [n_seq] logits, p = softmax(logits / temperature) (0 or less: all mass on the first largest logit).
+ * d_draft_probs [n_seq][n_draft_max][n_codebooks][vocab] are the probabilities q that the drafts were drawn from; NULL: the
+ * drafts were not drawn (q = 1 at the drafted code). The codes are judged in order, frame by frame and codebook by codebook:
+ * code x is kept iff u q(x) < p(x), u = d_u_accept [n_seq][n_draft_max][n_codebooks]. Behind the first code that is not
+ * kept, in frame k codebook c, the sequence ends: d_n_accept[s] = k whole frames are kept, and d_codes[s] ([n_seq][n_codebooks])
+ * is the frame that follows them: the kept codes of frame k before c, at c a draw from max(p - q, 0) (from p where that
+ * has no mass), behind c draws from p of frame k. With every code kept it is a draw from p of the frame behind the last draft.
+ * A draw takes the first code whose cumulative mass exceeds u (total mass), u = d_u_draw [n_seq][n_codebooks], and if rounding leaves none, the last with
+ * mass. So the frames are distributed as the target's own, codebook by codebook. Probabilities, sums and comparisons in 64 bits.
+ * Random numbers are doubles in [0, 1). A drafted code outside [0, vocab) is not kept. Probabilities that are no
+ * numbers or have no mass give some code in range. vocab is at most 2^20. The workspace (z2h_verify_ws_bytes; 0: the sizes are refused; 256-byte aligned)
+ * holds one call at a time. */
+int64_t z2h_verify_ws_bytes(int n_seq, int n_draft_max, int n_codebooks, int vocab);
+int z2h_verify(z2h_ctx * ctx, int n_seq, int n_draft_max, int n_codebooks, int vocab, const int32_t * d_draft,
+               const int32_t * d_n_draft, const float * d_target, const float * d_temperature, const float * d_draft_probs,
+               const double * d_u_accept, const double * d_u_draw, int32_t * d_n_accept, int32_t * d_codes, void * d_ws,
+               int64_t ws_bytes, void * stream);
+
 /* Debug capture of per-layer intermediates of the following steps (off by default). */
 enum {
     Z2H_CAP_RES_IN = 0, Z2H_CAP_ATTN_IN, Z2H_CAP_Q, Z2H_CAP_K, Z2H_CAP_V, Z2H_CAP_GATE, Z2H_CAP_ATTN_O,

@@ -1,0 +1,100 @@
+// The checks and index rules of the operators on device tensors (csrc/z2h_ops_rules.h), without a GPU: prints "ok" or the
+// first thing that is wrong.
+#include "../../zonos2.cpp_amd/csrc/z2h_ops_rules.h"
+#include <cstdio>
+#include <cstdlib>
+#include <limits>
+#include <vector>
+
+#define EXPECT(cond) do { if (!(cond)) { std::printf("line %d: %s\n", __LINE__, #cond); std::exit(1); } } while (0)
+
+static z2h_pages good_pages() {
+    static const int32_t table[4] = {0, 1, 2, 3};
+    z2h_pages p{};
+    p.k = (void *) 256; p.v = (void *) 512; p.table = table;
+    p.type = Z2H_F16; p.n_pages = 4; p.page_rows = 16; p.n_head_kv = 2; p.head_dim = 64; p.n_seq = 2; p.table_len = 2;
+    p.page_stride = 2 * 16 * 64;
+    return p;
+}
+
+static void pages() {
+    const z2h_pages good = good_pages();
+    EXPECT(!z2o::check_pages(&good));
+    EXPECT(z2o::check_pages(nullptr));
+    auto bad = [](auto change) { z2h_pages p = good_pages(); change(p); return z2o::check_pages(&p) != nullptr; };
+    EXPECT(bad([](auto & p) { p.k = nullptr; }));
+    EXPECT(bad([](auto & p) { p.v = (void *) 520; }));
+    EXPECT(bad([](auto & p) { p.table = nullptr; }));
+    EXPECT(bad([](auto & p) { p.type = Z2H_F32; }));
+    EXPECT(bad([](auto & p) { p.type = Z2H_Q8_0; }));
+    EXPECT(bad([](auto & p) { p.head_dim = 16; }));
+    EXPECT(bad([](auto & p) { p.head_dim = 96; }));
+    EXPECT(bad([](auto & p) { p.page_rows = 8; p.page_stride = 1 << 20; }));
+    EXPECT(bad([](auto & p) { p.page_rows = 24; p.page_stride = 1 << 20; }));
+    EXPECT(bad([](auto & p) { p.page_rows = 8192; p.page_stride = 1 << 28; }));
+    EXPECT(bad([](auto & p) { p.page_stride -= 8; }));
+    EXPECT(bad([](auto & p) { p.page_stride += 4; }));
+    EXPECT(bad([](auto & p) { p.n_pages = 0; }));
+    EXPECT(bad([](auto & p) { p.n_head_kv = 0; }));
+    EXPECT(bad([](auto & p) { p.n_seq = 0; }));
+    EXPECT(bad([](auto & p) { p.table_len = 0; }));
+    EXPECT(bad([](auto & p) { p.table_len = std::numeric_limits<int32_t>::max(); }));
+    EXPECT(!bad([](auto & p) { p.page_stride += 8; }));
+    // look-ups: every entry out of range is -1, never an address
+    const int32_t table[6] = {0, 3, -1, 4, 2, std::numeric_limits<int32_t>::min()};
+    auto at = [&](int seq, int pos) { return z2o::page_of(table, 2, 3, 4, 4, seq, pos); };
+    EXPECT(at(0, 0) == 0 && at(0, 15) == 0 && at(0, 16) == 3 && at(0, 31) == 3 && at(0, 32) == -1);
+    EXPECT(at(1, 0) == -1 && at(1, 16) == 2 && at(1, 40) == -1);
+    EXPECT(at(0, 48) == -1 && at(0, -1) == -1 && at(-1, 0) == -1 && at(2, 0) == -1 && at(0, std::numeric_limits<int>::max()) == -1);
+    for (int s = 4; s <= 12; ++s) EXPECT(z2o::page_shift_of(1 << s) == s);
+}
+
+static void rope() {
+    z2h_rope r{10000.0f, 64, 0, 1.0f, 0.0f, 0.0f, 0, 1.0f};
+    EXPECT(!z2o::check_rope(&r, 64) && !z2o::check_rope(&r, 128) && z2o::check_rope(&r, 32) && z2o::check_rope(nullptr, 64));
+    EXPECT(z2o::check_rope(&r, 256) && z2o::check_rope(&r, 0) && z2o::check_rope(&r, 65));
+    auto bad = [&](auto change) { z2h_rope x = r; change(x); return z2o::check_rope(&x, 128) != nullptr; };
+    const float nan = std::numeric_limits<float>::quiet_NaN(), inf = std::numeric_limits<float>::infinity();
+    EXPECT(bad([](auto & x) { x.n_dims = 63; }) && bad([](auto & x) { x.n_dims = -2; }) && bad([](auto & x) { x.n_dims = 130; }));
+    EXPECT(!bad([](auto & x) { x.n_dims = 0; }));
+    for (float v : {0.0f, -1.0f, nan, inf}) {
+        EXPECT(bad([&](auto & x) { x.base = v; }) && bad([&](auto & x) { x.factor = v; }) && bad([&](auto & x) { x.mscale = v; }));
+    }
+    EXPECT(bad([](auto & x) { x.orig_ctx = -1; }) && bad([](auto & x) { x.orig_ctx = 1; }));
+    EXPECT(!bad([](auto & x) { x.orig_ctx = 1; x.high_turns = 1.0f; }) && bad([&](auto & x) { x.orig_ctx = 1; x.high_turns = nan; }));
+    double t[64];
+    const double two_pi = 6.283185307179586476925;
+    z2o::rope_turns(r, t);
+    EXPECT(std::fabs(t[0] - 1.0 / two_pi) < 1e-16 && std::fabs(t[16] * two_pi - 0.01) < 1e-17);
+    r.factor = 4.0f;
+    z2o::rope_turns(r, t);
+    EXPECT(std::fabs(t[0] - 0.25 / two_pi) < 1e-16);
+    r.orig_ctx = 4096; r.low_turns = 1.0f; r.high_turns = 32.0f;                       // fast pairs as they are, slow ones by 4
+    z2o::rope_turns(r, t);
+    EXPECT(std::fabs(t[0] - 1.0 / two_pi) < 1e-16);
+    EXPECT(std::fabs(t[31] / (std::pow(10000.0, -62.0 / 64) / 4 / two_pi) - 1.0) < 1e-12);
+    for (int i = 1; i < 32; ++i) EXPECT(t[i] < t[i - 1]);
+}
+
+static void rows() {
+    EXPECT(!z2o::check_rows((void *) 64, 128, 2, 64, Z2H_F16) && z2o::check_rows((void *) 64, 127, 2, 64, Z2H_F16));
+    EXPECT(z2o::check_rows(nullptr, 128, 2, 64, Z2H_F16) && z2o::check_rows((void *) 65, 128, 2, 64, Z2H_F16));
+    EXPECT(z2o::check_rows((void *) 66, 128, 2, 64, Z2H_F32) && z2o::check_rows((void *) 64, 128, 2, 64, Z2H_Q8_0));
+    EXPECT(z2o::check_rows((void *) 64, 0, 65536, 65536, Z2H_F16));
+    z2h_pages p = good_pages();
+    EXPECT(!z2o::check_attn(&p, 2, 0, 0) && !z2o::check_attn(&p, 128, 5, 2) && z2o::check_attn(&p, 130, 5, 2) && z2o::check_attn(&p, 3, 5, 2));
+    EXPECT(z2o::check_attn(&p, 0, 5, 2) && z2o::check_attn(&p, 2, -1, 2) && z2o::check_attn(&p, 2, 5, 3) && z2o::check_attn(&p, 2, 5, -1));
+    EXPECT(z2o::check_attn(&p, 128, 1 << 20, 0) && !z2o::check_attn(&p, 64, 1 << 20, 0));
+    EXPECT(!z2o::check_attn_type(Z2H_F32, Z2H_F16) && !z2o::check_attn_type(Z2H_F16, Z2H_F16) && !z2o::check_attn_type(Z2H_BF16, Z2H_BF16));
+    EXPECT(z2o::check_attn_type(Z2H_F32, Z2H_BF16) && z2o::check_attn_type(Z2H_BF16, Z2H_F16) && z2o::check_attn_type(Z2H_Q4_K, Z2H_F16));
+    EXPECT(!z2o::check_verify(0, 0, 1, 1) && !z2o::check_verify(64, 7, 9, 1 << 20) && z2o::check_verify(1, 1, 1, (1 << 20) + 1));
+    EXPECT(z2o::check_verify(-1, 1, 1, 5) && z2o::check_verify(1, -1, 1, 5) && z2o::check_verify(1, 1, 0, 5) && z2o::check_verify(1, 1, 1, 0));
+    EXPECT(z2o::check_verify(1 << 20, 4096, 1024, 5));
+}
+
+int main() {
+    pages();
+    rope();
+    rows();
+    std::puts("ok");
+}

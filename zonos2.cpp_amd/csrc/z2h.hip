@@ -14,6 +14,7 @@
 #include "z2h_attn.h"
 #include <hip/hip_ext.h>
 #include "z2_formats.h"
+#include "z2h_ctx_ops.h"
 
 #include <algorithm>
 #include <atomic>
@@ -1607,6 +1608,11 @@ struct DeviceScope {
     ~DeviceScope() { if (ok && prev >= 0) (void) hipSetDevice(prev); }
 };
 } // namespace
+
+int z2h_ctx_fail(z2h_ctx * ctx, int code, const char * what) noexcept {
+    try { return seterr(ctx, code, what); } catch (...) { return code; }
+}
+int z2h_ctx_device(const z2h_ctx * ctx) noexcept { return ctx->device; }
 
 // ====================================================================== C ABI
 extern "C" {

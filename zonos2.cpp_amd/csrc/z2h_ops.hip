@@ -1,0 +1,201 @@
+// z2h_ops.hip — the operators on device tensors of include/z2h.h: rotary rows, paged append, attention over shared
+// prefixes, draft verification. A translation unit of their own: z2h.hip's kernels keep their code layout.
+#include "z2h.h"
+#include "z2h_ctx_ops.h"
+#include "z2h_ops_rules.h"
+#include "z2h_rope.h"
+#include "z2h_paged.h"
+#include "z2h_verify.h"
+
+using namespace z2d;
+
+namespace {
+
+// makes the context's device current for a scope and restores the caller's on every way out
+struct OnDevice {
+    int prev = -1;
+    bool ok = false, moved = false;
+    explicit OnDevice(const z2h_ctx * ctx) {
+        const int device = z2h_ctx_device(ctx);
+        if (hipGetDevice(&prev) != hipSuccess) return;
+        moved = prev != device;
+        ok = !moved || hipSetDevice(device) == hipSuccess;
+    }
+    ~OnDevice() { if (ok && moved) (void) hipSetDevice(prev); }
+};
+
+int launched(z2h_ctx * ctx) {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? Z2H_OK : z2h_ctx_fail(ctx, Z2H_EDEVICE, hipGetErrorString(e));
+}
+
+#define CHECK(expr) do { if (const char * e_ = (expr)) return z2h_ctx_fail(ctx, Z2H_EINVAL, e_); } while (0)
+#define REQUIRE(cond, what) do { if (!(cond)) return z2h_ctx_fail(ctx, Z2H_EINVAL, what); } while (0)
+#define ON_DEVICE OnDevice on_(ctx); if (!on_.ok) return z2h_ctx_fail(ctx, Z2H_EDEVICE, "hipSetDevice failed")
+
+template <typename T, typename TC>
+void rope_launch(const RopeArgs & a, int n_rows, bool halves, hipStream_t stream) {
+    if (halves) hipLaunchKernelGGL((k_rope_append<T, TC, true>), dim3(n_rows), dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((k_rope_append<T, TC, false>), dim3(n_rows), dim3(256), 0, stream, a);
+}
+template <typename T>
+void rope_launch(const RopeArgs & a, int n_rows, bool halves, int cache, hipStream_t stream) {
+    if (cache == Z2H_BF16) rope_launch<T, __bf16>(a, n_rows, halves, stream);
+    else rope_launch<T, _Float16>(a, n_rows, halves, stream);
+}
+int rope_run(z2h_ctx * ctx, RopeArgs & a, const z2h_rope * rope, int n_rows, int type, int cache, void * stream) {
+    a.mscale = rope->mscale;
+    a.n_dims = rope->n_dims;
+    z2o::rope_turns(*rope, a.turn);
+    ON_DEVICE;
+    const bool halves = rope->halves != 0;
+    switch (type) {
+        case Z2H_F32: rope_launch<float>(a, n_rows, halves, cache, (hipStream_t) stream); break;
+        case Z2H_F16: rope_launch<_Float16>(a, n_rows, halves, cache, (hipStream_t) stream); break;
+        default: rope_launch<__bf16>(a, n_rows, halves, cache, (hipStream_t) stream); break;
+    }
+    return launched(ctx);
+}
+
+template <int HD>
+void attn_launch(const PagedArgs & a, int type, hipStream_t stream) {
+    const dim3 grid(a.n_rows, a.n_head);
+    switch (type) {
+        case Z2H_F32: hipLaunchKernelGGL((k_paged_attn_row<HD, float, _Float16>), grid, dim3(256), 0, stream, a); break;
+        case Z2H_F16: hipLaunchKernelGGL((k_paged_attn_row<HD, _Float16, _Float16>), grid, dim3(256), 0, stream, a); break;
+        default: hipLaunchKernelGGL((k_paged_attn_row<HD, __bf16, __bf16>), grid, dim3(256), 0, stream, a); break;
+    }
+}
+
+const char * check_ws(const void * ws, int64_t have, int64_t need) {
+    if (!ws || (uintptr_t) ws % 256) return "workspace must be 256-byte aligned";
+    return have < need ? "workspace too small" : nullptr;
+}
+
+} // namespace
+
+extern "C" {
+
+int z2h_rope_rows(z2h_ctx * ctx, const z2h_rope * rope, int n_rows, int n_head, int head_dim, int type, const void * d_x,
+                  int64_t x_stride, void * d_out, int64_t out_stride, const int32_t * d_pos, void * stream) {
+    if (!ctx) return Z2H_EINVAL;
+    CHECK(z2o::check_rope(rope, head_dim));
+    REQUIRE(n_rows >= 0 && n_head > 0 && n_head <= 65536, "rope: row or head count out of range");
+    CHECK(z2o::check_rows(d_x, x_stride, n_head, head_dim, type));
+    CHECK(z2o::check_rows(d_out, out_stride, n_head, head_dim, type));
+    REQUIRE(d_x != d_out || x_stride == out_stride, "rope: in place with different strides");
+    REQUIRE(d_pos, "null positions");
+    if (n_rows == 0) return Z2H_OK;
+    RopeArgs a{};
+    a.hd = head_dim; a.nh = n_head;
+    a.pos = d_pos;
+    a.q = d_x; a.qs = x_stride; a.q_out = d_out; a.qos = out_stride;
+    return rope_run(ctx, a, rope, n_rows, type, Z2H_F16, stream);
+}
+
+int z2h_paged_append(z2h_ctx * ctx, const z2h_pages * pages, const z2h_rope * rope, int n_rows, const int32_t * d_seq,
+                     const int32_t * d_pos, int type, const void * d_k, int64_t k_stride, const void * d_v, int64_t v_stride,
+                     int n_head, const void * d_q, int64_t q_stride, void * d_q_out, int64_t q_out_stride, void * stream) {
+    if (!ctx) return Z2H_EINVAL;
+    CHECK(z2o::check_pages(pages));
+    CHECK(z2o::check_rope(rope, pages->head_dim));
+    REQUIRE(n_rows >= 0, "append: n_rows out of range");
+    REQUIRE(d_seq && d_pos, "append: null sequences or positions");
+    CHECK(z2o::check_rows(d_k, k_stride, pages->n_head_kv, pages->head_dim, type));
+    CHECK(z2o::check_rows(d_v, v_stride, pages->n_head_kv, pages->head_dim, type));
+    if (d_q) {
+        REQUIRE(n_head > 0 && n_head <= 65536, "append: n_head out of range");
+        CHECK(z2o::check_rows(d_q, q_stride, n_head, pages->head_dim, type));
+        CHECK(z2o::check_rows(d_q_out, q_out_stride, n_head, pages->head_dim, type));
+        REQUIRE(d_q != d_q_out || q_stride == q_out_stride, "append: queries in place with different strides");
+    }
+    if (n_rows == 0) return Z2H_OK;
+    RopeArgs a{};
+    a.hd = pages->head_dim; a.nh = d_q ? n_head : 0; a.nkv = pages->n_head_kv;
+    a.seq = d_seq; a.pos = d_pos;
+    a.q = d_q; a.qs = q_stride; a.q_out = d_q_out; a.qos = q_out_stride;
+    a.k = d_k; a.ks = k_stride; a.v = d_v; a.vs = v_stride;
+    a.kc = pages->k; a.vc = pages->v; a.page_stride = pages->page_stride;
+    a.table = pages->table; a.n_seq = pages->n_seq; a.table_len = pages->table_len; a.n_pages = pages->n_pages;
+    a.page_shift = z2o::page_shift_of(pages->page_rows);
+    return rope_run(ctx, a, rope, n_rows, type, pages->type, stream);
+}
+
+int64_t z2h_paged_ws_bytes(z2h_ctx * ctx, const z2h_pages * pages, int n_head, int n_rows, int n_group) {
+    if (!ctx) return 0;
+    if (const char * e = z2o::check_attn(pages, n_head, n_rows, n_group)) { z2h_ctx_fail(ctx, Z2H_EINVAL, e); return 0; }
+    return z2o::attn_ws(*pages, n_head, n_rows, n_group).bytes;
+}
+
+int z2h_paged_plan(z2h_ctx * ctx, const z2h_pages * pages, int n_head, int n_rows, const int32_t * d_row_start,
+                   const int32_t * d_kv_len, int n_group, const int32_t * d_group_start, const int32_t * d_prefix_len,
+                   void * d_ws, int64_t ws_bytes, void * stream) {
+    if (!ctx) return Z2H_EINVAL;
+    CHECK(z2o::check_attn(pages, n_head, n_rows, n_group));
+    REQUIRE(d_row_start && d_kv_len && (n_group == 0 || (d_group_start && d_prefix_len)), "plan: null table");
+    const z2o::AttnWs w = z2o::attn_ws(*pages, n_head, n_rows, n_group);
+    CHECK(check_ws(d_ws, ws_bytes, w.bytes));
+    PlanArgs a{};
+    a.row_start = d_row_start; a.kv_len = d_kv_len; a.group_start = d_group_start; a.prefix_len = d_prefix_len;
+    a.n_seq = pages->n_seq; a.n_rows = n_rows; a.n_group = n_group; a.n_head = n_head; a.nkv = pages->n_head_kv; a.hd = pages->head_dim;
+    a.cap = pages->table_len * pages->page_rows;
+    a.ws = (uint8_t *) d_ws;
+    ON_DEVICE;
+    hipLaunchKernelGGL(k_paged_plan, dim3(n_rows / 256 + 1), dim3(256), 0, (hipStream_t) stream, a, w.rows);
+    return launched(ctx);
+}
+
+int z2h_paged_attn(z2h_ctx * ctx, const z2h_pages * pages, int n_head, int n_rows, int n_group, float scale, int type,
+                   const void * d_q, int64_t q_stride, void * d_out, int64_t out_stride, void * d_ws, int64_t ws_bytes,
+                   void * stream) {
+    if (!ctx) return Z2H_EINVAL;
+    CHECK(z2o::check_attn(pages, n_head, n_rows, n_group));
+    CHECK(z2o::check_attn_type(type, pages->type));
+    CHECK(z2o::check_rows(d_q, q_stride, n_head, pages->head_dim, type));
+    CHECK(z2o::check_rows(d_out, out_stride, n_head, pages->head_dim, type));
+    REQUIRE(d_q != d_out || q_stride == out_stride, "attention: in place with different strides");
+    REQUIRE(std::isfinite(scale), "attention: scale must be finite");
+    const z2o::AttnWs w = z2o::attn_ws(*pages, n_head, n_rows, n_group);
+    CHECK(check_ws(d_ws, ws_bytes, w.bytes));
+    if (n_rows == 0) return Z2H_OK;
+    PagedArgs a{};
+    a.k = pages->k; a.v = pages->v; a.page_stride = pages->page_stride; a.qs = q_stride; a.os = out_stride; a.rows_at = w.rows;
+    a.table = pages->table; a.n_seq = pages->n_seq; a.table_len = pages->table_len; a.n_pages = pages->n_pages;
+    a.page_shift = z2o::page_shift_of(pages->page_rows);
+    a.nkv = pages->n_head_kv; a.n_head = n_head; a.n_rows = n_rows; a.n_group = n_group; a.scale = scale;
+    a.q = d_q; a.out = d_out; a.ws = (uint8_t *) d_ws;
+    ON_DEVICE;
+    switch (pages->head_dim) {
+        case 32: attn_launch<32>(a, type, (hipStream_t) stream); break;
+        case 64: attn_launch<64>(a, type, (hipStream_t) stream); break;
+        default: attn_launch<128>(a, type, (hipStream_t) stream); break;
+    }
+    return launched(ctx);
+}
+
+int64_t z2h_verify_ws_bytes(int n_seq, int n_draft_max, int n_codebooks, int vocab) {
+    return z2o::check_verify(n_seq, n_draft_max, n_codebooks, vocab) ? 0 : z2o::verify_ws_bytes(n_seq, n_draft_max, n_codebooks, vocab);
+}
+
+int z2h_verify(z2h_ctx * ctx, int n_seq, int n_draft_max, int n_codebooks, int vocab, const int32_t * d_draft,
+               const int32_t * d_n_draft, const float * d_target, const float * d_temperature, const float * d_draft_probs,
+               const double * d_u_accept, const double * d_u_draw, int32_t * d_n_accept, int32_t * d_codes, void * d_ws,
+               int64_t ws_bytes, void * stream) {
+    if (!ctx) return Z2H_EINVAL;
+    CHECK(z2o::check_verify(n_seq, n_draft_max, n_codebooks, vocab));
+    REQUIRE(d_target && d_u_draw && d_n_accept && d_codes && (n_draft_max == 0 || (d_draft && d_u_accept)), "verify: null argument");
+    CHECK(check_ws(d_ws, ws_bytes, z2o::verify_ws_bytes(n_seq, n_draft_max, n_codebooks, vocab)));
+    if (n_seq == 0) return Z2H_OK;
+    VerifyArgs a{};
+    a.n_seq = n_seq; a.K = n_draft_max; a.C = n_codebooks; a.V = vocab;
+    a.draft = d_draft; a.n_draft = d_n_draft; a.target = d_target; a.temperature = d_temperature; a.draft_probs = d_draft_probs;
+    a.u_accept = d_u_accept; a.u_draw = d_u_draw; a.n_accept = d_n_accept; a.codes = d_codes;
+    a.stats = (double *) d_ws;
+    ON_DEVICE;
+    if (d_temperature)
+        hipLaunchKernelGGL(k_verify_stats, dim3(n_seq * (n_draft_max + 1) * n_codebooks), dim3(256), 0, (hipStream_t) stream, a);
+    hipLaunchKernelGGL(k_verify, dim3(n_seq * n_codebooks), dim3(256), (size_t) ((vocab + 255) / 256) * 8, (hipStream_t) stream, a);
+    return launched(ctx);
+}
+
+} // extern "C"

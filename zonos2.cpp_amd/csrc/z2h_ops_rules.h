@@ -1,0 +1,123 @@
+// z2h_ops_rules.h — the argument checks, sizes and index rules of the operators on device tensors (z2h_ops.hip), as plain
+// functions: the kernels use the index rules as they stand here, and a CPU test runs all of them without a GPU.
+#pragma once
+#include "z2h.h"
+#include <cmath>
+#include <cstdint>
+
+#if defined(__HIPCC__)
+#define Z2O_HD __host__ __device__ inline
+#else
+#define Z2O_HD inline
+#endif
+
+namespace z2o {
+
+constexpr int MAX_GROUP = 64;                      // query heads per key head
+constexpr int64_t MAX_ROW_HEADS = 1ll << 26;       // rows x heads of one attention call
+constexpr int MAX_VOCAB = 1 << 20;
+constexpr int MAX_ROPE_DIMS = 128;
+
+// ---- checks: nullptr, or what is wrong
+inline const char * check_rope(const z2h_rope * r, int head_dim) {
+    if (!r) return "null rope";
+    if (head_dim <= 0 || head_dim > MAX_ROPE_DIMS || head_dim % 2) return "rope: head_dim must be even and at most 128";
+    if (r->n_dims < 0 || r->n_dims > head_dim || r->n_dims % 2) return "rope: n_dims must be even, 0 .. head_dim";
+    if (!(r->base > 0.0f) || !std::isfinite(r->base)) return "rope: base must be positive";
+    if (!(r->factor > 0.0f) || !std::isfinite(r->factor)) return "rope: factor must be positive";
+    if (!(r->mscale > 0.0f) || !std::isfinite(r->mscale)) return "rope: mscale must be positive";
+    if (r->orig_ctx < 0) return "rope: orig_ctx must not be negative";
+    if (r->orig_ctx > 0 && !(std::isfinite(r->low_turns) && std::isfinite(r->high_turns) && r->high_turns > r->low_turns))
+        return "rope: high_turns must be above low_turns";
+    return nullptr;
+}
+
+inline const char * check_pages(const z2h_pages * p) {
+    if (!p) return "null pages";
+    if (!p->k || !p->v || !p->table) return "pages: null buffer or table";
+    if (p->type != Z2H_F16 && p->type != Z2H_BF16) return "pages: the cache must be F16 or BF16";
+    if (p->head_dim != 32 && p->head_dim != 64 && p->head_dim != 128) return "pages: head_dim must be 32, 64 or 128";
+    if (p->page_rows < 16 || p->page_rows > 4096 || (p->page_rows & (p->page_rows - 1))) return "pages: page_rows must be a power of two, 16 .. 4096";
+    if (p->n_pages <= 0 || p->n_head_kv <= 0 || p->n_head_kv > 1024 || p->n_seq <= 0 || p->n_seq > (1 << 24) || p->table_len <= 0)
+        return "pages: counts out of range";
+    if ((int64_t) p->table_len * p->page_rows > (1ll << 30)) return "pages: a sequence of more than 2^30 rows";
+    if (p->page_stride < (int64_t) p->n_head_kv * p->page_rows * p->head_dim) return "pages: page_stride below a page's size";
+    if (p->page_stride % 8 || (uintptr_t) p->k % 16 || (uintptr_t) p->v % 16) return "pages: k, v and page_stride must be 16-byte aligned";
+    return nullptr;
+}
+
+inline int type_size(int type) { return type == Z2H_F32 ? 4 : type == Z2H_F16 || type == Z2H_BF16 ? 2 : 0; }
+
+// a row tensor of n_head heads: rows `stride` elements apart, elements aligned to their size
+inline const char * check_rows(const void * p, int64_t stride, int n_head, int head_dim, int type) {
+    if (!p) return "null row tensor";
+    if (!type_size(type)) return "row type must be F32, F16 or BF16";
+    if (stride < (int64_t) n_head * head_dim) return "row stride below a row's size";
+    if ((uintptr_t) p % type_size(type)) return "row tensor not aligned to its elements";
+    return nullptr;
+}
+
+inline const char * check_attn(const z2h_pages * p, int n_head, int n_rows, int n_group) {
+    if (const char * e = check_pages(p)) return e;
+    if (n_head <= 0 || n_head % p->n_head_kv || n_head / p->n_head_kv > MAX_GROUP) return "n_head must be 1 .. 64 times n_head_kv";
+    if (n_rows < 0 || (int64_t) n_rows * n_head > MAX_ROW_HEADS) return "n_rows out of range";
+    if (n_group < 0 || n_group > p->n_seq) return "n_group out of range (0 .. n_seq)";
+    return nullptr;
+}
+
+inline const char * check_attn_type(int type, int cache) {
+    if (type == Z2H_F32 || type == Z2H_F16) return cache == Z2H_F16 ? nullptr : "F32 and F16 queries need F16 pages";
+    if (type == Z2H_BF16) return cache == Z2H_BF16 ? nullptr : "BF16 queries need BF16 pages";
+    return "query type must be F32, F16 or BF16";
+}
+
+inline const char * check_verify(int n_seq, int n_draft_max, int n_codebooks, int vocab) {
+    if (n_seq < 0 || n_seq > (1 << 20) || n_draft_max < 0 || n_draft_max > 4096 || n_codebooks <= 0 || n_codebooks > 1024)
+        return "verify: counts out of range";
+    if (vocab <= 0 || vocab > MAX_VOCAB) return "verify: vocab out of range (1 .. 2^20)";
+    if ((int64_t) n_seq * (n_draft_max + 1) * n_codebooks > (1ll << 30)) return "verify: too many rows";
+    return nullptr;
+}
+
+// ---- rotary frequencies: turns per position of every pair (theta' / 2 pi)
+inline void rope_turns(const z2h_rope & r, double * turns) {
+    const double two_pi = 6.283185307179586476925;
+    for (int i = 0; i < r.n_dims / 2; ++i) {
+        const double theta = std::pow((double) r.base, -2.0 * i / r.n_dims);
+        double keep = 0.0;
+        if (r.orig_ctx > 0) {
+            keep = (r.orig_ctx * theta / two_pi - (double) r.low_turns) / ((double) r.high_turns - (double) r.low_turns);
+            keep = keep < 0.0 ? 0.0 : keep > 1.0 ? 1.0 : keep;
+        }
+        turns[i] = theta * (keep + (1.0 - keep) / (double) r.factor) / two_pi;
+    }
+}
+
+// ---- pages
+// The page that holds row `pos` of sequence `seq`; -1 where the sequence, the position or the entry is out of range.
+Z2O_HD int page_of(const int32_t * table, int n_seq, int table_len, int n_pages, int page_shift, int seq, int pos) {
+    if (seq < 0 || seq >= n_seq || pos < 0 || (pos >> page_shift) >= table_len) return -1;
+    const int page = table[(int64_t) seq * table_len + (pos >> page_shift)];
+    return page >= 0 && page < n_pages ? page : -1;
+}
+inline int page_shift_of(int page_rows) { int s = 0; while ((1 << s) < page_rows) ++s; return s; }
+
+// ---- attention workspace
+struct AttnWs {
+    int64_t rows = 0, bytes = 0;                   // offsets in bytes; the header is at 0
+};
+inline int64_t align256(int64_t n) { return (n + 255) & ~(int64_t) 255; }
+inline AttnWs attn_ws(const z2h_pages & p, int n_head, int n_rows, int n_group) {
+    (void) p; (void) n_head; (void) n_group;
+    AttnWs w;
+    w.rows = 256;
+    w.bytes = w.rows + align256((int64_t) n_rows * 32);
+    return w;
+}
+
+inline int64_t verify_ws_bytes(int n_seq, int n_draft_max, int n_codebooks, int vocab) {
+    (void) vocab;
+    return align256((int64_t) n_seq * (n_draft_max + 1) * n_codebooks * 16 + 256);
+}
+
+} // namespace z2o

@@ -9,6 +9,7 @@ import numpy as np
 
 from .lib import _load
 
+F32, F16, BF16 = 0, 1, 30                       # element types of the operators on device tensors
 OK, EINVAL, ENOMEM, EDEVICE, ESTATE, ENOTSUP = range(6)
 CAP = {n: i for i, n in enumerate(
     ("res_in", "attn_in", "q", "k", "v", "gate", "attn_o", "attn_out", "ffn_in", "router_state", "router_logits",
@@ -69,6 +70,13 @@ def lib() -> C.CDLL:
         "z2h_set_prefill_chunk": (i32, [vp, i32]),
         "z2h_sample_feed": (i32, [vp, i32, vp, vp, vp, i32, vp, vp]),
         "z2h_step_resident": (i32, [vp, i32]),
+        "z2h_rope_rows": (i32, [vp, vp, i32, i32, i32, i32, vp, i64, vp, i64, vp, vp]),
+        "z2h_paged_append": (i32, [vp, vp, vp, i32, vp, vp, i32, vp, i64, vp, i64, i32, vp, i64, vp, i64, vp]),
+        "z2h_paged_ws_bytes": (i64, [vp, vp, i32, i32, i32]),
+        "z2h_paged_plan": (i32, [vp, vp, i32, i32, vp, vp, i32, vp, vp, vp, i64, vp]),
+        "z2h_paged_attn": (i32, [vp, vp, i32, i32, i32, C.c_float, i32, vp, i64, vp, i64, vp, i64, vp]),
+        "z2h_verify_ws_bytes": (i64, [i32, i32, i32, i32]),
+        "z2h_verify": (i32, [vp, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, vp]),
         "z2h_last_error": (C.c_char_p, [vp]),
         "z2h_destroy": (None, [vp]),
     }
@@ -86,7 +94,8 @@ EXPORTS = ("z2h_model_create", "z2h_model_upload_tensor", "z2h_model_finalize", 
            "z2h_set_expert_mask", "z2h_set_logit_bias", "z2h_set_capture", "z2h_capture_bytes",
            "z2h_read_capture", "z2h_device_bytes", "z2h_set_graphs", "z2h_profile_begin", "z2h_profile_end", "z2h_sample", "z2h_set_prefill_chunk",
            "z2h_sample_feed", "z2h_step_resident", "z2h_create_batch_rows", "z2h_step_mixed",
-           "z2h_last_error", "z2h_destroy")
+           "z2h_rope_rows", "z2h_paged_append", "z2h_paged_ws_bytes", "z2h_paged_plan", "z2h_paged_attn", "z2h_verify_ws_bytes",
+           "z2h_verify", "z2h_last_error", "z2h_destroy")
 KERNEL_FAMILIES = ("resnorm", "gemv_qkv", "qkv_post", "attn", "attn_combine", "gemv_wo", "router_down", "router_tail",
                    "gemv_gateup", "gemv_down", "gemv_dense", "gemv_head", "swiglu")
 
@@ -99,6 +108,22 @@ class Sampling(C.Structure):
     """z2h_sampling (include/z2h.h)."""
     _fields_ = [("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float), ("min_p", C.c_float),
                 ("rep_penalty", C.c_float), ("rep_codebooks", C.c_int32), ("greedy", C.c_int32), ("reserved", C.c_int32)]
+
+
+class Rope(C.Structure):
+    """z2h_rope (include/z2h.h)."""
+    _fields_ = [("base", C.c_float), ("n_dims", C.c_int32), ("halves", C.c_int32), ("factor", C.c_float),
+                ("low_turns", C.c_float), ("high_turns", C.c_float), ("orig_ctx", C.c_int32), ("mscale", C.c_float)]
+
+    def __init__(self, base=10000.0, n_dims=0, halves=0, factor=1.0, low_turns=0.0, high_turns=0.0, orig_ctx=0, mscale=1.0):
+        super().__init__(base, n_dims, halves, factor, low_turns, high_turns, orig_ctx, mscale)
+
+
+class Pages(C.Structure):
+    """z2h_pages (include/z2h.h): one layer's paged cache; k, v and table are device pointers (ints)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_int64), ("type", C.c_int32), ("n_pages", C.c_int32),
+                ("page_rows", C.c_int32), ("n_head_kv", C.c_int32), ("head_dim", C.c_int32), ("n_seq", C.c_int32),
+                ("table_len", C.c_int32), ("table", C.c_void_p)]
 
 
 class Z2HError(RuntimeError):
@@ -330,6 +355,44 @@ class Context:
         self.check(lib().z2h_sample(self.ctx, n, C.c_void_p(d_logits) if d_logits else None, C.cast(arr, C.c_void_p),
                                     _p(hist), _p(hist_len), cap, _p(u), _p(codes)))
         return codes
+
+    # ---- operators on device tensors: pointers are ints (torch's data_ptr()), 0 = NULL; stream is a hipStream_t
+    # handle, 0 or None = the null stream
+    def rope_rows(self, rope, n_rows, n_head, head_dim, type, d_x, x_stride, d_out, out_stride, d_pos, stream=None):
+        self.check(lib().z2h_rope_rows(self.ctx, C.byref(rope), n_rows, n_head, head_dim, type, d_x, x_stride, d_out, out_stride,
+                                       d_pos, stream))
+
+    def paged_append(self, pages, rope, n_rows, d_seq, d_pos, type, d_k, k_stride, d_v, v_stride, n_head=0, d_q=0, q_stride=0,
+                     d_q_out=0, q_out_stride=0, stream=None):
+        self.check(lib().z2h_paged_append(self.ctx, C.byref(pages), C.byref(rope), n_rows, d_seq, d_pos, type, d_k, k_stride,
+                                          d_v, v_stride, n_head, d_q, q_stride, d_q_out, q_out_stride, stream))
+
+    def paged_ws_bytes(self, pages, n_head, n_rows, n_group) -> int:
+        n = int(lib().z2h_paged_ws_bytes(self.ctx, C.byref(pages), n_head, n_rows, n_group))
+        if n <= 0:
+            raise Z2HError(EINVAL, lib().z2h_last_error(self.ctx).decode())
+        return n
+
+    def paged_plan(self, pages, n_head, n_rows, d_row_start, d_kv_len, n_group, d_group_start, d_prefix_len, d_ws, ws_bytes,
+                   stream=None):
+        self.check(lib().z2h_paged_plan(self.ctx, C.byref(pages), n_head, n_rows, d_row_start, d_kv_len, n_group, d_group_start,
+                                        d_prefix_len, d_ws, ws_bytes, stream))
+
+    def paged_attn(self, pages, n_head, n_rows, n_group, scale, type, d_q, q_stride, d_out, out_stride, d_ws, ws_bytes,
+                   stream=None):
+        self.check(lib().z2h_paged_attn(self.ctx, C.byref(pages), n_head, n_rows, n_group, scale, type, d_q, q_stride, d_out,
+                                        out_stride, d_ws, ws_bytes, stream))
+
+    def verify_ws_bytes(self, n_seq, n_draft_max, n_codebooks, vocab) -> int:
+        n = int(lib().z2h_verify_ws_bytes(n_seq, n_draft_max, n_codebooks, vocab))
+        if n <= 0:
+            raise Z2HError(EINVAL, "z2h_verify: sizes out of range")
+        return n
+
+    def verify(self, n_seq, n_draft_max, n_codebooks, vocab, d_draft, d_n_draft, d_target, d_temperature, d_draft_probs,
+               d_u_accept, d_u_draw, d_n_accept, d_codes, d_ws, ws_bytes, stream=None):
+        self.check(lib().z2h_verify(self.ctx, n_seq, n_draft_max, n_codebooks, vocab, d_draft, d_n_draft, d_target, d_temperature,
+                                    d_draft_probs, d_u_accept, d_u_draw, d_n_accept, d_codes, d_ws, ws_bytes, stream))
 
     def device_bytes(self, what: int) -> int:
         return int(lib().z2h_device_bytes(self.ctx, what))
