@@ -1,6 +1,7 @@
 // The checks and index rules of the operators on device tensors (csrc/z2h_ops_rules.h), without a GPU: prints "ok" or the
 // first thing that is wrong.
 #include "../../zonos2.cpp_amd/csrc/z2h_ops_rules.h"
+#include <algorithm>
 #include <cstdio>
 #include <cstdlib>
 #include <limits>
@@ -92,7 +93,56 @@ static void rows() {
     EXPECT(z2o::check_verify(1 << 20, 4096, 1024, 5));
 }
 
+// the work of random batches, cut as the plan cuts it, fits the workspace
+static void workspace() {
+    unsigned long long x = 12345;
+    auto rnd = [&](int n) { x = x * 6364136223846793005ull + 1442695040888963407ull; return (int) ((x >> 33) % (unsigned) n); };
+    for (int trial = 0; trial < 3000; ++trial) {
+        z2h_pages p = good_pages();
+        const int group = 1 + rnd(trial % 2 ? 8 : z2o::MAX_GROUP);
+        p.n_head_kv = 1 + rnd(16); p.n_seq = 1 + rnd(trial % 7 ? 20 : 300);
+        const int heads = group * p.n_head_kv, target = 1 + rnd(2000);
+        std::vector<int> rows(p.n_seq), len(p.n_seq), gs{0}, pre;
+        int n_rows = 0;
+        for (int s = 0; s < p.n_seq; ++s) { rows[s] = rnd(3) ? rnd(3) : rnd(400); len[s] = rnd(2) ? rnd(200) : rnd(30000); n_rows += rows[s]; }
+        while (gs.back() < p.n_seq) { gs.push_back(std::min(p.n_seq, gs.back() + 1 + rnd(40))); pre.push_back(rnd(2) ? 0 : rnd(20000)); }
+        const z2o::AttnWs w = z2o::attn_ws(p, heads, n_rows, (int) pre.size(), target);
+        struct Tile { int rows, key0, key1; };
+        std::vector<Tile> tiles;
+        const int tr = z2o::tile_rows(group);
+        EXPECT(tr >= 1 && tr * group <= z2o::TILE_RH);
+        auto span = [&](int r, int k0, int k1) { for (int i = 0; i < r; i += tr) tiles.push_back({std::min(tr, r - i), k0, k1}); };
+        for (size_t g = 0; g < pre.size(); ++g) {
+            int r = 0;
+            for (int s = gs[g]; s < gs[g + 1]; ++s) { r += rows[s]; span(rows[s], std::min(pre[g], len[gs[g]]), len[s]); }
+            if (pre[g] > 0) span(r, 0, std::min(pre[g], len[gs[g]]));
+        }
+        int64_t total = 0, items = 0, parts = 0;
+        for (auto & t : tiles) total += z2o::tile_keys(t.key0, t.key1) * p.n_head_kv;
+        const int chunk = z2o::chunk_keys(total, target);
+        EXPECT(chunk >= 128 && chunk % 128 == 0);
+        for (auto & t : tiles) {
+            const int64_t n = z2o::chunk_count(z2o::tile_keys(t.key0, t.key1), chunk);
+            items += n * p.n_head_kv;
+            parts += n * p.n_head_kv * t.rows * group;
+        }
+        EXPECT((int64_t) tiles.size() <= w.max_tiles || n_rows == 0);
+        EXPECT(items <= w.max_items && parts <= w.max_parts);
+        EXPECT(w.rows % 256 == 0 && w.tiles % 256 == 0 && w.items % 256 == 0 && w.ml % 256 == 0 && w.o % 256 == 0);
+        EXPECT(w.bytes >= w.o + w.max_parts * p.head_dim * 4 && w.o >= w.ml + w.max_parts * 8 && w.ml >= w.items + w.max_items * 32);
+    }
+    // the largest call's counts stay below 2^31
+    z2h_pages p = good_pages();
+    p.n_seq = 1 << 20; p.n_head_kv = 1;
+    const z2o::AttnWs w = z2o::attn_ws(p, 64, 1 << 20, 1 << 20, 4096);
+    EXPECT(w.max_parts < (1ll << 31) && w.max_items < (1ll << 31) && w.max_tiles < (1ll << 31));
+    p.n_head_kv = 1024; p.page_stride = 1ll << 30;
+    const z2o::AttnWs v = z2o::attn_ws(p, 1024, 1 << 16, 1 << 20, 4096);
+    EXPECT(v.max_parts < (1ll << 31) && v.max_items < (1ll << 31));
+}
+
 int main() {
+    workspace();
     pages();
     rope();
     rows();

@@ -7,6 +7,9 @@
 #include "z2h_paged.h"
 #include "z2h_verify.h"
 
+#include <algorithm>
+#include <atomic>
+
 using namespace z2d;
 
 namespace {
@@ -57,13 +60,30 @@ int rope_run(z2h_ctx * ctx, RopeArgs & a, const z2h_rope * rope, int n_rows, int
     return launched(ctx);
 }
 
+// blocks that fit the device at once (two of k_paged_attn per compute unit), and the chunks that a plan aims at
+int compute_units(int device) {
+    static std::atomic<int> known[64] = {};
+    const bool slot = device >= 0 && device < 64;
+    int n = slot ? known[device].load(std::memory_order_relaxed) : 0;
+    if (n <= 0) {
+        if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || n <= 0) return 0;
+        if (slot) known[device].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+int attn_target(int n_cu) { return 4 * n_cu; }
+
+template <int HD, typename T, typename TC>
+void attn_launch(const PagedArgs & a, int blocks, hipStream_t stream) {
+    hipLaunchKernelGGL((k_paged_attn<HD, T, TC>), dim3(blocks), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((k_paged_join<HD, T>), dim3((a.n_rows * a.n_head + 3) / 4), dim3(256), 0, stream, a);
+}
 template <int HD>
-void attn_launch(const PagedArgs & a, int type, hipStream_t stream) {
-    const dim3 grid(a.n_rows, a.n_head);
+void attn_launch(const PagedArgs & a, int type, int blocks, hipStream_t stream) {
     switch (type) {
-        case Z2H_F32: hipLaunchKernelGGL((k_paged_attn_row<HD, float, _Float16>), grid, dim3(256), 0, stream, a); break;
-        case Z2H_F16: hipLaunchKernelGGL((k_paged_attn_row<HD, _Float16, _Float16>), grid, dim3(256), 0, stream, a); break;
-        default: hipLaunchKernelGGL((k_paged_attn_row<HD, __bf16, __bf16>), grid, dim3(256), 0, stream, a); break;
+        case Z2H_F32: attn_launch<HD, float, _Float16>(a, blocks, stream); break;
+        case Z2H_F16: attn_launch<HD, _Float16, _Float16>(a, blocks, stream); break;
+        default: attn_launch<HD, __bf16, __bf16>(a, blocks, stream); break;
     }
 }
 
@@ -124,7 +144,9 @@ int z2h_paged_append(z2h_ctx * ctx, const z2h_pages * pages, const z2h_rope * ro
 int64_t z2h_paged_ws_bytes(z2h_ctx * ctx, const z2h_pages * pages, int n_head, int n_rows, int n_group) {
     if (!ctx) return 0;
     if (const char * e = z2o::check_attn(pages, n_head, n_rows, n_group)) { z2h_ctx_fail(ctx, Z2H_EINVAL, e); return 0; }
-    return z2o::attn_ws(*pages, n_head, n_rows, n_group).bytes;
+    const int n_cu = compute_units(z2h_ctx_device(ctx));
+    if (!n_cu) { z2h_ctx_fail(ctx, Z2H_EDEVICE, "compute-unit count query failed"); return 0; }
+    return z2o::attn_ws(*pages, n_head, n_rows, n_group, attn_target(n_cu)).bytes;
 }
 
 int z2h_paged_plan(z2h_ctx * ctx, const z2h_pages * pages, int n_head, int n_rows, const int32_t * d_row_start,
@@ -133,15 +155,20 @@ int z2h_paged_plan(z2h_ctx * ctx, const z2h_pages * pages, int n_head, int n_row
     if (!ctx) return Z2H_EINVAL;
     CHECK(z2o::check_attn(pages, n_head, n_rows, n_group));
     REQUIRE(d_row_start && d_kv_len && (n_group == 0 || (d_group_start && d_prefix_len)), "plan: null table");
-    const z2o::AttnWs w = z2o::attn_ws(*pages, n_head, n_rows, n_group);
+    const int n_cu = compute_units(z2h_ctx_device(ctx));
+    if (!n_cu) return z2h_ctx_fail(ctx, Z2H_EDEVICE, "compute-unit count query failed");
+    const z2o::AttnWs w = z2o::attn_ws(*pages, n_head, n_rows, n_group, attn_target(n_cu));
     CHECK(check_ws(d_ws, ws_bytes, w.bytes));
     PlanArgs a{};
     a.row_start = d_row_start; a.kv_len = d_kv_len; a.group_start = d_group_start; a.prefix_len = d_prefix_len;
-    a.n_seq = pages->n_seq; a.n_rows = n_rows; a.n_group = n_group; a.n_head = n_head; a.nkv = pages->n_head_kv; a.hd = pages->head_dim;
+    a.n_seq = pages->n_seq; a.n_rows = n_rows; a.n_group = n_group; a.n_head = n_head; a.nkv = pages->n_head_kv;
     a.cap = pages->table_len * pages->page_rows;
-    a.ws = (uint8_t *) d_ws;
+    a.target = attn_target(n_cu);
+    uint8_t * ws = (uint8_t *) d_ws;
+    a.head = (int32_t *) ws; a.rows = (PlanRow *) (ws + w.rows); a.tiles = (PlanTile *) (ws + w.tiles); a.items = (PlanItem *) (ws + w.items);
+    a.max_tiles = (int) w.max_tiles; a.max_items = (int) w.max_items; a.max_parts = (int) w.max_parts;
     ON_DEVICE;
-    hipLaunchKernelGGL(k_paged_plan, dim3(n_rows / 256 + 1), dim3(256), 0, (hipStream_t) stream, a, w.rows);
+    hipLaunchKernelGGL(k_paged_plan, dim3(1), dim3(PLAN_T), 0, (hipStream_t) stream, a);
     return launched(ctx);
 }
 
@@ -155,20 +182,26 @@ int z2h_paged_attn(z2h_ctx * ctx, const z2h_pages * pages, int n_head, int n_row
     CHECK(z2o::check_rows(d_out, out_stride, n_head, pages->head_dim, type));
     REQUIRE(d_q != d_out || q_stride == out_stride, "attention: in place with different strides");
     REQUIRE(std::isfinite(scale), "attention: scale must be finite");
-    const z2o::AttnWs w = z2o::attn_ws(*pages, n_head, n_rows, n_group);
+    const int n_cu = compute_units(z2h_ctx_device(ctx));
+    if (!n_cu) return z2h_ctx_fail(ctx, Z2H_EDEVICE, "compute-unit count query failed");
+    const z2o::AttnWs w = z2o::attn_ws(*pages, n_head, n_rows, n_group, attn_target(n_cu));
     CHECK(check_ws(d_ws, ws_bytes, w.bytes));
     if (n_rows == 0) return Z2H_OK;
     PagedArgs a{};
-    a.k = pages->k; a.v = pages->v; a.page_stride = pages->page_stride; a.qs = q_stride; a.os = out_stride; a.rows_at = w.rows;
+    a.k = pages->k; a.v = pages->v; a.page_stride = pages->page_stride; a.qs = q_stride; a.os = out_stride;
     a.table = pages->table; a.n_seq = pages->n_seq; a.table_len = pages->table_len; a.n_pages = pages->n_pages;
     a.page_shift = z2o::page_shift_of(pages->page_rows);
     a.nkv = pages->n_head_kv; a.n_head = n_head; a.n_rows = n_rows; a.n_group = n_group; a.scale = scale;
-    a.q = d_q; a.out = d_out; a.ws = (uint8_t *) d_ws;
+    a.q = d_q; a.out = d_out;
+    uint8_t * ws = (uint8_t *) d_ws;
+    a.head = (const int32_t *) ws; a.rows = (const PlanRow *) (ws + w.rows); a.items = (const PlanItem *) (ws + w.items);
+    a.part_ml = (float2 *) (ws + w.ml); a.part_o = (float *) (ws + w.o);
+    const int blocks = (int) std::min<int64_t>(w.max_items, 2 * n_cu);
     ON_DEVICE;
     switch (pages->head_dim) {
-        case 32: attn_launch<32>(a, type, (hipStream_t) stream); break;
-        case 64: attn_launch<64>(a, type, (hipStream_t) stream); break;
-        default: attn_launch<128>(a, type, (hipStream_t) stream); break;
+        case 32: attn_launch<32>(a, type, blocks, (hipStream_t) stream); break;
+        case 64: attn_launch<64>(a, type, blocks, (hipStream_t) stream); break;
+        default: attn_launch<128>(a, type, blocks, (hipStream_t) stream); break;
     }
     return launched(ctx);
 }

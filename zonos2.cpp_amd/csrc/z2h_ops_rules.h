@@ -102,16 +102,46 @@ Z2O_HD int page_of(const int32_t * table, int n_seq, int table_len, int n_pages,
 }
 inline int page_shift_of(int page_rows) { int s = 0; while ((1 << s) < page_rows) ++s; return s; }
 
+// ---- attention: how the work is cut
+// A span is a run of query rows over a run of cache rows: a group's rows over its shared prefix, a sequence's rows over the
+// rest. Its rows are cut into tiles of at most TILE_RH row-heads of one key head (32 per wave). A tile of at most
+// NARROW_RH row-heads is walked by four waves over keys of their own, a larger one by four waves over the same keys.
+constexpr int TILE_RH = 128, NARROW_RH = 32;
+Z2O_HD int tile_rows(int group) { return TILE_RH / group; }              // group <= MAX_GROUP: two rows at least
+// Keys of a tile are counted from a multiple of 64 and cut into chunks of whole steps: 128 keys where the waves take 32 each,
+// 64 where they share them.
+Z2O_HD int64_t tile_keys(int key0, int key1) { return key1 > key0 ? (int64_t) key1 - (key0 & ~63) : 0; }
+// keys per chunk: all work (keys x key heads over all tiles) divided over `target` blocks, so that blocks have alike work whatever
+// the sequences' lengths
+Z2O_HD int chunk_keys(int64_t total, int target) {
+    const int64_t c = (total + target - 1) / target;
+    return (int) (((c < 128 ? 128 : c) + 127) / 128 * 128);
+}
+Z2O_HD int chunk_count(int64_t keys, int chunk) { return (int) ((keys + chunk - 1) / chunk); }
+
 // ---- attention workspace
 struct AttnWs {
-    int64_t rows = 0, bytes = 0;                   // offsets in bytes; the header is at 0
+    int64_t rows = 0, tiles = 0, items = 0, ml = 0, o = 0, bytes = 0;    // offsets in bytes; the header is at 0
+    int64_t max_tiles = 0, max_items = 0, max_parts = 0;
 };
 inline int64_t align256(int64_t n) { return (n + 255) & ~(int64_t) 255; }
-inline AttnWs attn_ws(const z2h_pages & p, int n_head, int n_rows, int n_group) {
-    (void) p; (void) n_head; (void) n_group;
+// Every row is in at most one tile of its group's span and one of its sequence's, and a span's last tile may be partly filled.
+// Chunks of a tile: at most keys / chunk + 1, so over all tiles and key heads at most target + tiles x key heads; and of
+// partial results, row-heads of the tile each, min(TILE_RH, all rows' of one key head) x target + 2 x rows x heads.
+inline AttnWs attn_ws(const z2h_pages & p, int n_head, int n_rows, int n_group, int target) {
     AttnWs w;
+    const int group = n_head / p.n_head_kv, tr = tile_rows(group);
+    const int64_t by_span = (int64_t) p.n_seq + n_group + 2 * ((n_rows + tr - 1) / tr), by_row = 2 * (int64_t) n_rows;
+    const int64_t rh = (int64_t) n_rows * group;
+    w.max_tiles = by_span < by_row ? by_span : by_row;
+    w.max_items = n_rows ? target + w.max_tiles * p.n_head_kv : 0;
+    w.max_parts = n_rows ? (rh < TILE_RH ? rh : TILE_RH) * target + 2 * (int64_t) n_rows * n_head : 0;
     w.rows = 256;
-    w.bytes = w.rows + align256((int64_t) n_rows * 32);
+    w.tiles = w.rows + align256((int64_t) n_rows * 32);
+    w.items = w.tiles + align256(w.max_tiles * 32);
+    w.ml = w.items + align256(w.max_items * 32);
+    w.o = w.ml + align256(w.max_parts * 8);
+    w.bytes = w.o + align256(w.max_parts * p.head_dim * 4);
     return w;
 }
 
