@@ -88,7 +88,7 @@ static void rows() {
     EXPECT(z2o::check_attn(&p, 128, 1 << 20, 0) && !z2o::check_attn(&p, 64, 1 << 20, 0));
     EXPECT(!z2o::check_attn_type(Z2H_F32, Z2H_F16) && !z2o::check_attn_type(Z2H_F16, Z2H_F16) && !z2o::check_attn_type(Z2H_BF16, Z2H_BF16));
     EXPECT(z2o::check_attn_type(Z2H_F32, Z2H_BF16) && z2o::check_attn_type(Z2H_BF16, Z2H_F16) && z2o::check_attn_type(Z2H_Q4_K, Z2H_F16));
-    EXPECT(!z2o::check_verify(0, 0, 1, 1) && !z2o::check_verify(64, 7, 9, 1 << 20) && z2o::check_verify(1, 1, 1, (1 << 20) + 1));
+    EXPECT(!z2o::check_verify(0, 0, 1, 1) && !z2o::check_verify(64, 7, 9, 1 << 20) && z2o::check_verify(1 << 20, 7, 9, 1025) && z2o::check_verify(1, 1, 1, (1 << 20) + 1));
     EXPECT(z2o::check_verify(-1, 1, 1, 5) && z2o::check_verify(1, -1, 1, 5) && z2o::check_verify(1, 1, 0, 5) && z2o::check_verify(1, 1, 1, 0));
     EXPECT(z2o::check_verify(1 << 20, 4096, 1024, 5));
 }

@@ -223,11 +223,22 @@ int z2h_verify(z2h_ctx * ctx, int n_seq, int n_draft_max, int n_codebooks, int v
     a.n_seq = n_seq; a.K = n_draft_max; a.C = n_codebooks; a.V = vocab;
     a.draft = d_draft; a.n_draft = d_n_draft; a.target = d_target; a.temperature = d_temperature; a.draft_probs = d_draft_probs;
     a.u_accept = d_u_accept; a.u_draw = d_u_draw; a.n_accept = d_n_accept; a.codes = d_codes;
-    a.stats = (double *) d_ws;
+    a.n_chunk = z2o::verify_chunks(vocab);
+    a.stats = (VerifyStat *) d_ws;
+    a.sums = (double *) ((uint8_t *) d_ws + z2o::verify_stats_bytes(n_seq, n_draft_max, n_codebooks, vocab));
+    const hipStream_t st = (hipStream_t) stream;
+    const int draws = n_seq * n_codebooks;
     ON_DEVICE;
     if (d_temperature)
-        hipLaunchKernelGGL(k_verify_stats, dim3(n_seq * (n_draft_max + 1) * n_codebooks), dim3(256), 0, (hipStream_t) stream, a);
-    hipLaunchKernelGGL(k_verify, dim3(n_seq * n_codebooks), dim3(256), (size_t) ((vocab + 255) / 256) * 8, (hipStream_t) stream, a);
+        hipLaunchKernelGGL(k_verify_stats, dim3(n_seq * (n_draft_max + 1) * n_codebooks * a.n_chunk), dim3(256), 0, st, a);
+    // rows of more codes than a block's 256 threads take in a few rounds get 1024
+    if (vocab <= 4096) hipLaunchKernelGGL(k_verify<256>, dim3(draws), dim3(256), 0, st, a);
+    else if (vocab <= z2o::VERIFY_ONE) hipLaunchKernelGGL(k_verify<1024>, dim3(draws), dim3(1024), 0, st, a);
+    else {
+        a.n_share = (vocab + 8191) / 8192;
+        hipLaunchKernelGGL(k_verify_sums, dim3(draws * a.n_share), dim3(256), 0, st, a);
+        hipLaunchKernelGGL(k_verify_pick, dim3(draws), dim3(256), 0, st, a);
+    }
     return launched(ctx);
 }
 

@@ -71,14 +71,6 @@ inline const char * check_attn_type(int type, int cache) {
     return "query type must be F32, F16 or BF16";
 }
 
-inline const char * check_verify(int n_seq, int n_draft_max, int n_codebooks, int vocab) {
-    if (n_seq < 0 || n_seq > (1 << 20) || n_draft_max < 0 || n_draft_max > 4096 || n_codebooks <= 0 || n_codebooks > 1024)
-        return "verify: counts out of range";
-    if (vocab <= 0 || vocab > MAX_VOCAB) return "verify: vocab out of range (1 .. 2^20)";
-    if ((int64_t) n_seq * (n_draft_max + 1) * n_codebooks > (1ll << 30)) return "verify: too many rows";
-    return nullptr;
-}
-
 // ---- rotary frequencies: turns per position of every pair (theta' / 2 pi)
 inline void rope_turns(const z2h_rope & r, double * turns) {
     const double two_pi = 6.283185307179586476925;
@@ -145,9 +137,25 @@ inline AttnWs attn_ws(const z2h_pages & p, int n_head, int n_rows, int n_group, 
     return w;
 }
 
+// ---- verification
+constexpr int VERIFY_CHUNK = 16384;                // logits of a row per block of k_verify_stats
+constexpr int VERIFY_ONE = 32768;                  // longest rows that one block draws from
+constexpr int VERIFY_STAT_BYTES = 24;
+inline int verify_chunks(int vocab) { return (vocab + VERIFY_CHUNK - 1) / VERIFY_CHUNK; }
+constexpr int64_t MAX_VERIFY_BLOCKS = 1ll << 23;
+inline const char * check_verify(int n_seq, int n_draft_max, int n_codebooks, int vocab) {
+    if (n_seq < 0 || n_seq > (1 << 20) || n_draft_max < 0 || n_draft_max > 4096 || n_codebooks <= 0 || n_codebooks > 1024)
+        return "verify: counts out of range";
+    if (vocab <= 0 || vocab > MAX_VOCAB) return "verify: vocab out of range (1 .. 2^20)";
+    if ((int64_t) n_seq * (n_draft_max + 1) * n_codebooks * verify_chunks(vocab) > MAX_VERIFY_BLOCKS) return "verify: too many rows";
+    return nullptr;
+}
+inline int64_t verify_stats_bytes(int n_seq, int n_draft_max, int n_codebooks, int vocab) {
+    return align256((int64_t) n_seq * (n_draft_max + 1) * n_codebooks * verify_chunks(vocab) * VERIFY_STAT_BYTES);
+}
 inline int64_t verify_ws_bytes(int n_seq, int n_draft_max, int n_codebooks, int vocab) {
-    (void) vocab;
-    return align256((int64_t) n_seq * (n_draft_max + 1) * n_codebooks * 16 + 256);
+    const int64_t sums = vocab > VERIFY_ONE ? (int64_t) n_seq * n_codebooks * ((vocab + 255) / 256) * 8 : 0;
+    return 256 + verify_stats_bytes(n_seq, n_draft_max, n_codebooks, vocab) + align256(sums);
 }
 
 } // namespace z2o

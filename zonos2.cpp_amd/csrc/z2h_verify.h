@@ -1,129 +1,335 @@
 // z2h_verify.h — verification of drafted frames against the target's probabilities.
+//
+// The codes of a sequence's drafts are tested independently (u q(x) < p(x)); the first that fails decides which row each
+// codebook is drawn from, so every block finds it for itself from the handful of values it takes, and no launch waits for
+// another's verdict. A draw needs the mass of a row twice, whole and up to the code: masses are summed in pieces of 256
+// codes, the piece is found by a scan of the piece sums and the code by a scan of the piece. Everything is in 64 bits (an
+// exponential there is about 25 instructions at the full rate), so that draws are those of the definition; sums are formed
+// in a fixed order.
+//   k_verify_stats   logits: a row's largest logit, its first place, and the mass over it
+//   k_verify         the verdict and, for rows of at most VERIFY_ONE codes, the draws: one block per (sequence, codebook)
+//   k_verify_sums / k_verify_pick   longer rows: piece sums by several blocks per row, then the draw
+// Bound by reading the rows once where there are many codes, by the dependent loads of a verdict where there are few.
 #pragma once
 #include "z2h_common.h"
 #include "z2h_ops_rules.h"
 
 namespace z2d {
 
+struct VerifyStat { double max, mass; int64_t first; };          // of a chunk of a row
+static_assert(sizeof(VerifyStat) == z2o::VERIFY_STAT_BYTES, "workspace layout");
+
 struct VerifyArgs {
-    int n_seq, K, C, V;
+    int n_seq, K, C, V, n_chunk, n_share;
     const int32_t * draft, * n_draft;
     const float * target, * temperature, * draft_probs;
     const double * u_accept, * u_draw;
     int32_t * n_accept, * codes;
-    double * stats;                                // [row][2]: largest logit, mass over it
+    VerifyStat * stats;                                          // [row][n_chunk]
+    double * sums;                                               // [sequence][codebook][piece]
 };
 
-// the mass of a code whose logit is x in a row whose largest is mx (temperature > 0), or its probability
-__device__ __forceinline__ double code_mass(float x, bool logits, double mx, double T) {
-    return logits ? z_exp_d(((double) x - mx) / T) : (double) x;
+__device__ __forceinline__ double wave_max_d(double v) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v = fmax(v, __shfl_xor(v, o));
+    return v;
+}
+// sum over the lanes up to this one
+__device__ __forceinline__ double wave_scan_d(double v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double y = __shfl_up(v, o);
+        if (lane >= o) v += y;
+    }
+    return v;
 }
 
-// Of each logits row, one block: its largest logit and the sum of exp((x - largest) / temperature).
+// One block per (row, chunk): VERIFY_CHUNK logits of a row. The whole share is requested before the first is used.
 __global__ void __launch_bounds__(256) k_verify_stats(VerifyArgs a) {
-    __shared__ double s_w[4];
-    const int64_t row = blockIdx.x;
-    const int s = (int) (row / ((int64_t) (a.K + 1) * a.C)), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const float * x = a.target + row * a.V;
+    __shared__ double s_m[4], s_z[4];
+    __shared__ int s_i[4];
+    constexpr int N = z2o::VERIFY_CHUNK / 256;
+    const int64_t row = blockIdx.x / a.n_chunk;
+    const int chunk = blockIdx.x % a.n_chunk;
+    const int s = (int) (row / ((int64_t) (a.K + 1) * a.C)), k = (int) (row / a.C % (a.K + 1));
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c0 = chunk * z2o::VERIFY_CHUNK;
+    if (a.n_draft && k > min(max(a.n_draft[s], 0), a.K)) return;           // behind the last draft's successor
+    const int n = min(z2o::VERIFY_CHUNK, a.V - c0);
+    const float * x = a.target + row * a.V + c0;
     const double T = a.temperature[s];
-    float mx = -__builtin_inff();
-    for (int i = tid; i < a.V; i += 256) mx = fmaxf(mx, x[i]);
-    mx = wave_max_f(mx);
-    if (lane == 0) s_w[wave] = mx;
+    float v[N], m = -__builtin_inff();
+    // rows much shorter than a chunk take one round of it
+    const int rounds = (n + 2047) / 2048;
+#pragma unroll
+    for (int r = 0; r < N / 8; ++r)
+        if (r < rounds)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int i = tid + 256 * (8 * r + e);
+                v[8 * r + e] = i < n ? x[i] : -__builtin_inff();
+            }
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int r = 0; r < N / 8; ++r)
+        if (r < rounds)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (v[8 * r + e] > m || at == 0x7fffffff) { if (tid + 256 * (8 * r + e) < n) { m = v[8 * r + e]; at = tid + 256 * (8 * r + e); } }
+    const float wm = wave_max_f(m);
+    int wi = m == wm ? at : 0x7fffffff;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) wi = min(wi, __shfl_xor(wi, o));
+    if (lane == 0) { s_m[wave] = wm; s_i[wave] = wi; }
     __syncthreads();
-    const double m = fmax(fmax(s_w[0], s_w[1]), fmax(s_w[2], s_w[3]));
-    __syncthreads();
+    const double mx = fmax(fmax(s_m[0], s_m[1]), fmax(s_m[2], s_m[3]));
     double z = 0.0;
-    if (T > 0.0) for (int i = tid; i < a.V; i += 256) z += z_exp_d(((double) x[i] - m) / T);
+    if (T > 0.0) {
+        const double inv = 1.0 / T;
+#pragma unroll
+        for (int r = 0; r < N / 8; ++r)
+            if (r < rounds)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const double w = z_exp_d(((double) v[8 * r + e] - mx) * inv);
+                    z += tid + 256 * (8 * r + e) < n ? w : 0.0;
+                }
+    }
     z = wave_tree_d(z);
-    if (lane == 0) s_w[wave] = z;
+    if (lane == 0) s_z[wave] = z;
     __syncthreads();
-    if (tid == 0) { a.stats[2 * row] = m; a.stats[2 * row + 1] = (s_w[0] + s_w[1]) + (s_w[2] + s_w[3]); }
+    if (tid == 0) {
+        int first = 0x7fffffff;
+        for (int w = 0; w < 4; ++w) if (s_m[w] == mx) first = min(first, s_i[w]);
+        a.stats[row * a.n_chunk + chunk] = VerifyStat{mx, (s_z[0] + s_z[1]) + (s_z[2] + s_z[3]), c0 + (int64_t) (first == 0x7fffffff ? 0 : first)};
+    }
 }
 
-// One block per (sequence, codebook): the first code that is not kept, then this codebook's code of the frame behind.
-__global__ void __launch_bounds__(256) k_verify(VerifyArgs a) {
-    extern __shared__ double s_piece[];            // mass of every 256 codes
-    __shared__ int s_first, s_pick;
-    __shared__ double s_tot;
-    const int s = blockIdx.x / a.C, cb = blockIdx.x % a.C, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// a whole row's numbers from its chunks'
+__device__ __forceinline__ VerifyStat row_stat(const VerifyArgs & a, int64_t row, double T) {
+    const VerifyStat * s = a.stats + row * a.n_chunk;
+    VerifyStat r = s[0];
+    if (a.n_chunk == 1) return r;
+    for (int c = 1; c < a.n_chunk; ++c) if (s[c].max > r.max) { r.max = s[c].max; r.first = s[c].first; }
+    r.mass = 0.0;
+    const double inv = 1.0 / T;
+    if (T > 0.0) for (int c = 0; c < a.n_chunk; ++c) r.mass += s[c].mass * z_exp_d((s[c].max - r.max) * inv);
+    return r;
+}
+
+// One (sequence, codebook): the verdict, and the masses of the row its code is drawn from.
+struct VerifyRow {
+    const float * x, * q;              // target row; draft row whose mass is taken off (or null)
+    VerifyStat st;
+    double inv_T;
+    int V, drafted;                    // drafted: the code of all the draft's mass, where q is null (-1: none)
+    bool logits, greedy, rest;
+
+    // mass of code i, whose target value is x and whose draft probability is qi
+    __device__ __forceinline__ double mass(int i, float xi, float qi, bool off) const {
+        double p = greedy ? (i == st.first ? 1.0 : 0.0) : logits ? z_exp_d(((double) xi - st.max) * inv_T) / st.mass : (double) xi;
+        if (off) { p -= q ? (double) qi : i == drafted ? 1.0 : 0.0; p = p > 0.0 ? p : 0.0; }
+        return p;
+    }
+    __device__ __forceinline__ double mass_at(int i, bool off) const { return i < V ? mass(i, x[i], q && off ? q[i] : 0.0f, off) : 0.0; }
+    // sum over piece b's 256 codes, by a wave
+    template <int NB>
+    __device__ __forceinline__ void pieces(const int (&b)[NB], bool off, double (&sum)[NB]) const {
+        const int lane = threadIdx.x & 63;
+        float xv[NB][4], qv[NB][4];
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = 256 * b[n] + 64 * e + lane, j = i < V ? i : V - 1;
+                xv[n][e] = x[j];
+                qv[n][e] = q && off ? q[j] : 0.0f;
+            }
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            double w = 0.0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = 256 * b[n] + 64 * e + lane;
+                const double p = mass(i, xv[n][e], qv[n][e], off);
+                w += i < V ? p : 0.0;
+            }
+            sum[n] = wave_tree_d(w);
+        }
+    }
+};
+
+// The block's verdict on a sequence: the index of the first code that is not kept (or of the code behind the last).
+__device__ __forceinline__ int verify_first(const VerifyArgs & a, int s, int n_code, int * s_first) {
     const bool logits = a.temperature != nullptr;
-    const double T = logits ? a.temperature[s] : 1.0;
+    const double T = logits ? (double) a.temperature[s] : 1.0;
     const bool greedy = logits && !(T > 0.0);
-    const int nd = a.n_draft ? min(max(a.n_draft[s], 0), a.K) : a.K, n_code = nd * a.C;
     const int64_t row0 = (int64_t) s * (a.K + 1) * a.C, d0 = (int64_t) s * a.K * a.C;
-    if (tid == 0) s_first = n_code;
+    if (threadIdx.x == 0) *s_first = n_code;
     __syncthreads();
-    // the first of the row's largest logits, for greedy rows
-    auto first_max = [&](int64_t row) {
-        const float * x = a.target + row * a.V;
-        for (int i = 0; i < a.V; ++i) if ((double) x[i] == a.stats[2 * row]) return i;
-        return 0;
-    };
-    for (int j = tid; j < n_code; j += 256) {
+    for (int j = threadIdx.x; j < n_code; j += blockDim.x) {
         const int x = a.draft[d0 + j];
-        const int64_t row = row0 + j;
         bool keep = x >= 0 && x < a.V;
         if (keep) {
             const double u = a.u_accept[d0 + j], q = a.draft_probs ? (double) a.draft_probs[(d0 + j) * a.V + x] : 1.0;
-            if (greedy) keep = x == first_max(row) && u * q < 1.0;
-            else if (logits) keep = u * q < code_mass(a.target[row * a.V + x], true, a.stats[2 * row], T) / a.stats[2 * row + 1];
-            else keep = u * q < (double) a.target[row * a.V + x];
+            const float t = a.target[(row0 + j) * a.V + x];
+            double p = t;
+            if (logits) {
+                const VerifyStat st = row_stat(a, row0 + j, T);
+                p = greedy ? (x == st.first ? 1.0 : 0.0) : z_exp_d(((double) t - st.max) * (1.0 / T)) / st.mass;
+            }
+            keep = u * q < p;
         }
-        if (!keep) atomicMin(&s_first, j);
+        if (!keep) atomicMin(s_first, j);
     }
     __syncthreads();
-    const int first = s_first, k = first / a.C, c = first % a.C;
+    return *s_first;
+}
+__device__ __forceinline__ int verify_codes(const VerifyArgs & a, int s) { return (a.n_draft ? min(max(a.n_draft[s], 0), a.K) : a.K) * a.C; }
+
+// false: the code is the draft's own (taken over here)
+__device__ __forceinline__ bool verify_row(const VerifyArgs & a, int s, int cb, int first, int n_code, bool write, VerifyRow & r) {
+    const int k = first / a.C, c = first % a.C;
     const bool rejected = first < n_code;
-    if (cb == 0 && tid == 0) a.n_accept[s] = k;
+    const int64_t d0 = (int64_t) s * a.K * a.C;
+    if (write && cb == 0 && threadIdx.x == 0) a.n_accept[s] = k;
     if (rejected && cb < c) {
-        if (tid == 0) a.codes[(int64_t) s * a.C + cb] = a.draft[d0 + (int64_t) k * a.C + cb];
-        return;
+        if (write && threadIdx.x == 0) a.codes[(int64_t) s * a.C + cb] = a.draft[d0 + (int64_t) k * a.C + cb];
+        return false;
     }
-    const int64_t row = row0 + (int64_t) k * a.C + cb;
-    const float * x = a.target + row * a.V;
-    const double mx = logits ? a.stats[2 * row] : 0.0, Z = logits ? a.stats[2 * row + 1] : 1.0;
-    const int best = greedy ? first_max(row) : 0;
-    const int drafted = rejected ? a.draft[d0 + first] : -1;
-    const float * qr = a.draft_probs && rejected ? a.draft_probs + (d0 + first) * a.V : nullptr;
-    const int n_piece = (a.V + 255) / 256;
-    for (int pass = rejected && cb == c ? 0 : 1; pass < 2; ++pass) {
-        auto mass = [&](int i) {
-            if (i >= a.V) return 0.0;
-            double p = greedy ? (i == best ? 1.0 : 0.0) : code_mass(x[i], logits, mx, T) / Z;
-            if (pass == 0) { p -= qr ? (double) qr[i] : i == drafted ? 1.0 : 0.0; p = p > 0.0 ? p : 0.0; }
-            return p;
-        };
-        __syncthreads();
-        for (int b = wave; b < n_piece; b += 4) {
-            double w = 0.0;
-            for (int e = 0; e < 4; ++e) w += mass(256 * b + 4 * lane + e);
-            w = wave_tree_d(w);
-            if (lane == 0) s_piece[b] = w;
+    const int64_t row = ((int64_t) s * (a.K + 1) + k) * a.C + cb;
+    r.logits = a.temperature != nullptr;
+    const double T = r.logits ? (double) a.temperature[s] : 1.0;
+    r.greedy = r.logits && !(T > 0.0);
+    r.inv_T = 1.0 / T;
+    r.x = a.target + row * a.V;
+    r.V = a.V;
+    r.rest = rejected && cb == c;
+    r.q = r.rest && a.draft_probs ? a.draft_probs + (d0 + first) * a.V : nullptr;
+    r.drafted = r.rest ? a.draft[d0 + first] : -1;
+    if (r.logits) r.st = row_stat(a, row, T);
+    return true;
+}
+
+// piece sums of a row over the waves of the block: pieces [b0, b1) to out[b]
+template <int NT>
+__device__ __forceinline__ void row_pieces(const VerifyRow & r, bool off, int b0, int b1, double * out) {
+    constexpr int NB = 4, NW = NT / 64;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int b = b0 + wave; b < b1; b += NB * NW) {
+        int at[NB];
+        double sum[NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) at[n] = min(b + n * NW, b1 - 1);
+        r.template pieces<NB>(at, off, sum);
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+            if (lane == 0 && b + n * NW < b1) out[b + n * NW] = sum[n];
+    }
+}
+
+// by one wave: the code that u draws from a row's masses, given its piece sums; -1 where the row has no mass
+__device__ __forceinline__ int pick_code(const VerifyRow & r, bool off, const double * sum, int n_piece, double u) {
+    const int lane = threadIdx.x & 63;
+    double total = 0.0;
+    int last = -1;
+    for (int b0 = 0; b0 < n_piece; b0 += 64) {
+        const double w = b0 + lane < n_piece ? sum[b0 + lane] : 0.0;
+        const uint64_t some = __ballot(w > 0.0);
+        if (some) last = b0 + 63 - __builtin_clzll(some);
+        total += __shfl(wave_scan_d(w), 63);
+    }
+    if (!(total > 0.0)) return -1;
+    const double want = u * total;
+    double base = 0.0;
+    int piece = -1;
+    for (int b0 = 0; b0 < n_piece && piece < 0; b0 += 64) {
+        const double w = b0 + lane < n_piece ? sum[b0 + lane] : 0.0, cum = wave_scan_d(w);
+        const uint64_t over = __ballot(w > 0.0 && base + cum > want);
+        if (over) {
+            const int l = __ffsll((unsigned long long) over) - 1;
+            piece = b0 + l;
+            const double below = __shfl(cum, l > 0 ? l - 1 : 0);
+            base += l > 0 ? below : 0.0;
+        } else base += __shfl(cum, 63);
+    }
+    const bool none = piece < 0;                                 // rounding left no crossing: the last code with mass
+    if (none) piece = last;
+    double w[4], own = 0.0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { w[e] = r.mass_at(256 * piece + 4 * lane + e, off); own += w[e]; }
+    const double cum = wave_scan_d(own);
+    double run = base + (cum - own);
+    int hit = 0x7fffffff, end = -1;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        run += w[e];
+        if (w[e] > 0.0) {
+            end = 256 * piece + 4 * lane + e;
+            if (!none && run > want) hit = min(hit, end);
         }
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) { hit = min(hit, __shfl_xor(hit, o)); end = max(end, __shfl_xor(end, o)); }
+    return hit != 0x7fffffff ? hit : end;
+}
+
+template <int NT>
+__global__ void __launch_bounds__(NT) k_verify(VerifyArgs a) {
+    __shared__ double s_sum[z2o::VERIFY_ONE / 256];
+    __shared__ int s_first, s_none;
+    const int s = blockIdx.x / a.C, cb = blockIdx.x % a.C, n_code = verify_codes(a, s), n_piece = (a.V + 255) / 256;
+    const int first = verify_first(a, s, n_code, &s_first);
+    VerifyRow r{};
+    if (!verify_row(a, s, cb, first, n_code, true, r)) return;
+    const int64_t at = (int64_t) s * a.C + cb;
+    for (bool off = r.rest;; off = false) {
+        row_pieces<NT>(r, off, 0, n_piece, s_sum);
         __syncthreads();
-        if (tid == 0) {
-            double tot = 0.0, cum = 0.0;
-            for (int b = 0; b < n_piece; ++b) tot += s_piece[b];
-            const double want = a.u_draw[(int64_t) s * a.C + cb] * tot;
-            int b = 0, last = 0;
-            for (; b < n_piece; ++b) { if (s_piece[b] > 0.0) last = b; if (cum + s_piece[b] > want) break; cum += s_piece[b]; }
-            const bool none = b == n_piece;          // rounding left no crossing: the last code with mass
-            if (none) b = last;
-            int pick = -1, lastc = 256 * b;
-            for (int i = 256 * b; i < min(a.V, 256 * b + 256); ++i) {
-                const double w = mass(i);
-                if (w > 0.0) lastc = i;
-                cum += w;
-                if (!none && cum > want) { pick = i; break; }
+        if (threadIdx.x < 64) {
+            const int code = pick_code(r, off, s_sum, n_piece, a.u_draw[at]);
+            if (threadIdx.x == 0) {
+                s_none = code < 0;
+                a.codes[at] = max(code, 0);
             }
-            s_pick = pick >= 0 ? pick : lastc;
-            s_tot = tot;
         }
         __syncthreads();
-        if (s_tot > 0.0 || pass == 1) break;
+        if (!off || !s_none) break;                              // no mass in the rest: from p itself
     }
-    if (tid == 0) a.codes[(int64_t) s * a.C + cb] = s_pick;
+}
+
+// One block per (sequence, codebook, share of the row's pieces).
+__global__ void __launch_bounds__(256) k_verify_sums(VerifyArgs a) {
+    __shared__ int s_first;
+    const int draw = blockIdx.x / a.n_share, share = blockIdx.x % a.n_share, s = draw / a.C, cb = draw % a.C, n_code = verify_codes(a, s), n_piece = (a.V + 255) / 256;
+    const int first = verify_first(a, s, n_code, &s_first);
+    VerifyRow r{};
+    if (!verify_row(a, s, cb, first, n_code, false, r)) return;
+    const int per = (n_piece + a.n_share - 1) / a.n_share, b0 = share * per;
+    row_pieces<256>(r, r.rest, b0, min(n_piece, b0 + per), a.sums + (int64_t) draw * n_piece);
+}
+
+__global__ void __launch_bounds__(256) k_verify_pick(VerifyArgs a) {
+    __shared__ int s_first, s_none;
+    const int s = blockIdx.x / a.C, cb = blockIdx.x % a.C, n_code = verify_codes(a, s), n_piece = (a.V + 255) / 256;
+    const int first = verify_first(a, s, n_code, &s_first);
+    VerifyRow r{};
+    if (!verify_row(a, s, cb, first, n_code, true, r)) return;
+    const int64_t at = (int64_t) s * a.C + cb;
+    double * sum = a.sums + at * n_piece;
+    for (bool off = r.rest;; off = false) {
+        if (threadIdx.x < 64) {
+            const int code = pick_code(r, off, sum, n_piece, a.u_draw[at]);
+            if (threadIdx.x == 0) {
+                s_none = code < 0;
+                a.codes[at] = max(code, 0);
+            }
+        }
+        __syncthreads();
+        if (!off || !s_none) break;
+        row_pieces<256>(r, false, 0, n_piece, sum);              // no mass in the rest: from p itself
+        __syncthreads();
+    }
 }
 
 } // namespace z2d
