@@ -235,7 +235,8 @@ int z2h_verify(z2h_ctx * ctx, int n_seq, int n_draft_max, int n_codebooks, int v
     if (vocab <= 4096) hipLaunchKernelGGL(k_verify<256>, dim3(draws), dim3(256), 0, st, a);
     else if (vocab <= z2o::VERIFY_ONE) hipLaunchKernelGGL(k_verify<1024>, dim3(draws), dim3(1024), 0, st, a);
     else {
-        a.n_share = (vocab + 8191) / 8192;
+        // shares of 1024 codes (a round of the block's loads) or more, about 512 blocks in all
+        a.n_share = std::min((vocab + 1023) / 1024, std::max(1, 512 / draws));
         hipLaunchKernelGGL(k_verify_sums, dim3(draws * a.n_share), dim3(256), 0, st, a);
         hipLaunchKernelGGL(k_verify_pick, dim3(draws), dim3(256), 0, st, a);
     }

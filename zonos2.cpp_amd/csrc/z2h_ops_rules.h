@@ -138,7 +138,7 @@ inline AttnWs attn_ws(const z2h_pages & p, int n_head, int n_rows, int n_group, 
 }
 
 // ---- verification
-constexpr int VERIFY_CHUNK = 16384;                // logits of a row per block of k_verify_stats
+constexpr int VERIFY_CHUNK = 8192;                 // logits of a row per block of k_verify_stats
 constexpr int VERIFY_ONE = 32768;                  // longest rows that one block draws from
 constexpr int VERIFY_STAT_BYTES = 24;
 inline int verify_chunks(int vocab) { return (vocab + VERIFY_CHUNK - 1) / VERIFY_CHUNK; }

@@ -69,18 +69,23 @@ __global__ void __launch_bounds__(256) k_verify_stats(VerifyArgs a) {
                 const int i = tid + 256 * (8 * r + e);
                 v[8 * r + e] = i < n ? x[i] : -__builtin_inff();
             }
-    int at = 0x7fffffff;
 #pragma unroll
     for (int r = 0; r < N / 8; ++r)
         if (r < rounds)
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (v[8 * r + e] > m || at == 0x7fffffff) { if (tid + 256 * (8 * r + e) < n) { m = v[8 * r + e]; at = tid + 256 * (8 * r + e); } }
-    const float wm = wave_max_f(m);
-    int wi = m == wm ? at : 0x7fffffff;
+            for (int e = 0; e < 8; ++e) m = fmaxf(m, v[8 * r + e]);
+    m = wave_max_f(m);
+    int at = 0x7fffffff;
+    if (!(T > 0.0)) {                                            // all mass on the first of the largest
 #pragma unroll
-    for (int o = 32; o; o >>= 1) wi = min(wi, __shfl_xor(wi, o));
-    if (lane == 0) { s_m[wave] = wm; s_i[wave] = wi; }
+        for (int r = 0; r < N / 8; ++r)
+            if (r < rounds)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) if (v[8 * r + e] == m) at = min(at, tid + 256 * (8 * r + e));
+#pragma unroll
+        for (int o = 32; o; o >>= 1) at = min(at, __shfl_xor(at, o));
+    }
+    if (lane == 0) { s_m[wave] = m; s_i[wave] = at; }
     __syncthreads();
     const double mx = fmax(fmax(s_m[0], s_m[1]), fmax(s_m[2], s_m[3]));
     double z = 0.0;
@@ -101,19 +106,31 @@ __global__ void __launch_bounds__(256) k_verify_stats(VerifyArgs a) {
     if (tid == 0) {
         int first = 0x7fffffff;
         for (int w = 0; w < 4; ++w) if (s_m[w] == mx) first = min(first, s_i[w]);
-        a.stats[row * a.n_chunk + chunk] = VerifyStat{mx, (s_z[0] + s_z[1]) + (s_z[2] + s_z[3]), c0 + (int64_t) (first == 0x7fffffff ? 0 : first)};
+        a.stats[row * a.n_chunk + chunk] = VerifyStat{mx, (s_z[0] + s_z[1]) + (s_z[2] + s_z[3]), c0 + (int64_t) (first < n ? first : 0)};
     }
 }
 
-// a whole row's numbers from its chunks'
+// a whole row's numbers from its chunks' (several at a time in flight)
 __device__ __forceinline__ VerifyStat row_stat(const VerifyArgs & a, int64_t row, double T) {
     const VerifyStat * s = a.stats + row * a.n_chunk;
     VerifyStat r = s[0];
-    if (a.n_chunk == 1) return r;
-    for (int c = 1; c < a.n_chunk; ++c) if (s[c].max > r.max) { r.max = s[c].max; r.first = s[c].first; }
-    r.mass = 0.0;
+    constexpr int M = 8;
     const double inv = 1.0 / T;
-    if (T > 0.0) for (int c = 0; c < a.n_chunk; ++c) r.mass += s[c].mass * z_exp_d((s[c].max - r.max) * inv);
+    for (int c0 = 1; c0 < a.n_chunk; c0 += M) {
+        VerifyStat t[M];
+#pragma unroll
+        for (int u = 0; u < M; ++u) t[u] = s[min(c0 + u, a.n_chunk - 1)];
+        double m = r.max;
+#pragma unroll
+        for (int u = 0; u < M; ++u) if (t[u].max > m) { m = t[u].max; r.first = t[u].first; }
+        if (T > 0.0) {
+            double z = r.mass * z_exp_d((r.max - m) * inv);
+#pragma unroll
+            for (int u = 0; u < M; ++u) z += c0 + u < a.n_chunk ? t[u].mass * z_exp_d((t[u].max - m) * inv) : 0.0;
+            r.mass = z;
+        }
+        r.max = m;
+    }
     return r;
 }
 
@@ -121,20 +138,21 @@ __device__ __forceinline__ VerifyStat row_stat(const VerifyArgs & a, int64_t row
 struct VerifyRow {
     const float * x, * q;              // target row; draft row whose mass is taken off (or null)
     VerifyStat st;
-    double inv_T;
+    double inv_T, inv_mass;
     int V, drafted;                    // drafted: the code of all the draft's mass, where q is null (-1: none)
     bool logits, greedy, rest;
 
     // mass of code i, whose target value is x and whose draft probability is qi
     __device__ __forceinline__ double mass(int i, float xi, float qi, bool off) const {
-        double p = greedy ? (i == st.first ? 1.0 : 0.0) : logits ? z_exp_d(((double) xi - st.max) * inv_T) / st.mass : (double) xi;
+        double p = greedy ? (i == st.first ? 1.0 : 0.0) : logits ? z_exp_d(((double) xi - st.max) * inv_T) * inv_mass : (double) xi;
         if (off) { p -= q ? (double) qi : i == drafted ? 1.0 : 0.0; p = p > 0.0 ? p : 0.0; }
         return p;
     }
     __device__ __forceinline__ double mass_at(int i, bool off) const { return i < V ? mass(i, x[i], q && off ? q[i] : 0.0f, off) : 0.0; }
     // sum over piece b's 256 codes, by a wave
+    // (pieces n >= live are left out)
     template <int NB>
-    __device__ __forceinline__ void pieces(const int (&b)[NB], bool off, double (&sum)[NB]) const {
+    __device__ __forceinline__ void pieces(const int (&b)[NB], int live, bool off, double (&sum)[NB]) const {
         const int lane = threadIdx.x & 63;
         float xv[NB][4], qv[NB][4];
 #pragma unroll
@@ -147,6 +165,7 @@ struct VerifyRow {
             }
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
+            if (n >= live) break;
             double w = 0.0;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -159,33 +178,35 @@ struct VerifyRow {
     }
 };
 
+__device__ __forceinline__ int verify_codes(const VerifyArgs & a, int s) { return (a.n_draft ? min(max(a.n_draft[s], 0), a.K) : a.K) * a.C; }
+
 // The block's verdict on a sequence: the index of the first code that is not kept (or of the code behind the last).
-__device__ __forceinline__ int verify_first(const VerifyArgs & a, int s, int n_code, int * s_first) {
+// A thread's values are requested before the number of drafts is known: the buffers hold all K.
+__device__ __forceinline__ int verify_first(const VerifyArgs & a, int s, int & n_code, int * s_first) {
     const bool logits = a.temperature != nullptr;
     const double T = logits ? (double) a.temperature[s] : 1.0;
     const bool greedy = logits && !(T > 0.0);
     const int64_t row0 = (int64_t) s * (a.K + 1) * a.C, d0 = (int64_t) s * a.K * a.C;
-    if (threadIdx.x == 0) *s_first = n_code;
+    if (threadIdx.x == 0) *s_first = 0x7fffffff;
+    n_code = verify_codes(a, s);
     __syncthreads();
-    for (int j = threadIdx.x; j < n_code; j += blockDim.x) {
-        const int x = a.draft[d0 + j];
-        bool keep = x >= 0 && x < a.V;
-        if (keep) {
-            const double u = a.u_accept[d0 + j], q = a.draft_probs ? (double) a.draft_probs[(d0 + j) * a.V + x] : 1.0;
-            const float t = a.target[(row0 + j) * a.V + x];
-            double p = t;
-            if (logits) {
-                const VerifyStat st = row_stat(a, row0 + j, T);
-                p = greedy ? (x == st.first ? 1.0 : 0.0) : z_exp_d(((double) t - st.max) * (1.0 / T)) / st.mass;
-            }
-            keep = u * q < p;
+    const int all = a.K * a.C;
+    for (int j = threadIdx.x; j < all; j += blockDim.x) {
+        const int x = a.draft[d0 + j], xc = min(max(x, 0), a.V - 1);
+        const double u = a.u_accept[d0 + j];
+        if (j >= n_code) break;
+        const double q = a.draft_probs ? (double) a.draft_probs[(d0 + j) * a.V + xc] : 1.0;
+        const float t = a.target[(row0 + j) * a.V + xc];
+        double p = t;
+        if (logits) {
+            const VerifyStat st = row_stat(a, row0 + j, T);
+            p = greedy ? (x == st.first ? 1.0 : 0.0) : z_exp_d(((double) t - st.max) * (1.0 / T)) / st.mass;
         }
-        if (!keep) atomicMin(s_first, j);
+        if (!(x == xc && u * q < p)) atomicMin(s_first, j);
     }
     __syncthreads();
-    return *s_first;
+    return min(*s_first, n_code);
 }
-__device__ __forceinline__ int verify_codes(const VerifyArgs & a, int s) { return (a.n_draft ? min(max(a.n_draft[s], 0), a.K) : a.K) * a.C; }
 
 // false: the code is the draft's own (taken over here)
 __device__ __forceinline__ bool verify_row(const VerifyArgs & a, int s, int cb, int first, int n_code, bool write, VerifyRow & r) {
@@ -207,7 +228,7 @@ __device__ __forceinline__ bool verify_row(const VerifyArgs & a, int s, int cb, 
     r.rest = rejected && cb == c;
     r.q = r.rest && a.draft_probs ? a.draft_probs + (d0 + first) * a.V : nullptr;
     r.drafted = r.rest ? a.draft[d0 + first] : -1;
-    if (r.logits) r.st = row_stat(a, row, T);
+    if (r.logits) { r.st = row_stat(a, row, T); r.inv_mass = 1.0 / r.st.mass; }
     return true;
 }
 
@@ -216,12 +237,12 @@ template <int NT>
 __device__ __forceinline__ void row_pieces(const VerifyRow & r, bool off, int b0, int b1, double * out) {
     constexpr int NB = 4, NW = NT / 64;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int b = b0 + wave; b < b1; b += NB * NW) {
+    for (int b = __builtin_amdgcn_readfirstlane(b0 + wave); b < b1; b += NB * NW) {
         int at[NB];
         double sum[NB];
 #pragma unroll
         for (int n = 0; n < NB; ++n) at[n] = min(b + n * NW, b1 - 1);
-        r.template pieces<NB>(at, off, sum);
+        r.template pieces<NB>(at, (b1 - b + NW - 1) / NW, off, sum);
 #pragma unroll
         for (int n = 0; n < NB; ++n)
             if (lane == 0 && b + n * NW < b1) out[b + n * NW] = sum[n];
@@ -231,30 +252,30 @@ __device__ __forceinline__ void row_pieces(const VerifyRow & r, bool off, int b0
 // by one wave: the code that u draws from a row's masses, given its piece sums; -1 where the row has no mass
 __device__ __forceinline__ int pick_code(const VerifyRow & r, bool off, const double * sum, int n_piece, double u) {
     const int lane = threadIdx.x & 63;
-    double total = 0.0;
-    int last = -1;
-    for (int b0 = 0; b0 < n_piece; b0 += 64) {
-        const double w = b0 + lane < n_piece ? sum[b0 + lane] : 0.0;
-        const uint64_t some = __ballot(w > 0.0);
-        if (some) last = b0 + 63 - __builtin_clzll(some);
-        total += __shfl(wave_scan_d(w), 63);
+    // a run of pieces per lane; the run, then the piece in it
+    const int per = (n_piece + 63) / 64, p0 = per * lane, p1 = min(n_piece, p0 + per);
+    double own_run = 0.0;
+    for (int b = p0; b < p1; b += 8) {
+        double t[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t[e] = b + e < p1 ? sum[b + e] : 0.0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) own_run += t[e];
     }
+    const double runs = wave_scan_d(own_run), total = __shfl(runs, 63);
     if (!(total > 0.0)) return -1;
     const double want = u * total;
-    double base = 0.0;
-    int piece = -1;
-    for (int b0 = 0; b0 < n_piece && piece < 0; b0 += 64) {
-        const double w = b0 + lane < n_piece ? sum[b0 + lane] : 0.0, cum = wave_scan_d(w);
-        const uint64_t over = __ballot(w > 0.0 && base + cum > want);
-        if (over) {
-            const int l = __ffsll((unsigned long long) over) - 1;
-            piece = b0 + l;
-            const double below = __shfl(cum, l > 0 ? l - 1 : 0);
-            base += l > 0 ? below : 0.0;
-        } else base += __shfl(cum, 63);
-    }
-    const bool none = piece < 0;                                 // rounding left no crossing: the last code with mass
-    if (none) piece = last;
+    const uint64_t over = __ballot(own_run > 0.0 && runs > want), some = __ballot(own_run > 0.0);
+    const bool none = over == 0;                                 // rounding left no crossing: the last code with mass
+    const int l = none ? 63 - __builtin_clzll(some) : __ffsll((unsigned long long) over) - 1;
+    double base = l > 0 ? __shfl(runs, max(l - 1, 0)) : 0.0;
+    const int q0 = per * l, nq = min(n_piece, q0 + per) - q0;    // at most 64 pieces
+    const double ws = lane < nq ? sum[q0 + lane] : 0.0, cum_p = wave_scan_d(ws);
+    const uint64_t over_p = __ballot(ws > 0.0 && base + cum_p > want), some_p = __ballot(ws > 0.0);
+    const bool none_p = none || over_p == 0;
+    const int lp = none_p ? 63 - __builtin_clzll(some_p | 1) : __ffsll((unsigned long long) over_p) - 1;
+    base += lp > 0 ? __shfl(cum_p, max(lp - 1, 0)) : 0.0;
+    const int piece = q0 + lp;
     double w[4], own = 0.0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) { w[e] = r.mass_at(256 * piece + 4 * lane + e, off); own += w[e]; }
@@ -266,7 +287,7 @@ __device__ __forceinline__ int pick_code(const VerifyRow & r, bool off, const do
         run += w[e];
         if (w[e] > 0.0) {
             end = 256 * piece + 4 * lane + e;
-            if (!none && run > want) hit = min(hit, end);
+            if (!none_p && run > want) hit = min(hit, end);
         }
     }
 #pragma unroll
@@ -278,7 +299,8 @@ template <int NT>
 __global__ void __launch_bounds__(NT) k_verify(VerifyArgs a) {
     __shared__ double s_sum[z2o::VERIFY_ONE / 256];
     __shared__ int s_first, s_none;
-    const int s = blockIdx.x / a.C, cb = blockIdx.x % a.C, n_code = verify_codes(a, s), n_piece = (a.V + 255) / 256;
+    const int s = blockIdx.x / a.C, cb = blockIdx.x % a.C, n_piece = (a.V + 255) / 256;
+    int n_code;
     const int first = verify_first(a, s, n_code, &s_first);
     VerifyRow r{};
     if (!verify_row(a, s, cb, first, n_code, true, r)) return;
@@ -301,7 +323,8 @@ __global__ void __launch_bounds__(NT) k_verify(VerifyArgs a) {
 // One block per (sequence, codebook, share of the row's pieces).
 __global__ void __launch_bounds__(256) k_verify_sums(VerifyArgs a) {
     __shared__ int s_first;
-    const int draw = blockIdx.x / a.n_share, share = blockIdx.x % a.n_share, s = draw / a.C, cb = draw % a.C, n_code = verify_codes(a, s), n_piece = (a.V + 255) / 256;
+    const int draw = blockIdx.x / a.n_share, share = blockIdx.x % a.n_share, s = draw / a.C, cb = draw % a.C, n_piece = (a.V + 255) / 256;
+    int n_code;
     const int first = verify_first(a, s, n_code, &s_first);
     VerifyRow r{};
     if (!verify_row(a, s, cb, first, n_code, false, r)) return;
@@ -311,7 +334,8 @@ __global__ void __launch_bounds__(256) k_verify_sums(VerifyArgs a) {
 
 __global__ void __launch_bounds__(256) k_verify_pick(VerifyArgs a) {
     __shared__ int s_first, s_none;
-    const int s = blockIdx.x / a.C, cb = blockIdx.x % a.C, n_code = verify_codes(a, s), n_piece = (a.V + 255) / 256;
+    const int s = blockIdx.x / a.C, cb = blockIdx.x % a.C, n_piece = (a.V + 255) / 256;
+    int n_code;
     const int first = verify_first(a, s, n_code, &s_first);
     VerifyRow r{};
     if (!verify_row(a, s, cb, first, n_code, true, r)) return;
