@@ -225,12 +225,15 @@ int z2h_verify(z2h_ctx * ctx, int n_seq, int n_draft_max, int n_codebooks, int v
     a.u_accept = d_u_accept; a.u_draw = d_u_draw; a.n_accept = d_n_accept; a.codes = d_codes;
     a.n_chunk = z2o::verify_chunks(vocab);
     a.stats = (VerifyStat *) d_ws;
-    a.sums = (double *) ((uint8_t *) d_ws + z2o::verify_stats_bytes(n_seq, n_draft_max, n_codebooks, vocab));
+    uint8_t * draws_at = (uint8_t *) d_ws + z2o::verify_stats_bytes(n_seq, n_draft_max, n_codebooks, vocab);
+    a.draws = (VerifyDraw *) draws_at;
+    a.sums = (double *) (draws_at + z2o::align256((int64_t) n_seq * n_codebooks * z2o::VERIFY_DRAW_BYTES));
     const hipStream_t st = (hipStream_t) stream;
     const int draws = n_seq * n_codebooks;
     ON_DEVICE;
-    if (d_temperature)
-        hipLaunchKernelGGL(k_verify_stats, dim3(n_seq * (n_draft_max + 1) * n_codebooks * a.n_chunk), dim3(256), 0, st, a);
+    const int rows = n_seq * (n_draft_max + 1) * n_codebooks;
+    if (d_temperature && vocab <= z2o::VERIFY_SHORT) hipLaunchKernelGGL(k_verify_stats<256>, dim3(rows), dim3(256), 0, st, a);
+    else if (d_temperature) hipLaunchKernelGGL(k_verify_stats<1024>, dim3(rows * a.n_chunk), dim3(1024), 0, st, a);
     // rows of more codes than a block's 256 threads take in a few rounds get 1024
     if (vocab <= 4096) hipLaunchKernelGGL(k_verify<256>, dim3(draws), dim3(256), 0, st, a);
     else if (vocab <= z2o::VERIFY_ONE) hipLaunchKernelGGL(k_verify<1024>, dim3(draws), dim3(1024), 0, st, a);

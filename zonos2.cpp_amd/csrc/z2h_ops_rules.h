@@ -138,9 +138,10 @@ inline AttnWs attn_ws(const z2h_pages & p, int n_head, int n_rows, int n_group, 
 }
 
 // ---- verification
-constexpr int VERIFY_CHUNK = 8192;                 // logits of a row per block of k_verify_stats
+constexpr int VERIFY_PER_THREAD = 32;              // logits of a row per thread of k_verify_stats
+constexpr int VERIFY_SHORT = 256 * VERIFY_PER_THREAD, VERIFY_CHUNK = 1024 * VERIFY_PER_THREAD;
 constexpr int VERIFY_ONE = 32768;                  // longest rows that one block draws from
-constexpr int VERIFY_STAT_BYTES = 24;
+constexpr int VERIFY_STAT_BYTES = 24, VERIFY_DRAW_BYTES = 32;
 inline int verify_chunks(int vocab) { return (vocab + VERIFY_CHUNK - 1) / VERIFY_CHUNK; }
 constexpr int64_t MAX_VERIFY_BLOCKS = 1ll << 23;
 inline const char * check_verify(int n_seq, int n_draft_max, int n_codebooks, int vocab) {
@@ -154,8 +155,9 @@ inline int64_t verify_stats_bytes(int n_seq, int n_draft_max, int n_codebooks, i
     return align256((int64_t) n_seq * (n_draft_max + 1) * n_codebooks * verify_chunks(vocab) * VERIFY_STAT_BYTES);
 }
 inline int64_t verify_ws_bytes(int n_seq, int n_draft_max, int n_codebooks, int vocab) {
-    const int64_t sums = vocab > VERIFY_ONE ? (int64_t) n_seq * n_codebooks * ((vocab + 255) / 256) * 8 : 0;
-    return 256 + verify_stats_bytes(n_seq, n_draft_max, n_codebooks, vocab) + align256(sums);
+    const int64_t draws = vocab > VERIFY_ONE ? (int64_t) n_seq * n_codebooks : 0;
+    return 256 + verify_stats_bytes(n_seq, n_draft_max, n_codebooks, vocab) + align256(draws * VERIFY_DRAW_BYTES) +
+           align256(draws * ((vocab + 255) / 256) * 8);
 }
 
 } // namespace z2o

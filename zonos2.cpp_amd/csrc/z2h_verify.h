@@ -19,6 +19,9 @@ namespace z2d {
 struct VerifyStat { double max, mass; int64_t first; };          // of a chunk of a row
 static_assert(sizeof(VerifyStat) == z2o::VERIFY_STAT_BYTES, "workspace layout");
 
+struct VerifyDraw { int first, n_code; VerifyStat st; };         // a verdict and the numbers of the row that follows from it
+static_assert(sizeof(VerifyDraw) == z2o::VERIFY_DRAW_BYTES, "workspace layout");
+
 struct VerifyArgs {
     int n_seq, K, C, V, n_chunk, n_share;
     const int32_t * draft, * n_draft;
@@ -26,8 +29,36 @@ struct VerifyArgs {
     const double * u_accept, * u_draw;
     int32_t * n_accept, * codes;
     VerifyStat * stats;                                          // [row][n_chunk]
+    VerifyDraw * draws;                                          // [sequence][codebook]
     double * sums;                                               // [sequence][codebook][piece]
 };
+
+// exp(x) for x <= 0: z_exp_d's reduction and polynomial, with the whole part rounded in 32 bits and put into the
+// exponent by an integer add (64-bit rounding, conversion and scaling instructions take four times as long as a 64-bit fma).
+// Below -700 it is 0 (there z_exp_d is under 1e-304).
+__device__ __forceinline__ double exp_mass(double x) {
+    const float nf = rintf(fmaxf((float) x, -708.0f) * 1.44269504f);
+    const double n = (double) nf;
+    double r = __builtin_fma(-n, 0x1.62e42fee00000p-1, x);
+    r = __builtin_fma(-n, 0x1.a39ef35793c76p-33, r);
+    double p = 0x1.6124613a86d09p-33;                                    // 1/13!
+    p = __builtin_fma(p, r, 0x1.1eed8eff8d898p-29);
+    p = __builtin_fma(p, r, 0x1.ae64567f544e4p-26);
+    p = __builtin_fma(p, r, 0x1.27e4fb7789f5cp-22);
+    p = __builtin_fma(p, r, 0x1.71de3a556c734p-19);
+    p = __builtin_fma(p, r, 0x1.a01a01a01a01ap-16);
+    p = __builtin_fma(p, r, 0x1.a01a01a01a01ap-13);
+    p = __builtin_fma(p, r, 0x1.6c16c16c16c17p-10);
+    p = __builtin_fma(p, r, 0x1.1111111111111p-7);
+    p = __builtin_fma(p, r, 0x1.5555555555555p-5);
+    p = __builtin_fma(p, r, 0x1.5555555555555p-3);
+    p = __builtin_fma(p, r, 0.5);
+    p = __builtin_fma(p, r, 1.0);
+    p = __builtin_fma(p, r, 1.0);
+    const uint64_t b = __builtin_bit_cast(uint64_t, p) + ((uint64_t) (uint32_t) (int) nf << 52);
+    const double e = __builtin_bit_cast(double, b);
+    return x < -700.0 ? 0.0 : e;                                         // (no number stays none)
+}
 
 __device__ __forceinline__ double wave_max_d(double v) {
 #pragma unroll
@@ -45,28 +76,29 @@ __device__ __forceinline__ double wave_scan_d(double v) {
     return v;
 }
 
-// One block per (row, chunk): VERIFY_CHUNK logits of a row. The whole share is requested before the first is used.
-__global__ void __launch_bounds__(256) k_verify_stats(VerifyArgs a) {
-    __shared__ double s_m[4], s_z[4];
-    __shared__ int s_i[4];
-    constexpr int N = z2o::VERIFY_CHUNK / 256;
+// One block of NT threads per (row, chunk): NT x 32 logits of a row, all requested before the first is used.
+template <int NT>
+__global__ void __launch_bounds__(NT) k_verify_stats(VerifyArgs a) {
+    constexpr int NW = NT / 64, N = z2o::VERIFY_PER_THREAD;
+    __shared__ double s_m[NW], s_z[NW];
+    __shared__ int s_i[NW];
     const int64_t row = blockIdx.x / a.n_chunk;
     const int chunk = blockIdx.x % a.n_chunk;
     const int s = (int) (row / ((int64_t) (a.K + 1) * a.C)), k = (int) (row / a.C % (a.K + 1));
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c0 = chunk * z2o::VERIFY_CHUNK;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c0 = chunk * NT * N;
     if (a.n_draft && k > min(max(a.n_draft[s], 0), a.K)) return;           // behind the last draft's successor
-    const int n = min(z2o::VERIFY_CHUNK, a.V - c0);
+    const int n = min(NT * N, a.V - c0);
     const float * x = a.target + row * a.V + c0;
     const double T = a.temperature[s];
     float v[N], m = -__builtin_inff();
     // rows much shorter than a chunk take one round of it
-    const int rounds = (n + 2047) / 2048;
+    const int rounds = (n + 8 * NT - 1) / (8 * NT);
 #pragma unroll
     for (int r = 0; r < N / 8; ++r)
         if (r < rounds)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const int i = tid + 256 * (8 * r + e);
+                const int i = tid + NT * (8 * r + e);
                 v[8 * r + e] = i < n ? x[i] : -__builtin_inff();
             }
 #pragma unroll
@@ -81,13 +113,15 @@ __global__ void __launch_bounds__(256) k_verify_stats(VerifyArgs a) {
         for (int r = 0; r < N / 8; ++r)
             if (r < rounds)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) if (v[8 * r + e] == m) at = min(at, tid + 256 * (8 * r + e));
+                for (int e = 0; e < 8; ++e) if (v[8 * r + e] == m) at = min(at, tid + NT * (8 * r + e));
 #pragma unroll
         for (int o = 32; o; o >>= 1) at = min(at, __shfl_xor(at, o));
     }
     if (lane == 0) { s_m[wave] = m; s_i[wave] = at; }
     __syncthreads();
-    const double mx = fmax(fmax(s_m[0], s_m[1]), fmax(s_m[2], s_m[3]));
+    double mx = s_m[0];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) mx = fmax(mx, s_m[w]);
     double z = 0.0;
     if (T > 0.0) {
         const double inv = 1.0 / T;
@@ -96,8 +130,8 @@ __global__ void __launch_bounds__(256) k_verify_stats(VerifyArgs a) {
             if (r < rounds)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const double w = z_exp_d(((double) v[8 * r + e] - mx) * inv);
-                    z += tid + 256 * (8 * r + e) < n ? w : 0.0;
+                    const double w = exp_mass(((double) v[8 * r + e] - mx) * inv);
+                    z += tid + NT * (8 * r + e) < n ? w : 0.0;
                 }
     }
     z = wave_tree_d(z);
@@ -105,18 +139,23 @@ __global__ void __launch_bounds__(256) k_verify_stats(VerifyArgs a) {
     __syncthreads();
     if (tid == 0) {
         int first = 0x7fffffff;
-        for (int w = 0; w < 4; ++w) if (s_m[w] == mx) first = min(first, s_i[w]);
-        a.stats[row * a.n_chunk + chunk] = VerifyStat{mx, (s_z[0] + s_z[1]) + (s_z[2] + s_z[3]), c0 + (int64_t) (first < n ? first : 0)};
+        double mass = 0.0;
+        for (int w = 0; w < NW; ++w) {
+            if (s_m[w] == mx) first = min(first, s_i[w]);
+            mass += s_z[w];
+        }
+        a.stats[row * a.n_chunk + chunk] = VerifyStat{mx, mass, c0 + (int64_t) (first < n ? first : 0)};
     }
 }
 
-// a whole row's numbers from its chunks' (several at a time in flight)
+// a whole row's numbers from its chunks' (eight at a time in flight)
 __device__ __forceinline__ VerifyStat row_stat(const VerifyArgs & a, int64_t row, double T) {
     const VerifyStat * s = a.stats + row * a.n_chunk;
-    VerifyStat r = s[0];
+    if (a.n_chunk == 1) return s[0];
+    VerifyStat r{-__builtin_inf(), 0.0, 0};
     constexpr int M = 8;
     const double inv = 1.0 / T;
-    for (int c0 = 1; c0 < a.n_chunk; c0 += M) {
+    for (int c0 = 0; c0 < a.n_chunk; c0 += M) {
         VerifyStat t[M];
 #pragma unroll
         for (int u = 0; u < M; ++u) t[u] = s[min(c0 + u, a.n_chunk - 1)];
@@ -124,9 +163,9 @@ __device__ __forceinline__ VerifyStat row_stat(const VerifyArgs & a, int64_t row
 #pragma unroll
         for (int u = 0; u < M; ++u) if (t[u].max > m) { m = t[u].max; r.first = t[u].first; }
         if (T > 0.0) {
-            double z = r.mass * z_exp_d((r.max - m) * inv);
+            double z = c0 ? r.mass * exp_mass((r.max - m) * inv) : 0.0;
 #pragma unroll
-            for (int u = 0; u < M; ++u) z += c0 + u < a.n_chunk ? t[u].mass * z_exp_d((t[u].max - m) * inv) : 0.0;
+            for (int u = 0; u < M; ++u) z += c0 + u < a.n_chunk && t[u].max > -__builtin_inf() ? t[u].mass * exp_mass((t[u].max - m) * inv) : 0.0;
             r.mass = z;
         }
         r.max = m;
@@ -144,7 +183,7 @@ struct VerifyRow {
 
     // mass of code i, whose target value is x and whose draft probability is qi
     __device__ __forceinline__ double mass(int i, float xi, float qi, bool off) const {
-        double p = greedy ? (i == st.first ? 1.0 : 0.0) : logits ? z_exp_d(((double) xi - st.max) * inv_T) * inv_mass : (double) xi;
+        double p = greedy ? (i == st.first ? 1.0 : 0.0) : logits ? exp_mass(((double) xi - st.max) * inv_T) * inv_mass : (double) xi;
         if (off) { p -= q ? (double) qi : i == drafted ? 1.0 : 0.0; p = p > 0.0 ? p : 0.0; }
         return p;
     }
@@ -182,34 +221,45 @@ __device__ __forceinline__ int verify_codes(const VerifyArgs & a, int s) { retur
 
 // The block's verdict on a sequence: the index of the first code that is not kept (or of the code behind the last).
 // A thread's values are requested before the number of drafts is known: the buffers hold all K.
-__device__ __forceinline__ int verify_first(const VerifyArgs & a, int s, int & n_code, int * s_first) {
+constexpr int KEPT_STATS = 256;
+struct Verdict { int first; VerifyStat stat[KEPT_STATS]; };        // of code j's row, those of the frame behind the drafts too
+__device__ __forceinline__ int verify_first(const VerifyArgs & a, int s, int & n_code, Verdict & o) {
     const bool logits = a.temperature != nullptr;
     const double T = logits ? (double) a.temperature[s] : 1.0;
     const bool greedy = logits && !(T > 0.0);
     const int64_t row0 = (int64_t) s * (a.K + 1) * a.C, d0 = (int64_t) s * a.K * a.C;
-    if (threadIdx.x == 0) *s_first = 0x7fffffff;
+    if (threadIdx.x == 0) o.first = 0x7fffffff;
     n_code = verify_codes(a, s);
     __syncthreads();
     const int all = a.K * a.C;
-    for (int j = threadIdx.x; j < all; j += blockDim.x) {
-        const int x = a.draft[d0 + j], xc = min(max(x, 0), a.V - 1);
-        const double u = a.u_accept[d0 + j];
-        if (j >= n_code) break;
+    for (int j = threadIdx.x; j < all + a.C; j += blockDim.x) {
+        const int jd = min(j, all - 1), x = all ? a.draft[d0 + jd] : 0, xc = min(max(x, 0), a.V - 1);
+        const double u = all ? a.u_accept[d0 + jd] : 0.0;
+        if (j >= n_code) {
+            if (logits && j < n_code + a.C && j < KEPT_STATS) o.stat[j] = row_stat(a, row0 + j, T);
+            break;
+        }
         const double q = a.draft_probs ? (double) a.draft_probs[(d0 + j) * a.V + xc] : 1.0;
         const float t = a.target[(row0 + j) * a.V + xc];
         double p = t;
         if (logits) {
             const VerifyStat st = row_stat(a, row0 + j, T);
-            p = greedy ? (x == st.first ? 1.0 : 0.0) : z_exp_d(((double) t - st.max) * (1.0 / T)) / st.mass;
+            if (j < KEPT_STATS) o.stat[j] = st;
+            p = greedy ? (x == st.first ? 1.0 : 0.0) : exp_mass(((double) t - st.max) * (1.0 / T)) / st.mass;
         }
-        if (!(x == xc && u * q < p)) atomicMin(s_first, j);
+        if (!(x == xc && u * q < p)) atomicMin(&o.first, j);
     }
     __syncthreads();
-    return min(*s_first, n_code);
+    return min(o.first, n_code);
+}
+
+__device__ __forceinline__ const VerifyStat * kept_stat(const VerifyArgs & a, const Verdict & v, int first, int cb) {
+    const int j = first / a.C * a.C + cb;
+    return j < KEPT_STATS ? &v.stat[j] : nullptr;
 }
 
 // false: the code is the draft's own (taken over here)
-__device__ __forceinline__ bool verify_row(const VerifyArgs & a, int s, int cb, int first, int n_code, bool write, VerifyRow & r) {
+__device__ __forceinline__ bool verify_row(const VerifyArgs & a, int s, int cb, int first, int n_code, const VerifyStat * st, bool write, VerifyRow & r) {
     const int k = first / a.C, c = first % a.C;
     const bool rejected = first < n_code;
     const int64_t d0 = (int64_t) s * a.K * a.C;
@@ -228,7 +278,7 @@ __device__ __forceinline__ bool verify_row(const VerifyArgs & a, int s, int cb, 
     r.rest = rejected && cb == c;
     r.q = r.rest && a.draft_probs ? a.draft_probs + (d0 + first) * a.V : nullptr;
     r.drafted = r.rest ? a.draft[d0 + first] : -1;
-    if (r.logits) { r.st = row_stat(a, row, T); r.inv_mass = 1.0 / r.st.mass; }
+    if (r.logits) { r.st = st ? *st : row_stat(a, row, T); r.inv_mass = 1.0 / r.st.mass; }
     return true;
 }
 
@@ -298,12 +348,13 @@ __device__ __forceinline__ int pick_code(const VerifyRow & r, bool off, const do
 template <int NT>
 __global__ void __launch_bounds__(NT) k_verify(VerifyArgs a) {
     __shared__ double s_sum[z2o::VERIFY_ONE / 256];
-    __shared__ int s_first, s_none;
+    __shared__ Verdict s_v;
+    __shared__ int s_none;
     const int s = blockIdx.x / a.C, cb = blockIdx.x % a.C, n_piece = (a.V + 255) / 256;
     int n_code;
-    const int first = verify_first(a, s, n_code, &s_first);
+    const int first = verify_first(a, s, n_code, s_v);
     VerifyRow r{};
-    if (!verify_row(a, s, cb, first, n_code, true, r)) return;
+    if (!verify_row(a, s, cb, first, n_code, kept_stat(a, s_v, first, cb), true, r)) return;
     const int64_t at = (int64_t) s * a.C + cb;
     for (bool off = r.rest;; off = false) {
         row_pieces<NT>(r, off, 0, n_piece, s_sum);
@@ -322,23 +373,26 @@ __global__ void __launch_bounds__(NT) k_verify(VerifyArgs a) {
 
 // One block per (sequence, codebook, share of the row's pieces).
 __global__ void __launch_bounds__(256) k_verify_sums(VerifyArgs a) {
-    __shared__ int s_first;
+    __shared__ Verdict s_v;
     const int draw = blockIdx.x / a.n_share, share = blockIdx.x % a.n_share, s = draw / a.C, cb = draw % a.C, n_piece = (a.V + 255) / 256;
     int n_code;
-    const int first = verify_first(a, s, n_code, &s_first);
+    const int first = verify_first(a, s, n_code, s_v);
     VerifyRow r{};
-    if (!verify_row(a, s, cb, first, n_code, false, r)) return;
+    if (!verify_row(a, s, cb, first, n_code, kept_stat(a, s_v, first, cb), false, r)) {
+        if (share == 0 && threadIdx.x == 0) a.draws[draw] = VerifyDraw{first, n_code, VerifyStat{}};
+        return;
+    }
+    if (share == 0 && threadIdx.x == 0) a.draws[draw] = VerifyDraw{first, n_code, r.st};
     const int per = (n_piece + a.n_share - 1) / a.n_share, b0 = share * per;
     row_pieces<256>(r, r.rest, b0, min(n_piece, b0 + per), a.sums + (int64_t) draw * n_piece);
 }
 
 __global__ void __launch_bounds__(256) k_verify_pick(VerifyArgs a) {
-    __shared__ int s_first, s_none;
+    __shared__ int s_none;
     const int s = blockIdx.x / a.C, cb = blockIdx.x % a.C, n_piece = (a.V + 255) / 256;
-    int n_code;
-    const int first = verify_first(a, s, n_code, &s_first);
+    const VerifyDraw v = a.draws[blockIdx.x];
     VerifyRow r{};
-    if (!verify_row(a, s, cb, first, n_code, true, r)) return;
+    if (!verify_row(a, s, cb, v.first, v.n_code, &v.st, true, r)) return;
     const int64_t at = (int64_t) s * a.C + cb;
     double * sum = a.sums + at * n_piece;
     for (bool off = r.rest;; off = false) {
