@@ -234,9 +234,7 @@ int z2h_verify(z2h_ctx * ctx, int n_seq, int n_draft_max, int n_codebooks, int v
     const int rows = n_seq * (n_draft_max + 1) * n_codebooks;
     if (d_temperature && vocab <= z2o::VERIFY_SHORT) hipLaunchKernelGGL(k_verify_stats<256>, dim3(rows), dim3(256), 0, st, a);
     else if (d_temperature) hipLaunchKernelGGL(k_verify_stats<1024>, dim3(rows * a.n_chunk), dim3(1024), 0, st, a);
-    // rows of more codes than a block's 256 threads take in a few rounds get 1024
-    if (vocab <= 4096) hipLaunchKernelGGL(k_verify<256>, dim3(draws), dim3(256), 0, st, a);
-    else if (vocab <= z2o::VERIFY_ONE) hipLaunchKernelGGL(k_verify<1024>, dim3(draws), dim3(1024), 0, st, a);
+    if (vocab <= z2o::VERIFY_ONE) hipLaunchKernelGGL(k_verify, dim3(draws), dim3(256), 0, st, a);
     else {
         // shares of 1024 codes (a round of the block's loads) or more, about 512 blocks in all
         a.n_share = std::min((vocab + 1023) / 1024, std::max(1, 512 / draws));

@@ -7,7 +7,7 @@
 // exponential there is about 25 instructions at the full rate), so that draws are those of the definition; sums are formed
 // in a fixed order.
 //   k_verify_stats   logits: a row's largest logit, its first place, and the mass over it
-//   k_verify         the verdict and, for rows of at most VERIFY_ONE codes, the draws: one block per (sequence, codebook)
+//   k_verify         rows of at most VERIFY_ONE codes: the verdict and the draw, one block per (sequence, codebook)
 //   k_verify_sums / k_verify_pick   longer rows: piece sums by several blocks per row, then the draw
 // Bound by reading the rows once where there are many codes, by the dependent loads of a verdict where there are few.
 #pragma once
@@ -33,11 +33,10 @@ struct VerifyArgs {
     double * sums;                                               // [sequence][codebook][piece]
 };
 
-// exp(x) for x <= 0: z_exp_d's reduction and polynomial, with the whole part rounded in 32 bits and put into the
-// exponent by an integer add (64-bit rounding, conversion and scaling instructions take four times as long as a 64-bit fma).
-// Below -700 it is 0 (there z_exp_d is under 1e-304).
-__device__ __forceinline__ double exp_mass(double x) {
-    const float nf = rintf(fmaxf((float) x, -708.0f) * 1.44269504f);
+// exp(x) for x in [-708, 0]: z_exp_d's reduction and polynomial, with the whole part rounded in 32 bits and put into the
+// exponent by an integer add (64-bit rounding and scaling instructions take four times as long as a 64-bit fma).
+__device__ __forceinline__ double exp_core(double x) {
+    const float nf = rintf((float) x * 1.44269504f);
     const double n = (double) nf;
     double r = __builtin_fma(-n, 0x1.62e42fee00000p-1, x);
     r = __builtin_fma(-n, 0x1.a39ef35793c76p-33, r);
@@ -56,15 +55,14 @@ __device__ __forceinline__ double exp_mass(double x) {
     p = __builtin_fma(p, r, 1.0);
     p = __builtin_fma(p, r, 1.0);
     const uint64_t b = __builtin_bit_cast(uint64_t, p) + ((uint64_t) (uint32_t) (int) nf << 52);
-    const double e = __builtin_bit_cast(double, b);
-    return x < -700.0 ? 0.0 : e;                                         // (no number stays none)
+    return __builtin_bit_cast(double, b);
+}
+// exp(x) for x <= 0; 0 below -700 (z_exp_d is under 1e-304 there) and for what is no number
+__device__ __forceinline__ double exp_mass(double x) {
+    const double e = exp_core(fmax(x, -708.0));
+    return x >= -700.0 ? e : 0.0;
 }
 
-__device__ __forceinline__ double wave_max_d(double v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v = fmax(v, __shfl_xor(v, o));
-    return v;
-}
 // sum over the lanes up to this one
 __device__ __forceinline__ double wave_scan_d(double v) {
     const int lane = threadIdx.x & 63;
@@ -101,40 +99,43 @@ __global__ void __launch_bounds__(NT) k_verify_stats(VerifyArgs a) {
                 const int i = tid + NT * (8 * r + e);
                 v[8 * r + e] = i < n ? x[i] : -__builtin_inff();
             }
+    // Each thread on its own, eight logits at a time as they come in: its largest, and its mass over it.
+    const double inv = 1.0 / T;
+    double z = 0.0;
 #pragma unroll
     for (int r = 0; r < N / 8; ++r)
-        if (r < rounds)
+        if (r < rounds) {
+            float mr = m;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) m = fmaxf(m, v[8 * r + e]);
-    m = wave_max_f(m);
+            for (int e = 0; e < 8; ++e) mr = fmaxf(mr, v[8 * r + e]);
+            if (T > 0.0) {
+                const double md = mr;
+                z = r ? z * exp_mass(((double) m - md) * inv) : 0.0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    // (hidden codes and the places behind the row's end add e^-708)
+                    z += exp_core(fmax(((double) v[8 * r + e] - md) * inv, -708.0));
+                }
+            }
+            m = mr;
+        }
+    const float wm = wave_max_f(m);
     int at = 0x7fffffff;
     if (!(T > 0.0)) {                                            // all mass on the first of the largest
 #pragma unroll
         for (int r = 0; r < N / 8; ++r)
             if (r < rounds)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) if (v[8 * r + e] == m) at = min(at, tid + NT * (8 * r + e));
+                for (int e = 0; e < 8; ++e) if (v[8 * r + e] == wm) at = min(at, tid + NT * (8 * r + e));
 #pragma unroll
         for (int o = 32; o; o >>= 1) at = min(at, __shfl_xor(at, o));
     }
-    if (lane == 0) { s_m[wave] = m; s_i[wave] = at; }
+    if (lane == 0) { s_m[wave] = wm; s_i[wave] = at; }
     __syncthreads();
     double mx = s_m[0];
 #pragma unroll
     for (int w = 1; w < NW; ++w) mx = fmax(mx, s_m[w]);
-    double z = 0.0;
-    if (T > 0.0) {
-        const double inv = 1.0 / T;
-#pragma unroll
-        for (int r = 0; r < N / 8; ++r)
-            if (r < rounds)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const double w = exp_mass(((double) v[8 * r + e] - mx) * inv);
-                    z += tid + NT * (8 * r + e) < n ? w : 0.0;
-                }
-    }
-    z = wave_tree_d(z);
+    z = wave_tree_d(z * exp_mass(((double) m - mx) * inv));
     if (lane == 0) s_z[wave] = z;
     __syncthreads();
     if (tid == 0) {
@@ -165,7 +166,7 @@ __device__ __forceinline__ VerifyStat row_stat(const VerifyArgs & a, int64_t row
         if (T > 0.0) {
             double z = c0 ? r.mass * exp_mass((r.max - m) * inv) : 0.0;
 #pragma unroll
-            for (int u = 0; u < M; ++u) z += c0 + u < a.n_chunk && t[u].max > -__builtin_inf() ? t[u].mass * exp_mass((t[u].max - m) * inv) : 0.0;
+            for (int u = 0; u < M; ++u) z += c0 + u < a.n_chunk ? t[u].mass * exp_mass((t[u].max - m) * inv) : 0.0;
             r.mass = z;
         }
         r.max = m;
@@ -283,9 +284,8 @@ __device__ __forceinline__ bool verify_row(const VerifyArgs & a, int s, int cb, 
 }
 
 // piece sums of a row over the waves of the block: pieces [b0, b1) to out[b]
-template <int NT>
 __device__ __forceinline__ void row_pieces(const VerifyRow & r, bool off, int b0, int b1, double * out) {
-    constexpr int NB = 4, NW = NT / 64;
+    constexpr int NB = 4, NW = 4;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int b = __builtin_amdgcn_readfirstlane(b0 + wave); b < b1; b += NB * NW) {
         int at[NB];
@@ -345,8 +345,7 @@ __device__ __forceinline__ int pick_code(const VerifyRow & r, bool off, const do
     return hit != 0x7fffffff ? hit : end;
 }
 
-template <int NT>
-__global__ void __launch_bounds__(NT) k_verify(VerifyArgs a) {
+__global__ void __launch_bounds__(256) k_verify(VerifyArgs a) {
     __shared__ double s_sum[z2o::VERIFY_ONE / 256];
     __shared__ Verdict s_v;
     __shared__ int s_none;
@@ -357,7 +356,7 @@ __global__ void __launch_bounds__(NT) k_verify(VerifyArgs a) {
     if (!verify_row(a, s, cb, first, n_code, kept_stat(a, s_v, first, cb), true, r)) return;
     const int64_t at = (int64_t) s * a.C + cb;
     for (bool off = r.rest;; off = false) {
-        row_pieces<NT>(r, off, 0, n_piece, s_sum);
+        row_pieces(r, off, 0, n_piece, s_sum);
         __syncthreads();
         if (threadIdx.x < 64) {
             const int code = pick_code(r, off, s_sum, n_piece, a.u_draw[at]);
@@ -384,7 +383,7 @@ __global__ void __launch_bounds__(256) k_verify_sums(VerifyArgs a) {
     }
     if (share == 0 && threadIdx.x == 0) a.draws[draw] = VerifyDraw{first, n_code, r.st};
     const int per = (n_piece + a.n_share - 1) / a.n_share, b0 = share * per;
-    row_pieces<256>(r, r.rest, b0, min(n_piece, b0 + per), a.sums + (int64_t) draw * n_piece);
+    row_pieces(r, r.rest, b0, min(n_piece, b0 + per), a.sums + (int64_t) draw * n_piece);
 }
 
 __global__ void __launch_bounds__(256) k_verify_pick(VerifyArgs a) {
@@ -405,7 +404,7 @@ __global__ void __launch_bounds__(256) k_verify_pick(VerifyArgs a) {
         }
         __syncthreads();
         if (!off || !s_none) break;
-        row_pieces<256>(r, false, 0, n_piece, sum);              // no mass in the rest: from p itself
+        row_pieces(r, false, 0, n_piece, sum);              // no mass in the rest: from p itself
         __syncthreads();
     }
 }
