@@ -91,14 +91,27 @@ __global__ void __launch_bounds__(NT) k_verify_stats(VerifyArgs a) {
     float v[N], m = -__builtin_inff();
     // rows much shorter than a chunk take one round of it
     const int rounds = (n + 8 * NT - 1) / (8 * NT);
+    // value e of round r is logit `place(r, e)`: long rows are read 16 bytes at a time
+    auto place = [&](int r, int e) { return NT == 256 ? tid + NT * (8 * r + e) : 4 * (tid + NT * (2 * r + e / 4)) + e % 4; };
+    const bool wide = NT > 256 && ((uintptr_t) x & 15) == 0 && n % 4 == 0;
 #pragma unroll
     for (int r = 0; r < N / 8; ++r)
-        if (r < rounds)
+        if (r < rounds) {
+            if (wide) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int i = tid + NT * (8 * r + e);
-                v[8 * r + e] = i < n ? x[i] : -__builtin_inff();
+                for (int e = 0; e < 8; e += 4) {
+                    const int i = place(r, e);
+                    const float4 y = i < n ? *(const float4 *) (x + i) : make_float4(m, m, m, m);
+                    v[8 * r + e] = y.x; v[8 * r + e + 1] = y.y; v[8 * r + e + 2] = y.z; v[8 * r + e + 3] = y.w;
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int i = place(r, e);
+                    v[8 * r + e] = i < n ? x[i] : -__builtin_inff();
+                }
             }
+        }
     // Each thread on its own, eight logits at a time as they come in: its largest, and its mass over it.
     const double inv = 1.0 / T;
     double z = 0.0;
@@ -126,7 +139,7 @@ __global__ void __launch_bounds__(NT) k_verify_stats(VerifyArgs a) {
         for (int r = 0; r < N / 8; ++r)
             if (r < rounds)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) if (v[8 * r + e] == wm) at = min(at, tid + NT * (8 * r + e));
+                for (int e = 0; e < 8; ++e) if (v[8 * r + e] == wm) at = min(at, place(r, e));
 #pragma unroll
         for (int o = 32; o; o >>= 1) at = min(at, __shfl_xor(at, o));
     }
