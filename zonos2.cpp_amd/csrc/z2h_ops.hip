@@ -38,8 +38,19 @@ int launched(z2h_ctx * ctx) {
 
 template <typename T, typename TC>
 void rope_launch(const RopeArgs & a, int n_rows, bool halves, hipStream_t stream) {
-    if (halves) hipLaunchKernelGGL((k_rope_append<T, TC, true>), dim3(n_rows), dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((k_rope_append<T, TC, false>), dim3(n_rows), dim3(256), 0, stream, a);
+    // 16-byte accesses where every row, head and unit of pairs allows them
+    constexpr int N = 16 / (int) sizeof(T);
+    const auto al = [](const void * p, int64_t stride) { return !p || ((uintptr_t) p % 16 == 0 && stride * (int64_t) sizeof(T) % 16 == 0); };
+    const bool wide = a.hd % N == 0 && (a.n_dims / 2) % (halves ? N : N / 2) == 0 && (a.hd - a.n_dims) % N == 0 &&
+                      al(a.q, a.qs) && al(a.q_out, a.qos) && al(a.k, a.ks) && al(a.v, a.vs);
+    // few rows: their heads over several blocks, so that a row is one round of loads
+    const int np = !wide ? 1 : halves ? N : N / 2, units = a.n_dims / 2 / np + (a.hd - a.n_dims) / (wide ? N : 1);
+    const int rounds = (a.nh + a.nkv + 256 / units - 1) / (256 / units);
+    const dim3 grid(n_rows, std::min(rounds, std::max(1, 1024 / n_rows)));
+    if (halves && wide) hipLaunchKernelGGL((k_rope_append<T, TC, true, true>), grid, dim3(256), 0, stream, a);
+    else if (halves) hipLaunchKernelGGL((k_rope_append<T, TC, true, false>), grid, dim3(256), 0, stream, a);
+    else if (wide) hipLaunchKernelGGL((k_rope_append<T, TC, false, true>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((k_rope_append<T, TC, false, false>), grid, dim3(256), 0, stream, a);
 }
 template <typename T>
 void rope_launch(const RopeArgs & a, int n_rows, bool halves, int cache, hipStream_t stream) {

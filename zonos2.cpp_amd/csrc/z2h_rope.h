@@ -1,4 +1,9 @@
 // z2h_rope.h — rotary positions of rows of heads, and appending rotated rows to a paged cache.
+//
+//   (x, y) -> (x cos a - y sin a, x sin a + y cos a),  a = position * theta'
+// theta' is formed on the host in 64 bits (rope_turns) and travels with the kernel's arguments; the angle is reduced in 64 bits, so
+// positions up to 2^31 keep it to 4e-8 turns. A block's threads form the cosines and sines of their pairs once per row and
+// use them for all its heads. Bound by reading and writing the rows once; single tokens by the launch.
 #pragma once
 #include "z2h_common.h"
 #include "z2h_ops_rules.h"
@@ -39,48 +44,95 @@ struct RopeArgs {
     int n_seq, table_len, n_pages, page_shift;
 };
 
-// One row per block: its pairs' cos and sin once, then every head. Pairs (and the dims behind them) over the threads.
-template <typename T, typename TC, bool HALVES>
+template <int N, typename T> struct VecOf { typedef T type __attribute__((ext_vector_type(N))); };
+template <typename T> struct VecOf<1, T> { struct type { T x; __device__ T & operator[](int) { return x; } __device__ const T & operator[](int) const { return x; } }; };
+template <int N, typename T>
+__device__ __forceinline__ void load_f32(float (&o)[N], const T * p) {
+    const typename VecOf<N, T>::type x = *(const typename VecOf<N, T>::type *) p;
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = (float) x[i];
+}
+template <int N, typename T>
+__device__ __forceinline__ void store_as(T * p, const float (&o)[N]) {
+    typename VecOf<N, T>::type x;
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = (T) o[i];
+    *(typename VecOf<N, T>::type *) p = x;
+}
+
+// values a thread takes of a row at a time: 16 bytes of T, or one pair
+template <typename T, bool WIDE> struct RopeUnit { static constexpr int N = WIDE ? 16 / (int) sizeof(T) : 1; };
+
+// grid (rows, shares of the heads). A thread keeps one unit of a head (pairs, or dims behind them) and walks the heads: rotated
+// query heads, then rotated key heads and copied value heads. WIDE: rows, strides and pairs allow 16-byte accesses.
+template <typename T, typename TC, bool HALVES, bool WIDE>
 __global__ void __launch_bounds__(256) k_rope_append(RopeArgs a) {
+    constexpr int N = RopeUnit<T, WIDE>::N, NP = HALVES ? N : WIDE ? N / 2 : 1;      // values behind the pairs; pairs per unit
     const int t = blockIdx.x, tid = threadIdx.x;
-    const int seq = a.seq ? a.seq[t] : 0;
+    const int seq = a.seq ? a.seq[t] : 0, pos = a.pos[t];
     if (a.seq && (seq < 0 || seq >= a.n_seq)) return;
-    const int pos = a.pos[t], np = a.n_dims / 2, rest = a.hd - a.n_dims, U = np + rest, HL = 256 / U;
+    const int half = a.n_dims / 2, up = half / NP, U = up + (a.hd - a.n_dims) / N, HL = 256 / U;
     const int u = tid % U, hl = tid / U;
-    if (hl >= HL) return;
     int page = -1;
     if (a.k) page = z2o::page_of(a.table, a.n_seq, a.table_len, a.n_pages, a.page_shift, seq, pos);
     const int64_t cell = page < 0 ? 0 : page * a.page_stride + (int64_t) (pos & ((1 << a.page_shift) - 1)) * a.hd;
     const int64_t head_step = (int64_t) a.hd << a.page_shift;
-    float c = 0.0f, s = 0.0f;
-    const bool pair = u < np;
-    if (pair) {
-        turn_sincos((double) pos * a.turn[u], s, c);
-        c *= a.mscale; s *= a.mscale;
-    }
-    const int i0 = pair ? (HALVES ? u : 2 * u) : a.n_dims + u - np, i1 = pair ? (HALVES ? u + np : 2 * u + 1) : i0;
-    for (int h = hl; h < a.nh; h += HL) {
-        const T * x = (const T *) a.q + t * a.qs + (int64_t) h * a.hd;
-        T * y = (T *) a.q_out + t * a.qos + (int64_t) h * a.hd;
-        const float x0 = (float) x[i0], x1 = (float) x[i1];
-        if (!pair) y[i0] = (T) x0;
-        else {
-            y[i0] = (T) (x0 * c - x1 * s);
-            y[i1] = (T) (x0 * s + x1 * c);
+    if (hl < HL) {
+        if (u < up) {
+            float c[NP], s[NP];
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                turn_sincos((double) pos * a.turn[u * NP + i], s[i], c[i]);
+                c[i] *= a.mscale; s[i] *= a.mscale;
+            }
+            auto turn = [&](const T * x, auto * y) {
+                if constexpr (HALVES) {
+                    float p[NP], q[NP], r[NP], w[NP];
+                    load_f32(p, x + u * NP); load_f32(q, x + half + u * NP);
+#pragma unroll
+                    for (int i = 0; i < NP; ++i) { r[i] = p[i] * c[i] - q[i] * s[i]; w[i] = p[i] * s[i] + q[i] * c[i]; }
+                    store_as(y + u * NP, r); store_as(y + half + u * NP, w);
+                } else if constexpr (WIDE) {
+                    float p[2 * NP], r[2 * NP];
+                    load_f32(p, x + 2 * NP * u);
+#pragma unroll
+                    for (int i = 0; i < NP; ++i) {
+                        r[2 * i] = p[2 * i] * c[i] - p[2 * i + 1] * s[i];
+                        r[2 * i + 1] = p[2 * i] * s[i] + p[2 * i + 1] * c[i];
+                    }
+                    store_as(y + 2 * NP * u, r);
+                } else {
+                    const float p = (float) x[2 * u], q = (float) x[2 * u + 1];
+                    typedef __remove_reference_t(decltype(*y)) O;
+                    y[2 * u] = (O) (p * c[0] - q * s[0]);
+                    y[2 * u + 1] = (O) (p * s[0] + q * c[0]);
+                }
+            };
+            for (int h = hl + blockIdx.y * HL; h < a.nh + a.nkv; h += HL * gridDim.y) {
+                if (h < a.nh) turn((const T *) a.q + t * a.qs + (int64_t) h * a.hd, (T *) a.q_out + t * a.qos + (int64_t) h * a.hd);
+                else if (page >= 0) turn((const T *) a.k + t * a.ks + (int64_t) (h - a.nh) * a.hd, (TC *) a.kc + cell + (h - a.nh) * head_step);
+            }
+        } else {
+            const int d = a.n_dims + (u - up) * N;
+            float x[N];
+            for (int h = hl + blockIdx.y * HL; h < a.nh + a.nkv; h += HL * gridDim.y) {
+                if (h < a.nh) {
+                    load_f32(x, (const T *) a.q + t * a.qs + (int64_t) h * a.hd + d);
+                    store_as((T *) a.q_out + t * a.qos + (int64_t) h * a.hd + d, x);
+                } else if (page >= 0) {
+                    load_f32(x, (const T *) a.k + t * a.ks + (int64_t) (h - a.nh) * a.hd + d);
+                    store_as((TC *) a.kc + cell + (h - a.nh) * head_step + d, x);
+                }
+            }
         }
     }
     if (page < 0) return;
-    for (int g = hl; g < a.nkv; g += HL) {
-        const T * x = (const T *) a.k + t * a.ks + (int64_t) g * a.hd, * v = (const T *) a.v + t * a.vs + (int64_t) g * a.hd;
-        TC * y = (TC *) a.kc + cell + g * head_step, * w = (TC *) a.vc + cell + g * head_step;
-        const float x0 = (float) x[i0], x1 = (float) x[i1];
-        if (!pair) { y[i0] = (TC) x0; w[i0] = (TC) (float) v[i0]; }
-        else {
-            y[i0] = (TC) (x0 * c - x1 * s);
-            y[i1] = (TC) (x0 * s + x1 * c);
-            w[i0] = (TC) (float) v[i0];
-            w[i1] = (TC) (float) v[i1];
-        }
+    const int uv = a.hd / N;
+    for (int i = tid + 256 * blockIdx.y; i < a.nkv * uv; i += 256 * gridDim.y) {
+        const int g = i / uv, d = i % uv * N;
+        float x[N];
+        load_f32(x, (const T *) a.v + t * a.vs + (int64_t) g * a.hd + d);
+        store_as((TC *) a.vc + cell + g * head_step + d, x);
     }
 }
 
