@@ -77,14 +77,21 @@ __global__ void __launch_bounds__(256) k_rope_append(RopeArgs a) {
     if (a.k) page = z2o::page_of(a.table, a.n_seq, a.table_len, a.n_pages, a.page_shift, seq, pos);
     const int64_t cell = page < 0 ? 0 : page * a.page_stride + (int64_t) (pos & ((1 << a.page_shift) - 1)) * a.hd;
     const int64_t head_step = (int64_t) a.hd << a.page_shift;
+    // the row's cosines and sines once for all heads: a thread's own would take more time than its loads (8 pairs of a bf16
+    // unit, 4099 rows of 32 heads: 20.5 us against 14.0)
+    __shared__ float s_c[z2o::MAX_ROPE_DIMS / 2], s_s[z2o::MAX_ROPE_DIMS / 2];
+    if (tid < half) {
+        float c, s;
+        turn_sincos((double) pos * a.turn[tid], s, c);
+        s_c[tid] = c * a.mscale;
+        s_s[tid] = s * a.mscale;
+    }
+    lds_sync();
     if (hl < HL) {
         if (u < up) {
             float c[NP], s[NP];
 #pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                turn_sincos((double) pos * a.turn[u * NP + i], s[i], c[i]);
-                c[i] *= a.mscale; s[i] *= a.mscale;
-            }
+            for (int i = 0; i < NP; ++i) { c[i] = s_c[u * NP + i]; s[i] = s_s[u * NP + i]; }
             auto turn = [&](const T * x, auto * y) {
                 if constexpr (HALVES) {
                     float p[NP], q[NP], r[NP], w[NP];
