@@ -299,14 +299,16 @@ struct AttnWave {
         }
     }
 
-    // keys key0 .. key0 + 32 NT of the tiles; keys outside [from, min(to, vis)) are hidden
+    // keys key0 .. key0 + 32 NT, in LDS from row r0 on; keys outside [from, min(to, vis)) are hidden. One body for all steps: a second
+    // one for steps that hide something costs the compiler another set of accumulators (256 registers and 126 spilled against 237).
     template <int NT>
     __device__ __forceinline__ void step(const TC * sk, const TC * sv, int r0, int key0, int from, int to, int lane) {
+        const int end = min(to, vis);
         v16f_t s[NT];
         scores<NT>(s, sk, r0, lane);
-        const int end = min(to, vis), h4 = 4 * (lane >> 5);
-        const bool edge = __any(key0 < from || key0 + 32 * NT > end);
-        if (edge) {
+        __builtin_amdgcn_sched_barrier(0);                       // no V read ahead of the weights: registers
+        if (__any(key0 < from || key0 + 32 * NT > end)) {
+            const int h4 = 4 * (lane >> 5);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -322,9 +324,10 @@ struct AttnWave {
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[n][i]);
         mx = fmaxf(mx, other_half(mx)) * c;
         // the maximum moves only where a score exceeds it by 2^8: rarely behind the first keys
-        if (__any(mx > m + (8.0f + BIAS))) {
-            const float mn = mx > m + (8.0f + BIAS) ? mx - BIAS : m;
-            const float w = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+        const bool up = mx > m + (8.0f + BIAS);
+        if (__any(up)) {
+            const float mn = up ? mx - BIAS : m;
+            const float w = mn == m || m == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - mn);   // (nothing to scale yet)
             m = mn;
             l *= w;
 #pragma unroll
@@ -332,7 +335,6 @@ struct AttnWave {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[dt][i] *= w;
         }
-        if (edge) infinite_values<NT>(s, sv, r0, lane);
         const float mu = m == -__builtin_inff() ? 0.0f : m;
         v8 p[2 * NT], pl[SPLIT ? 2 * NT : 1];
         float sum = 0.0f;
@@ -344,20 +346,15 @@ struct AttnWave {
                 const TC hi = (TC) w;
                 p[2 * n + (i >> 3)][i & 7] = hi;
                 if constexpr (SPLIT) pl[2 * n + (i >> 3)][i & 7] = (TC) (w - (float) hi);
-                // the sum is over the weights as the products take them, so that their rounding has no mean effect
-                sum += SPLIT ? w : (float) hi;
+                sum += w;
             }
         l += sum;
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int t = 0; t < 2 * NT; ++t)
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-                s8_t v = values(sv, r0 + 16 * t, dt, lane);
-                if (edge) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] = not_finite(v[j]) ? (short) 0 : v[j];
-                }
-                const v8 vf = __builtin_bit_cast(v8, v);
+                const v8 vf = __builtin_bit_cast(v8, values(sv, r0 + 16 * t, dt, lane));
                 o[dt] = mfma32<TC>(vf, p[t], o[dt]);
                 if constexpr (SPLIT) o[dt] = mfma32<TC>(vf, pl[t], o[dt]);
             }
@@ -372,43 +369,72 @@ struct AttnWave {
         const s4_t x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *) (at + 8 * HD));
         return __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
     }
-    static constexpr unsigned EXP = __is_same(TC, _Float16) ? 0x7c00u : 0x7f80u;
-    static __device__ __forceinline__ bool not_finite(short x) { return ((unsigned) (unsigned short) x & EXP) == EXP; }
-
-    // Where some rows hide keys that others see, a hidden value that is not finite must not reach them as 0 x inf: `step` leaves such
-    // values out of its operand, and here rows that see one get infinity (or both infinities: NaN) by a product of indicators.
+    // Where some rows hide keys that others see (or that nobody has), a value that is not finite must not reach a row as 0 x inf. Such a
+    // tile's values are set to 0 in LDS, and before that rows that see one get infinity (or both infinities: NaN): the product
+    // of two numbers that are infinite together.
     template <int NT>
-    __device__ __forceinline__ void infinite_values(const v16f_t (&s)[NT], const TC * sv, int r0, int lane) {
+    __device__ __forceinline__ void infinite_values(const TC * sv, int r0, int key0, int from, int to, int lane) {
+        typedef typename Vec8<__bf16>::type b8;
+        const int end = min(to, vis), h4 = 4 * (lane >> 5);
+        const __bf16 big = (__bf16) 3e38f, none = (__bf16) 0.0f;
+#pragma unroll 1
+        for (int t = 0; t < 2 * NT; ++t) {
+            b8 seen;
 #pragma unroll
-        for (int t = 0; t < 2 * NT; ++t)
+            for (int j = 0; j < 8; ++j) {
+                const int key = key0 + 16 * t + 8 * (j >> 2) + h4 + (j & 3);
+                seen[j] = key >= from && key < end ? big : none;
+            }
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
                 const s8_t v = values(sv, r0 + 16 * t, dt, lane);
-                bool any = false;
+                b8 up, down;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) any |= not_finite(v[j]);
-                if (!__any(any)) continue;
-                v8 seen;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) seen[j] = (TC) (s[t >> 1][8 * (t & 1) + j] == -__builtin_inff() ? 0.0f : 1.0f);
-#pragma unroll
-                for (int sign = 0; sign < 2; ++sign) {
-                    v8 is;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const unsigned x = (unsigned short) v[j];
-                        const bool nan = (x & 0x7fffu) != EXP, neg = x & 0x8000u;
-                        is[j] = (TC) (not_finite(v[j]) && (nan || neg == (sign == 1)) ? 1.0f : 0.0f);
-                    }
-                    const v16f_t z = {};
-                    const v16f_t hit = mfma32<TC>(is, seen, z);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (hit[i] > 0.0f) o[dt][i] += sign ? -__builtin_inff() : __builtin_inff();
+                for (int j = 0; j < 8; ++j) {
+                    const unsigned x = (unsigned short) v[j];
+                    const bool nan = (x & 0x7fffu) > EXP, neg = x & 0x8000u, bad = (x & EXP) == EXP;
+                    up[j] = bad && (nan || !neg) ? big : none;
+                    down[j] = bad && (nan || neg) ? -big : none;
                 }
+                o[dt] = mfma32<__bf16>(up, seen, o[dt]);
+                o[dt] = mfma32<__bf16>(down, seen, o[dt]);
             }
+        }
     }
+    static constexpr unsigned EXP = __is_same(TC, _Float16) ? 0x7c00u : 0x7f80u;
 };
+
+// 16 rows of V in LDS: does one hold a value that is not finite; those values set to 0
+template <int HD, typename TC>
+__device__ __forceinline__ bool rows_not_finite(const TC * sv, int lane) {
+    constexpr unsigned EXP = __is_same(TC, _Float16) ? 0x7c00u : 0x7f80u;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i) {
+        const u4_t x = *(const u4_t *) (sv + 8 * (lane + 64 * i));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bad |= (x[j] & EXP) == EXP || (x[j] & (EXP << 16)) == EXP << 16;
+    }
+    return bad;
+}
+template <int HD, typename TC>
+__device__ __forceinline__ void clean_rows(TC * sv, int lane) {
+    constexpr unsigned EXP = __is_same(TC, _Float16) ? 0x7c00u : 0x7f80u;
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i) {
+        u4_t x = *(const u4_t *) (sv + 8 * (lane + 64 * i));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if ((x[j] & EXP) == EXP) x[j] &= 0xffff0000u;
+            if ((x[j] & (EXP << 16)) == EXP << 16) x[j] &= 0xffffu;
+        }
+        *(u4_t *) (sv + 8 * (lane + 64 * i)) = x;
+    }
+}
+
+// the wave's own loads have arrived; its own LDS reads have been answered
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); asm volatile("" ::: "memory"); }
+__device__ __forceinline__ void wait_lds() { asm volatile("" ::: "memory"); __builtin_amdgcn_s_waitcnt(0xc07f); }
 
 template <typename T>
 __device__ __forceinline__ void store4(T * p, float x0, float x1, float x2, float x3) {
@@ -421,21 +447,53 @@ __device__ __forceinline__ void store4(T * p, float x0, float x1, float x2, floa
     }
 }
 
+// 16 bytes per lane from global memory to the 1024 bytes of LDS at `to` (of one mind over the wave), in lane order, in flight until the
+// wave waits for its loads
+template <typename TC>
+__device__ __forceinline__ void to_lds(const TC * from, TC * to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) from, (__attribute__((address_space(3))) void *) to, 16, 0, 0);
+}
+
+// The lanes' places in the rows that a wave moves at a time: 64 / NC rows, row i's pieces permuted as Tile has them (the lane of
+// LDS piece x reads piece x ^ permutation of its row).
+template <int HD, typename TC>
+struct Mover {
+    static constexpr int NC = HD / 8, ROWS = 64 / NC;            // rows per instruction
+    int k[16 / ROWS], v;                                         // element offsets within 16 rows, per instruction; V's differ by whole rows
+    __device__ __forceinline__ explicit Mover(int lane) {
+        const int row = lane / NC, x = lane % NC;
+#pragma unroll
+        for (int i = 0; i < 16 / ROWS; ++i) k[i] = Tile<HD>::k_at(i * ROWS + row, x);
+        v = Tile<HD>::v_at(row, x);
+    }
+    // 16 rows from `at` (elements from the start of k and v) to the rows of LDS at sk, sv
+    // (rows 16 apart are permuted alike)
+    __device__ __forceinline__ void rows16(const PagedArgs & a, int64_t at, TC * sk, TC * sv) const {
+#pragma unroll
+        for (int i = 0; i < 16 / ROWS; ++i) {
+            to_lds((const TC *) a.k + at + k[i], sk + i * ROWS * HD);
+            to_lds((const TC *) a.v + at + i * ROWS * HD + v, sv + i * ROWS * HD);
+        }
+    }
+};
+
 template <int HD, typename T, typename TC>
 __global__ void __launch_bounds__(256, 2) k_paged_attn(PagedArgs a) {
-    constexpr int NC = HD / 8, ROWS = 128;
-    __shared__ __attribute__((aligned(16))) TC s_kv[2 * ROWS * HD];
+    // two buffers of 64 keys; arrays of their own, so that loads on their way to one do not hold up reads of the other
+    __shared__ __attribute__((aligned(1024))) TC s_k0[64 * HD], s_k1[64 * HD], s_v0[64 * HD], s_v1[64 * HD];
     __shared__ float2 s_ml[4][32];
-    TC * s_k = s_kv, * s_v = s_kv + ROWS * HD;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, group = a.n_head / a.nkv;
+    __shared__ int s_vis[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = a.n_head / a.nkv;
     if (!plan_fits(a)) return;
     const int n_items = a.head[PH_ITEMS], mask = (1 << a.page_shift) - 1;
+    const Mover<HD, TC> mv(lane);
     for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
         const PlanItem it = a.items[item];
         const int heads = it.rows * group;
         if (heads == 0) continue;
         const int64_t head_at = (int64_t) it.head << a.page_shift;
-        // elements from the start of k and v to the 16 rows that begin with `key` (one page holds them; the wave is of one mind)
+        // elements from the start of k and v to the 16 rows that begin with `key` (one page holds them; any key gives an address
+        // inside the cache)
         auto rows_at = [&](int key) __attribute__((always_inline)) {
             key = __builtin_amdgcn_readfirstlane(key);
             const int page = max(0, z2o::page_of(a.table, a.n_seq, a.table_len, a.n_pages, a.page_shift, it.seq, key));
@@ -443,56 +501,49 @@ __global__ void __launch_bounds__(256, 2) k_paged_attn(PagedArgs a) {
         };
         AttnWave<HD, T, TC> w;
         if (heads <= z2o::NARROW_RH) {
-            // ---- every wave takes 32 keys of each 128 and has its own part of LDS: nothing to wait for but its loads
-            constexpr int N = 32 * NC / 64;                      // loads of 16 bytes per lane: 32 rows
-            u4_t kr[N], vr[N];
-            TC * wk = s_k + 32 * wave * HD, * wv = s_v + 32 * wave * HD;
-            const int lrow = lane / NC, piece = lane % NC;
-            auto load = [&](int64_t at0, int64_t at1) __attribute__((always_inline)) {
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const int row = i * (64 / NC) + lrow;
-                    const int64_t at = (i < N / 2 ? at0 : at1) + (row & 15) * HD + 8 * piece;
-                    kr[i] = *(const u4_t *) ((const TC *) a.k + at);
-                    vr[i] = *(const u4_t *) ((const TC *) a.v + at);
-                }
-            };
+            // ---- every wave takes 32 keys of each 128 and has its own part of LDS: nothing to wait for but its own loads
+            TC * wk = (wave & 2 ? s_k1 : s_k0) + 32 * (wave & 1) * HD, * wv = (wave & 2 ? s_v1 : s_v0) + 32 * (wave & 1) * HD;
             int key = (it.key0 & ~31) + 32 * wave;
-            load(rows_at(key), rows_at(key + 16));
+            if (key < it.key1) { mv.rows16(a, rows_at(key), wk, wv); mv.rows16(a, rows_at(key + 16), wk + 16 * HD, wv + 16 * HD); }
             int64_t n0 = rows_at(key + 128), n1 = rows_at(key + 144);
             w.init(a, it, 0, lane);
             for (; key < it.key1; key += 128) {
-                const bool cut = key < it.key0 || key + 32 > it.key1;     // rows of no key: not read into the products
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const int row = i * (64 / NC) + lrow;
-                    if (cut && (key + row < it.key0 || key + row >= it.key1)) vr[i] = u4_t{0, 0, 0, 0};
-                    *(u4_t *) (wk + Tile<HD>::k_at(row, piece)) = kr[i];
-                    *(u4_t *) (wv + Tile<HD>::v_at(row, piece)) = vr[i];
+                wait_loads();
+                if (__any(key < it.key0 || key + 32 > min(it.key1, w.vis)) &&
+                    __any(rows_not_finite<HD>(wv, lane) || rows_not_finite<HD>(wv + 16 * HD, lane))) {
+                    w.template infinite_values<1>(wv, 0, key, it.key0, it.key1, lane);
+                    wait_lds();
+                    clean_rows<HD>(wv, lane);
+                    clean_rows<HD>(wv + 16 * HD, lane);
+                    wait_lds();
                 }
+                w.template step<1>(wk, wv, 0, key, it.key0, it.key1, lane);
                 if (key + 128 < it.key1) {
-                    load(n0, n1);
+                    wait_lds();
+                    mv.rows16(a, n0, wk, wv);
+                    mv.rows16(a, n1, wk + 16 * HD, wv + 16 * HD);
                     n0 = rows_at(key + 256); n1 = rows_at(key + 272);
                 }
-                asm volatile("" ::: "memory");
-                w.template step<1>(wk, wv, 0, key, it.key0, it.key1, lane);
-                asm volatile("" ::: "memory");
             }
-            // ---- the four waves' results, scaled to one maximum, meet in LDS
+            // ---- the four waves' results, scaled to one maximum, meet in LDS: each dim quarter in an array of its own
             w.l += other_half(w.l);
             if (lane < 32) s_ml[wave][lane] = make_float2(w.m, w.l);
             __syncthreads();
             const int rh = lane & 31;
             const float m = fmaxf(fmaxf(s_ml[0][rh].x, s_ml[1][rh].x), fmaxf(s_ml[2][rh].x, s_ml[3][rh].x));
             const float f = w.m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(w.m - m);
-            float * s_o = (float *) s_kv;                        // [4][32][HD]: the block's LDS exactly
-            static_assert(4 * 32 * HD * 4 <= sizeof(TC) * 2 * ROWS * HD, "merge area");
+            // wave i's [32][HD] floats: 32 keys' K and V of a wave are as many bytes, so two arrays of 64 rows hold one wave's
+            auto s_o = [&](int i, int r, int d) __attribute__((always_inline)) {
+                TC * at = i == 0 ? s_k0 : i == 1 ? s_k1 : i == 2 ? s_v0 : s_v1;
+                return (float *) at + r * HD + d;
+            };
+            static_assert(32 * HD * 4 <= sizeof(s_k0), "merge area");
             if (rh < heads) {
 #pragma unroll
                 for (int dt = 0; dt < HD / 32; ++dt)
 #pragma unroll
                     for (int i = 0; i < 16; i += 4)
-                        *(float4 *) (s_o + (wave * 32 + rh) * HD + 32 * dt + 2 * i + 4 * (lane >> 5)) =
+                        *(float4 *) s_o(wave, rh, 32 * dt + 2 * i + 4 * (lane >> 5)) =
                             make_float4(w.o[dt][i] * f, w.o[dt][i + 1] * f, w.o[dt][i + 2] * f, w.o[dt][i + 3] * f);
             }
             __syncthreads();
@@ -505,7 +556,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_attn(PagedArgs a) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float2 ml = s_ml[i][r];
-                    const float4 y = *(const float4 *) (s_o + (i * 32 + r) * HD + d);
+                    const float4 y = *(const float4 *) s_o(i, r, d);
                     ll += ml.x == -__builtin_inff() ? 0.0f : ml.y * __builtin_amdgcn_exp2f(ml.x - mm);
                     x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
                 }
@@ -520,45 +571,40 @@ __global__ void __launch_bounds__(256, 2) k_paged_attn(PagedArgs a) {
             }
             __syncthreads();
         } else {
-            // ---- every wave takes 32 row-heads; 64 keys at a time in LDS for all, the next 64 on their way in registers
-            constexpr int N = 16 * NC / 64;                      // loads per lane: the wave's 16 of the 64 rows
-            u4_t kr[N], vr[N];
-            const int lrow = 16 * wave + lane / NC, piece = lane % NC;
-            auto load = [&](int64_t at0) __attribute__((always_inline)) {
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const int64_t at = at0 + (i * (64 / NC) + lane / NC) * HD + 8 * piece;
-                    kr[i] = *(const u4_t *) ((const TC *) a.k + at);
-                    vr[i] = *(const u4_t *) ((const TC *) a.v + at);
-                }
-            };
-            auto put = [&](int key, int buf) __attribute__((always_inline)) {
-                const bool cut = key < it.key0 || key + 64 > it.key1;
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const int row = lrow + i * (64 / NC);
-                    if (cut && (key + row < it.key0 || key + row >= it.key1)) vr[i] = u4_t{0, 0, 0, 0};
-                    *(u4_t *) (s_k + 64 * buf * HD + Tile<HD>::k_at(row, piece)) = kr[i];
-                    *(u4_t *) (s_v + 64 * buf * HD + Tile<HD>::v_at(row, piece)) = vr[i];
-                }
-            };
-            int key = it.key0 & ~63, buf = 0;
+            // ---- every wave takes 32 row-heads; 64 keys at a time in LDS for all, the next 64 on their way into the other buffer
             const int mine = 16 * wave;
-            load(rows_at(key + mine));
+            int key = it.key0 & ~63;
+            mv.rows16(a, rows_at(key + mine), s_k0 + mine * HD, s_v0 + mine * HD);
             int64_t next = rows_at(key + 64 + mine);
             w.init(a, it, 32 * wave, lane);
-            put(key, 0);
-            lds_sync();
             const bool live = 32 * wave < heads;
-            for (; key < it.key1; key += 64, buf ^= 1) {
-                const bool more = key + 64 < it.key1;
-                if (more) {
-                    load(next);
+            int least = w.vis;                                   // the fewest cache rows that a row of the tile sees
+#pragma unroll
+            for (int o = 16; o; o >>= 1) least = min(least, __shfl_xor(least, o));
+            if (lane == 0) s_vis[wave] = least;
+            __syncthreads();
+            least = min(min(s_vis[0], s_vis[1]), min(s_vis[2], s_vis[3]));
+            const int whole = min(it.key1, __builtin_amdgcn_readfirstlane(least));     // steps up to here hide nothing behind them
+            // one stage: its keys have arrived for every wave, and nobody reads the other buffer any more
+            auto stage = [&](const TC * sk, TC * sv, TC * ok, TC * ov) __attribute__((always_inline)) {
+                __syncthreads();
+                if (key + 64 < it.key1) {
+                    mv.rows16(a, next, ok + mine * HD, ov + mine * HD);
                     next = rows_at(key + 128 + mine);
                 }
-                if (live) w.template step<2>(s_k, s_v, 64 * buf, key, it.key0, it.key1, lane);
-                if (more) put(key + 64, buf ^ 1);
-                lds_sync();
+                if ((key < it.key0 || key + 64 > whole) && __syncthreads_or(rows_not_finite<HD>(sv + mine * HD, lane))) {
+                    if (live) w.template infinite_values<2>(sv, 0, key, it.key0, it.key1, lane);
+                    __syncthreads();
+                    clean_rows<HD>(sv + mine * HD, lane);
+                    __syncthreads();
+                }
+                if (live) w.template step<2>(sk, sv, 0, key, it.key0, it.key1, lane);
+                key += 64;
+            };
+            while (key < it.key1) {
+                stage(s_k0, s_v0, s_k1, s_v1);
+                if (key >= it.key1) break;
+                stage(s_k1, s_v1, s_k0, s_v0);
             }
             w.l += other_half(w.l);
             const int rh = 32 * wave + (lane & 31);
@@ -577,6 +623,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_attn(PagedArgs a) {
                     }
                 if (!it.direct && lane < 32) a.part_ml[it.part0 + rh] = make_float2(w.m, w.l);
             }
+            __syncthreads();
         }
     }
 }
