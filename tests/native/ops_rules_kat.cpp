@@ -101,7 +101,7 @@ static void workspace() {
         z2h_pages p = good_pages();
         const int group = 1 + rnd(trial % 2 ? 8 : z2o::MAX_GROUP);
         p.n_head_kv = 1 + rnd(16); p.n_seq = 1 + rnd(trial % 7 ? 20 : 300);
-        const int heads = group * p.n_head_kv, target = 1 + rnd(2000);
+        const int heads = group * p.n_head_kv, target = 1 + rnd(1000);
         std::vector<int> rows(p.n_seq), len(p.n_seq), gs{0}, pre;
         int n_rows = 0;
         for (int s = 0; s < p.n_seq; ++s) { rows[s] = rnd(3) ? rnd(3) : rnd(400); len[s] = rnd(2) ? rnd(200) : rnd(30000); n_rows += rows[s]; }
@@ -117,28 +117,67 @@ static void workspace() {
             for (int s = gs[g]; s < gs[g + 1]; ++s) { r += rows[s]; span(rows[s], std::min(pre[g], len[gs[g]]), len[s]); }
             if (pre[g] > 0) span(r, 0, std::min(pre[g], len[gs[g]]));
         }
-        int64_t total = 0, items = 0, parts = 0;
-        for (auto & t : tiles) total += z2o::tile_keys(t.key0, t.key1) * p.n_head_kv;
-        const int chunk = z2o::chunk_keys(total, target);
-        EXPECT(chunk >= 128 && chunk % 128 == 0);
-        for (auto & t : tiles) {
-            const int64_t n = z2o::chunk_count(z2o::tile_keys(t.key0, t.key1), chunk);
-            items += n * p.n_head_kv;
-            parts += n * p.n_head_kv * t.rows * group;
+        const int shift = trial % 5 == 0 ? 1 + rnd(3) : 0;                             // (of calls far larger than these)
+        int64_t parts = 0;
+        for (const bool wide : {false, true}) {
+            const int most_shares = wide ? target : 4 * target, head = z2o::piece_cost(wide);
+            int64_t in_row = 0;
+            int whole = 0;
+            auto mine = [&](const Tile & t) { return z2o::is_wide(t.rows * group) == wide; };
+            auto units_of = [&](const Tile & t) { return mine(t) ? z2o::strip_units(t.key0, t.key1, wide, shift) : 0; };
+            for (auto & t : tiles) in_row += z2o::strip_cost(units_of(t), head) * p.n_head_kv;
+            for (int j = z2o::WHOLE_SHARES - 1; j >= 0; --j) {
+                int64_t n = 0;
+                const int share = z2o::whole_share(j);
+                EXPECT(share >= 1 && (j == 0 || share > z2o::whole_share(j - 1)));
+                for (auto & t : tiles) n += (units_of(t) + share - 1) / share * p.n_head_kv;
+                if (n <= most_shares) whole = share;
+            }
+            z2o::Cut cut = z2o::choose_cut(z2o::row_share(in_row, most_shares, head), whole, head);
+            if (trial % 3 == 0) cut = z2o::Cut{z2o::row_share(in_row, most_shares, head), head};
+            const int share = cut.share;
+            int64_t begin = 0, total = 0;
+            for (auto & t : tiles) total += z2o::strip_pitch(z2o::strip_cost(units_of(t), cut.head), cut) * p.n_head_kv;
+            const int64_t shares = (total + share - 1) / share;
+            EXPECT(shares <= most_shares && total < (1ll << 31));
+            for (auto & t : tiles) {
+                if (!mine(t)) continue;
+                const int units = (int) units_of(t), cost = (int) z2o::strip_cost(units, cut.head), most = z2o::max_pieces(cost, share);
+                const int64_t pitch = z2o::strip_pitch(cost, cut);
+                parts += (int64_t) most * p.n_head_kv * t.rows * group;
+                for (int g = 0; g < p.n_head_kv; ++g, begin += pitch) {
+                    // the pieces of the shares that touch the strip are its units, each once, and are numbered in order
+                    int u = 0, at = 0, n = -1;
+                    if (!units) { EXPECT(z2o::strip_piece((int) begin, units, cut, 0).n == 0); continue; }
+                    EXPECT(cut.head || begin % share == 0);
+                    for (int b = (int) (begin / share); (int64_t) b * share < begin + pitch; ++b) {
+                        EXPECT(b < shares);
+                        const z2o::Piece q = z2o::strip_piece((int) begin, units, cut, b);
+                        EXPECT(n < 0 || q.n == n);
+                        n = q.n;
+                        if (q.u0 >= q.u1) continue;
+                        EXPECT(q.u0 == u && q.at == at && q.at < q.n);
+                        u = q.u1;
+                        ++at;
+                    }
+                    EXPECT(u == units && at == n && n <= most);
+                    EXPECT(z2o::strip_piece((int) begin, units, cut, 0).n == n);
+                }
+            }
         }
         EXPECT((int64_t) tiles.size() <= w.max_tiles || n_rows == 0);
-        EXPECT(items <= w.max_items && parts <= w.max_parts);
-        EXPECT(w.rows % 256 == 0 && w.tiles % 256 == 0 && w.items % 256 == 0 && w.ml % 256 == 0 && w.o % 256 == 0);
-        EXPECT(w.bytes >= w.o + w.max_parts * p.head_dim * 4 && w.o >= w.ml + w.max_parts * 8 && w.ml >= w.items + w.max_items * 32);
+        EXPECT(parts <= w.max_parts);
+        EXPECT(w.rows % 256 == 0 && w.tiles % 256 == 0 && w.starts % 256 == 0 && w.ml % 256 == 0 && w.o % 256 == 0);
+        EXPECT(w.bytes >= w.o + w.max_parts * p.head_dim * 4 && w.o >= w.ml + w.max_parts * 8 && w.ml >= w.starts + 5 * target * 8ll);
     }
     // the largest call's counts stay below 2^31
     z2h_pages p = good_pages();
     p.n_seq = 1 << 20; p.n_head_kv = 1;
     const z2o::AttnWs w = z2o::attn_ws(p, 64, 1 << 20, 1 << 20, 4096);
-    EXPECT(w.max_parts < (1ll << 31) && w.max_items < (1ll << 31) && w.max_tiles < (1ll << 31));
+    EXPECT(w.max_parts < (1ll << 31) && w.max_tiles < (1ll << 31));
     p.n_head_kv = 1024; p.page_stride = 1ll << 30;
     const z2o::AttnWs v = z2o::attn_ws(p, 1024, 1 << 16, 1 << 20, 4096);
-    EXPECT(v.max_parts < (1ll << 31) && v.max_items < (1ll << 31));
+    EXPECT(v.max_parts < (1ll << 31));
 }
 
 int main() {

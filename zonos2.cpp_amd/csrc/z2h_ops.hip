@@ -71,7 +71,6 @@ int rope_run(z2h_ctx * ctx, RopeArgs & a, const z2h_rope * rope, int n_rows, int
     return launched(ctx);
 }
 
-// blocks that fit the device at once (two of k_paged_attn per compute unit), and the chunks that a plan aims at
 int compute_units(int device) {
     static std::atomic<int> known[64] = {};
     const bool slot = device >= 0 && device < 64;
@@ -82,7 +81,8 @@ int compute_units(int device) {
     }
     return n;
 }
-int attn_target(int n_cu) { return 4 * n_cu; }
+// blocks of k_paged_attn: as many as the device holds at once
+int attn_blocks(int n_cu) { return 2 * n_cu; }
 
 template <int HD, typename T, typename TC>
 void attn_launch(const PagedArgs & a, int blocks, hipStream_t stream) {
@@ -157,7 +157,7 @@ int64_t z2h_paged_ws_bytes(z2h_ctx * ctx, const z2h_pages * pages, int n_head, i
     if (const char * e = z2o::check_attn(pages, n_head, n_rows, n_group)) { z2h_ctx_fail(ctx, Z2H_EINVAL, e); return 0; }
     const int n_cu = compute_units(z2h_ctx_device(ctx));
     if (!n_cu) { z2h_ctx_fail(ctx, Z2H_EDEVICE, "compute-unit count query failed"); return 0; }
-    return z2o::attn_ws(*pages, n_head, n_rows, n_group, attn_target(n_cu)).bytes;
+    return z2o::attn_ws(*pages, n_head, n_rows, n_group, attn_blocks(n_cu)).bytes;
 }
 
 int z2h_paged_plan(z2h_ctx * ctx, const z2h_pages * pages, int n_head, int n_rows, const int32_t * d_row_start,
@@ -168,16 +168,16 @@ int z2h_paged_plan(z2h_ctx * ctx, const z2h_pages * pages, int n_head, int n_row
     REQUIRE(d_row_start && d_kv_len && (n_group == 0 || (d_group_start && d_prefix_len)), "plan: null table");
     const int n_cu = compute_units(z2h_ctx_device(ctx));
     if (!n_cu) return z2h_ctx_fail(ctx, Z2H_EDEVICE, "compute-unit count query failed");
-    const z2o::AttnWs w = z2o::attn_ws(*pages, n_head, n_rows, n_group, attn_target(n_cu));
+    const z2o::AttnWs w = z2o::attn_ws(*pages, n_head, n_rows, n_group, attn_blocks(n_cu));
     CHECK(check_ws(d_ws, ws_bytes, w.bytes));
     PlanArgs a{};
     a.row_start = d_row_start; a.kv_len = d_kv_len; a.group_start = d_group_start; a.prefix_len = d_prefix_len;
     a.n_seq = pages->n_seq; a.n_rows = n_rows; a.n_group = n_group; a.n_head = n_head; a.nkv = pages->n_head_kv;
     a.cap = pages->table_len * pages->page_rows;
-    a.target = attn_target(n_cu);
+    a.blocks = attn_blocks(n_cu);
     uint8_t * ws = (uint8_t *) d_ws;
-    a.head = (int32_t *) ws; a.rows = (PlanRow *) (ws + w.rows); a.tiles = (PlanTile *) (ws + w.tiles); a.items = (PlanItem *) (ws + w.items);
-    a.max_tiles = (int) w.max_tiles; a.max_items = (int) w.max_items; a.max_parts = (int) w.max_parts;
+    a.head = (int32_t *) ws; a.rows = (PlanRow *) (ws + w.rows); a.tiles = (PlanTile *) (ws + w.tiles); a.starts = (int2 *) (ws + w.starts);
+    a.max_tiles = (int) w.max_tiles; a.max_parts = (int) w.max_parts;
     ON_DEVICE;
     hipLaunchKernelGGL(k_paged_plan, dim3(1), dim3(PLAN_T), 0, (hipStream_t) stream, a);
     return launched(ctx);
@@ -195,7 +195,7 @@ int z2h_paged_attn(z2h_ctx * ctx, const z2h_pages * pages, int n_head, int n_row
     REQUIRE(std::isfinite(scale), "attention: scale must be finite");
     const int n_cu = compute_units(z2h_ctx_device(ctx));
     if (!n_cu) return z2h_ctx_fail(ctx, Z2H_EDEVICE, "compute-unit count query failed");
-    const z2o::AttnWs w = z2o::attn_ws(*pages, n_head, n_rows, n_group, attn_target(n_cu));
+    const z2o::AttnWs w = z2o::attn_ws(*pages, n_head, n_rows, n_group, attn_blocks(n_cu));
     CHECK(check_ws(d_ws, ws_bytes, w.bytes));
     if (n_rows == 0) return Z2H_OK;
     PagedArgs a{};
@@ -205,9 +205,12 @@ int z2h_paged_attn(z2h_ctx * ctx, const z2h_pages * pages, int n_head, int n_row
     a.nkv = pages->n_head_kv; a.n_head = n_head; a.n_rows = n_rows; a.n_group = n_group; a.scale = scale;
     a.q = d_q; a.out = d_out;
     uint8_t * ws = (uint8_t *) d_ws;
-    a.head = (const int32_t *) ws; a.rows = (const PlanRow *) (ws + w.rows); a.items = (const PlanItem *) (ws + w.items);
+    a.head = (const int32_t *) ws; a.rows = (const PlanRow *) (ws + w.rows); a.tiles = (const PlanTile *) (ws + w.tiles);
+    a.starts = (const int2 *) (ws + w.starts);
     a.part_ml = (float2 *) (ws + w.ml); a.part_o = (float *) (ws + w.o);
-    const int blocks = (int) std::min<int64_t>(w.max_items, 2 * n_cu);
+    const int blocks = attn_blocks(n_cu);
+    a.max_tiles = (int) w.max_tiles;
+    a.blocks = blocks;
     ON_DEVICE;
     switch (pages->head_dim) {
         case 32: attn_launch<32>(a, type, blocks, (hipStream_t) stream); break;

@@ -99,42 +99,76 @@ inline int page_shift_of(int page_rows) { int s = 0; while ((1 << s) < page_rows
 
 // ---- attention: how the work is cut
 // A span is a run of query rows over a run of cache rows: a group's rows over its shared prefix, a sequence's rows over the
-// rest. Its rows are cut into tiles of at most TILE_RH row-heads of one key head (32 per wave). A tile of at most
-// NARROW_RH row-heads is walked by four waves over keys of their own, a larger one by four waves over the same keys.
+// rest. Its rows are cut into tiles of at most TILE_RH row-heads of one key head. A tile of more than NARROW_RH row-heads is
+// wide: the four waves of a block take 32 row-heads each of the same keys. Any other is narrow: one wave has all its row-heads.
+// A strip is a tile with one of its key heads. All strips of a kind are dealt out in shares of equal work, one per block (wide) or
+// per wave (narrow), whatever the sequences' lengths; so every block has as much of either kind as any other.
 constexpr int TILE_RH = 128, NARROW_RH = 32;
 Z2O_HD int tile_rows(int group) { return TILE_RH / group; }              // group <= MAX_GROUP: two rows at least
-// Keys of a tile are counted from a multiple of 64 and cut into chunks of whole steps: 128 keys where the waves take 32 each,
-// 64 where they share them.
-Z2O_HD int64_t tile_keys(int key0, int key1) { return key1 > key0 ? (int64_t) key1 - (key0 & ~63) : 0; }
-// keys per chunk: all work (keys x key heads over all tiles) divided over `target` blocks, so that blocks have alike work whatever
-// the sequences' lengths
-Z2O_HD int chunk_keys(int64_t total, int target) {
-    const int64_t c = (total + target - 1) / target;
-    return (int) (((c < 128 ? 128 : c) + 127) / 128 * 128);
+Z2O_HD bool is_wide(int row_heads) { return row_heads > NARROW_RH; }
+// Keys of a strip are counted in units, the keys of one step (times 2^shift in calls of more than 2^28 units), from a multiple of 64 on.
+Z2O_HD int unit_keys(bool wide) { return wide ? 64 : 32; }
+Z2O_HD int64_t strip_units(int key0, int key1, bool wide, int shift) {
+    const int64_t k = unit_keys(wide);
+    return key1 > key0 ? (((int64_t) key1 - (key0 & ~63) + k - 1) / k + (1ll << shift) - 1) >> shift : 0;
 }
-Z2O_HD int chunk_count(int64_t keys, int chunk) { return (int) ((keys + chunk - 1) / chunk); }
+// What it takes to begin and end a piece of a strip, in steps (query rows, page numbers, partial results: 6 us beside steps of
+// about 2 and 3).
+Z2O_HD int piece_cost(bool wide) { return wide ? 2 : 3; }
+// Two ways to cut. Whole shares (`head` 0): every strip is cut into pieces of `share` units, the last one shorter; strips begin at
+// multiples of the share, so that a share is a piece of one strip, and strips over the same keys have their pieces side by side. In a
+// row (`head`: the cost of a piece): all strips one behind the other, cut into shares of equal cost, so that a share has the end of
+// one strip, whole strips and the beginning of another; for batches of more or longer strips than there are shares.
+struct Cut { int share, head; };
+Z2O_HD int64_t strip_cost(int64_t units, int head) { return units ? head + units : 0; }
+Z2O_HD int64_t strip_pitch(int64_t cost, Cut cut) { return cut.head ? cost : (cost + cut.share - 1) / cut.share * cut.share; }
+Z2O_HD int row_share(int64_t cost, int max_shares, int head) {
+    const int64_t s = (cost + max_shares - 1) / max_shares;
+    return (int) (s <= head ? head + 1 : s);                             // a unit at least
+}
+constexpr int WHOLE_SHARES = 24;                                         // whole shares that are tried: 2, 3, 4, 6, 8, 12, ... units
+Z2O_HD int whole_share(int i) { return (i & 1 ? 3 : 2) << i / 2; }
+// Of a call whose strips in a row give shares of `in_row`, and whose smallest whole share that needs no more than there are is
+// `whole` (0: none): whole ones where they take no longer (a share in a row usually has parts of two strips).
+Z2O_HD Cut choose_cut(int in_row, int whole, int head) { return whole && whole <= in_row + head ? Cut{whole, 0} : Cut{in_row, head}; }
+
+// The piece of a strip that share `b` has: units [u0, u1), the `at`-th of `n` pieces. The strip begins at `begin` of the row of strips.
+struct Piece { int u0, u1, at, n; };
+Z2O_HD int units_before(int cost, int units) { return cost <= 0 ? 0 : cost < units ? cost : units; }
+Z2O_HD Piece strip_piece(int begin, int units, Cut cut, int b) {
+    if (!units) return Piece{0, 0, 0, 0};
+    const int share = cut.share, b0 = begin / share, b1 = (begin + cut.head + units - 1) / share, from = begin + cut.head;
+    // a first piece may be too short for a unit; the others are not
+    const int none = b1 > b0 && (b0 + 1) * share - from <= 0;
+    Piece p;
+    p.u0 = b <= b0 ? 0 : units_before(b * share - from, units);
+    p.u1 = b >= b1 ? units : units_before((b + 1) * share - from, units);
+    p.at = b - b0 - none;
+    p.n = b1 - b0 + 1 - none;
+    return p;
+}
+Z2O_HD int max_pieces(int cost, int share) { return cost ? cost / share + 2 : 0; }
 
 // ---- attention workspace
 struct AttnWs {
-    int64_t rows = 0, tiles = 0, items = 0, ml = 0, o = 0, bytes = 0;    // offsets in bytes; the header is at 0
-    int64_t max_tiles = 0, max_items = 0, max_parts = 0;
+    int64_t rows = 0, tiles = 0, starts = 0, ml = 0, o = 0, bytes = 0;   // offsets in bytes; the header is at 0
+    int64_t max_tiles = 0, max_parts = 0;
 };
 inline int64_t align256(int64_t n) { return (n + 255) & ~(int64_t) 255; }
 // Every row is in at most one tile of its group's span and one of its sequence's, and a span's last tile may be partly filled.
-// Chunks of a tile: at most keys / chunk + 1, so over all tiles and key heads at most target + tiles x key heads; and of
-// partial results, row-heads of the tile each, min(TILE_RH, all rows' of one key head) x target + 2 x rows x heads.
-inline AttnWs attn_ws(const z2h_pages & p, int n_head, int n_rows, int n_group, int target) {
+// Pieces of a strip: at most cost / share + 2, so over all strips of a kind at most shares + 2 strips, of as many partial results as the
+// tile has row-heads: blocks x min(TILE_RH, all rows' of one key head) + 4 blocks x min(NARROW_RH, ...) + 4 x rows x heads.
+inline AttnWs attn_ws(const z2h_pages & p, int n_head, int n_rows, int n_group, int blocks) {
     AttnWs w;
     const int group = n_head / p.n_head_kv, tr = tile_rows(group);
     const int64_t by_span = (int64_t) p.n_seq + n_group + 2 * ((n_rows + tr - 1) / tr), by_row = 2 * (int64_t) n_rows;
     const int64_t rh = (int64_t) n_rows * group;
     w.max_tiles = by_span < by_row ? by_span : by_row;
-    w.max_items = n_rows ? target + w.max_tiles * p.n_head_kv : 0;
-    w.max_parts = n_rows ? (rh < TILE_RH ? rh : TILE_RH) * target + 2 * (int64_t) n_rows * n_head : 0;
+    w.max_parts = n_rows ? blocks * ((rh < TILE_RH ? rh : TILE_RH) + 4 * (rh < NARROW_RH ? rh : NARROW_RH)) + 4 * (int64_t) n_rows * n_head : 0;
     w.rows = 256;
     w.tiles = w.rows + align256((int64_t) n_rows * 32);
-    w.items = w.tiles + align256(w.max_tiles * 32);
-    w.ml = w.items + align256(w.max_items * 32);
+    w.starts = w.tiles + align256(w.max_tiles * 32);
+    w.ml = w.starts + align256((int64_t) blocks * 5 * 8);
     w.o = w.ml + align256(w.max_parts * 8);
     w.bytes = w.o + align256(w.max_parts * p.head_dim * 4);
     return w;

@@ -3,10 +3,10 @@
 //   o = sum_i p_i v_i / sum_i p_i,  p_i = 2^(x_i - m),  x_i = scale log2(e) q.k_i
 // in one pass over the keys with a running m; partial (m, sum p, sum p v) of disjoint keys join by scaling to the larger m. So a
 // row's keys may be cut anywhere: its group's shared prefix is walked once for all rows of the group (their queries side
-// by side in one product), the rest of its keys with its own sequence, and both in chunks of alike work.
-//   k_paged_plan     one block: tiles, chunks and the places of their partial results, from the lengths (z2h_ops_rules.h)
-//   k_paged_attn     one item = (tile of query rows, key head, chunk of keys) per block
-//   k_paged_join     one wave per (row, head): its chunks' partial results
+// by side in one product), the rest of its keys with its own sequence, and both where shares of equal work end.
+//   k_paged_plan     one block: tiles of query rows, the shares and the places of partial results, from the lengths (z2h_ops_rules.h)
+//   k_paged_attn     a share of the wide strips per block and of the narrow ones per wave
+//   k_paged_join     one wave per (row, head): its pieces' partial results
 // Single tokens are bound by reading the cache once; groups of many rows and prompt chunks by the products and the exponentials.
 #pragma once
 #include "z2h_common.h"
@@ -15,24 +15,27 @@
 namespace z2d {
 
 constexpr int PLAN_MAGIC = 0x50414745;
-enum { PH_MAGIC = 0, PH_ROWS, PH_HEADS, PH_GROUPS, PH_SEQS, PH_KV_HEADS, PH_ITEMS, PH_CHUNK };
+enum { PH_MAGIC = 0, PH_ROWS, PH_HEADS, PH_GROUPS, PH_SEQS, PH_KV_HEADS, PH_SHIFT, PH_KIND, PH_COUNT = PH_KIND + 8 };
+enum { PK_TILES = 0, PK_SHARES, PK_SHARE, PK_HEAD };             // of each kind, narrow then wide, from PH_KIND on
 
-// per row: what it sees, and where its partial results are: chunk c, key head g, head h of the group at
-// base + c * step + g * (step / key heads) + h, in its group's prefix and in its own keys
-struct PlanRow { int vis, pre_base, pre_n, pre_step, own_base, own_n, own_step, spare; };
-struct PlanTile { int row0, rows, key0, key1, seq, chunks, item0, part0; };
-struct PlanItem { int row0, rows, key0, key1, seq, head, part0, direct; };
-static_assert(sizeof(PlanRow) == 32 && sizeof(PlanTile) == 32 && sizeof(PlanItem) == 32, "workspace layout");
+// per row: what it sees, and its tiles in its group's prefix and in its own keys (-1: none), and its place in their row-heads
+struct PlanRow { int vis, pre_tile, pre_at, own_tile, own_at, spare[3]; };
+// A tile's strips begin at `begin` + key head x pitch in the row of all strips of its kind; partial result `at` of its strip g is at part0 +
+// (g x pieces + at) x row-heads, `pieces` the most that any of its strips has; alone: its rows have no other tile. Wide tiles are
+// kept from the table's first place on, narrow ones from its last backwards.
+struct PlanTile { int row0, rows, key0, key1, seq, alone, begin, part0; };
+static_assert(sizeof(PlanRow) == 32 && sizeof(PlanTile) == 32, "workspace layout");
 
 struct PlanArgs {
     const int32_t * row_start, * kv_len, * group_start, * prefix_len;
-    int n_seq, n_rows, n_group, n_head, nkv, cap, target;
+    int n_seq, n_rows, n_group, n_head, nkv, cap, blocks;
     int32_t * head;
     PlanRow * rows;
     PlanTile * tiles;
-    PlanItem * items;
-    int max_tiles, max_items, max_parts;
+    int2 * starts;                                               // a share's first strip: tile of its kind, key head; [blocks] wide, [4 blocks] narrow
+    int max_tiles, max_parts;
 };
+__device__ __forceinline__ int tile_place(int i, bool wide, int max_tiles) { return wide ? i : max_tiles - 1 - i; }
 
 // the last index i of [0, n) with start[i] <= x (start ascending; -1: none)
 __device__ __forceinline__ int last_at_or_before(const int32_t * start, int n, int x) {
@@ -71,21 +74,17 @@ __device__ __forceinline__ int block_scan(int v, int * s_wave, int & total) {
 __global__ void __launch_bounds__(PLAN_T) k_paged_plan(PlanArgs a) {
     __shared__ int s_wave[PLAN_T / 64];
     __shared__ unsigned long long s_total;
-    constexpr int LDS_TILES = 4096;
-    __shared__ int s_item0[LDS_TILES];
+    constexpr int LDS_TILES = 8192;
+    __shared__ int s_begin[LDS_TILES];
     const int tid = threadIdx.x, group = a.n_head / a.nkv, tr = z2o::tile_rows(group);
-    for (int t = tid; t < a.n_rows; t += PLAN_T) a.rows[t] = PlanRow{0, 0, 0, 0, 0, 0, 0, 0};
-    if (tid == 0) {
-        s_total = 0;
-        a.head[PH_MAGIC] = PLAN_MAGIC; a.head[PH_ROWS] = a.n_rows; a.head[PH_HEADS] = a.n_head; a.head[PH_GROUPS] = a.n_group;
-        a.head[PH_SEQS] = a.n_seq; a.head[PH_KV_HEADS] = a.nkv;
-    }
+    for (int t = tid; t < a.n_rows; t += PLAN_T) a.rows[t] = PlanRow{0, -1, 0, -1, 0, {0, 0, 0}};
+    if (tid == 0) s_total = 0;
     auto start_of = [&](int s) { return min(max(a.row_start[s], 0), a.n_rows); };
     auto len_of = [&](int s) { return min(max(a.kv_len[s], 0), a.cap); };
     auto group_of = [&](int g) { return min(max(a.group_start[g], 0), a.n_seq); };
-    // ---- tiles of every span: the groups' prefixes, then the sequences' own keys
-    int n_tiles = 0;
-    unsigned long long work = 0;
+    // ---- tiles of every span: the groups' prefixes, then the sequences' own keys. A span's tiles have tr rows each but for the last.
+    int n_tiles[2] = {0, 0};                                     // narrow, wide
+    unsigned long long units = 0;
     for (int base = 0; base < a.n_group + a.n_seq; base += PLAN_T) {
         const int x = base + tid;
         int r0 = 0, r1 = 0, key0 = 0, key1 = 0, seq = 0, len = 0;
@@ -103,64 +102,98 @@ __global__ void __launch_bounds__(PLAN_T) k_paged_plan(PlanArgs a) {
             if (g >= 0 && g < a.n_group) key0 = max(0, min(a.prefix_len[g], len_of(group_of(g))));
         }
         const bool some = r1 > r0 && (own || key1 > 0);
+        const int n = some ? (r1 - r0 + tr - 1) / tr : 0, last = some ? r1 - r0 - (n - 1) * tr : 0;
+        const int n_wide = !some ? 0 : z2o::is_wide(last * group) ? n : z2o::is_wide(tr * group) ? n - 1 : 0;
         int all;
-        const int at = n_tiles + block_scan(some ? (r1 - r0 + tr - 1) / tr : 0, s_wave, all);
-        n_tiles = min(n_tiles + all, a.max_tiles);
-        if (some)
-            for (int i = 0, r = r0; r < r1; ++i, r += tr) {
-                if (at + i >= a.max_tiles) break;
-                const int rows = min(tr, r1 - r);
-                // own keys: up to what the tile's last row sees
-                const int end = own ? max(key0, min(key1, len - (r1 - r0) + (r + rows - r0))) : key1;
-                a.tiles[at + i] = PlanTile{r, rows, key0, end, seq, own ? (len - (r1 - r0) + (r - r0)) : -1, 0, own};
-                work += (unsigned long long) z2o::tile_keys(key0, end) * a.nkv;
-            }
-    }
-    atomicAdd(&s_total, work);                         // integers: the order does not matter
-    __syncthreads();
-    const int chunk = z2o::chunk_keys((int64_t) s_total, a.target);
-    // ---- chunks of every tile, the places of its items and partial results, and its rows' entries
-    int n_items = 0, n_parts = 0;
-    for (int base = 0; base < n_tiles; base += PLAN_T) {
-        const int i = base + tid;
-        PlanTile t{};
-        if (i < n_tiles) t = a.tiles[i];
-        const int see0 = t.chunks;                     // (own tiles: cache rows before the first row's own)
-        const bool own = t.part0;
-        const int chunks = i < n_tiles ? z2o::chunk_count(z2o::tile_keys(t.key0, t.key1), chunk) : 0, heads = t.rows * group;
-        int items, parts;
-        t.chunks = chunks;
-        t.item0 = n_items + block_scan(chunks * a.nkv, s_wave, items);
-        t.part0 = n_parts + block_scan(chunks * a.nkv * heads, s_wave, parts);
-        n_items = min(n_items + items, a.max_items);
-        n_parts = min(n_parts + parts, a.max_parts);
-        if (i < n_tiles) {
-            if (t.part0 + chunks * a.nkv * heads > a.max_parts) t.chunks = 0;   // (cannot be, by the sizes' rule)
-            a.tiles[i] = t;
-            if (i < LDS_TILES) s_item0[i] = t.item0;
-            for (int r = 0; r < t.rows; ++r) {
-                PlanRow & p = a.rows[t.row0 + r];
-                const int part = t.part0 + r * group, step = a.nkv * heads;
-                if (own) { p.vis = max(0, see0 + r + 1); p.own_base = part; p.own_n = t.chunks; p.own_step = step; }
-                else { p.pre_base = part; p.pre_n = t.chunks; p.pre_step = step; }
-            }
+        int at[2] = {n_tiles[0] + block_scan(n - n_wide, s_wave, all), 0};
+        n_tiles[0] += all;
+        at[1] = n_tiles[1] + block_scan(n_wide, s_wave, all);
+        n_tiles[1] += all;
+        for (int i = 0, r = r0; i < n; ++i, r += tr) {
+            const int rows = min(tr, r1 - r), before = len - (r1 - r0) + (r - r0);
+            const bool wide = z2o::is_wide(rows * group);
+            const int place = tile_place(at[wide]++, wide, a.max_tiles);
+            if (place < 0 || place >= a.max_tiles) continue;     // (cannot be, by the table's size)
+            // own keys: up to what the tile's last row sees (`before`: cache rows before its first row's own)
+            const int end = own ? max(key0, min(key1, before + rows)) : key1;
+            a.tiles[place] = PlanTile{r, rows, key0, end, seq, own && key0 == 0, own ? before : 0, own};
+            units += (unsigned long long) z2o::strip_units(key0, end, wide, 0) * a.nkv;
         }
     }
+    atomicAdd(&s_total, units);                                  // integers: the order does not matter
     __syncthreads();
-    if (tid == 0) { a.head[PH_ITEMS] = n_items; a.head[PH_CHUNK] = chunk; }
-    // ---- items: chunk by chunk of a tile, its key heads side by side
-    for (int i = tid; i < n_items; i += PLAN_T) {
-        int lo = 0, hi = n_tiles;
-        while (hi - lo > 1) {
-            const int m = (lo + hi) >> 1;
-            if ((m < LDS_TILES ? s_item0[m] : a.tiles[m].item0) <= i) lo = m; else hi = m;
+    int shift = 0, n_parts = 0;
+    while (s_total >> shift >= 1ull << 28) ++shift;
+#pragma unroll 1
+    for (int kind = 0; kind < 2; ++kind) {
+        const bool wide = kind;
+        const int count = min(n_tiles[kind], a.max_tiles), max_shares = wide ? a.blocks : 4 * a.blocks, head = z2o::piece_cost(wide);
+        int2 * starts = wide ? a.starts : a.starts + a.blocks;
+        auto tile = [&](int i) -> PlanTile & { return a.tiles[tile_place(i, wide, a.max_tiles)]; };
+        auto units_of = [&](const PlanTile & t) { return (int) z2o::strip_units(t.key0, t.key1, wide, shift); };
+        // ---- how to cut: what all strips cost in a row, and the smallest whole share that needs no more than there are
+        int row_cost = 0, all;
+        for (int i = tid; i < count; i += PLAN_T) row_cost += (int) z2o::strip_cost(units_of(tile(i)), head) * a.nkv;
+        block_scan(row_cost, s_wave, all);
+        const int in_row = z2o::row_share(all, max_shares, head);
+        int whole = 0;
+        if (count && (int64_t) count * a.nkv <= max_shares)      // (a share per strip at least)
+            for (int j = 0; j < z2o::WHOLE_SHARES && !whole && z2o::whole_share(j) <= in_row + head; ++j) {
+                const int share = z2o::whole_share(j);
+                int n = 0;
+                for (int i = tid; i < count; i += PLAN_T) n += (units_of(tile(i)) + share - 1) / share * a.nkv;
+                block_scan(min(n, 1 << 20), s_wave, all);
+                if (all <= max_shares) whole = share;
+            }
+        const z2o::Cut cut = z2o::choose_cut(in_row, whole, head);
+        // ---- where every tile's strips begin, the places of their partial results, and the rows' entries
+        int total = 0;
+        for (int base = 0; base < count; base += PLAN_T) {
+            const int i = base + tid;
+            PlanTile t{};
+            if (i < count) t = tile(i);
+            const int before = t.begin, heads = t.rows * group;
+            const bool own = t.part0;
+            const int cost = i < count ? (int) z2o::strip_cost(units_of(t), cut.head) : 0;
+            t.begin = total + block_scan((int) z2o::strip_pitch(cost, cut) * a.nkv, s_wave, all);
+            total += all;
+            t.part0 = n_parts + block_scan(z2o::max_pieces(cost, cut.share) * a.nkv * heads, s_wave, all);
+            n_parts += all;
+            if (i < count) {
+                const int place = tile_place(i, wide, a.max_tiles);
+                a.tiles[place] = t;
+                if (i < LDS_TILES) s_begin[i] = t.begin;
+                for (int r = 0; r < t.rows; ++r) {
+                    PlanRow & p = a.rows[t.row0 + r];
+                    if (own) { p.vis = max(0, before + r + 1); p.own_tile = cost ? place : -1; p.own_at = r * group; }
+                    else { p.pre_tile = place; p.pre_at = r * group; }
+                }
+            }
         }
-        const PlanTile t = a.tiles[lo];
-        const int c = (i - t.item0) / a.nkv, g = (i - t.item0) % a.nkv, from = (t.key0 & ~63) + c * chunk;
-        if (c >= t.chunks) { a.items[i] = PlanItem{0, 0, 0, 0, 0, 0, 0, 0}; continue; }
-        const bool direct = t.chunks == 1 && a.rows[t.row0].pre_n == 0 && a.rows[t.row0].own_n == 1;
-        a.items[i] = PlanItem{t.row0, t.rows, max(t.key0, from), min(t.key1, from + chunk), t.seq, g,
-                              t.part0 + (c * a.nkv + g) * t.rows * group, direct};
+        __syncthreads();
+        // ---- every share's first strip
+        const int shares = min((total + cut.share - 1) / cut.share, max_shares);
+        for (int b = tid; b < shares; b += PLAN_T) {
+            const int at = b * cut.share;
+            int lo = 0, hi = count;
+            while (hi - lo > 1) {
+                const int m = (lo + hi) >> 1;
+                if ((m < LDS_TILES ? s_begin[m] : tile(m).begin) <= at) lo = m; else hi = m;
+            }
+            const PlanTile t = tile(lo);
+            const int pitch = (int) z2o::strip_pitch(z2o::strip_cost(units_of(t), cut.head), cut);
+            starts[b] = make_int2(lo, pitch ? min((at - t.begin) / pitch, a.nkv - 1) : 0);
+        }
+        if (tid == 0) {
+            int32_t * k = a.head + PH_KIND + 4 * kind;
+            k[PK_TILES] = count; k[PK_SHARES] = shares; k[PK_SHARE] = cut.share; k[PK_HEAD] = cut.head;
+        }
+        __syncthreads();
+    }
+    if (tid == 0) {
+        const bool fits = n_parts <= a.max_parts;                // (always, by the sizes' rule)
+        a.head[PH_ROWS] = a.n_rows; a.head[PH_HEADS] = a.n_head; a.head[PH_GROUPS] = a.n_group; a.head[PH_SEQS] = a.n_seq;
+        a.head[PH_KV_HEADS] = a.nkv; a.head[PH_SHIFT] = shift; a.head[PH_MAGIC] = fits ? PLAN_MAGIC : 0;
     }
 }
 
@@ -174,7 +207,9 @@ struct PagedArgs {
     void * out;
     const int32_t * head;
     const PlanRow * rows;
-    const PlanItem * items;
+    const PlanTile * tiles;
+    const int2 * starts;
+    int max_tiles, blocks;
     float2 * part_ml;
     float * part_o;
 };
@@ -183,6 +218,48 @@ __device__ __forceinline__ bool plan_fits(const PagedArgs & a) {
     return a.head[PH_MAGIC] == PLAN_MAGIC && a.head[PH_ROWS] == a.n_rows && a.head[PH_HEADS] == a.n_head && a.head[PH_GROUPS] == a.n_group &&
            a.head[PH_SEQS] == a.n_seq && a.head[PH_KV_HEADS] == a.nkv;
 }
+
+// a piece of a strip: query rows, keys, and where its results go
+struct PlanItem { int row0, rows, key0, key1, seq, head, part0, direct; };
+struct PlanKind {
+    z2o::Cut cut;
+    int tiles, shares, shift;
+    bool wide;
+    __device__ __forceinline__ PlanKind(const PagedArgs & a, bool wide_) : wide(wide_) {
+        const int32_t * k = a.head + PH_KIND + 4 * (int) wide_;
+        tiles = k[PK_TILES]; shares = k[PK_SHARES]; cut = z2o::Cut{k[PK_SHARE], k[PK_HEAD]}; shift = a.head[PH_SHIFT];
+    }
+    // the piece that share b has of the tile's strip g, where that begins, and the most pieces that a strip of the tile has
+    __device__ __forceinline__ z2o::Piece piece(const PlanTile & t, int g, int b, int & begin, int & most) const {
+        const int units = (int) z2o::strip_units(t.key0, t.key1, wide, shift), cost = (int) z2o::strip_cost(units, cut.head);
+        most = z2o::max_pieces(cost, cut.share);
+        begin = t.begin + g * (int) z2o::strip_pitch(cost, cut);
+        return z2o::strip_piece(begin, units, cut, b);
+    }
+};
+// The pieces of share b, one after the other.
+struct ShareWalk {
+    int b, tile, g;
+    __device__ __forceinline__ ShareWalk(const PagedArgs & a, const PlanKind & k, int share) : b(share), tile(k.tiles), g(0) {
+        if (b < k.shares) { const int2 s = a.starts[k.wide ? b : a.blocks + b]; tile = s.x; g = s.y; }
+    }
+    __device__ __forceinline__ bool next(const PagedArgs & a, const PlanKind & k, int group, PlanItem & it) {
+        while (tile < k.tiles) {
+            const PlanTile t = a.tiles[tile_place(tile, k.wide, a.max_tiles)];
+            int begin, pieces;
+            const z2o::Piece p = k.piece(t, g, b, begin, pieces);
+            if (p.n && begin >= (b + 1) * k.cut.share) return false;
+            const int head = g;
+            if (p.n == 0 || ++g == a.nkv) { ++tile; g = 0; }
+            if (p.u0 >= p.u1) continue;
+            const int base = t.key0 & ~63, unit = z2o::unit_keys(k.wide) << k.shift;
+            it = PlanItem{t.row0, t.rows, max(t.key0, base + p.u0 * unit), min(t.key1, base + p.u1 * unit), t.seq, head,
+                          t.part0 + (head * pieces + p.at) * t.rows * group, t.alone && p.n == 1};
+            return true;
+        }
+        return false;
+    }
+};
 
 typedef float v16f_t __attribute__((ext_vector_type(16)));
 typedef unsigned u4_t __attribute__((ext_vector_type(4)));
@@ -478,153 +555,132 @@ struct Mover {
 };
 
 template <int HD, typename T, typename TC>
+struct PagedAttn {
+    const PagedArgs & a;
+    const Mover<HD, TC> mv;
+    const int lane, wave, group;
+    __device__ __forceinline__ PagedAttn(const PagedArgs & args, int lane_, int wave_)
+        : a(args), mv(lane_), lane(lane_), wave(wave_), group(args.n_head / args.nkv) {}
+
+    // elements from the start of k and v to the 16 rows that begin with `key` (one page holds them; any key gives an address inside
+    // the cache; the wave is of one mind)
+    __device__ __forceinline__ int64_t rows_at(const PlanItem & it, int key) const {
+        key = __builtin_amdgcn_readfirstlane(key);
+        const int page = max(0, z2o::page_of(a.table, a.n_seq, a.table_len, a.n_pages, a.page_shift, it.seq, key));
+        const int64_t head_row = ((int64_t) it.head << a.page_shift) + (key & ((1 << a.page_shift) - 1));
+        return (int64_t) __builtin_amdgcn_readfirstlane(page) * a.page_stride + head_row * HD;
+    }
+    // the row-heads first_rh .. first_rh + 31 of the piece: final, or partial
+    __device__ __forceinline__ void store(const PlanItem & it, AttnWave<HD, T, TC> & w, int first_rh) const {
+        const int heads = it.rows * group, rh = first_rh + (lane & 31);
+        w.l += other_half(w.l);
+        if (rh >= heads) return;
+        const float inv = !it.direct ? 1.0f : w.l == 0.0f ? 0.0f : 1.0f / w.l;
+        T * out = (T *) a.out + (it.row0 + rh / group) * a.os + (int64_t) (it.head * group + rh % group) * HD;
+        float * part = a.part_o + (int64_t) (it.part0 + rh) * HD;
+#pragma unroll
+        for (int dt = 0; dt < HD / 32; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const int d = 32 * dt + 2 * i + 4 * (lane >> 5);
+                const float4 x = make_float4(w.o[dt][i] * inv, w.o[dt][i + 1] * inv, w.o[dt][i + 2] * inv, w.o[dt][i + 3] * inv);
+                if (it.direct) store4(out + d, x.x, x.y, x.z, x.w);
+                else *(float4 *) (part + d) = x;
+            }
+        if (!it.direct && lane < 32) a.part_ml[it.part0 + rh] = make_float2(w.m, w.l);
+    }
+
+    // ---- narrow: the wave's own 32 rows of LDS (K at wk, V at wv), its own keys; nothing to wait for but its own loads
+    __device__ __forceinline__ void narrow(const PlanItem & it, TC * wk, TC * wv) const {
+        int key = it.key0 & ~31;
+        mv.rows16(a, rows_at(it, key), wk, wv);
+        mv.rows16(a, rows_at(it, key + 16), wk + 16 * HD, wv + 16 * HD);
+        int64_t n0 = rows_at(it, key + 32), n1 = rows_at(it, key + 48);
+        AttnWave<HD, T, TC> w;
+        w.init(a, it, 0, lane);
+        for (; key < it.key1; key += 32) {
+            wait_loads();
+            if (__any(key < it.key0 || key + 32 > min(it.key1, w.vis)) &&
+                __any(rows_not_finite<HD>(wv, lane) || rows_not_finite<HD>(wv + 16 * HD, lane))) {
+                w.template infinite_values<1>(wv, 0, key, it.key0, it.key1, lane);
+                wait_lds();
+                clean_rows<HD>(wv, lane);
+                clean_rows<HD>(wv + 16 * HD, lane);
+                wait_lds();
+            }
+            w.template step<1>(wk, wv, 0, key, it.key0, it.key1, lane);
+            wait_lds();
+            if (key + 32 < it.key1) {
+                mv.rows16(a, n0, wk, wv);
+                mv.rows16(a, n1, wk + 16 * HD, wv + 16 * HD);
+                n0 = rows_at(it, key + 64); n1 = rows_at(it, key + 80);
+            }
+        }
+        store(it, w, 0);
+    }
+
+    // ---- wide: every wave takes 32 row-heads; 64 keys at a time in LDS for all, the next 64 on their way into the other buffer
+    __device__ __forceinline__ void wide(const PlanItem & it, TC * s_k0, TC * s_v0, TC * s_k1, TC * s_v1, int * s_vis) const {
+        const int mine = 16 * wave;
+        int key = it.key0 & ~63;
+        mv.rows16(a, rows_at(it, key + mine), s_k0 + mine * HD, s_v0 + mine * HD);
+        int64_t next = rows_at(it, key + 64 + mine);
+        AttnWave<HD, T, TC> w;
+        w.init(a, it, 32 * wave, lane);
+        const bool live = 32 * wave < it.rows * group;
+        int least = w.vis;                                       // the fewest cache rows that a row of the tile sees
+#pragma unroll
+        for (int o = 16; o; o >>= 1) least = min(least, __shfl_xor(least, o));
+        if (lane == 0) s_vis[wave] = least;
+        __syncthreads();
+        least = min(min(s_vis[0], s_vis[1]), min(s_vis[2], s_vis[3]));
+        const int whole = min(it.key1, __builtin_amdgcn_readfirstlane(least));         // steps up to here hide nothing behind them
+        // one stage: its keys have arrived for every wave, and nobody reads the other buffer any more
+        auto stage = [&](const TC * sk, TC * sv, TC * ok, TC * ov) __attribute__((always_inline)) {
+            __syncthreads();
+            if (key + 64 < it.key1) {
+                mv.rows16(a, next, ok + mine * HD, ov + mine * HD);
+                next = rows_at(it, key + 128 + mine);
+            }
+            if ((key < it.key0 || key + 64 > whole) && __syncthreads_or(rows_not_finite<HD>(sv + mine * HD, lane))) {
+                if (live) w.template infinite_values<2>(sv, 0, key, it.key0, it.key1, lane);
+                __syncthreads();
+                clean_rows<HD>(sv + mine * HD, lane);
+                __syncthreads();
+            }
+            if (live) w.template step<2>(sk, sv, 0, key, it.key0, it.key1, lane);
+            key += 64;
+        };
+        while (key < it.key1) {
+            stage(s_k0, s_v0, s_k1, s_v1);
+            if (key >= it.key1) break;
+            stage(s_k1, s_v1, s_k0, s_v0);
+        }
+        store(it, w, 32 * wave);
+        __syncthreads();                                         // LDS is free
+    }
+};
+
+template <int HD, typename T, typename TC>
 __global__ void __launch_bounds__(256, 2) k_paged_attn(PagedArgs a) {
     // two buffers of 64 keys; arrays of their own, so that loads on their way to one do not hold up reads of the other
     __shared__ __attribute__((aligned(1024))) TC s_k0[64 * HD], s_k1[64 * HD], s_v0[64 * HD], s_v1[64 * HD];
-    __shared__ float2 s_ml[4][32];
     __shared__ int s_vis[4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = a.n_head / a.nkv;
+    const int wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
     if (!plan_fits(a)) return;
-    const int n_items = a.head[PH_ITEMS], mask = (1 << a.page_shift) - 1;
-    const Mover<HD, TC> mv(lane);
-    for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
-        const PlanItem it = a.items[item];
-        const int heads = it.rows * group;
-        if (heads == 0) continue;
-        const int64_t head_at = (int64_t) it.head << a.page_shift;
-        // elements from the start of k and v to the 16 rows that begin with `key` (one page holds them; any key gives an address
-        // inside the cache)
-        auto rows_at = [&](int key) __attribute__((always_inline)) {
-            key = __builtin_amdgcn_readfirstlane(key);
-            const int page = max(0, z2o::page_of(a.table, a.n_seq, a.table_len, a.n_pages, a.page_shift, it.seq, key));
-            return (int64_t) __builtin_amdgcn_readfirstlane(page) * a.page_stride + (head_at + (key & mask)) * HD;
-        };
-        AttnWave<HD, T, TC> w;
-        if (heads <= z2o::NARROW_RH) {
-            // ---- every wave takes 32 keys of each 128 and has its own part of LDS: nothing to wait for but its own loads
-            TC * wk = (wave & 2 ? s_k1 : s_k0) + 32 * (wave & 1) * HD, * wv = (wave & 2 ? s_v1 : s_v0) + 32 * (wave & 1) * HD;
-            int key = (it.key0 & ~31) + 32 * wave;
-            if (key < it.key1) { mv.rows16(a, rows_at(key), wk, wv); mv.rows16(a, rows_at(key + 16), wk + 16 * HD, wv + 16 * HD); }
-            int64_t n0 = rows_at(key + 128), n1 = rows_at(key + 144);
-            w.init(a, it, 0, lane);
-            for (; key < it.key1; key += 128) {
-                wait_loads();
-                if (__any(key < it.key0 || key + 32 > min(it.key1, w.vis)) &&
-                    __any(rows_not_finite<HD>(wv, lane) || rows_not_finite<HD>(wv + 16 * HD, lane))) {
-                    w.template infinite_values<1>(wv, 0, key, it.key0, it.key1, lane);
-                    wait_lds();
-                    clean_rows<HD>(wv, lane);
-                    clean_rows<HD>(wv + 16 * HD, lane);
-                    wait_lds();
-                }
-                w.template step<1>(wk, wv, 0, key, it.key0, it.key1, lane);
-                if (key + 128 < it.key1) {
-                    wait_lds();
-                    mv.rows16(a, n0, wk, wv);
-                    mv.rows16(a, n1, wk + 16 * HD, wv + 16 * HD);
-                    n0 = rows_at(key + 256); n1 = rows_at(key + 272);
-                }
-            }
-            // ---- the four waves' results, scaled to one maximum, meet in LDS: each dim quarter in an array of its own
-            w.l += other_half(w.l);
-            if (lane < 32) s_ml[wave][lane] = make_float2(w.m, w.l);
-            __syncthreads();
-            const int rh = lane & 31;
-            const float m = fmaxf(fmaxf(s_ml[0][rh].x, s_ml[1][rh].x), fmaxf(s_ml[2][rh].x, s_ml[3][rh].x));
-            const float f = w.m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(w.m - m);
-            // wave i's [32][HD] floats: 32 keys' K and V of a wave are as many bytes, so two arrays of 64 rows hold one wave's
-            auto s_o = [&](int i, int r, int d) __attribute__((always_inline)) {
-                TC * at = i == 0 ? s_k0 : i == 1 ? s_k1 : i == 2 ? s_v0 : s_v1;
-                return (float *) at + r * HD + d;
-            };
-            static_assert(32 * HD * 4 <= sizeof(s_k0), "merge area");
-            if (rh < heads) {
-#pragma unroll
-                for (int dt = 0; dt < HD / 32; ++dt)
-#pragma unroll
-                    for (int i = 0; i < 16; i += 4)
-                        *(float4 *) s_o(wave, rh, 32 * dt + 2 * i + 4 * (lane >> 5)) =
-                            make_float4(w.o[dt][i] * f, w.o[dt][i + 1] * f, w.o[dt][i + 2] * f, w.o[dt][i + 3] * f);
-            }
-            __syncthreads();
-            for (int e = tid; e < heads * (HD / 4); e += 256) {
-                const int r = e / (HD / 4), d = 4 * (e % (HD / 4));
-                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                float mm = s_ml[0][r].x, ll = 0.0f;
-#pragma unroll
-                for (int i = 1; i < 4; ++i) mm = fmaxf(mm, s_ml[i][r].x);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 ml = s_ml[i][r];
-                    const float4 y = *(const float4 *) s_o(i, r, d);
-                    ll += ml.x == -__builtin_inff() ? 0.0f : ml.y * __builtin_amdgcn_exp2f(ml.x - mm);
-                    x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-                }
-                if (it.direct) {
-                    const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-                    store4((T *) a.out + (it.row0 + r / group) * a.os + (int64_t) (it.head * group + r % group) * HD + d,
-                           x.x * inv, x.y * inv, x.z * inv, x.w * inv);
-                } else {
-                    *(float4 *) (a.part_o + (int64_t) (it.part0 + r) * HD + d) = x;
-                    if (d == 0) a.part_ml[it.part0 + r] = make_float2(mm, ll);
-                }
-            }
-            __syncthreads();
-        } else {
-            // ---- every wave takes 32 row-heads; 64 keys at a time in LDS for all, the next 64 on their way into the other buffer
-            const int mine = 16 * wave;
-            int key = it.key0 & ~63;
-            mv.rows16(a, rows_at(key + mine), s_k0 + mine * HD, s_v0 + mine * HD);
-            int64_t next = rows_at(key + 64 + mine);
-            w.init(a, it, 32 * wave, lane);
-            const bool live = 32 * wave < heads;
-            int least = w.vis;                                   // the fewest cache rows that a row of the tile sees
-#pragma unroll
-            for (int o = 16; o; o >>= 1) least = min(least, __shfl_xor(least, o));
-            if (lane == 0) s_vis[wave] = least;
-            __syncthreads();
-            least = min(min(s_vis[0], s_vis[1]), min(s_vis[2], s_vis[3]));
-            const int whole = min(it.key1, __builtin_amdgcn_readfirstlane(least));     // steps up to here hide nothing behind them
-            // one stage: its keys have arrived for every wave, and nobody reads the other buffer any more
-            auto stage = [&](const TC * sk, TC * sv, TC * ok, TC * ov) __attribute__((always_inline)) {
-                __syncthreads();
-                if (key + 64 < it.key1) {
-                    mv.rows16(a, next, ok + mine * HD, ov + mine * HD);
-                    next = rows_at(key + 128 + mine);
-                }
-                if ((key < it.key0 || key + 64 > whole) && __syncthreads_or(rows_not_finite<HD>(sv + mine * HD, lane))) {
-                    if (live) w.template infinite_values<2>(sv, 0, key, it.key0, it.key1, lane);
-                    __syncthreads();
-                    clean_rows<HD>(sv + mine * HD, lane);
-                    __syncthreads();
-                }
-                if (live) w.template step<2>(sk, sv, 0, key, it.key0, it.key1, lane);
-                key += 64;
-            };
-            while (key < it.key1) {
-                stage(s_k0, s_v0, s_k1, s_v1);
-                if (key >= it.key1) break;
-                stage(s_k1, s_v1, s_k0, s_v0);
-            }
-            w.l += other_half(w.l);
-            const int rh = 32 * wave + (lane & 31);
-            if (rh < heads) {
-                const float inv = !it.direct ? 1.0f : w.l == 0.0f ? 0.0f : 1.0f / w.l;
-                T * out = (T *) a.out + (it.row0 + rh / group) * a.os + (int64_t) (it.head * group + rh % group) * HD;
-                float * part = a.part_o + (int64_t) (it.part0 + rh) * HD;
-#pragma unroll
-                for (int dt = 0; dt < HD / 32; ++dt)
-#pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        const int d = 32 * dt + 2 * i + 4 * (lane >> 5);
-                        const float4 x = make_float4(w.o[dt][i] * inv, w.o[dt][i + 1] * inv, w.o[dt][i + 2] * inv, w.o[dt][i + 3] * inv);
-                        if (it.direct) store4(out + d, x.x, x.y, x.z, x.w);
-                        else *(float4 *) (part + d) = x;
-                    }
-                if (!it.direct && lane < 32) a.part_ml[it.part0 + rh] = make_float2(w.m, w.l);
-            }
-            __syncthreads();
-        }
+    const PagedAttn<HD, T, TC> p(a, threadIdx.x & 63, wave);
+    PlanItem it;
+    {
+        const PlanKind kind(a, true);
+        ShareWalk walk(a, kind, blockIdx.x);
+        while (walk.next(a, kind, p.group, it)) p.wide(it, s_k0, s_v0, s_k1, s_v1, s_vis);
+    }
+    {
+        // (the first shares on different compute units)
+        const PlanKind kind(a, false);
+        ShareWalk walk(a, kind, wave * a.blocks + blockIdx.x);
+        TC * wk = (wave & 2 ? s_k1 : s_k0) + 32 * (wave & 1) * HD, * wv = (wave & 2 ? s_v1 : s_v0) + 32 * (wave & 1) * HD;
+        while (walk.next(a, kind, p.group, it)) p.narrow(it, wk, wv);
     }
 }
 
@@ -636,13 +692,25 @@ __global__ void __launch_bounds__(256) k_paged_join(PagedArgs a) {
     if (id >= a.n_rows * a.n_head) return;
     const int row = id / a.n_head, head = id % a.n_head, group = a.n_head / a.nkv, g = head / group;
     const PlanRow r = a.rows[row];
-    if (r.pre_n == 0 && r.own_n == 1) return;                    // stored by its only chunk
-    const int n = r.pre_n + r.own_n;
-    auto part = [&](int i) {
-        const bool pre = i < r.pre_n;
-        const int step = pre ? r.pre_step : r.own_step;
-        return (pre ? r.pre_base + i * step : r.own_base + (i - r.pre_n) * step) + g * (step / a.nkv) + head % group;
+    // the pieces of the row's strip of a tile: how many, the first one's place and the step between places
+    auto pieces_of = [&](int tile, int at, int & first, int & step, bool & stored) {
+        if (tile < 0) return 0;
+        const PlanTile t = a.tiles[tile];
+        step = t.rows * group;
+        const PlanKind kind(a, z2o::is_wide(step));
+        int begin, most;
+        const int n = kind.piece(t, g, 0, begin, most).n;
+        first = t.part0 + g * most * step + at + head % group;
+        stored = t.alone && n == 1;
+        return n;
     };
+    int pre0 = 0, own0 = 0, pre_step = 0, own_step = 0;
+    bool stored = false, unused;
+    const int n_pre = pieces_of(r.pre_tile, r.pre_at, pre0, pre_step, unused);
+    const int n_own = pieces_of(r.own_tile, r.own_at, own0, own_step, stored);
+    if (stored) return;                                          // by its only piece
+    const int n = n_pre + n_own;
+    auto part = [&](int i) { return i < n_pre ? pre0 + i * pre_step : own0 + (i - n_pre) * own_step; };
     constexpr int E = HD >= 64 ? HD / 64 : 1;
     const int d = E * lane;
     float m = -__builtin_inff(), l = 0.0f, o[E] = {};
