@@ -167,8 +167,8 @@ static void workspace() {
         }
         EXPECT((int64_t) tiles.size() <= w.max_tiles || n_rows == 0);
         EXPECT(parts <= w.max_parts);
-        EXPECT(w.rows % 256 == 0 && w.tiles % 256 == 0 && w.starts % 256 == 0 && w.ml % 256 == 0 && w.o % 256 == 0);
-        EXPECT(w.bytes >= w.o + w.max_parts * p.head_dim * 4 && w.o >= w.ml + w.max_parts * 8 && w.ml >= w.starts + 5 * target * 8ll);
+        EXPECT(w.rows % 256 == 0 && w.tiles % 256 == 0 && w.shares % 256 == 0 && w.strips % 256 == 0 && w.ml % 256 == 0 && w.o % 256 == 0);
+        EXPECT(w.bytes >= w.o + w.max_parts * p.head_dim * 4 && w.o >= w.ml + w.max_parts * 8 && w.ml >= w.shares + 5 * target * 64ll);
     }
     // the largest call's counts stay below 2^31
     z2h_pages p = good_pages();

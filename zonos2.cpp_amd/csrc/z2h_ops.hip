@@ -176,7 +176,8 @@ int z2h_paged_plan(z2h_ctx * ctx, const z2h_pages * pages, int n_head, int n_row
     a.cap = pages->table_len * pages->page_rows;
     a.blocks = attn_blocks(n_cu);
     uint8_t * ws = (uint8_t *) d_ws;
-    a.head = (int32_t *) ws; a.rows = (PlanRow *) (ws + w.rows); a.tiles = (PlanTile *) (ws + w.tiles); a.starts = (int2 *) (ws + w.starts);
+    a.head = (int32_t *) ws; a.rows = (PlanRow *) (ws + w.rows); a.tiles = (PlanTile *) (ws + w.tiles); a.strips = (PlanStrip *) (ws + w.strips);
+    a.shares = (PlanShare *) (ws + w.shares);
     a.max_tiles = (int) w.max_tiles; a.max_parts = (int) w.max_parts;
     ON_DEVICE;
     hipLaunchKernelGGL(k_paged_plan, dim3(1), dim3(PLAN_T), 0, (hipStream_t) stream, a);
@@ -206,7 +207,7 @@ int z2h_paged_attn(z2h_ctx * ctx, const z2h_pages * pages, int n_head, int n_row
     a.q = d_q; a.out = d_out;
     uint8_t * ws = (uint8_t *) d_ws;
     a.head = (const int32_t *) ws; a.rows = (const PlanRow *) (ws + w.rows); a.tiles = (const PlanTile *) (ws + w.tiles);
-    a.starts = (const int2 *) (ws + w.starts);
+    a.strips = (const PlanStrip *) (ws + w.strips); a.shares = (const PlanShare *) (ws + w.shares);
     a.part_ml = (float2 *) (ws + w.ml); a.part_o = (float *) (ws + w.o);
     const int blocks = attn_blocks(n_cu);
     a.max_tiles = (int) w.max_tiles;

@@ -151,7 +151,7 @@ Z2O_HD int max_pieces(int cost, int share) { return cost ? cost / share + 2 : 0;
 
 // ---- attention workspace
 struct AttnWs {
-    int64_t rows = 0, tiles = 0, starts = 0, ml = 0, o = 0, bytes = 0;   // offsets in bytes; the header is at 0
+    int64_t rows = 0, tiles = 0, strips = 0, shares = 0, ml = 0, o = 0, bytes = 0;   // offsets in bytes; the header is at 0
     int64_t max_tiles = 0, max_parts = 0;
 };
 inline int64_t align256(int64_t n) { return (n + 255) & ~(int64_t) 255; }
@@ -167,8 +167,9 @@ inline AttnWs attn_ws(const z2h_pages & p, int n_head, int n_rows, int n_group, 
     w.max_parts = n_rows ? blocks * ((rh < TILE_RH ? rh : TILE_RH) + 4 * (rh < NARROW_RH ? rh : NARROW_RH)) + 4 * (int64_t) n_rows * n_head : 0;
     w.rows = 256;
     w.tiles = w.rows + align256((int64_t) n_rows * 32);
-    w.starts = w.tiles + align256(w.max_tiles * 32);
-    w.ml = w.starts + align256((int64_t) blocks * 5 * 8);
+    w.strips = w.tiles + align256(w.max_tiles * 32);
+    w.shares = w.strips + align256(w.max_tiles * p.n_head_kv * 8);
+    w.ml = w.shares + align256((int64_t) blocks * 5 * 64);
     w.o = w.ml + align256(w.max_parts * 8);
     w.bytes = w.o + align256(w.max_parts * p.head_dim * 4);
     return w;

@@ -15,8 +15,8 @@
 namespace z2d {
 
 constexpr int PLAN_MAGIC = 0x50414745;
-enum { PH_MAGIC = 0, PH_ROWS, PH_HEADS, PH_GROUPS, PH_SEQS, PH_KV_HEADS, PH_SHIFT, PH_KIND, PH_COUNT = PH_KIND + 8 };
-enum { PK_TILES = 0, PK_SHARES, PK_SHARE, PK_HEAD };             // of each kind, narrow then wide, from PH_KIND on
+enum { PH_MAGIC = 0, PH_ROWS, PH_HEADS, PH_GROUPS, PH_SEQS, PH_KV_HEADS, PH_SHIFT, PH_KIND, PH_COUNT = PH_KIND + 6 };
+enum { PK_TILES = 0, PK_SHARE, PK_HEAD };                        // of each kind, narrow then wide, from PH_KIND on
 
 // per row: what it sees, and its tiles in its group's prefix and in its own keys (-1: none), and its place in their row-heads
 struct PlanRow { int vis, pre_tile, pre_at, own_tile, own_at, spare[3]; };
@@ -24,7 +24,14 @@ struct PlanRow { int vis, pre_tile, pre_at, own_tile, own_at, spare[3]; };
 // (g x pieces + at) x row-heads, `pieces` the most that any of its strips has; alone: its rows have no other tile. Wide tiles are
 // kept from the table's first place on, narrow ones from its last backwards.
 struct PlanTile { int row0, rows, key0, key1, seq, alone, begin, part0; };
-static_assert(sizeof(PlanRow) == 32 && sizeof(PlanTile) == 32, "workspace layout");
+// a piece of a strip: query rows, keys, and where its results go
+struct PlanItem { int row0, rows, key0, key1, seq, head, part0, direct; };
+// what a block (wide) or a wave (narrow) begins with: its share's first piece (rows 0: none), and the strip that may have the next (tile
+// of its kind -1: none)
+struct PlanShare { PlanItem it; int share, tile, head, spare[5]; };
+// of a tile's strip: its first partial result, its pieces, the tile's row-heads, and whether its only piece stores the rows itself
+struct PlanStrip { int part0; unsigned short pieces; unsigned char heads, stored; };
+static_assert(sizeof(PlanRow) == 32 && sizeof(PlanTile) == 32 && sizeof(PlanShare) == 64 && sizeof(PlanStrip) == 8, "workspace layout");
 
 struct PlanArgs {
     const int32_t * row_start, * kv_len, * group_start, * prefix_len;
@@ -32,9 +39,11 @@ struct PlanArgs {
     int32_t * head;
     PlanRow * rows;
     PlanTile * tiles;
-    int2 * starts;                                               // a share's first strip: tile of its kind, key head; [blocks] wide, [4 blocks] narrow
+    PlanStrip * strips;                                          // [tile's place][key head]
+    PlanShare * shares;                                          // [blocks] wide, [blocks][4] narrow
     int max_tiles, max_parts;
 };
+
 __device__ __forceinline__ int tile_place(int i, bool wide, int max_tiles) { return wide ? i : max_tiles - 1 - i; }
 
 // the last index i of [0, n) with start[i] <= x (start ascending; -1: none)
@@ -69,6 +78,30 @@ __device__ __forceinline__ int block_scan(int v, int * s_wave, int & total) {
     total = all;
     return below + x - v;
 }
+
+struct PlanKind {
+    z2o::Cut cut;
+    int tiles, shift, max_tiles, nkv, group;
+    bool wide;
+    // the next piece that share b has, from the tile's strip `head` on: (tile, head) is then the strip behind it
+    __device__ __forceinline__ bool next(const PlanTile * all, int b, int & tile, int & head, PlanItem & it) const {
+        while (tile < tiles) {
+            const PlanTile t = all[tile_place(tile, wide, max_tiles)];
+            const int units = (int) z2o::strip_units(t.key0, t.key1, wide, shift), cost = (int) z2o::strip_cost(units, cut.head);
+            const int begin = t.begin + head * (int) z2o::strip_pitch(cost, cut);
+            if (units && begin >= (b + 1) * cut.share) return false;
+            const z2o::Piece p = z2o::strip_piece(begin, units, cut, b);
+            const int g = head;
+            if (units == 0 || ++head == nkv) { ++tile; head = 0; }
+            if (p.u0 >= p.u1) continue;
+            const int base = t.key0 & ~63, unit = z2o::unit_keys(wide) << shift;
+            it = PlanItem{t.row0, t.rows, max(t.key0, base + p.u0 * unit), min(t.key1, base + p.u1 * unit), t.seq, g,
+                          t.part0 + (g * z2o::max_pieces(cost, cut.share) + p.at) * t.rows * group, t.alone && p.n == 1};
+            return true;
+        }
+        return false;
+    }
+};
 
 // One block. Everything is clamped to the tables' sizes, so that whatever the lengths say no entry leads outside the buffers.
 __global__ void __launch_bounds__(PLAN_T) k_paged_plan(PlanArgs a) {
@@ -122,13 +155,12 @@ __global__ void __launch_bounds__(PLAN_T) k_paged_plan(PlanArgs a) {
     }
     atomicAdd(&s_total, units);                                  // integers: the order does not matter
     __syncthreads();
-    int shift = 0, n_parts = 0;
+    int shift = 0, n_parts = 0, n_wide_shares = 0;
     while (s_total >> shift >= 1ull << 28) ++shift;
 #pragma unroll 1
-    for (int kind = 0; kind < 2; ++kind) {
+    for (int kind = 1; kind >= 0; --kind) {
         const bool wide = kind;
         const int count = min(n_tiles[kind], a.max_tiles), max_shares = wide ? a.blocks : 4 * a.blocks, head = z2o::piece_cost(wide);
-        int2 * starts = wide ? a.starts : a.starts + a.blocks;
         auto tile = [&](int i) -> PlanTile & { return a.tiles[tile_place(i, wide, a.max_tiles)]; };
         auto units_of = [&](const PlanTile & t) { return (int) z2o::strip_units(t.key0, t.key1, wide, shift); };
         // ---- how to cut: what all strips cost in a row, and the smallest whole share that needs no more than there are
@@ -171,22 +203,49 @@ __global__ void __launch_bounds__(PLAN_T) k_paged_plan(PlanArgs a) {
             }
         }
         __syncthreads();
-        // ---- every share's first strip
-        const int shares = min((total + cut.share - 1) / cut.share, max_shares);
-        for (int b = tid; b < shares; b += PLAN_T) {
-            const int at = b * cut.share;
-            int lo = 0, hi = count;
-            while (hi - lo > 1) {
-                const int m = (lo + hi) >> 1;
-                if ((m < LDS_TILES ? s_begin[m] : tile(m).begin) <= at) lo = m; else hi = m;
-            }
-            const PlanTile t = tile(lo);
-            const int pitch = (int) z2o::strip_pitch(z2o::strip_cost(units_of(t), cut.head), cut);
-            starts[b] = make_int2(lo, pitch ? min((at - t.begin) / pitch, a.nkv - 1) : 0);
+        const PlanKind k{cut, count, shift, a.max_tiles, a.nkv, group, wide};
+        // ---- of every strip, where its results are
+        for (int64_t i = tid; i < (int64_t) count * a.nkv; i += PLAN_T) {
+            const int place = tile_place((int) (i / a.nkv), wide, a.max_tiles), g = (int) (i % a.nkv);
+            const PlanTile t = a.tiles[place];
+            const int units = units_of(t), cost = (int) z2o::strip_cost(units, cut.head), heads = t.rows * group;
+            const z2o::Piece p = z2o::strip_piece(t.begin + g * (int) z2o::strip_pitch(cost, cut), units, cut, 0);
+            a.strips[(int64_t) place * a.nkv + g] = PlanStrip{t.part0 + g * z2o::max_pieces(cost, cut.share) * heads, (unsigned short) p.n,
+                                                              (unsigned char) heads, (unsigned char) (t.alone && p.n == 1)};
         }
+        // ---- every share's first piece. Narrow shares go first to the blocks that have no wide one, a wave on each of them, then
+        // the next waves, and then to the others.
+        const int shares = min((total + cut.share - 1) / cut.share, max_shares), free = a.blocks - n_wide_shares;
+        for (int b = tid; b < max_shares; b += PLAN_T) {
+            PlanShare sh{};
+            sh.share = b;
+            sh.tile = -1;
+            if (b < shares) {
+                const int at = b * cut.share;
+                int lo = 0, hi = count;
+                while (hi - lo > 1) {
+                    const int m = (lo + hi) >> 1;
+                    if ((m < LDS_TILES ? s_begin[m] : tile(m).begin) <= at) lo = m; else hi = m;
+                }
+                const PlanTile t = tile(lo);
+                const int pitch = (int) z2o::strip_pitch(z2o::strip_cost(units_of(t), cut.head), cut);
+                sh.tile = lo;
+                sh.head = pitch ? min((at - t.begin) / pitch, a.nkv - 1) : 0;
+                if (!k.next(a.tiles, b, sh.tile, sh.head, sh.it)) sh.it.rows = 0;
+                if (!cut.head || sh.it.rows == 0) sh.tile = -1;          // whole shares have one piece
+            }
+            if (wide) a.shares[b] = sh;
+            else {
+                int block, wave;
+                if (b < 4 * free) { block = a.blocks - 1 - b % free; wave = b / free; }
+                else { const int c = b - 4 * free; block = n_wide_shares - 1 - c % n_wide_shares; wave = c / n_wide_shares; }
+                a.shares[a.blocks + 4 * block + wave] = sh;
+            }
+        }
+        if (wide) n_wide_shares = shares;
         if (tid == 0) {
-            int32_t * k = a.head + PH_KIND + 4 * kind;
-            k[PK_TILES] = count; k[PK_SHARES] = shares; k[PK_SHARE] = cut.share; k[PK_HEAD] = cut.head;
+            int32_t * h = a.head + PH_KIND + 3 * kind;
+            h[PK_TILES] = count; h[PK_SHARE] = cut.share; h[PK_HEAD] = cut.head;
         }
         __syncthreads();
     }
@@ -208,7 +267,8 @@ struct PagedArgs {
     const int32_t * head;
     const PlanRow * rows;
     const PlanTile * tiles;
-    const int2 * starts;
+    const PlanStrip * strips;
+    const PlanShare * shares;
     int max_tiles, blocks;
     float2 * part_ml;
     float * part_o;
@@ -218,48 +278,6 @@ __device__ __forceinline__ bool plan_fits(const PagedArgs & a) {
     return a.head[PH_MAGIC] == PLAN_MAGIC && a.head[PH_ROWS] == a.n_rows && a.head[PH_HEADS] == a.n_head && a.head[PH_GROUPS] == a.n_group &&
            a.head[PH_SEQS] == a.n_seq && a.head[PH_KV_HEADS] == a.nkv;
 }
-
-// a piece of a strip: query rows, keys, and where its results go
-struct PlanItem { int row0, rows, key0, key1, seq, head, part0, direct; };
-struct PlanKind {
-    z2o::Cut cut;
-    int tiles, shares, shift;
-    bool wide;
-    __device__ __forceinline__ PlanKind(const PagedArgs & a, bool wide_) : wide(wide_) {
-        const int32_t * k = a.head + PH_KIND + 4 * (int) wide_;
-        tiles = k[PK_TILES]; shares = k[PK_SHARES]; cut = z2o::Cut{k[PK_SHARE], k[PK_HEAD]}; shift = a.head[PH_SHIFT];
-    }
-    // the piece that share b has of the tile's strip g, where that begins, and the most pieces that a strip of the tile has
-    __device__ __forceinline__ z2o::Piece piece(const PlanTile & t, int g, int b, int & begin, int & most) const {
-        const int units = (int) z2o::strip_units(t.key0, t.key1, wide, shift), cost = (int) z2o::strip_cost(units, cut.head);
-        most = z2o::max_pieces(cost, cut.share);
-        begin = t.begin + g * (int) z2o::strip_pitch(cost, cut);
-        return z2o::strip_piece(begin, units, cut, b);
-    }
-};
-// The pieces of share b, one after the other.
-struct ShareWalk {
-    int b, tile, g;
-    __device__ __forceinline__ ShareWalk(const PagedArgs & a, const PlanKind & k, int share) : b(share), tile(k.tiles), g(0) {
-        if (b < k.shares) { const int2 s = a.starts[k.wide ? b : a.blocks + b]; tile = s.x; g = s.y; }
-    }
-    __device__ __forceinline__ bool next(const PagedArgs & a, const PlanKind & k, int group, PlanItem & it) {
-        while (tile < k.tiles) {
-            const PlanTile t = a.tiles[tile_place(tile, k.wide, a.max_tiles)];
-            int begin, pieces;
-            const z2o::Piece p = k.piece(t, g, b, begin, pieces);
-            if (p.n && begin >= (b + 1) * k.cut.share) return false;
-            const int head = g;
-            if (p.n == 0 || ++g == a.nkv) { ++tile; g = 0; }
-            if (p.u0 >= p.u1) continue;
-            const int base = t.key0 & ~63, unit = z2o::unit_keys(k.wide) << k.shift;
-            it = PlanItem{t.row0, t.rows, max(t.key0, base + p.u0 * unit), min(t.key1, base + p.u1 * unit), t.seq, head,
-                          t.part0 + (head * pieces + p.at) * t.rows * group, t.alone && p.n == 1};
-            return true;
-        }
-        return false;
-    }
-};
 
 typedef float v16f_t __attribute__((ext_vector_type(16)));
 typedef unsigned u4_t __attribute__((ext_vector_type(4)));
@@ -376,13 +394,15 @@ struct AttnWave {
         }
     }
 
-    // keys key0 .. key0 + 32 NT, in LDS from row r0 on; keys outside [from, min(to, vis)) are hidden. One body for all steps: a second
+    // keys key0 .. key0 + 32 NT, in the first rows of sk and sv; keys outside [from, min(to, vis)) are hidden. One body for all steps: a second
     // one for steps that hide something costs the compiler another set of accumulators (256 registers and 126 spilled against 237).
-    template <int NT>
-    __device__ __forceinline__ void step(const TC * sk, const TC * sv, int r0, int key0, int from, int to, int lane) {
-        const int end = min(to, vis);
+    // keys_done() is called when K has been read, values_ready() before V is.
+    template <int NT, typename F, typename G>
+    __device__ __forceinline__ void step(const TC * sk, const TC * sv, int key0, int from, int to, int lane, F keys_done, G values_ready) {
+        const int end = min(to, vis), r0 = 0;
         v16f_t s[NT];
         scores<NT>(s, sk, r0, lane);
+        keys_done();
         __builtin_amdgcn_sched_barrier(0);                       // no V read ahead of the weights: registers
         if (__any(key0 < from || key0 + 32 * NT > end)) {
             const int h4 = 4 * (lane >> 5);
@@ -427,6 +447,7 @@ struct AttnWave {
             }
         l += sum;
         __builtin_amdgcn_sched_barrier(0);
+        values_ready();
 #pragma unroll
         for (int t = 0; t < 2 * NT; ++t)
 #pragma unroll
@@ -509,8 +530,9 @@ __device__ __forceinline__ void clean_rows(TC * sv, int lane) {
     }
 }
 
-// the wave's own loads have arrived; its own LDS reads have been answered
-__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); asm volatile("" ::: "memory"); }
+// all of the wave's own loads but the last N have arrived; its own LDS reads have been answered
+template <int N>
+__device__ __forceinline__ void wait_loads_but() { static_assert(N < 16, ""); __builtin_amdgcn_s_waitcnt(0x0f70 | N); asm volatile("" ::: "memory"); }
 __device__ __forceinline__ void wait_lds() { asm volatile("" ::: "memory"); __builtin_amdgcn_s_waitcnt(0xc07f); }
 
 template <typename T>
@@ -543,14 +565,19 @@ struct Mover {
         for (int i = 0; i < 16 / ROWS; ++i) k[i] = Tile<HD>::k_at(i * ROWS + row, x);
         v = Tile<HD>::v_at(row, x);
     }
-    // 16 rows from `at` (elements from the start of k and v) to the rows of LDS at sk, sv
-    // (rows 16 apart are permuted alike)
-    __device__ __forceinline__ void rows16(const PagedArgs & a, int64_t at, TC * sk, TC * sv) const {
+    static constexpr int N = 16 / ROWS;                          // instructions for 16 rows of K or V
+    // 16 rows from `at` (elements from the start of k and v) to the rows of LDS at `to` (rows 16 apart are permuted alike)
+    __device__ __forceinline__ void keys16(const PagedArgs & a, int64_t at, TC * to) const {
 #pragma unroll
-        for (int i = 0; i < 16 / ROWS; ++i) {
-            to_lds((const TC *) a.k + at + k[i], sk + i * ROWS * HD);
-            to_lds((const TC *) a.v + at + i * ROWS * HD + v, sv + i * ROWS * HD);
-        }
+        for (int i = 0; i < N; ++i) to_lds((const TC *) a.k + at + k[i], to + i * ROWS * HD);
+    }
+    __device__ __forceinline__ void values16(const PagedArgs & a, int64_t at, TC * to) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) to_lds((const TC *) a.v + at + i * ROWS * HD + v, to + i * ROWS * HD);
+    }
+    __device__ __forceinline__ void rows16(const PagedArgs & a, int64_t at, TC * sk, TC * sv) const {
+        keys16(a, at, sk);
+        values16(a, at, sv);
     }
 };
 
@@ -590,31 +617,40 @@ struct PagedAttn {
         if (!it.direct && lane < 32) a.part_ml[it.part0 + rh] = make_float2(w.m, w.l);
     }
 
-    // ---- narrow: the wave's own 32 rows of LDS (K at wk, V at wv), its own keys; nothing to wait for but its own loads
+    // ---- narrow: the wave's own 32 rows of LDS (K at wk, V at wv), its own keys; nothing to wait for but its own loads. The next keys
+    // are requested when this step's scores are formed, the next values when its values have been used.
     __device__ __forceinline__ void narrow(const PlanItem & it, TC * wk, TC * wv) const {
         int key = it.key0 & ~31;
-        mv.rows16(a, rows_at(it, key), wk, wv);
-        mv.rows16(a, rows_at(it, key + 16), wk + 16 * HD, wv + 16 * HD);
-        int64_t n0 = rows_at(it, key + 32), n1 = rows_at(it, key + 48);
+        int64_t n0 = rows_at(it, key), n1 = rows_at(it, key + 16);
+        mv.keys16(a, n0, wk);
+        mv.keys16(a, n1, wk + 16 * HD);
+        mv.values16(a, n0, wv);
+        mv.values16(a, n1, wv + 16 * HD);
         AttnWave<HD, T, TC> w;
         w.init(a, it, 0, lane);
         for (; key < it.key1; key += 32) {
-            wait_loads();
-            if (__any(key < it.key0 || key + 32 > min(it.key1, w.vis)) &&
-                __any(rows_not_finite<HD>(wv, lane) || rows_not_finite<HD>(wv + 16 * HD, lane))) {
-                w.template infinite_values<1>(wv, 0, key, it.key0, it.key1, lane);
-                wait_lds();
-                clean_rows<HD>(wv, lane);
-                clean_rows<HD>(wv + 16 * HD, lane);
-                wait_lds();
+            const bool more = key + 32 < it.key1;
+            wait_loads_but<2 * Mover<HD, TC>::N>();              // the values may still be on their way
+            if (__any(key < it.key0 || key + 32 > min(it.key1, w.vis))) {
+                wait_loads_but<0>();
+                if (__any(rows_not_finite<HD>(wv, lane) || rows_not_finite<HD>(wv + 16 * HD, lane))) {
+                    w.template infinite_values<1>(wv, 0, key, it.key0, it.key1, lane);
+                    wait_lds();
+                    clean_rows<HD>(wv, lane);
+                    clean_rows<HD>(wv + 16 * HD, lane);
+                    wait_lds();
+                }
             }
-            w.template step<1>(wk, wv, 0, key, it.key0, it.key1, lane);
+            if (more) { n0 = rows_at(it, key + 32); n1 = rows_at(it, key + 48); }
+            w.template step<1>(wk, wv, key, it.key0, it.key1, lane, [&] {
+                wait_lds();
+                if (more) { mv.keys16(a, n0, wk); mv.keys16(a, n1, wk + 16 * HD); }
+            }, [&] {
+                if (more) wait_loads_but<2 * Mover<HD, TC>::N>();
+                else wait_loads_but<0>();
+            });
             wait_lds();
-            if (key + 32 < it.key1) {
-                mv.rows16(a, n0, wk, wv);
-                mv.rows16(a, n1, wk + 16 * HD, wv + 16 * HD);
-                n0 = rows_at(it, key + 64); n1 = rows_at(it, key + 80);
-            }
+            if (more) { mv.values16(a, n0, wv); mv.values16(a, n1, wv + 16 * HD); }
         }
         store(it, w, 0);
     }
@@ -648,7 +684,7 @@ struct PagedAttn {
                 clean_rows<HD>(sv + mine * HD, lane);
                 __syncthreads();
             }
-            if (live) w.template step<2>(sk, sv, 0, key, it.key0, it.key1, lane);
+            if (live) w.template step<2>(sk, sv, key, it.key0, it.key1, lane, [] {}, [] {});
             key += 64;
         };
         while (key < it.key1) {
@@ -669,18 +705,23 @@ __global__ void __launch_bounds__(256, 2) k_paged_attn(PagedArgs a) {
     const int wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
     if (!plan_fits(a)) return;
     const PagedAttn<HD, T, TC> p(a, threadIdx.x & 63, wave);
-    PlanItem it;
-    {
-        const PlanKind kind(a, true);
-        ShareWalk walk(a, kind, blockIdx.x);
-        while (walk.next(a, kind, p.group, it)) p.wide(it, s_k0, s_v0, s_k1, s_v1, s_vis);
+    // (both records are requested before either is used)
+    const PlanShare wide = a.shares[blockIdx.x], narrow = a.shares[a.blocks + 4 * blockIdx.x + wave];
+    auto rest = [&](bool kind, PlanShare & s) __attribute__((always_inline)) {
+        const int32_t * h = a.head + PH_KIND + 3 * (int) kind;
+        const PlanKind k{z2o::Cut{h[PK_SHARE], h[PK_HEAD]}, h[PK_TILES], a.head[PH_SHIFT], a.max_tiles, a.nkv, p.group, kind};
+        return s.tile >= 0 && k.next(a.tiles, s.share, s.tile, s.head, s.it);
+    };
+    if (wide.it.rows > 0) {
+        PlanShare s = wide;
+        do p.wide(s.it, s_k0, s_v0, s_k1, s_v1, s_vis); while (rest(true, s));
     }
-    {
-        // (the first shares on different compute units)
-        const PlanKind kind(a, false);
-        ShareWalk walk(a, kind, wave * a.blocks + blockIdx.x);
-        TC * wk = (wave & 2 ? s_k1 : s_k0) + 32 * (wave & 1) * HD, * wv = (wave & 2 ? s_v1 : s_v0) + 32 * (wave & 1) * HD;
-        while (walk.next(a, kind, p.group, it)) p.narrow(it, wk, wv);
+    if (narrow.it.rows > 0) {
+        PlanShare s = narrow;
+        // (a copy for each pair of arrays: loads on their way to one array do not hold up reads of the other)
+        const int at = 32 * (wave & 1) * HD;
+        if (wave & 2) { do p.narrow(s.it, s_k1 + at, s_v1 + at); while (rest(false, s)); }
+        else { do p.narrow(s.it, s_k0 + at, s_v0 + at); while (rest(false, s)); }
     }
 }
 
@@ -692,23 +733,11 @@ __global__ void __launch_bounds__(256) k_paged_join(PagedArgs a) {
     if (id >= a.n_rows * a.n_head) return;
     const int row = id / a.n_head, head = id % a.n_head, group = a.n_head / a.nkv, g = head / group;
     const PlanRow r = a.rows[row];
-    // the pieces of the row's strip of a tile: how many, the first one's place and the step between places
-    auto pieces_of = [&](int tile, int at, int & first, int & step, bool & stored) {
-        if (tile < 0) return 0;
-        const PlanTile t = a.tiles[tile];
-        step = t.rows * group;
-        const PlanKind kind(a, z2o::is_wide(step));
-        int begin, most;
-        const int n = kind.piece(t, g, 0, begin, most).n;
-        first = t.part0 + g * most * step + at + head % group;
-        stored = t.alone && n == 1;
-        return n;
-    };
-    int pre0 = 0, own0 = 0, pre_step = 0, own_step = 0;
-    bool stored = false, unused;
-    const int n_pre = pieces_of(r.pre_tile, r.pre_at, pre0, pre_step, unused);
-    const int n_own = pieces_of(r.own_tile, r.own_at, own0, own_step, stored);
-    if (stored) return;                                          // by its only piece
+    const PlanStrip pre = r.pre_tile >= 0 ? a.strips[(int64_t) r.pre_tile * a.nkv + g] : PlanStrip{0, 0, 0, 0};
+    const PlanStrip own = r.own_tile >= 0 ? a.strips[(int64_t) r.own_tile * a.nkv + g] : PlanStrip{0, 0, 0, 0};
+    if (own.stored) return;                                      // by its only piece
+    const int n_pre = pre.pieces, n_own = own.pieces, pre_step = pre.heads, own_step = own.heads;
+    const int pre0 = pre.part0 + r.pre_at + head % group, own0 = own.part0 + r.own_at + head % group;
     const int n = n_pre + n_own;
     auto part = [&](int i) { return i < n_pre ? pre0 + i * pre_step : own0 + (i - n_pre) * own_step; };
     constexpr int E = HD >= 64 ? HD / 64 : 1;
