@@ -79,14 +79,33 @@ __device__ __forceinline__ int block_scan(int v, int * s_wave, int & total) {
     return below + x - v;
 }
 
+// What a kernel only reads and a whole wave agrees on is read through the constant address space: as scalar loads, which do not queue behind
+// the wave's other loads (a page number read as a vector load waits for all K and V on their way: steps of 2.6 us against 1.6).
+template <typename T>
+__device__ __forceinline__ const __attribute__((address_space(4))) T * uniform(const T * p) { return (const __attribute__((address_space(4))) T *) p; }
+
+template <typename T>
+__device__ __forceinline__ void uniform_copy(T & to, const T * from) {
+    static_assert(sizeof(T) % 4 == 0, "");
+    int32_t x[sizeof(T) / 4];
+    const __attribute__((address_space(4))) int32_t * p = (const __attribute__((address_space(4))) int32_t *) from;
+#pragma unroll
+    for (int i = 0; i < (int) (sizeof(T) / 4); ++i) x[i] = p[i];
+    __builtin_memcpy(&to, x, sizeof(T));
+}
+
 struct PlanKind {
     z2o::Cut cut;
     int tiles, shift, max_tiles, nkv, group;
     bool wide;
     // the next piece that share b has, from the tile's strip `head` on: (tile, head) is then the strip behind it
+    // (KERNEL: not in the kernel that writes the tiles)
+    template <bool KERNEL>
     __device__ __forceinline__ bool next(const PlanTile * all, int b, int & tile, int & head, PlanItem & it) const {
         while (tile < tiles) {
-            const PlanTile t = all[tile_place(tile, wide, max_tiles)];
+            PlanTile t;
+            if constexpr (KERNEL) uniform_copy(t, all + tile_place(tile, wide, max_tiles));
+            else t = all[tile_place(tile, wide, max_tiles)];
             const int units = (int) z2o::strip_units(t.key0, t.key1, wide, shift), cost = (int) z2o::strip_cost(units, cut.head);
             const int begin = t.begin + head * (int) z2o::strip_pitch(cost, cut);
             if (units && begin >= (b + 1) * cut.share) return false;
@@ -231,7 +250,7 @@ __global__ void __launch_bounds__(PLAN_T) k_paged_plan(PlanArgs a) {
                 const int pitch = (int) z2o::strip_pitch(z2o::strip_cost(units_of(t), cut.head), cut);
                 sh.tile = lo;
                 sh.head = pitch ? min((at - t.begin) / pitch, a.nkv - 1) : 0;
-                if (!k.next(a.tiles, b, sh.tile, sh.head, sh.it)) sh.it.rows = 0;
+                if (!k.next<false>(a.tiles, b, sh.tile, sh.head, sh.it)) sh.it.rows = 0;
                 if (!cut.head || sh.it.rows == 0) sh.tile = -1;          // whole shares have one piece
             }
             if (wide) a.shares[b] = sh;
@@ -274,7 +293,9 @@ struct PagedArgs {
     float * part_o;
 };
 
-__device__ __forceinline__ bool plan_fits(const PagedArgs & a) {
+__device__ __forceinline__ bool plan_fits(const PagedArgs & args) {
+    struct { const __attribute__((address_space(4))) int32_t * head; int n_rows, n_head, n_group, n_seq, nkv; } a{
+        uniform(args.head), args.n_rows, args.n_head, args.n_group, args.n_seq, args.nkv};
     return a.head[PH_MAGIC] == PLAN_MAGIC && a.head[PH_ROWS] == a.n_rows && a.head[PH_HEADS] == a.n_head && a.head[PH_GROUPS] == a.n_group &&
            a.head[PH_SEQS] == a.n_seq && a.head[PH_KV_HEADS] == a.nkv;
 }
@@ -589,13 +610,12 @@ struct PagedAttn {
     __device__ __forceinline__ PagedAttn(const PagedArgs & args, int lane_, int wave_)
         : a(args), mv(lane_), lane(lane_), wave(wave_), group(args.n_head / args.nkv) {}
 
-    // elements from the start of k and v to the 16 rows that begin with `key` (one page holds them; any key gives an address inside
-    // the cache; the wave is of one mind)
+    // elements from the start of k and v to the 16 rows that begin with `key` >= 0 (one page holds them; any key and any page entry
+    // give an address inside the cache)
     __device__ __forceinline__ int64_t rows_at(const PlanItem & it, int key) const {
-        key = __builtin_amdgcn_readfirstlane(key);
-        const int page = max(0, z2o::page_of(a.table, a.n_seq, a.table_len, a.n_pages, a.page_shift, it.seq, key));
-        const int64_t head_row = ((int64_t) it.head << a.page_shift) + (key & ((1 << a.page_shift) - 1));
-        return (int64_t) __builtin_amdgcn_readfirstlane(page) * a.page_stride + head_row * HD;
+        const int at = min(key >> a.page_shift, a.table_len - 1), entry = uniform(a.table)[(int64_t) it.seq * a.table_len + at];
+        const int page = entry >= 0 && entry < a.n_pages ? entry : 0;
+        return page * a.page_stride + (((int64_t) it.head << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * HD;
     }
     // the row-heads first_rh .. first_rh + 31 of the piece: final, or partial
     __device__ __forceinline__ void store(const PlanItem & it, AttnWave<HD, T, TC> & w, int first_rh) const {
@@ -693,7 +713,7 @@ struct PagedAttn {
             stage(s_k1, s_v1, s_k0, s_v0);
         }
         store(it, w, 32 * wave);
-        __syncthreads();                                         // LDS is free
+        __syncthreads();                                         // LDS is free for the next piece
     }
 };
 
@@ -705,23 +725,28 @@ __global__ void __launch_bounds__(256, 2) k_paged_attn(PagedArgs a) {
     const int wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
     if (!plan_fits(a)) return;
     const PagedAttn<HD, T, TC> p(a, threadIdx.x & 63, wave);
-    // (both records are requested before either is used)
-    const PlanShare wide = a.shares[blockIdx.x], narrow = a.shares[a.blocks + 4 * blockIdx.x + wave];
+    PlanShare wide, narrow;
+    uniform_copy(wide, a.shares + blockIdx.x);
+    uniform_copy(narrow, a.shares + a.blocks + 4 * blockIdx.x + wave);
     auto rest = [&](bool kind, PlanShare & s) __attribute__((always_inline)) {
-        const int32_t * h = a.head + PH_KIND + 3 * (int) kind;
-        const PlanKind k{z2o::Cut{h[PK_SHARE], h[PK_HEAD]}, h[PK_TILES], a.head[PH_SHIFT], a.max_tiles, a.nkv, p.group, kind};
-        return s.tile >= 0 && k.next(a.tiles, s.share, s.tile, s.head, s.it);
+        const auto * h = uniform(a.head) + PH_KIND + 3 * (int) kind;
+        const PlanKind k{z2o::Cut{h[PK_SHARE], h[PK_HEAD]}, h[PK_TILES], uniform(a.head)[PH_SHIFT], a.max_tiles, a.nkv, p.group, kind};
+        return s.tile >= 0 && k.template next<true>(a.tiles, s.share, s.tile, s.head, s.it);
     };
-    if (wide.it.rows > 0) {
-        PlanShare s = wide;
-        do p.wide(s.it, s_k0, s_v0, s_k1, s_v1, s_vis); while (rest(true, s));
-    }
-    if (narrow.it.rows > 0) {
-        PlanShare s = narrow;
-        // (a copy for each pair of arrays: loads on their way to one array do not hold up reads of the other)
-        const int at = 32 * (wave & 1) * HD;
-        if (wave & 2) { do p.narrow(s.it, s_k1 + at, s_v1 + at); while (rest(false, s)); }
-        else { do p.narrow(s.it, s_k0 + at, s_v0 + at); while (rest(false, s)); }
+    // Half of the blocks (one of the two that a compute unit holds) begin with their narrow share: products and loads side by side.
+    const int first = 2 * (int) blockIdx.x >= a.blocks;
+#pragma unroll 1
+    for (int phase = 0; phase < 2; ++phase) {
+        if (phase == first) {
+            if (wide.it.rows > 0)
+                do p.wide(wide.it, s_k0, s_v0, s_k1, s_v1, s_vis); while (rest(true, wide));
+        } else if (narrow.it.rows > 0) {
+            // (a copy for each pair of arrays: loads on their way to one array do not hold up reads of the other)
+            const int at = 32 * (wave & 1) * HD;
+            if (wave & 2) { do p.narrow(narrow.it, s_k1 + at, s_v1 + at); while (rest(false, narrow)); }
+            else { do p.narrow(narrow.it, s_k0 + at, s_v0 + at); while (rest(false, narrow)); }
+        }
+        __syncthreads();                                         // every wave is done with its part of LDS
     }
 }
 
