@@ -83,6 +83,13 @@ __device__ __forceinline__ int block_scan(int v, int * s_wave, int & total) {
 // the wave's other loads (a page number read as a vector load waits for all K and V on their way: steps of 2.6 us against 1.6).
 template <typename T>
 __device__ __forceinline__ const __attribute__((address_space(4))) T * uniform(const T * p) { return (const __attribute__((address_space(4))) T *) p; }
+template <typename T>
+__device__ __forceinline__ T uniform_copy(const T * p) {
+    struct { int w[sizeof(T) / 4]; } x;
+#pragma unroll
+    for (int i = 0; i < (int) (sizeof(T) / 4); ++i) x.w[i] = uniform((const int *) p)[i];
+    return __builtin_bit_cast(T, x);
+}
 
 template <typename T>
 __device__ __forceinline__ void uniform_copy(T & to, const T * from) {
@@ -753,13 +760,13 @@ __global__ void __launch_bounds__(256, 2) k_paged_attn(PagedArgs a) {
 // One wave per (row, head): weights of its partial results from their maxima (a lane each, 64 at a time), then the dims over the lanes.
 template <int HD, typename T>
 __global__ void __launch_bounds__(256) k_paged_join(PagedArgs a) {
-    if (!plan_fits(a)) return;
-    const int lane = threadIdx.x & 63, id = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, id = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
     if (id >= a.n_rows * a.n_head) return;
     const int row = id / a.n_head, head = id % a.n_head, group = a.n_head / a.nkv, g = head / group;
-    const PlanRow r = a.rows[row];
-    const PlanStrip pre = r.pre_tile >= 0 ? a.strips[(int64_t) r.pre_tile * a.nkv + g] : PlanStrip{0, 0, 0, 0};
-    const PlanStrip own = r.own_tile >= 0 ? a.strips[(int64_t) r.own_tile * a.nkv + g] : PlanStrip{0, 0, 0, 0};
+    const PlanRow r = uniform_copy(a.rows + row);
+    if (!plan_fits(a)) return;
+    auto strip = [&](int tile) { return tile >= 0 ? uniform_copy(a.strips + (int64_t) tile * a.nkv + g) : PlanStrip{0, 0, 0, 0}; };
+    const PlanStrip pre = strip(r.pre_tile), own = strip(r.own_tile);
     if (own.stored) return;                                      // by its only piece
     const int n_pre = pre.pieces, n_own = own.pieces, pre_step = pre.heads, own_step = own.heads;
     const int pre0 = pre.part0 + r.pre_at + head % group, own0 = own.part0 + r.own_at + head % group;
@@ -767,9 +774,20 @@ __global__ void __launch_bounds__(256) k_paged_join(PagedArgs a) {
     auto part = [&](int i) { return i < n_pre ? pre0 + i * pre_step : own0 + (i - n_pre) * own_step; };
     constexpr int E = HD >= 64 ? HD / 64 : 1;
     const int d = E * lane;
-    float m = -__builtin_inff(), l = 0.0f, o[E] = {};
+    constexpr int MB = 8;                                        // results on their way, the first of them with the maxima
+    float m = -__builtin_inff(), l = 0.0f, o[E] = {}, x[MB][E];
+    auto request = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < MB; ++u) {
+            if (i0 + u >= n) break;
+            const float * p = a.part_o + (int64_t) part(i0 + u) * HD + d;
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[u][e] = d < HD ? p[e] : 0.0f;
+        }
+    };
     for (int i0 = 0; i0 < n; i0 += 64) {
         const float2 ml = i0 + lane < n ? a.part_ml[part(i0 + lane)] : make_float2(-__builtin_inff(), 0.0f);
+        request(i0);
         const float mn = fmaxf(m, wave_max_f(ml.x));
         const float w = ml.x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mn);
         const float w0 = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
@@ -778,19 +796,12 @@ __global__ void __launch_bounds__(256) k_paged_join(PagedArgs a) {
 #pragma unroll
         for (int e = 0; e < E; ++e) o[e] *= w0;
         const int k = min(64, n - i0);
-        constexpr int MB = 4;                                    // loads in flight
         for (int i = 0; i < k; i += MB) {
-            float x[MB][E];
+            if (i) request(i0 + i);
 #pragma unroll
             for (int u = 0; u < MB; ++u) {
-                const float * p = a.part_o + (int64_t) part(i0 + min(i + u, k - 1)) * HD + d;
-#pragma unroll
-                for (int e = 0; e < E; ++e) x[u][e] = d < HD ? p[e] : 0.0f;
-            }
-#pragma unroll
-            for (int u = 0; u < MB; ++u) {
-                const float wi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), min(i + u, 63)));
-                if (i + u < k)
+                if (i + u >= k) break;
+                const float wi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), i + u));
 #pragma unroll
                     for (int e = 0; e < E; ++e) o[e] = __builtin_fmaf(wi, x[u][e], o[e]);
             }
