@@ -245,10 +245,10 @@ int z2h_step_resident(z2h_ctx * ctx, int n_active);
 /* ---------------------------------------------------------------------------------------------------------
  * Operators on device tensors around a paged key / value cache (no reference counterpart: the reference keeps one
  * contiguous band per slot, src/zonos2-graph.cpp:639-690, and its decode step, like z2h_step, reads a prompt that
- * requests share once per request). For callers that keep their own buffers; z2h_step_paged below runs the
- * model's layers over them. They take a context for its device and its error string only: no tensor, no weights and no
- * z2h_finalize are needed, nothing is allocated, nothing synchronizes, and every call may be captured into a HIP graph.
- * All tensors are on the context's device. Work is enqueued on `stream` (a hipStream_t, NULL = the null stream); the
+ * requests share once per request). For callers that keep their own buffers; z2h_step_paged, at the end of the section,
+ * runs the model's layers over them. The operators take a context for its device and its error string only: no tensor,
+ * no weights and no z2h_finalize are needed, nothing is allocated, nothing synchronizes, and every call may be captured
+ * into a HIP graph. All tensors are on the context's device. Work is enqueued on `stream` (a hipStream_t, NULL = the null stream); the
  * caller's current device is the same on return. Strides are in elements.
  *
  * Tables of lengths, positions and pages are read on the device and are not checked on the host: an entry out of range
@@ -349,6 +349,30 @@ int z2h_verify(z2h_ctx * ctx, int n_seq, int n_draft_max, int n_codebooks, int v
                const int32_t * d_n_draft, const float * d_target, const float * d_temperature, const float * d_draft_probs,
                const double * d_u_accept, const double * d_u_draw, int32_t * d_n_accept, int32_t * d_codes, void * d_ws,
                int64_t ws_bytes, void * stream);
+
+/* The pass of z2h_step_mixed over a paged cache in place of the context's bands: the model's layers with z2h_paged_append,
+ * z2h_paged_plan and z2h_paged_attn in them. A prompt that sequences share is stored once and read once per pass, and a
+ * sequence may bring any number of rows: a chunk of its prompt, one frame, or a frame and the drafts behind it, whose logits
+ * z2h_verify then judges.
+ *
+ * `pages` describes layer 0 (Z2H_F16, the model's n_head_kv and head_dim; n_seq and table_len as the caller likes); layer
+ * L's k and v lie L * layer_stride elements behind (a multiple of 8, at least n_pages * page_stride), the page table is the
+ * same for all layers and stays as it is during the call. row_start [n_seq + 1], kv_len [n_seq], group_start
+ * [n_group + 1] and prefix_len [n_group] are on the host and mean what they do in z2h_paged_plan, with row_start[n_seq] = n_rows:
+ * sequence s's m rows become its cache rows kv_len[s] - m .. kv_len[s] - 1, row j of them attends to rows
+ * [0, kv_len[s] - m + j], of this pass or earlier ones. Only a group's first sequence may bring rows of the group's prefix.
+ * No two sequences' rows may lie in the same cache row.
+ *
+ * ids, emb_map, emb, n_emb, n_out and out_rows are those of z2h_step_mixed. The logits of the n_out rows go to d_logits (device,
+ * [n_out][n_codebooks][audio_vocab]; NULL: the context's own buffer) and, if out_logits is not NULL, to the host. d_ws is a
+ * workspace of z2h_step_paged_ws_bytes (0: refused, see z2h_last_error; 256-byte aligned). The call works on the
+ * context's stream and returns when it is done; work of other streams on the cache has to be done before. Not while a
+ * debug capture is on; a profiling window leaves out the paged operators' launches. */
+int64_t z2h_step_paged_ws_bytes(z2h_ctx * ctx, const z2h_pages * pages, int n_rows, int n_group);
+int z2h_step_paged(z2h_ctx * ctx, const z2h_pages * pages, int64_t layer_stride, int n_rows, const int32_t * row_start,
+                   const int32_t * kv_len, int n_group, const int32_t * group_start, const int32_t * prefix_len,
+                   const int32_t * ids, const int32_t * emb_map, const float * emb, int n_emb, int n_out,
+                   const int32_t * out_rows, float * out_logits, float * d_logits, void * d_ws, int64_t ws_bytes);
 
 /* Debug capture of per-layer intermediates of the following steps (off by default). */
 enum {

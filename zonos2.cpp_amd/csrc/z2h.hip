@@ -154,6 +154,7 @@ struct z2h_ctx {
     int4 * d_tiles = nullptr;         // [items_max] attention tile entries of a kv_pre pass (k_attn_tile)
     int4 * h_tiles = nullptr;         // pinned staging for them
     int32_t * h_pin = nullptr;        // pinned staging for step inputs (d_slot's block), then the error flag
+    std::vector<int32_t> paged_tables;   // z2h_step_paged: the tables on their way to its workspace
     std::vector<uint64_t> row_seen;   // z2h_step_mixed: one bit per cache row, all clear between calls
 
     // frame sampler: per-column settings, histories, draws and codes (device + pinned staging)
@@ -1117,12 +1118,13 @@ int dense_block(z2h_ctx * ctx, Layer & ly, int T) {
 // f32_prompt (per-slot prefill): the rows also keep their fp32 K/V in ctx->pf_kv and attend over those
 // (the reference's in-prompt attention, src/zonos2-graph.cpp:155-169) instead of the f16 cache rows.
 // head_rows: which rows get logits (rows [0, n_head) of d_logits): every row, none, the last row, or
-// the n_head rows listed in d_head_rows.
+// the n_head rows listed in d_head_rows. paged: the K/V rows go to its pages and the rows attend over them (z2h_step_paged).
 enum { HEAD_ALL = 0, HEAD_NONE = 1, HEAD_LAST = 2, HEAD_ROWS = 3 };
 int run_step(z2h_ctx * ctx, int T, const int32_t * h_npast, const int32_t * d_slot, const int32_t * d_npast,
              const int32_t * d_ids, const float * d_emb, float * d_logits, bool kv_pre = false,
              const int32_t * d_emb_map = nullptr, const int32_t * h_slot = nullptr, bool f32_prompt = false,
-             int head_rows = HEAD_ALL, const int32_t * d_head_rows = nullptr, int n_head = 0) {
+             int head_rows = HEAD_ALL, const int32_t * d_head_rows = nullptr, int n_head = 0,
+             const Z2hPagedPass * paged = nullptr) {
     const auto & hp = ctx->hp;
     const int d = hp.n_embd, nh = hp.n_head, nkv = hp.n_head_kv, hd = hp.head_dim;
     int rc;
@@ -1255,7 +1257,10 @@ int run_step(z2h_ctx * ctx, int T, const int32_t * h_npast, const int32_t * d_sl
         a.act = ctx->act;
         const int wo_act = act_of(ly.wo.type);
         bool in_block;
-        if (flash32) {
+        if (paged) {
+            in_block = false;
+            if ((rc = z2h_paged_layer(ctx, *paged, L, ctx->qkvg, ly.attn_temp, ctx->attn_o, ctx->stream))) return rc;
+        } else if (flash32) {
             in_block = (grp * hd) % 256 == 0;
             a.act_fmt = in_block ? wo_act : ACT_NONE;
             a.tiles = (const int4 *) ctx->d_tiles;
@@ -2094,6 +2099,126 @@ int z2h_step_mixed(z2h_ctx * ctx, int n_rows, const int32_t * slot_idx, const in
                           ctx->logits, /*kv_pre=*/true, emb_map ? d.emb_map : nullptr, h.slot, false,
                           HEAD_ROWS, d.head_rows, n_out)) return rc;
     return finish_pass(ctx, out_logits, (size_t) n_out * ctx->hp.n_codebooks * ctx->hp.audio_vocab);
+}
+
+// the tables that a paged pass keeps in front of the attention's workspace
+static int64_t paged_tables_bytes(const z2h_pages & p, int n_group) {
+    return ((int64_t) (2 * (int64_t) p.n_seq + 1 + 2 * (int64_t) n_group + 1) * 4 + 255) / 256 * 256;
+}
+static const char * check_paged(const z2h_ctx * ctx, const z2h_pages * p) {
+    if (!p) return "null pages";
+    if (p->type != Z2H_F16) return "the model's pages are f16";
+    if (p->n_head_kv != ctx->hp.n_head_kv || p->head_dim != ctx->hp.head_dim) return "pages of another head layout than the model's";
+    return nullptr;
+}
+
+int64_t z2h_step_paged_ws_bytes(z2h_ctx * ctx, const z2h_pages * pages, int n_rows, int n_group) {
+    if (!ctx) return 0;
+    if (const char * e = check_paged(ctx, pages)) { seterr(ctx, Z2H_EINVAL, e); return 0; }
+    const int64_t n = z2h_paged_ws_bytes(ctx, pages, ctx->hp.n_head, n_rows, n_group);
+    return n ? n + paged_tables_bytes(*pages, n_group) : 0;
+}
+
+static int paged_pass(z2h_ctx * ctx, const z2h_pages * pages, int64_t layer_stride, int n_rows, const int32_t * row_start, const int32_t * kv_len,
+                      int n_group, const int32_t * group_start, const int32_t * prefix_len, const int32_t * ids, const int32_t * emb_map,
+                      const float * emb, int n_emb, int n_out, const int32_t * out_rows, float * out_logits, float * d_logits, void * d_ws,
+                      int64_t ws_bytes) {
+    const auto & hp = ctx->hp;
+    const int W = ctx->W;
+    if (!row_start || !kv_len || !ids || (n_group > 0 && (!group_start || !prefix_len)) || (n_out > 0 && !out_rows))
+        return seterr(ctx, Z2H_EINVAL, "null argument");
+    if (!ctx->finalized) return seterr(ctx, Z2H_ESTATE, "z2h_finalize not called");
+    if (ctx->capture) return seterr(ctx, Z2H_ESTATE, "a paged pass while a capture is on");
+    if (const char * e = check_paged(ctx, pages)) return seterr(ctx, Z2H_EINVAL, e);
+    if (n_rows <= 0 || n_rows > ctx->Tmax) return seterr(ctx, Z2H_EINVAL, "n_rows out of range");
+    if (n_out < 0 || n_out > ctx->Tmax) return seterr(ctx, Z2H_EINVAL, "n_out out of range");
+    const int64_t ws_need = z2h_paged_ws_bytes(ctx, pages, hp.n_head, n_rows, n_group);        // (checks the pages)
+    if (!ws_need) return Z2H_EINVAL;
+    const int64_t tables = paged_tables_bytes(*pages, n_group);
+    if (!d_ws || (uintptr_t) d_ws % 256 || ws_bytes < ws_need + tables) return seterr(ctx, Z2H_EINVAL, "workspace misaligned or too small");
+    if (layer_stride % 8 || layer_stride < pages->n_pages * pages->page_stride || layer_stride > ((int64_t) 1 << 40))
+        return seterr(ctx, Z2H_EINVAL, "layer_stride out of range");
+    if (emb_map && (!emb || n_emb <= 0 || n_emb > ctx->Tmax)) return seterr(ctx, Z2H_EINVAL, "embedding rows out of range");
+    // ---- sequences and groups
+    const int S = pages->n_seq, cap = pages->table_len * pages->page_rows;
+    if (row_start[0] != 0 || row_start[S] != n_rows) return seterr(ctx, Z2H_EINVAL, "row_start does not span the rows");
+    for (int s = 0; s < S; ++s) {
+        const int m = row_start[s + 1] - row_start[s];
+        if (m < 0) return seterr(ctx, Z2H_EINVAL, "row_start is not ascending");
+        if (m && (kv_len[s] < m || kv_len[s] > cap)) return seterr(ctx, Z2H_EINVAL, "kv_len out of range");
+    }
+    for (int g = 0; g < n_group; ++g) {
+        if (group_start[g] < 0 || group_start[g] > group_start[g + 1] || group_start[g + 1] > S || prefix_len[g] < 0)
+            return seterr(ctx, Z2H_EINVAL, "groups are not ascending spans of the sequences");
+        for (int s = group_start[g] + 1; s < group_start[g + 1]; ++s) {
+            const int m = row_start[s + 1] - row_start[s];
+            if (m && kv_len[s] - m < prefix_len[g]) return seterr(ctx, Z2H_EINVAL, "a row of a group's prefix is not of its first sequence");
+        }
+    }
+    // ---- rows
+    for (int t = 0; t < n_rows; ++t) {
+        const int em = emb_map ? emb_map[t] : -1;
+        if (em < -1 || em >= n_emb) return seterr(ctx, Z2H_EINVAL, "emb_map entry out of range");
+        if (em < 0)
+            for (int k = 0; k < W; ++k) {
+                const int id = ids[(size_t) t * W + k];
+                if (id < 0 || id >= ctx->m->tab_rows[k]) return seterr(ctx, Z2H_EINVAL, "token id out of range");
+            }
+    }
+    for (int i = 0; i < n_out; ++i)
+        if (out_rows[i] < 0 || out_rows[i] >= n_rows) return seterr(ctx, Z2H_EINVAL, "out_rows entry out of range");
+    HIPX(hipSetDevice(ctx->device));
+    ctx->resident_T = ctx->resident_last = 0;
+    const PassInputs h = pass_inputs(ctx->h_pin, n_rows, W), d = pass_inputs(ctx->d_slot, n_rows, W);
+    for (int s = 0; s < S; ++s)
+        for (int t = row_start[s]; t < row_start[s + 1]; ++t) { h.slot[t] = s; h.n_past[t] = kv_len[s] - (row_start[s + 1] - t); }
+    std::memcpy(h.ids, ids, (size_t) n_rows * W * 4);
+    for (int t = 0; t < n_rows; ++t) {
+        h.emb_map[t] = emb_map ? emb_map[t] : -1;
+        if (h.emb_map[t] >= 0) for (int k = 0; k < W; ++k) h.ids[(size_t) t * W + k] = 0;     // unused ids
+    }
+    if (n_out > 0) std::memcpy(h.head_rows, out_rows, (size_t) n_out * 4);
+    if (int rc = upload_inputs(ctx, (size_t) n_rows * (3 + W) + n_out)) return rc;
+    if (emb_map) HIPX(hipMemcpyAsync(ctx->d_emb, emb, (size_t) n_emb * hp.n_embd * 4, hipMemcpyHostToDevice, ctx->stream));
+    int32_t * d_rows = (int32_t *) d_ws, * d_len = d_rows + S + 1, * d_groups = d_len + S, * d_prefix = d_groups + n_group + 1;
+    auto & tab = ctx->paged_tables;                                  // (kept: the copy may read it until the pass is done)
+    tab.assign(row_start, row_start + S + 1);
+    tab.insert(tab.end(), kv_len, kv_len + S);
+    if (n_group > 0) {
+        tab.insert(tab.end(), group_start, group_start + n_group + 1);
+        tab.insert(tab.end(), prefix_len, prefix_len + n_group);
+    }
+    HIPX(hipMemcpyAsync(d_ws, tab.data(), tab.size() * 4, hipMemcpyHostToDevice, ctx->stream));
+    Z2hPagedPass pass{};
+    pass.pages = *pages; pass.layer_stride = layer_stride;
+    pass.rope = z2h_rope{hp.rope_freq_base, hp.head_dim, 0, 1.0f, 0.0f, 0.0f, 0, 1.0f};
+    pass.n_rows = n_rows; pass.n_head = hp.n_head; pass.n_group = n_group;
+    pass.R = (hp.n_head + 2 * hp.n_head_kv) * hp.head_dim + hp.n_head;
+    pass.qk_eps = hp.qk_norm_eps; pass.scale = 1.0f / std::sqrt((float) hp.head_dim);
+    pass.d_seq = d.slot; pass.d_pos = d.n_past;
+    pass.d_ws = (uint8_t *) d_ws + tables; pass.ws_bytes = ws_need;
+    float * logits = d_logits ? d_logits : ctx->logits;
+    int rc = z2h_paged_plan(ctx, pages, hp.n_head, n_rows, d_rows, d_len, n_group, d_groups, d_prefix, pass.d_ws, ws_need, ctx->stream);
+    if (!rc) rc = run_step(ctx, n_rows, nullptr, d.slot, d.n_past, d.ids, emb_map ? ctx->d_emb : nullptr, logits, false,
+                           emb_map ? d.emb_map : nullptr, nullptr, false, HEAD_ROWS, d.head_rows, n_out, &pass);
+    if (rc) { (void) hipStreamSynchronize(ctx->stream); return rc; }
+    const size_t n = (size_t) n_out * hp.n_codebooks * hp.audio_vocab;
+    if (d_logits && out_logits && n) HIPX(hipMemcpyAsync(out_logits, d_logits, n * 4, hipMemcpyDeviceToHost, ctx->stream));
+    return finish_pass(ctx, d_logits ? nullptr : out_logits, n);
+}
+
+int z2h_step_paged(z2h_ctx * ctx, const z2h_pages * pages, int64_t layer_stride, int n_rows, const int32_t * row_start, const int32_t * kv_len,
+                   int n_group, const int32_t * group_start, const int32_t * prefix_len, const int32_t * ids, const int32_t * emb_map,
+                   const float * emb, int n_emb, int n_out, const int32_t * out_rows, float * out_logits, float * d_logits, void * d_ws,
+                   int64_t ws_bytes) {
+    if (!ctx) return Z2H_EINVAL;
+    try {
+        return paged_pass(ctx, pages, layer_stride, n_rows, row_start, kv_len, n_group, group_start, prefix_len, ids, emb_map, emb, n_emb, n_out,
+                          out_rows, out_logits, d_logits, d_ws, ws_bytes);
+    } catch (...) {
+        (void) hipStreamSynchronize(ctx->stream);
+        return z2h_ctx_fail(ctx, Z2H_ENOMEM, "out of host memory");
+    }
 }
 
 int z2h_set_prefill_chunk(z2h_ctx * ctx, int rows) {

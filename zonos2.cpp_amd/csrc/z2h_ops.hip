@@ -6,6 +6,7 @@
 #include "z2h_rope.h"
 #include "z2h_paged.h"
 #include "z2h_verify.h"
+#include "z2h_paged_step.h"
 
 #include <algorithm>
 #include <atomic>
@@ -260,3 +261,25 @@ int z2h_verify(z2h_ctx * ctx, int n_seq, int n_draft_max, int n_codebooks, int v
 }
 
 } // extern "C"
+
+int z2h_paged_layer(z2h_ctx * ctx, const Z2hPagedPass & s, int layer, float * qkvg, const float * temp, float * out, void * stream) {
+    z2h_pages pages = s.pages;
+    const int64_t at = 2 * layer * s.layer_stride;
+    pages.k = (uint8_t *) pages.k + at;
+    pages.v = (uint8_t *) pages.v + at;
+    const int nh = s.n_head, nkv = pages.n_head_kv, hd = pages.head_dim;
+    const HeadRows h{qkvg, s.R, s.n_rows, nh, nkv, hd, temp, s.qk_eps, out};
+    float * k = qkvg + nh * hd, * v = k + nkv * hd;
+    {
+        ON_DEVICE;
+        hipLaunchKernelGGL(k_head_norm, dim3((s.n_rows * (nh + nkv) + 3) / 4), dim3(256), 0, (hipStream_t) stream, h);
+        if (int rc = launched(ctx)) return rc;
+    }
+    if (int rc = z2h_paged_append(ctx, &pages, &s.rope, s.n_rows, s.d_seq, s.d_pos, Z2H_F32, k, s.R, v, s.R, nh, qkvg, s.R, qkvg, s.R, stream))
+        return rc;
+    if (int rc = z2h_paged_attn(ctx, &pages, nh, s.n_rows, s.n_group, s.scale, Z2H_F32, qkvg, s.R, out, (int64_t) nh * hd, s.d_ws, s.ws_bytes, stream))
+        return rc;
+    ON_DEVICE;
+    hipLaunchKernelGGL(k_head_gate, dim3(s.n_rows, (nh * hd + 1023) / 1024), dim3(256), 0, (hipStream_t) stream, h);
+    return launched(ctx);
+}

@@ -77,6 +77,8 @@ def lib() -> C.CDLL:
         "z2h_paged_attn": (i32, [vp, vp, i32, i32, i32, C.c_float, i32, vp, i64, vp, i64, vp, i64, vp]),
         "z2h_verify_ws_bytes": (i64, [i32, i32, i32, i32]),
         "z2h_verify": (i32, [vp, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, vp]),
+        "z2h_step_paged_ws_bytes": (i64, [vp, vp, i32, i32]),
+        "z2h_step_paged": (i32, [vp, vp, i64, i32, vp, vp, i32, vp, vp, vp, vp, vp, i32, i32, vp, vp, vp, vp, i64]),
         "z2h_last_error": (C.c_char_p, [vp]),
         "z2h_destroy": (None, [vp]),
     }
@@ -95,7 +97,7 @@ EXPORTS = ("z2h_model_create", "z2h_model_upload_tensor", "z2h_model_finalize", 
            "z2h_read_capture", "z2h_device_bytes", "z2h_set_graphs", "z2h_profile_begin", "z2h_profile_end", "z2h_sample", "z2h_set_prefill_chunk",
            "z2h_sample_feed", "z2h_step_resident", "z2h_create_batch_rows", "z2h_step_mixed",
            "z2h_rope_rows", "z2h_paged_append", "z2h_paged_ws_bytes", "z2h_paged_plan", "z2h_paged_attn", "z2h_verify_ws_bytes",
-           "z2h_verify", "z2h_last_error", "z2h_destroy")
+           "z2h_verify", "z2h_step_paged_ws_bytes", "z2h_step_paged", "z2h_last_error", "z2h_destroy")
 KERNEL_FAMILIES = ("resnorm", "gemv_qkv", "qkv_post", "attn", "attn_combine", "gemv_wo", "router_down", "router_tail",
                    "gemv_gateup", "gemv_down", "gemv_dense", "gemv_head", "swiglu")
 
@@ -393,6 +395,31 @@ class Context:
                d_u_accept, d_u_draw, d_n_accept, d_codes, d_ws, ws_bytes, stream=None):
         self.check(lib().z2h_verify(self.ctx, n_seq, n_draft_max, n_codebooks, vocab, d_draft, d_n_draft, d_target, d_temperature,
                                     d_draft_probs, d_u_accept, d_u_draw, d_n_accept, d_codes, d_ws, ws_bytes, stream))
+
+    def step_paged_ws_bytes(self, pages, n_rows, n_group) -> int:
+        n = int(lib().z2h_step_paged_ws_bytes(self.ctx, C.byref(pages), n_rows, n_group))
+        if n <= 0:
+            raise Z2HError(EINVAL, lib().z2h_last_error(self.ctx).decode())
+        return n
+
+    def step_paged(self, pages, layer_stride, row_start, kv_len, ids, out_rows, d_ws, ws_bytes, group_start=None, prefix_len=None,
+                   emb_map=None, emb=None, d_logits=0):
+        """z2h_step_paged: rows of any sequences over a paged cache; returns the logits of out_rows (they stay at the device
+        address d_logits if one is given, and None is returned)."""
+        rs, kl = np.ascontiguousarray(row_start, np.int32), np.ascontiguousarray(kv_len, np.int32)
+        assert len(rs) == pages.n_seq + 1 and len(kl) == pages.n_seq
+        gs = None if group_start is None else np.ascontiguousarray(group_start, np.int32)
+        pl = None if prefix_len is None else np.ascontiguousarray(prefix_len, np.int32)
+        ng = 0 if pl is None else len(pl)
+        assert ng == 0 or len(gs) == ng + 1
+        ids, orow = np.ascontiguousarray(ids, np.int32), np.ascontiguousarray(out_rows, np.int32)
+        em = None if emb_map is None else np.ascontiguousarray(emb_map, np.int32)
+        e = None if emb is None else np.ascontiguousarray(emb, np.float32)
+        out = None if d_logits else np.empty((len(orow), self.hp["n_codebooks"] * self.hp["audio_vocab"]), np.float32)
+        self.check(lib().z2h_step_paged(self.ctx, C.byref(pages), layer_stride, len(ids), _p(rs), _p(kl), ng, _p(gs), _p(pl), _p(ids),
+                                        _p(em), _p(e), 0 if e is None else e.shape[0], len(orow), _p(orow), _p(out), d_logits,
+                                        d_ws, ws_bytes))
+        return out
 
     def device_bytes(self, what: int) -> int:
         return int(lib().z2h_device_bytes(self.ctx, what))
