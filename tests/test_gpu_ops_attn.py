@@ -89,6 +89,19 @@ def test_long_prefix(ctx):
     _check(ctx, "f16", lens, [1, 1, 1, 2], 8, 2, 128, 64, [(0, 4, 20000)])
 
 
+@pytest.mark.parametrize("typ", ["f32", "bf16"])
+def test_repeated_calls_agree_bit_for_bit(ctx, typ):
+    """Long shared prefix, several wide tiles, two of them partly filled: keys and values pass through LDS in many steps, which
+    waves that have nothing to multiply help to fill. No answer depends on who came first."""
+    c, row_start, q, a, first = _check(ctx, typ, [4100 + 3 * s for s in range(18)], [1] * 18, 32, 2, 128, 64, groups=[(0, 18, 4096)])
+    d = q.to(DEV)
+    outs = [torch.empty_like(first) for _ in range(40)]
+    for o in outs:
+        a.run(d.view(len(d), -1), o.view(len(d), -1), 128 ** -0.5)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, first) for o in outs)
+
+
 def test_peaked_and_large_queries(ctx):
     """Scores far apart (softmax near one-hot), and queries that f16 could not hold as fp32 rows."""
     _check(ctx, "f32", [300, 40], [1, 3], 8, 2, 64, 16, qscale=30.0)

@@ -85,20 +85,11 @@ template <typename T>
 __device__ __forceinline__ const __attribute__((address_space(4))) T * uniform(const T * p) { return (const __attribute__((address_space(4))) T *) p; }
 template <typename T>
 __device__ __forceinline__ T uniform_copy(const T * p) {
+    static_assert(sizeof(T) % 4 == 0, "");
     struct { int w[sizeof(T) / 4]; } x;
 #pragma unroll
     for (int i = 0; i < (int) (sizeof(T) / 4); ++i) x.w[i] = uniform((const int *) p)[i];
     return __builtin_bit_cast(T, x);
-}
-
-template <typename T>
-__device__ __forceinline__ void uniform_copy(T & to, const T * from) {
-    static_assert(sizeof(T) % 4 == 0, "");
-    int32_t x[sizeof(T) / 4];
-    const __attribute__((address_space(4))) int32_t * p = (const __attribute__((address_space(4))) int32_t *) from;
-#pragma unroll
-    for (int i = 0; i < (int) (sizeof(T) / 4); ++i) x[i] = p[i];
-    __builtin_memcpy(&to, x, sizeof(T));
 }
 
 struct PlanKind {
@@ -111,7 +102,7 @@ struct PlanKind {
     __device__ __forceinline__ bool next(const PlanTile * all, int b, int & tile, int & head, PlanItem & it) const {
         while (tile < tiles) {
             PlanTile t;
-            if constexpr (KERNEL) uniform_copy(t, all + tile_place(tile, wide, max_tiles));
+            if constexpr (KERNEL) t = uniform_copy(all + tile_place(tile, wide, max_tiles));
             else t = all[tile_place(tile, wide, max_tiles)];
             const int units = (int) z2o::strip_units(t.key0, t.key1, wide, shift), cost = (int) z2o::strip_cost(units, cut.head);
             const int begin = t.begin + head * (int) z2o::strip_pitch(cost, cut);
@@ -427,6 +418,8 @@ struct AttnWave {
     // keys_done() is called when K has been read, values_ready() before V is.
     template <int NT, typename F, typename G>
     __device__ __forceinline__ void step(const TC * sk, const TC * sv, int key0, int from, int to, int lane, F keys_done, G values_ready) {
+        // fp32 queries at head size 128 fill the registers: the fragments' places anew in each step (kept, 15 registers are spilled)
+        if constexpr (SPLIT) asm("" : "+v"(lane));
         const int end = min(to, vis), r0 = 0;
         v16f_t s[NT];
         scores<NT>(s, sk, r0, lane);
@@ -700,6 +693,7 @@ struct PagedAttn {
         const int whole = min(it.key1, __builtin_amdgcn_readfirstlane(least));         // steps up to here hide nothing behind them
         // one stage: its keys have arrived for every wave, and nobody reads the other buffer any more
         auto stage = [&](const TC * sk, TC * sv, TC * ok, TC * ov) __attribute__((always_inline)) {
+            wait_loads_but<0>();                                 // (the barrier itself does not wait for loads to LDS)
             __syncthreads();
             if (key + 64 < it.key1) {
                 mv.rows16(a, next, ok + mine * HD, ov + mine * HD);
@@ -732,9 +726,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_attn(PagedArgs a) {
     const int wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
     if (!plan_fits(a)) return;
     const PagedAttn<HD, T, TC> p(a, threadIdx.x & 63, wave);
-    PlanShare wide, narrow;
-    uniform_copy(wide, a.shares + blockIdx.x);
-    uniform_copy(narrow, a.shares + a.blocks + 4 * blockIdx.x + wave);
+    PlanShare wide = uniform_copy(a.shares + blockIdx.x), narrow = uniform_copy(a.shares + a.blocks + 4 * blockIdx.x + wave);
     auto rest = [&](bool kind, PlanShare & s) __attribute__((always_inline)) {
         const auto * h = uniform(a.head) + PH_KIND + 3 * (int) kind;
         const PlanKind k{z2o::Cut{h[PK_SHARE], h[PK_HEAD]}, h[PK_TILES], uniform(a.head)[PH_SHIFT], a.max_tiles, a.nkv, p.group, kind};
