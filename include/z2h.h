@@ -25,6 +25,9 @@
  *   z2h_moe_forward       build_moe                    src/zonos2-graph.cpp:191-239 (one MoE layer)
  *   z2h_set_expert_mask   zonos2_set_expert_mask       src/zonos2.cpp:203-239, src/zonos2.h:136
  *   z2h_destroy           zonos2_batch_free            src/zonos2-graph.cpp:692-701 (+ drops the model reference)
+ * Without a reference counterpart: the mixed pass, the operators on device tensors around a paged cache (z2h_rope_rows,
+ * z2h_paged_append, z2h_paged_plan, z2h_paged_attn, z2h_verify) with the paged pass over them (z2h_step_paged), capture,
+ * graph and profiling switches.
  */
 #ifndef Z2H_H
 #define Z2H_H
@@ -308,18 +311,20 @@ int z2h_paged_append(z2h_ctx * ctx, const z2h_pages * pages, const z2h_rope * ro
  * may then be called any number of times (every layer of a step) with the same shapes and workspace. Sequence s has
  * query rows [d_row_start[s], d_row_start[s + 1]) of the batch (d_row_start [n_seq + 1] ascending from 0 to n_rows; no
  * rows: the sequence sits this call out) and d_kv_len[s] cache rows, its query rows' own among them: row j of m sees
- * rows [0, d_kv_len[s] - m + j]. A row that sees nothing gives zeros. Group g is sequences
- * [d_group_start[g], d_group_start[g + 1]) (d_group_start [n_group + 1] ascending), whose first d_prefix_len[g] cache rows
- * hold the same values: they are read through the group's first sequence, and only as many as it has. Sequences outside every
- * group share nothing; n_group may be 0. A page entry outside [0, n_pages) reads as page 0; lengths are clamped to the table.
+ * rows [0, d_kv_len[s] - m + j]. A row that sees nothing gives zeros. Group g is sequences [d_group_start[g],
+ * d_group_start[g + 1]) (d_group_start [n_group + 1] ascending), whose first d_prefix_len[g] cache rows hold the same
+ * values: they are read through the group's first sequence, and only as many as it has. Sequences outside every group
+ * share nothing; n_group may be 0. A page entry outside [0, n_pages) reads as page 0; lengths are clamped to the
+ * table.
  *
- * z2h_paged_attn: d_out = softmax(scale q k^T) v for d_q [n_rows][n_head][head_dim], rows q_stride / out_stride apart, n_head a
- * multiple of n_head_kv, at most 64 query heads per key head; query head h reads key head h / (n_head / n_head_kv). `type` is Z2H_F32 or
- * Z2H_F16 over Z2H_F16 pages, or Z2H_BF16 over Z2H_BF16 pages. d_out may be d_q (with the same stride). Softmax and sums in fp32;
- * results do not depend on timing (no atomics).
+ * z2h_paged_attn: d_out = softmax(scale q k^T) v for d_q [n_rows][n_head][head_dim], rows q_stride / out_stride apart,
+ * n_head a multiple of n_head_kv, at most 64 query heads per key head; query head h reads key head h / (n_head /
+ * n_head_kv). `type` is Z2H_F32 or Z2H_F16 over Z2H_F16 pages, or Z2H_BF16 over Z2H_BF16 pages. d_out may be d_q (with
+ * the same stride). Softmax and sums in fp32; results do not depend on timing (no atomics).
  *
- * The workspace (z2h_paged_ws_bytes; 0 = the shapes are refused, see z2h_last_error; 256-byte aligned) holds the plan and the partial results of one call at a time: calls and graphs
- * that may overlap need one each. z2h_paged_attn with another shape than the plan's leaves d_out as it was. */
+ * The workspace (z2h_paged_ws_bytes; 0 = the shapes are refused, see z2h_last_error; 256-byte aligned) holds the plan
+ * and the partial results of one call at a time: calls and graphs that may overlap need one each. z2h_paged_attn with
+ * another shape than the plan's leaves d_out as it was. */
 int64_t z2h_paged_ws_bytes(z2h_ctx * ctx, const z2h_pages * pages, int n_head, int n_rows, int n_group);
 int z2h_paged_plan(z2h_ctx * ctx, const z2h_pages * pages, int n_head, int n_rows, const int32_t * d_row_start,
                    const int32_t * d_kv_len, int n_group, const int32_t * d_group_start, const int32_t * d_prefix_len,
@@ -329,45 +334,46 @@ int z2h_paged_attn(z2h_ctx * ctx, const z2h_pages * pages, int n_head, int n_row
                    void * stream);
 
 /* Verification of drafted frames against the target's probabilities, with the random numbers given (the device
- * counterpart of z2h_sample for speculative decoding). Sequence s has d_n_draft[s] drafted frames (clamped to 0 .. n_draft_max; NULL:
- * n_draft_max each) of n_codebooks codes, d_draft [n_seq][n_draft_max][n_codebooks]. d_target [n_seq][n_draft_max + 1]
- * [n_codebooks][vocab] is what the target model says at each drafted frame and behind the last: probabilities, or with
- * d_temperature [n_seq] logits, p = softmax(logits / temperature) (0 or less: all mass on the first largest logit).
- * d_draft_probs [n_seq][n_draft_max][n_codebooks][vocab] are the probabilities q that the drafts were drawn from; NULL: the
- * drafts were not drawn (q = 1 at the drafted code). The codes are judged in order, frame by frame and codebook by codebook:
- * code x is kept iff u q(x) < p(x), u = d_u_accept [n_seq][n_draft_max][n_codebooks]. Behind the first code that is not
- * kept, in frame k codebook c, the sequence ends: d_n_accept[s] = k whole frames are kept, and d_codes[s] ([n_seq][n_codebooks])
- * is the frame that follows them: the kept codes of frame k before c, at c a draw from max(p - q, 0) (from p where that
- * has no mass), behind c draws from p of frame k. With every code kept it is a draw from p of the frame behind the last draft.
- * A draw takes the first code whose cumulative mass exceeds u (total mass), u = d_u_draw [n_seq][n_codebooks], and if rounding leaves none, the last with
- * mass. So the frames are distributed as the target's own, codebook by codebook. Probabilities, sums and comparisons in 64 bits.
- * Random numbers are doubles in [0, 1). A drafted code outside [0, vocab) is not kept. Probabilities that are no
- * numbers or have no mass give some code in range. vocab is at most 2^20. The workspace (z2h_verify_ws_bytes; 0: the sizes are refused; 256-byte aligned)
- * holds one call at a time. */
+ * counterpart of z2h_sample for speculative decoding). Sequence s has d_n_draft[s] drafted frames (clamped to 0 ..
+ * n_draft_max; NULL: n_draft_max each) of n_codebooks codes, d_draft [n_seq][n_draft_max][n_codebooks]. d_target
+ * [n_seq][n_draft_max + 1] [n_codebooks][vocab] is what the target model says at each drafted frame and behind the
+ * last: probabilities, or with d_temperature [n_seq] logits, p = softmax(logits / temperature) (0 or less: all mass on
+ * the first largest logit). d_draft_probs [n_seq][n_draft_max][n_codebooks][vocab] are the probabilities q that the
+ * drafts were drawn from; NULL: the drafts were not drawn (q = 1 at the drafted code). The codes are judged in order,
+ * frame by frame and codebook by codebook: code x is kept iff u q(x) < p(x), u = d_u_accept
+ * [n_seq][n_draft_max][n_codebooks]. Behind the first code that is not kept, in frame k codebook c, the sequence ends:
+ * d_n_accept[s] = k whole frames are kept, and d_codes[s] ([n_seq][n_codebooks]) is the frame that follows them: the
+ * kept codes of frame k before c, at c a draw from max(p - q, 0) (from p where that has no mass), behind c draws from
+ * p of frame k. With every code kept it is a draw from p of the frame behind the last draft. A draw takes the first
+ * code whose cumulative mass exceeds u (total mass), u = d_u_draw [n_seq][n_codebooks], and if rounding leaves none,
+ * the last with mass. So the frames are distributed as the target's own, codebook by codebook. Probabilities, sums and
+ * comparisons in 64 bits. Random numbers are doubles in [0, 1). A drafted code outside [0, vocab) is not kept.
+ * Probabilities that are no numbers or have no mass give some code in range. vocab is at most 2^20. The workspace
+ * (z2h_verify_ws_bytes; 0: the sizes are refused; 256-byte aligned) holds one call at a time. */
 int64_t z2h_verify_ws_bytes(int n_seq, int n_draft_max, int n_codebooks, int vocab);
 int z2h_verify(z2h_ctx * ctx, int n_seq, int n_draft_max, int n_codebooks, int vocab, const int32_t * d_draft,
                const int32_t * d_n_draft, const float * d_target, const float * d_temperature, const float * d_draft_probs,
                const double * d_u_accept, const double * d_u_draw, int32_t * d_n_accept, int32_t * d_codes, void * d_ws,
                int64_t ws_bytes, void * stream);
 
-/* The pass of z2h_step_mixed over a paged cache in place of the context's bands: the model's layers with z2h_paged_append,
- * z2h_paged_plan and z2h_paged_attn in them. A prompt that sequences share is stored once and read once per pass, and a
- * sequence may bring any number of rows: a chunk of its prompt, one frame, or a frame and the drafts behind it, whose logits
- * z2h_verify then judges.
+/* The pass of z2h_step_mixed over a paged cache in place of the context's bands: the model's layers with
+ * z2h_paged_append, z2h_paged_plan and z2h_paged_attn in them. A prompt that sequences share is stored once and read
+ * once per pass, and a sequence may bring any number of rows: a chunk of its prompt, one frame, or a frame and the
+ * drafts behind it, whose logits z2h_verify then judges.
  *
- * `pages` describes layer 0 (Z2H_F16, the model's n_head_kv and head_dim; n_seq and table_len as the caller likes); layer
- * L's k and v lie L * layer_stride elements behind (a multiple of 8, at least n_pages * page_stride), the page table is the
- * same for all layers and stays as it is during the call. row_start [n_seq + 1], kv_len [n_seq], group_start
- * [n_group + 1] and prefix_len [n_group] are on the host and mean what they do in z2h_paged_plan, with row_start[n_seq] = n_rows:
- * sequence s's m rows become its cache rows kv_len[s] - m .. kv_len[s] - 1, row j of them attends to rows
- * [0, kv_len[s] - m + j], of this pass or earlier ones. Only a group's first sequence may bring rows of the group's prefix.
- * No two sequences' rows may lie in the same cache row.
+ * `pages` describes layer 0 (Z2H_F16, the model's n_head_kv and head_dim; n_seq and table_len as the caller likes);
+ * layer L's k and v lie L * layer_stride elements behind (a multiple of 8, at least n_pages * page_stride), the page
+ * table is the same for all layers and stays as it is during the call. row_start [n_seq + 1], kv_len [n_seq],
+ * group_start [n_group + 1] and prefix_len [n_group] are on the host and mean what they do in z2h_paged_plan, with
+ * row_start[n_seq] = n_rows: sequence s's m rows become its cache rows kv_len[s] - m .. kv_len[s] - 1, row j of them
+ * attends to rows [0, kv_len[s] - m + j], of this pass or earlier ones. Only a group's first sequence may bring rows
+ * of the group's prefix. No two sequences' rows may lie in the same cache row.
  *
- * ids, emb_map, emb, n_emb, n_out and out_rows are those of z2h_step_mixed. The logits of the n_out rows go to d_logits (device,
- * [n_out][n_codebooks][audio_vocab]; NULL: the context's own buffer) and, if out_logits is not NULL, to the host. d_ws is a
- * workspace of z2h_step_paged_ws_bytes (0: refused, see z2h_last_error; 256-byte aligned). The call works on the
- * context's stream and returns when it is done; work of other streams on the cache has to be done before. Not while a
- * debug capture is on; a profiling window leaves out the paged operators' launches. */
+ * ids, emb_map, emb, n_emb, n_out and out_rows are those of z2h_step_mixed. The logits of the n_out rows go to
+ * d_logits (device, [n_out][n_codebooks][audio_vocab]; NULL: the context's own buffer) and, if out_logits is not NULL,
+ * to the host. d_ws is a workspace of z2h_step_paged_ws_bytes (0: refused, see z2h_last_error; 256-byte aligned). The
+ * call works on the context's stream and returns when it is done; work of other streams on the cache has to be done
+ * before. Not while a debug capture is on; a profiling window leaves out the paged operators' launches. */
 int64_t z2h_step_paged_ws_bytes(z2h_ctx * ctx, const z2h_pages * pages, int n_rows, int n_group);
 int z2h_step_paged(z2h_ctx * ctx, const z2h_pages * pages, int64_t layer_stride, int n_rows, const int32_t * row_start,
                    const int32_t * kv_len, int n_group, const int32_t * group_start, const int32_t * prefix_len,
