@@ -8,9 +8,9 @@
 //   k_paged_attn     a share of the wide strips per block and of the narrow ones per wave
 //   k_paged_join     one wave per (row, head): its pieces' partial results
 // Single tokens are bound by reading the cache once; groups of many rows and prompt chunks by the products and the exponentials.
-// Measured (attention + join): 64 single rows over 2048 shared and 16 to 2048 own keys, 4 key heads of 128: 21.8 + 7.2 us for
-// 60 MB; 256 rows over 16384 shared keys, 8 key heads of 128, 32 query heads: 110 + 9 us for 253 MB and 69 GFLOP at 630 TFLOP/s;
-// 4 prompt chunks of 333 rows behind 1500 shared ones: 41 + 11 us; one row over 700 keys: 10.6 + 3.8 us, of dependent loads.
+// Measured (attention + join): 64 single rows over 2048 shared and 16 to 2048 own keys, 4 key heads of 128: 20.5 + 7.2 us for
+// 60 MB; 256 rows over 16384 shared keys, 8 key heads of 128, 32 query heads: 104 + 9 us for 253 MB and 69 GFLOP at 670 TFLOP/s;
+// 4 prompt chunks of 333 rows behind 1500 shared ones: 40 + 11 us; one row over 700 keys: 10.0 + 3.8 us, of dependent loads.
 #pragma once
 #include "z2h_common.h"
 #include "z2h_ops_rules.h"
@@ -326,10 +326,11 @@ __device__ __forceinline__ float other_half(float v) {
 // {16 t + 4 h + j, 16 t + 8 + 4 h + j} (h the lane's half, j < 4): P never moves between lanes. V^T's operand for these keys is two
 // transposing LDS reads of 4 keys x 16 dims each from V rows stored as they are. K and V rows lie in LDS with their 16-byte
 // pieces permuted by row, so that both reads take all banks (no conflict counted).
-// A step of 64 keys takes a wave 4.5 thousand cycles beside the other block's wave: K Q 1.0, the softmax 1.0, P V 1.3, the barrier 0.2, the
-// rest the requests of the next keys. The matrix units are busy for 35 % of the kernel and the vector units for 38 % (256 rows over 16384
-// shared keys). Two waves per SIMD are what 253 registers leave: 32 query registers, 64 of O, 32 of scores at head size 128.
-// More row-heads per wave would halve the LDS reads per product, but not the exponentials, and leave one wave per SIMD.
+// A step of 64 keys takes a wave 4.0 thousand cycles beside the other block's wave: K Q with the requests of the next keys 1.2, the softmax
+// 0.9, P V 0.9, the barrier 0.1, the rest masks and addresses. 256 rows over 16384 shared keys: 110 us with operands read just before each
+// product and all requests behind the barrier, 104 so. Products and vector instructions each take 40 % of the cycles. Two waves per
+// SIMD are what the registers leave: 32 of queries, 64 of O, 32 of scores at head size 128. More row-heads per wave would halve the
+// LDS reads per product, but not the exponentials, and leave one wave per SIMD.
 template <int HD>
 struct Tile {
     static constexpr int NC = HD / 8, RP = 128 / HD;             // 16-byte pieces of a row, rows per 256 bytes
@@ -347,6 +348,7 @@ struct AttnWave {
     v16f_t o[DT];
     float m, l, c;                                               // m includes -BIAS: f16 weights up to 2^14, kept to 2^-24
     int vis;
+    int k_place[KS], v_place[DT];                                // where the lane's operands lie in 16 keys' rows (elements)
 
     __device__ __forceinline__ void init(const PagedArgs & a, const PlanItem & it, int first_rh, int lane) {
         const int group = a.n_head / a.nkv, rh = first_rh + (lane & 31), h8 = 8 * (lane >> 5);
@@ -396,6 +398,14 @@ struct AttnWave {
                 q[ks][j] = (TC) y;
                 if constexpr (SPLIT) ql[ks][j] = (TC) (y - (float) q[ks][j]);
             }
+        const int i16 = lane & 15, r = 4 * (lane >> 5) + (i16 >> 2);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) k_place[ks] = Tile<HD>::k_at(lane & 31, 2 * ks + (lane >> 5));
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+            const int d = 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
+            v_place[dt] = Tile<HD>::v_at(r, d >> 3) + (d & 7);
+        }
         m = -__builtin_inff();
         l = 0.0f;
 #pragma unroll
@@ -404,33 +414,51 @@ struct AttnWave {
             for (int i = 0; i < 16; ++i) o[dt][i] = 0.0f;
     }
 
-    // scores of NT tiles of 32 keys whose rows lie at LDS rows r0, r0 + 32, ...
-    template <int NT>
-    __device__ __forceinline__ void scores(v16f_t (&s)[NT], const TC * sk, int r0, int lane) const {
+    // PRODUCTS products in order, whose LDS operands are requested AHEAD products before they are used; beside(i) is called behind product
+    // i. The barriers keep the compiler from what it does by itself: to read, wait and multiply in turn.
+    template <int PRODUCTS, typename READ, typename MUL, typename B>
+    static __device__ __forceinline__ void products(READ read, MUL mul, B beside) {
+        constexpr int MOST = SPLIT ? 2 : 4, AHEAD = PRODUCTS < MOST ? PRODUCTS : MOST;   // (fp32 queries leave registers for two)
+        v8 f[AHEAD];
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            v16f_t acc = {};
-            const TC * rows = sk + (r0 + 32 * n) * HD;
+        for (int i = 0; i < AHEAD; ++i) f[i] = read(i);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const v8 kf = *(const v8 *) (rows + Tile<HD>::k_at(lane & 31, 2 * ks + (lane >> 5)));
-                acc = mfma32<TC>(kf, q[ks], acc);
-                if constexpr (SPLIT) acc = mfma32<TC>(kf, ql[ks], acc);
-            }
-            s[n] = acc;
+        for (int i = 0; i < PRODUCTS; ++i) {
+            mul(i, f[i % AHEAD]);
+            if (i + AHEAD < PRODUCTS) f[i % AHEAD] = read(i + AHEAD);
+            beside(i);
+            __builtin_amdgcn_sched_barrier(0);
         }
+    }
+
+    // scores of NT tiles of 32 keys whose rows lie at LDS rows r0, r0 + 32, ...
+    template <int NT, typename B>
+    __device__ __forceinline__ void scores(v16f_t (&s)[NT], const TC * sk, int r0, int lane, B beside) const {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[n] = v16f_t{};
+        products<KS * NT>(
+            [&](int i) __attribute__((always_inline)) { return *(const v8 *) (sk + k_place[i / NT] + (r0 + 32 * (i % NT)) * HD); },
+            [&](int i, v8 kf) __attribute__((always_inline)) {
+                s[i % NT] = mfma32<TC>(kf, q[i / NT], s[i % NT]);
+                if constexpr (SPLIT) s[i % NT] = mfma32<TC>(kf, ql[i / NT], s[i % NT]);
+            }, beside);
     }
 
     // keys key0 .. key0 + 32 NT, in the first rows of sk and sv; keys outside [from, min(to, vis)) are hidden. One body for all steps: a second
     // one for steps that hide something costs the compiler another set of accumulators (256 registers and 126 spilled against 237).
     // keys_done() is called when K has been read, values_ready() before V is.
-    template <int NT, typename F, typename G>
-    __device__ __forceinline__ void step(const TC * sk, const TC * sv, int key0, int from, int to, int lane, F keys_done, G values_ready) {
-        // fp32 queries at head size 128 fill the registers: the fragments' places anew in each step (kept, 15 registers are spilled)
-        if constexpr (SPLIT) asm("" : "+v"(lane));
+    template <int NT, typename B, typename F, typename G>
+    __device__ __forceinline__ void step(const TC * sk, const TC * sv, int key0, int from, int to, int lane, B beside, F keys_done, G values_ready) {
+        // (the places stay one register each, to which every read adds a constant: left to itself the compiler keeps one for every buffer)
+#pragma unroll
+        for (int i = 0; i < KS; ++i) asm("" : "+v"(k_place[i]));
+#pragma unroll
+        for (int i = 0; i < DT; ++i) asm("" : "+v"(v_place[i]));
         const int end = min(to, vis), r0 = 0;
         v16f_t s[NT];
-        scores<NT>(s, sk, r0, lane);
+        scores<NT>(s, sk, r0, lane, beside);
         keys_done();
         __builtin_amdgcn_sched_barrier(0);                       // no V read ahead of the weights: registers
         if (__any(key0 < from || key0 + 32 * NT > end)) {
@@ -480,20 +508,16 @@ struct AttnWave {
         l += sum;
         __builtin_amdgcn_sched_barrier(0);
         values_ready();
-#pragma unroll
-        for (int t = 0; t < 2 * NT; ++t)
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-                const v8 vf = __builtin_bit_cast(v8, values(sv, r0 + 16 * t, dt, lane));
-                o[dt] = mfma32<TC>(vf, p[t], o[dt]);
-                if constexpr (SPLIT) o[dt] = mfma32<TC>(vf, pl[t], o[dt]);
-            }
+        products<2 * NT * DT>([&](int i) __attribute__((always_inline)) { return __builtin_bit_cast(v8, values(sv, r0 + 16 * (i / DT), i % DT)); },
+                              [&](int i, v8 vf) __attribute__((always_inline)) {
+                                  o[i % DT] = mfma32<TC>(vf, p[i / DT], o[i % DT]);
+                                  if constexpr (SPLIT) o[i % DT] = mfma32<TC>(vf, pl[i / DT], o[i % DT]);
+                              }, [](int) {});
     }
 
     // V^T operand of 16 keys from LDS row r0 on, dims 32 dt ..: lanes 16 g + i read keys 4 (g / 2) + i / 4, dims 16 (g & 1) + 4 (i & 3)
-    static __device__ __forceinline__ s8_t values(const TC * sv, int r0, int dt, int lane) {
-        const int i16 = lane & 15, r = 4 * (lane >> 5) + (i16 >> 2), d = 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
-        const TC * at = sv + r0 * HD + Tile<HD>::v_at(r, d >> 3) + (d & 7);
+    __device__ __forceinline__ s8_t values(const TC * sv, int r0, int dt) const {
+        const TC * at = sv + v_place[dt] + r0 * HD;
         typedef __attribute__((address_space(3))) s4_t lds4;
         const s4_t x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *) at);
         const s4_t x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *) (at + 8 * HD));
@@ -517,7 +541,7 @@ struct AttnWave {
             }
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-                const s8_t v = values(sv, r0 + 16 * t, dt, lane);
+                const s8_t v = values(sv, r0 + 16 * t, dt);
                 b8 up, down;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -607,6 +631,11 @@ struct Mover {
 #pragma unroll
         for (int i = 0; i < N; ++i) to_lds((const TC *) a.v + at + i * ROWS * HD + v, to + i * ROWS * HD);
     }
+    // instruction i of these, K's before V's (none from 2 N on)
+    __device__ __forceinline__ void rows16_part(const PagedArgs & a, int64_t at, TC * sk, TC * sv, int i) const {
+        if (i < N) to_lds((const TC *) a.k + at + k[i], sk + i * ROWS * HD);
+        else if (i < 2 * N) to_lds((const TC *) a.v + at + (i - N) * ROWS * HD + v, sv + (i - N) * ROWS * HD);
+    }
     __device__ __forceinline__ void rows16(const PagedArgs & a, int64_t at, TC * sk, TC * sv) const {
         keys16(a, at, sk);
         values16(a, at, sv);
@@ -621,10 +650,14 @@ struct PagedAttn {
     __device__ __forceinline__ PagedAttn(const PagedArgs & args, int lane_, int wave_)
         : a(args), mv(lane_), lane(lane_), wave(wave_), group(args.n_head / args.nkv) {}
 
-    // elements from the start of k and v to the 16 rows that begin with `key` >= 0 (one page holds them; any key and any page entry
-    // give an address inside the cache)
-    __device__ __forceinline__ int64_t rows_at(const PlanItem & it, int key) const {
-        const int at = min(key >> a.page_shift, a.table_len - 1), entry = uniform(a.table)[(int64_t) it.seq * a.table_len + at];
+    // the page that holds `key` >= 0, as the table has it: a scalar load that is requested a step ahead of its use, where no wait for LDS
+    // follows soon (these loads come back in any order, so that such a wait is one for them too)
+    __device__ __forceinline__ int entry_at(const PlanItem & it, int key) const {
+        return uniform(a.table)[(int64_t) it.seq * a.table_len + min(key >> a.page_shift, a.table_len - 1)];
+    }
+    // elements from the start of k and v to the 16 rows that begin with `key` (one page holds them; any key and any page entry give
+    // an address inside the cache)
+    __device__ __forceinline__ int64_t rows_of(const PlanItem & it, int key, int entry) const {
         const int page = entry >= 0 && entry < a.n_pages ? entry : 0;
         return page * a.page_stride + (((int64_t) it.head << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * HD;
     }
@@ -652,7 +685,10 @@ struct PagedAttn {
     // are requested when this step's scores are formed, the next values when its values have been used.
     __device__ __forceinline__ void narrow(const PlanItem & it, TC * wk, TC * wv) const {
         int key = it.key0 & ~31;
-        int64_t n0 = rows_at(it, key), n1 = rows_at(it, key + 16);
+        int e0 = entry_at(it, key), e1 = entry_at(it, key + 16);
+        int64_t n0 = rows_of(it, key, e0), n1 = rows_of(it, key + 16, e1);
+        e0 = entry_at(it, key + 32);
+        e1 = entry_at(it, key + 48);
         mv.keys16(a, n0, wk);
         mv.keys16(a, n1, wk + 16 * HD);
         mv.values16(a, n0, wv);
@@ -672,10 +708,13 @@ struct PagedAttn {
                     wait_lds();
                 }
             }
-            if (more) { n0 = rows_at(it, key + 32); n1 = rows_at(it, key + 48); }
-            w.template step<1>(wk, wv, key, it.key0, it.key1, lane, [&] {
+            n0 = rows_of(it, key + 32, e0);
+            n1 = rows_of(it, key + 48, e1);
+            w.template step<1>(wk, wv, key, it.key0, it.key1, lane, [](int) {}, [&] {
                 wait_lds();
                 if (more) { mv.keys16(a, n0, wk); mv.keys16(a, n1, wk + 16 * HD); }
+                e0 = entry_at(it, key + 64);
+                e1 = entry_at(it, key + 80);
             }, [&] {
                 if (more) wait_loads_but<2 * Mover<HD, TC>::N>();
                 else wait_loads_but<0>();
@@ -688,10 +727,11 @@ struct PagedAttn {
 
     // ---- wide: every wave takes 32 row-heads; 64 keys at a time in LDS for all, the next 64 on their way into the other buffer
     __device__ __forceinline__ void wide(const PlanItem & it, TC * s_k0, TC * s_v0, TC * s_k1, TC * s_v1, int * s_vis) const {
+        static_assert(AttnWave<HD, T, TC>::KS == 2 * Mover<HD, TC>::N, "two requests beside every fourth of 2 KS products are all of them");
         const int mine = 16 * wave;
         int key = it.key0 & ~63;
-        mv.rows16(a, rows_at(it, key + mine), s_k0 + mine * HD, s_v0 + mine * HD);
-        int64_t next = rows_at(it, key + 64 + mine);
+        mv.rows16(a, rows_of(it, key + mine, entry_at(it, key + mine)), s_k0 + mine * HD, s_v0 + mine * HD);
+        int entry = entry_at(it, key + 64 + mine);
         AttnWave<HD, T, TC> w;
         w.init(a, it, 32 * wave, lane);
         const bool live = 32 * wave < it.rows * group;
@@ -706,24 +746,36 @@ struct PagedAttn {
         auto stage = [&](const TC * sk, TC * sv, TC * ok, TC * ov) __attribute__((always_inline)) {
             wait_loads_but<0>();                                 // (the barrier itself does not wait for loads to LDS)
             __syncthreads();
-            if (key + 64 < it.key1) {
-                mv.rows16(a, next, ok + mine * HD, ov + mine * HD);
-                next = rows_at(it, key + 128 + mine);
-            }
+            const bool more = key + 64 < it.key1;
             if ((key < it.key0 || key + 64 > whole) && __syncthreads_or(rows_not_finite<HD>(sv + mine * HD, lane))) {
                 if (live) w.template infinite_values<2>(sv, 0, key, it.key0, it.key1, lane);
                 __syncthreads();
                 clean_rows<HD>(sv + mine * HD, lane);
                 __syncthreads();
             }
-            if (live) w.template step<2>(sk, sv, key, it.key0, it.key1, lane, [] {}, [] {});
+            // the next keys and values are requested two instructions at a time beside the products: all at once they hold the wave up
+            // where the other block's narrow shares fill the queue
+            const int64_t next = rows_of(it, key + 64 + mine, entry);
+            if (live)
+                w.template step<2>(sk, sv, key, it.key0, it.key1, lane, [&](int i) __attribute__((always_inline)) {
+                    if (i % 4 == 0 && more) {
+                        mv.rows16_part(a, next, ok + mine * HD, ov + mine * HD, i / 2);
+                        mv.rows16_part(a, next, ok + mine * HD, ov + mine * HD, i / 2 + 1);
+                    }
+                }, [&] { entry = entry_at(it, key + 128 + mine); }, [] {});
+            else {
+                if (more) mv.rows16(a, next, ok + mine * HD, ov + mine * HD);
+                entry = entry_at(it, key + 128 + mine);
+            }
             key += 64;
         };
+        __builtin_amdgcn_s_setprio(1);                           // before narrow shares, which wait for memory anyway (110 -> 107 us)
         while (key < it.key1) {
             stage(s_k0, s_v0, s_k1, s_v1);
             if (key >= it.key1) break;
             stage(s_k1, s_v1, s_k0, s_v0);
         }
+        __builtin_amdgcn_s_setprio(0);
         store(it, w, 32 * wave);
         __syncthreads();                                         // LDS is free for the next piece
     }
