@@ -88,7 +88,10 @@ int attn_blocks(int n_cu) { return 2 * n_cu; }
 template <int HD, typename T, typename TC>
 void attn_launch(const PagedArgs & a, int blocks, hipStream_t stream) {
     hipLaunchKernelGGL((k_paged_attn<HD, T, TC>), dim3(blocks), dim3(256), 0, stream, a);
-    hipLaunchKernelGGL((k_paged_join<HD, T>), dim3((a.n_rows * a.n_head + 3) / 4), dim3(256), 0, stream, a);
+    // a block per (row, head) while the device holds all of them at once: 1024 of 24 partial results each 7.0 us against 5.3, 8192 of 10
+    // each 9.4 against 14.9
+    if (a.n_rows * a.n_head <= 4 * blocks) hipLaunchKernelGGL((k_paged_join<HD, T, true>), dim3(a.n_rows * a.n_head), dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((k_paged_join<HD, T, false>), dim3((a.n_rows * a.n_head + 3) / 4), dim3(256), 0, stream, a);
 }
 template <int HD>
 void attn_launch(const PagedArgs & a, int type, int blocks, hipStream_t stream) {

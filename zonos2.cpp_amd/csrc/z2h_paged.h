@@ -8,7 +8,7 @@
 //   k_paged_attn     a share of the wide strips per block and of the narrow ones per wave
 //   k_paged_join     one wave per (row, head): its pieces' partial results
 // Single tokens are bound by reading the cache once; groups of many rows and prompt chunks by the products and the exponentials.
-// Measured (attention + join): 64 single rows over 2048 shared and 16 to 2048 own keys, 4 key heads of 128: 20.5 + 7.2 us for
+// Measured (attention + join): 64 single rows over 2048 shared and 16 to 2048 own keys, 4 key heads of 128: 20.5 + 5.3 us for
 // 60 MB; 256 rows over 16384 shared keys, 8 key heads of 128, 32 query heads: 104 + 9 us for 253 MB and 69 GFLOP at 670 TFLOP/s;
 // 4 prompt chunks of 333 rows behind 1500 shared ones: 40 + 11 us; one row over 700 keys: 10.0 + 3.8 us, of dependent loads.
 #pragma once
@@ -812,10 +812,14 @@ __global__ void __launch_bounds__(256, 2) k_paged_attn(PagedArgs a) {
     }
 }
 
-// One wave per (row, head): weights of its partial results from their maxima (a lane each, 64 at a time), then the dims over the lanes.
-template <int HD, typename T>
+// One wave per (row, head), or with SHARED its block's four waves: weights of its partial results from their maxima (a lane each, 64 at a
+// time), then the dims over the lanes. Bound by its chain of loads (row, strips, maxima, results), which four waves shorten, and with many
+// rows by reading the results.
+template <int HD, typename T, bool SHARED>
 __global__ void __launch_bounds__(256) k_paged_join(PagedArgs a) {
-    const int lane = threadIdx.x & 63, id = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    constexpr int STEP = SHARED ? 4 : 1;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
+    const int id = SHARED ? (int) blockIdx.x : 4 * (int) blockIdx.x + wave, from = SHARED ? wave : 0;
     if (id >= a.n_rows * a.n_head) return;
     const int row = id / a.n_head, head = id % a.n_head, group = a.n_head / a.nkv, g = head / group;
     const PlanRow r = uniform_copy(a.rows + row);
@@ -825,8 +829,11 @@ __global__ void __launch_bounds__(256) k_paged_join(PagedArgs a) {
     if (own.stored) return;                                      // by its only piece
     const int n_pre = pre.pieces, n_own = own.pieces, pre_step = pre.heads, own_step = own.heads;
     const int pre0 = pre.part0 + r.pre_at + head % group, own0 = own.part0 + r.own_at + head % group;
-    const int n = n_pre + n_own;
-    auto part = [&](int i) { return i < n_pre ? pre0 + i * pre_step : own0 + (i - n_pre) * own_step; };
+    const int n = max(0, (n_pre + n_own - from + STEP - 1) / STEP);  // this wave's
+    auto part = [&](int i) {
+        i = i * STEP + from;
+        return i < n_pre ? pre0 + i * pre_step : own0 + (i - n_pre) * own_step;
+    };
     constexpr int E = HD >= 64 ? HD / 64 : 1;
     const int d = E * lane;
     constexpr int MB = 8;                                        // results on their way, the first of them with the maxima
@@ -860,6 +867,25 @@ __global__ void __launch_bounds__(256) k_paged_join(PagedArgs a) {
 #pragma unroll
                     for (int e = 0; e < E; ++e) o[e] = __builtin_fmaf(wi, x[u][e], o[e]);
             }
+        }
+    }
+    if constexpr (SHARED) {
+        __shared__ float s_o[4][64 * E], s_m[4], s_l[4];
+        if (lane == 0) { s_m[wave] = m; s_l[wave] = l; }
+#pragma unroll
+        for (int e = 0; e < E; ++e) s_o[wave][d + e] = o[e];
+        __syncthreads();
+        if (wave) return;
+        m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+        l = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float c = s_m[w] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(s_m[w] - m);
+            l = __builtin_fmaf(c, s_l[w], l);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = __builtin_fmaf(c, s_o[w][d + e], o[e]);
         }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
