@@ -327,7 +327,7 @@ __device__ __forceinline__ float other_half(float v) {
 // transposing LDS reads of 4 keys x 16 dims each from V rows stored as they are. K and V rows lie in LDS with their 16-byte
 // pieces permuted by row, so that both reads take all banks (no conflict counted).
 // A step of 64 keys takes a wave 4.0 thousand cycles beside the other block's wave: K Q with the requests of the next keys 1.2, the softmax
-// 0.9, P V 0.9, the barrier 0.1, the rest masks and addresses. 256 rows over 16384 shared keys: 110 us with operands read just before each
+// 1.0, P V 0.8, the barrier 0.15, the rest masks and addresses. 256 rows over 16384 shared keys: 110 us with operands read just before each
 // product and all requests behind the barrier, 104 so. Products and vector instructions each take 40 % of the cycles. Two waves per
 // SIMD are what the registers leave: 32 of queries, 64 of O, 32 of scores at head size 128. More row-heads per wave would halve the
 // LDS reads per product, but not the exponentials, and leave one wave per SIMD.
