@@ -1,0 +1,146 @@
+"""z2h_paged_plan / z2h_paged_attn where they are easily wrong: infinities in the cache, wherever they lie and whatever way their keys are
+walked (a piece that stores its rows itself, pieces that are joined, tiles of one wave and of four)."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from ops_helpers import DEV, TYPES, Attn, Cache, check, context, half_step
+from zonos2_amd import z2h
+
+pytestmark = pytest.mark.gpu
+INF = float("inf")
+UP = {torch.float32: 2.0 ** -21, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}   # half a step of a weight as it meets the values
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = context()
+    yield c
+    c.close()
+
+
+def reference(cache, q, row_start, kv_len, scale, dtype, up=None):
+    """64-bit attention and the tolerance that ops_helpers.attention derives, by products over a sequence's rows at once. A key with a score
+    of minus infinity has no weight; a value that is not finite reaches the rows that see it whatever its weight."""
+    R, nh, hd = q.shape
+    kvh, grp = cache.kvh, nh // cache.kvh
+    up = UP[dtype] if up is None else up
+    uq = 2.0 ** -21 if dtype == torch.float32 else 0.0
+    ref, tol = torch.zeros_like(q), torch.zeros_like(q)
+    for s in range(len(kv_len)):
+        r0, m, n = int(row_start[s]), int(row_start[s + 1] - row_start[s]), int(kv_len[s])
+        if m == 0 or n == 0:
+            continue
+        k, v = (t.transpose(0, 1).contiguous() for t in cache.rows(s, n))                 # [kvh][n][hd]
+        x = q[r0:r0 + m].reshape(m, kvh, grp, hd).transpose(0, 1).reshape(kvh, m * grp, hd)
+        see = (n - m + torch.arange(m) + 1).clamp(min=0).repeat_interleave(grp)            # cache rows that each row sees
+        hidden = torch.arange(n)[None, :] >= see[:, None]
+        sc = scale * torch.matmul(x, k.transpose(1, 2).contiguous())
+        size = torch.matmul(x.abs(), torch.nan_to_num(k, 0.0, 0.0, 0.0).abs().transpose(1, 2).contiguous())
+        sc = sc.masked_fill(hidden, -INF)
+        p = torch.nan_to_num(torch.softmax(sc, -1), 0.0) if bool((see == 0).any()) else torch.softmax(sc, -1)
+        v0 = torch.nan_to_num(v, 0.0, 0.0, 0.0)
+        o = torch.matmul(p, v0)
+        shown = (~hidden).double()
+        for bad, sign in (((v == INF) | v.isnan(), INF), ((v == -INF) | v.isnan(), -INF)):
+            if bool(bad.any()):
+                o = torch.where(torch.matmul(shown, bad.double()) > 0, o + sign, o)
+        ds = abs(scale) * size.masked_fill(hidden, 0.0).amax(-1) * (8 * 2.0 ** -24 * math.sqrt(hd) + uq)
+        rel = 2 * ds + 94 * 2.0 ** -24 + up + 8 * torch.sqrt(see.double()) * 2.0 ** -24
+        t = rel[..., None] * torch.matmul(torch.nan_to_num(p, 0.0), v0.abs())
+        for dst, val in ((ref, o), (tol, t)):
+            dst[r0:r0 + m] = val.reshape(kvh, m, grp, hd).transpose(0, 1).reshape(m, nh, hd)
+    return ref, tol + half_step(torch.nan_to_num(ref, 0.0, 0.0, 0.0), dtype) * (1 + 2.0 ** -10)
+
+
+def case(typ, lens, rows, heads, kvh, hd, page, groups=(), seed=0, qscale=1.0, **cache):
+    dtype = TYPES[typ][1]
+    c = Cache(lens, kvh, hd, page, torch.bfloat16 if typ == "bf16" else torch.float16, seed + 1, shared=groups, **cache)
+    row_start = np.concatenate([[0], np.cumsum(rows)]).astype(int)
+    g = torch.Generator().manual_seed(seed + 2)
+    return c, row_start, (torch.randn((int(row_start[-1]), heads, hd), generator=g) * qscale).to(dtype)
+
+
+def run(ctx, typ, c, row_start, q, lens, groups=(), scale=0.125, in_place=False):
+    a = Attn(ctx, c, q.shape[1], row_start, lens, groups, typ)
+    d = q.to(DEV)
+    out = d if in_place else torch.full_like(d, 7.0)
+    a.plan()
+    a.run(d.view(len(d), -1), out.view(len(d), -1), scale)
+    torch.cuda.synchronize()
+    return out
+
+
+# ---- infinities in the cache
+SHAPES = {
+    # one piece that stores its rows, two pieces, several
+    "few": dict(lens=[40, 70, 300], rows=[2, 6, 1], heads=4, kvh=2, hd=64, page=16, groups=()),
+    # a shared prefix for 160 row-heads of each key head: a tile of four waves, one of a wave, and the sequences' own keys
+    "shared": dict(lens=[300 + s % 40 for s in range(1, 41)], rows=[1] * 40, heads=8, kvh=2, hd=128, page=16, groups=[(0, 40, 300)]),
+    # whole prompts: tiles of four waves whose rows see more and more
+    "prompt": dict(lens=[150], rows=[150], heads=4, kvh=2, hd=32, page=16, groups=()),
+}
+
+
+def _infinite(ctx, typ, shape, qscale, poison, change=None, in_place=False):
+    print(f"infinite {typ} {shape} {qscale} {poison}", flush=True)
+    p = SHAPES[shape]
+    c, row_start, q = case(typ, **p, seed=11, qscale=qscale)
+    if change is not None:
+        change(q)
+    for which, seq, key, head, dim, value in poison:
+        c.cell(which, seq, key)[head, dim] = value
+    c.upload()
+    ref, tol = reference(c, q.double(), row_start, p["lens"], 0.125, q.dtype)
+    check(run(ctx, typ, c, row_start, q, p["lens"], p["groups"], in_place=in_place), ref, tol, typ)
+    return ref
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", list(SHAPES))
+@pytest.mark.parametrize("qscale", [1.0, 30.0])             # (30: most weights are below what f16 holds)
+def test_infinite_values_wherever_they_lie(ctx, typ, shape, qscale):
+    ref = _infinite(ctx, typ, shape, qscale, [(1, 0, 0, 0, 1, INF), (1, 0, 3, 0, 5, INF), (1, 0, 20, 1, 9, -INF), (1, 0, 7, 1, 11, INF),
+                                              (1, 0, 33, 1, 11, -INF), (1, 0, 39, 0, 2, INF), (1, 0, 12, 0, 30, float("nan"))])
+    assert torch.isinf(ref).any() and torch.isnan(ref).any() and torch.isfinite(ref).any()
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", list(SHAPES))
+def test_infinite_values_in_place(ctx, typ, shape):
+    _infinite(ctx, typ, shape, 3.0, [(1, 0, 2, 0, 5, INF), (1, 0, 30, 1, 9, -INF)], in_place=True)
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", list(SHAPES))
+def test_infinite_keys(ctx, typ, shape):
+    """A row whose component there has the other sign gives the key no weight, one with the same sign (or 0) has no answer."""
+    def change(q):
+        q[0, 0, 7], q[0, 1, 7], q[1, :, 7] = 0.0, -1e-30 if q.dtype == torch.float32 else -1e-4, -0.5
+    ref = _infinite(ctx, typ, shape, 1.0, [(0, 0, 3, 0, 7, INF), (0, 0, 25, 1, 6, -INF)], change)
+    assert torch.isnan(ref).any() and torch.isfinite(ref).any()
+    assert typ != "f32" or torch.isfinite(ref[0, 1]).all()
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+def test_infinite_keys_and_values(ctx, typ):
+    def change(q):
+        q[..., 7] = -q[..., 7].abs() - 0.01
+    ref = _infinite(ctx, typ, "shared", 1.0, [(0, 0, 3, 0, 7, INF), (0, 0, 150, 1, 7, INF), (1, 0, 200, 0, 4, INF), (1, 0, 64, 1, 4, -INF)], change)
+    assert not torch.isnan(ref).any() and torch.isinf(ref).any()
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16"])
+def test_infinities_with_large_queries_and_a_negative_scale(ctx, typ):
+    """Scores formed once more keep to the range of the queries and to the scale's sign."""
+    p = SHAPES["few"]
+    c, row_start, q = case(typ, **p, seed=12)
+    big = 1e30 if typ == "f32" else 1e3
+    q *= big
+    c.cell(1, 1, 5)[:, 3] = INF
+    c.upload()
+    scale = float(np.float32(-0.125 / big))
+    ref, tol = reference(c, q.double(), row_start, p["lens"], scale, q.dtype)
+    check(run(ctx, typ, c, row_start, q, p["lens"], scale=scale), ref, tol, typ)

@@ -306,6 +306,8 @@ typedef float v16f_t __attribute__((ext_vector_type(16)));
 typedef unsigned u4_t __attribute__((ext_vector_type(4)));
 typedef short s4_t __attribute__((ext_vector_type(4)));
 typedef short s8_t __attribute__((ext_vector_type(8)));
+template <typename T> struct CacheOf { typedef _Float16 type; };  // pages that queries of T go with
+template <> struct CacheOf<__bf16> { typedef __bf16 type; };
 template <typename TC> struct Vec8 { typedef TC type __attribute__((ext_vector_type(8))); };
 
 template <typename TC>
@@ -313,6 +315,7 @@ __device__ __forceinline__ v16f_t mfma32(typename Vec8<TC>::type a, typename Vec
     if constexpr (__is_same(TC, _Float16)) return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
+__device__ __forceinline__ bool is_finite(float v) { return fabsf(v) < __builtin_inff(); }
 // the value of the lane 32 away
 __device__ __forceinline__ float other_half(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
@@ -523,6 +526,17 @@ struct AttnWave {
         const s4_t x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *) (at + 8 * HD));
         return __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
     }
+    // What is not finite in the cache meets both parts of a number in two parts, which may differ in sign or be 0, and weights that are too
+    // small for the cache's type: the product is then NaN where the definition has infinity (values) or a weight of 0 (keys), never
+    // anything else that is wrong. So rows that hold NaN are formed once more, by k_paged_join (walk_row).
+    __device__ __forceinline__ bool any_nan() const {
+        bool nan = false;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) nan |= o[dt][i] != o[dt][i];
+        return nan;
+    }
     // Where some rows hide keys that others see (or that nobody has), a value that is not finite must not reach a row as 0 x inf. Such a
     // tile's values are set to 0 in LDS, and before that rows that see one get infinity (or both infinities: NaN): the product
     // of two numbers that are infinite together.
@@ -661,11 +675,16 @@ struct PagedAttn {
         const int page = entry >= 0 && entry < a.n_pages ? entry : 0;
         return page * a.page_stride + (((int64_t) it.head << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * HD;
     }
-    // the row-heads first_rh .. first_rh + 31 of the piece: final, or partial
+    // the row-heads first_rh .. first_rh + 31 of the piece: final, or partial. Final ones that hold NaN are left to k_paged_join (their
+    // queries may lie where the results go), which finds them by a mark in the place of their maximum and sum.
     __device__ __forceinline__ void store(const PlanItem & it, AttnWave<HD, T, TC> & w, int first_rh) const {
         const int heads = it.rows * group, rh = first_rh + (lane & 31);
         w.l += other_half(w.l);
+        float nan = it.direct && w.any_nan() ? 1.0f : 0.0f;
+        nan = fmaxf(nan, other_half(nan));
         if (rh >= heads) return;
+        if (lane < 32) a.part_ml[it.part0 + rh] = it.direct ? make_float2(0.0f, nan) : make_float2(w.m, w.l);
+        if (nan != 0.0f) return;
         const float inv = !it.direct ? 1.0f : w.l == 0.0f ? 0.0f : 1.0f / w.l;
         T * out = (T *) a.out + (it.row0 + rh / group) * a.os + (int64_t) (it.head * group + rh % group) * HD;
         float * part = a.part_o + (int64_t) (it.part0 + rh) * HD;
@@ -678,7 +697,6 @@ struct PagedAttn {
                 if (it.direct) store4(out + d, x.x, x.y, x.z, x.w);
                 else *(float4 *) (part + d) = x;
             }
-        if (!it.direct && lane < 32) a.part_ml[it.part0 + rh] = make_float2(w.m, w.l);
     }
 
     // ---- narrow: the wave's own 32 rows of LDS (K at wk, V at wv), its own keys; nothing to wait for but its own loads. The next keys
@@ -812,6 +830,75 @@ __global__ void __launch_bounds__(256, 2) k_paged_attn(PagedArgs a) {
     }
 }
 
+// A (row, head) in plain fp32, by one wave: 64 keys at a time, a lane each for the scores, then the dims over the lanes. A value that is
+// not finite reaches the row whatever its weight. For rows whose results hold NaN (see AttnWave): 2 ms over 16384 keys, of chains of loads.
+template <int HD, typename T, typename TC, int E>
+__device__ __forceinline__ void walk_row(const PagedArgs & a, const PlanRow & r, int row, int head, float * s_q, float (&o)[E], float & l) {
+    const int lane = threadIdx.x & 63, g = head / (a.n_head / a.nkv), d = E * lane;
+    const T * src = (const T *) a.q + row * a.qs + (int64_t) head * HD;
+    float mx = 0.0f;
+    for (int i = lane; i < HD; i += 64) mx = fmaxf(mx, fabsf((float) src[i]));
+    mx = wave_max_f(mx);
+    int up = 0;                                                  // (a power of two keeps the scores of large queries finite)
+    if (mx > 0.0f && mx < __builtin_inff()) (void) frexpf(mx, &up);
+    up = max(up, -120);
+    for (int i = lane; i < HD; i += 64) s_q[i] = a.scale == 0.0f ? 0.0f : ldexpf((float) src[i], -up);
+    wait_lds();
+    const float c = copysignf(fminf(ldexpf(fabsf(a.scale) * 1.44269504088896341f, up), 0x1p127f), a.scale);
+    float m = -__builtin_inff();
+    l = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.0f;
+    for (int part = 0; part < 2; ++part) {
+        const int place = part ? r.own_tile : r.pre_tile;
+        if (place < 0) continue;
+        const PlanTile t = a.tiles[place];
+        const int end = min(t.key1, r.vis);
+        for (int key0 = t.key0; key0 < end; key0 += 64) {
+            const int key = min(key0 + lane, end - 1), entry = a.table[(int64_t) t.seq * a.table_len + min(key >> a.page_shift, a.table_len - 1)];
+            const int page = entry >= 0 && entry < a.n_pages ? entry : 0;
+            const int64_t at = page * a.page_stride + (((int64_t) g << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * HD;
+            const typename Vec8<TC>::type * k = (const typename Vec8<TC>::type *) ((const TC *) a.k + at);
+            float x[4] = {};
+#pragma unroll 2                                                 // (64 registers at most, for the join's occupancy)
+            for (int i = 0; i < HD / 8; ++i) {
+                const typename Vec8<TC>::type kk = k[i];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j & 3] = __builtin_fmaf(s_q[8 * i + j], (float) kk[j], x[j & 3]);
+            }
+            float s = ((x[0] + x[1]) + (x[2] + x[3])) * c;
+            if (key0 + lane >= end) s = -__builtin_inff();
+            if (__any(!(s < __builtin_inff()))) {                // infinity or no number: nor is any weight a number
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[e] = __builtin_nanf("");
+                return;
+            }
+            const float mn = fmaxf(m, wave_max_f(s));
+            const float w0 = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+            const float w = s == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(s - mn);
+            m = mn;
+            l = l * w0 + wave_tree_f(w);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = is_finite(o[e]) ? o[e] * w0 : o[e];
+            const int n = min(64, end - key0), lo = (int) (uint64_t) at, hi = (int) ((uint64_t) at >> 32);
+            for (int i0 = 0; i0 < n; i0 += 8) {                 // (lanes from n on have the last key, with no weight)
+                float wi[8], v[8][E];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    wi[u] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), i0 + u));
+                    const uint64_t from = (uint64_t) (unsigned) __builtin_amdgcn_readlane(hi, i0 + u) << 32 | (unsigned) __builtin_amdgcn_readlane(lo, i0 + u);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) v[u][e] = d < HD ? (float) ((const TC *) a.v)[from + d + e] : 0.0f;
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) o[e] = is_finite(v[u][e]) ? __builtin_fmaf(wi[u], v[u][e], o[e]) : o[e] + v[u][e];
+            }
+        }
+    }
+}
+
 // One wave per (row, head), or with SHARED its block's four waves: weights of its partial results from their maxima (a lane each, 64 at a
 // time), then the dims over the lanes. Bound by its chain of loads (row, strips, maxima, results), which four waves shorten, and with many
 // rows by reading the results.
@@ -826,10 +913,12 @@ __global__ void __launch_bounds__(256) k_paged_join(PagedArgs a) {
     if (!plan_fits(a)) return;
     auto strip = [&](int tile) { return tile >= 0 ? uniform_copy(a.strips + (int64_t) tile * a.nkv + g) : PlanStrip{0, 0, 0, 0}; };
     const PlanStrip pre = strip(r.pre_tile), own = strip(r.own_tile);
-    if (own.stored) return;                                      // by its only piece
     const int n_pre = pre.pieces, n_own = own.pieces, pre_step = pre.heads, own_step = own.heads;
     const int pre0 = pre.part0 + r.pre_at + head % group, own0 = own.part0 + r.own_at + head % group;
-    const int n = max(0, (n_pre + n_own - from + STEP - 1) / STEP);  // this wave's
+    // stored by its only piece, unless that one found NaN
+    const bool again = own.stored && uniform(a.part_ml)[own0].y != 0.0f;
+    if (own.stored && (!again || from)) return;
+    const int n = again ? 0 : max(0, (n_pre + n_own - from + STEP - 1) / STEP);  // this wave's
     auto part = [&](int i) {
         i = i * STEP + from;
         return i < n_pre ? pre0 + i * pre_step : own0 + (i - n_pre) * own_step;
@@ -869,7 +958,7 @@ __global__ void __launch_bounds__(256) k_paged_join(PagedArgs a) {
             }
         }
     }
-    if constexpr (SHARED) {
+    if constexpr (SHARED) if (!again) {
         __shared__ float s_o[4][64 * E], s_m[4], s_l[4];
         if (lane == 0) { s_m[wave] = m; s_l[wave] = l; }
 #pragma unroll
@@ -887,6 +976,13 @@ __global__ void __launch_bounds__(256) k_paged_join(PagedArgs a) {
 #pragma unroll
             for (int e = 0; e < E; ++e) o[e] = __builtin_fmaf(c, s_o[w][d + e], o[e]);
         }
+    }
+    bool nan = again;
+#pragma unroll
+    for (int e = 0; e < E; ++e) nan |= o[e] != o[e];
+    if (__any(nan)) {
+        __shared__ float s_q[SHARED ? 1 : 4][HD];
+        walk_row<HD, T, typename CacheOf<T>::type>(a, r, row, head, s_q[SHARED ? 0 : wave], o, l);
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     T * out = (T *) a.out + row * a.os + (int64_t) head * HD + d;
