@@ -320,7 +320,8 @@ int z2h_paged_append(z2h_ctx * ctx, const z2h_pages * pages, const z2h_rope * ro
  * z2h_paged_attn: d_out = softmax(scale q k^T) v for d_q [n_rows][n_head][head_dim], rows q_stride / out_stride apart,
  * n_head a multiple of n_head_kv, at most 64 query heads per key head; query head h reads key head h / (n_head /
  * n_head_kv). `type` is Z2H_F32 or Z2H_F16 over Z2H_F16 pages, or Z2H_BF16 over Z2H_BF16 pages. d_out may be d_q (with
- * the same stride). Softmax and sums in fp32; results do not depend on timing (no atomics). Cache rows that a row does not see
+ * the same stride). Softmax and sums in fp32; the weights meet the
+ * values to 2^-16 of them (bf16) or 2^-22. Results do not depend on timing (no atomics). Cache rows that a row does not see
  * do not reach it, whatever they hold. A value that is not finite reaches every row that sees it; a key whose score is minus
  * infinity has no weight, and one whose score is infinity or no number leaves the row without a number. (Rows that see such a
  * cache row take longer: about 2 ms over 16384 keys.)

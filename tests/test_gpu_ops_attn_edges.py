@@ -1,5 +1,5 @@
 """z2h_paged_plan / z2h_paged_attn where they are easily wrong: infinities in the cache, wherever they lie and whatever way their keys are
-walked (a piece that stores its rows itself, pieces that are joined, tiles of one wave and of four)."""
+walked (a piece that stores its rows itself, pieces that are joined, tiles of one wave and of four); and how near the results come."""
 import math
 
 import numpy as np
@@ -144,3 +144,27 @@ def test_infinities_with_large_queries_and_a_negative_scale(ctx, typ):
     scale = float(np.float32(-0.125 / big))
     ref, tol = reference(c, q.double(), row_start, p["lens"], scale, q.dtype)
     check(run(ctx, typ, c, row_start, q, p["lens"], scale=scale), ref, tol, typ)
+
+
+# ---- how near 16-bit results come: the output's own rounding, and next to it what fp32 sums leave
+# A weight is carried as two numbers of the cache's type: off by half a step of half a step, 2^-22 of it in f16 and 2^-16 in bf16. In f16 the second
+# part is below the normal range where the weight is below 2^-3, and then off by 2^-25 at most; the largest weight is 2^6 or more, so n keys add
+# n 2^-31 of the largest value.
+TWO = {torch.float16: 2.0 ** -22, torch.bfloat16: 2.0 ** -16}
+
+
+@pytest.mark.parametrize("typ", ["f16", "bf16"])
+@pytest.mark.parametrize("shape", list(SHAPES) + ["long", "wide"])
+@pytest.mark.parametrize("qscale", [0.01, 1.0, 5.0])        # (weights all alike, as they usually are, and peaked)
+def test_16_bit_results_have_the_outputs_rounding_only(ctx, typ, shape, qscale):
+    p = SHAPES.get(shape) or {"long": dict(lens=[4097, 1000], rows=[1, 3], heads=8, kvh=2, hd=128, page=64, groups=()),
+                              "wide": dict(lens=[1500] * 33, rows=[1] * 33, heads=16, kvh=4, hd=64, page=32, groups=[(0, 33, 1480)])}[shape]
+    print(f"rounding {typ} {shape} {qscale}", flush=True)
+    c, row_start, q = case(typ, **p, seed=21, qscale=qscale)
+    ref, tol = reference(c, q.double(), row_start, p["lens"], 0.125, q.dtype, up=TWO[q.dtype])
+    if typ == "f16":
+        tol += max(p["lens"]) * 2.0 ** -31 * float(torch.nan_to_num(c.buf[1], 0.0).abs().max())
+    out = run(ctx, typ, c, row_start, q, p["lens"], p["groups"])
+    check(out, ref, tol, typ)
+    mine, least = (float((x.double().cpu() - ref).square().mean().sqrt()) for x in (out, ref.to(q.dtype)))
+    assert mine <= 1.01 * least                             # (some values on a border between two steps go to the other one)

@@ -8,9 +8,10 @@
 //   k_paged_attn     a share of the wide strips per block and of the narrow ones per wave
 //   k_paged_join     one wave per (row, head): its pieces' partial results
 // Single tokens are bound by reading the cache once; groups of many rows and prompt chunks by the products and the exponentials.
-// Measured (attention + join): 64 single rows over 2048 shared and 16 to 2048 own keys, 4 key heads of 128: 20.5 + 5.3 us for
-// 60 MB; 256 rows over 16384 shared keys, 8 key heads of 128, 32 query heads: 104 + 9 us for 253 MB and 69 GFLOP at 670 TFLOP/s;
-// 4 prompt chunks of 333 rows behind 1500 shared ones: 40 + 11 us; one row over 700 keys: 10.0 + 3.8 us, of dependent loads.
+// Measured (attention + join): 64 single rows over 2048 shared and 16 to 2048 own keys, 4 key heads of 128: 22.4 + 5.4 us for
+// 60 MB; 256 rows over 16384 shared keys, 8 key heads of 128, 32 query heads: 134 + 9.5 us for 253 MB and 69 GFLOP (103 with the
+// products of the weights' second parts, at 770 TFLOP/s); 4 prompt chunks of 333 rows behind 1500 shared ones: 50 + 11.7 us; one row over
+// 700 keys: 10.0 + 3.6 us, of dependent loads.
 #pragma once
 #include "z2h_common.h"
 #include "z2h_ops_rules.h"
@@ -346,7 +347,7 @@ template <int HD, typename T, typename TC>
 struct AttnWave {
     typedef typename Vec8<TC>::type v8;
     static constexpr int KS = HD / 16, DT = HD / 32, BIAS = __is_same(TC, _Float16) ? 6 : 0;
-    static constexpr bool SPLIT = __is_same(T, float);           // fp32 queries and weights as two f16 each
+    static constexpr bool SPLIT = __is_same(T, float);           // fp32 queries as two f16 each
     v8 q[KS], ql[SPLIT ? KS : 1];
     v16f_t o[DT];
     float m, l, c;                                               // m includes -BIAS: f16 weights up to 2^14, kept to 2^-24
@@ -493,10 +494,11 @@ struct AttnWave {
                 for (int i = 0; i < 16; ++i) o[dt][i] *= w;
         }
         const float mu = m == -__builtin_inff() ? 0.0f : m;
-        // The weights meet the values as numbers of the cache's type, each off by at most half a step (2^-11 of it in f16, 2^-8 in bf16),
-        // independent from key to key: over many keys far less than the output's own rounding, over few about as much. The sum l
-        // has them unrounded. For fp32 results a second f16 carries the rest: 2^-21.
-        v8 p[2 * NT], pl[SPLIT ? 2 * NT : 1];
+        // The weights meet the values as two numbers of the cache's type, the second carrying what the first's rounding leaves: off by 2^-22 of
+        // them in f16, 2^-16 in bf16. One alone (2^-11, 2^-8) errs as much as the output's own rounding, over any number of keys: with
+        // values of mean zero the output shrinks as the error does (1.3 times the rounding's rms in all; with one number 256 rows over 16384
+        // shared keys take 103 us and 4 chunks of 333 rows 40, with two 134 and 50).
+        v8 p[2 * NT], pl[2 * NT];
         float sum = 0.0f;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -505,7 +507,7 @@ struct AttnWave {
                 const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], c, -mu));
                 const TC hi = (TC) w;
                 p[2 * n + (i >> 3)][i & 7] = hi;
-                if constexpr (SPLIT) pl[2 * n + (i >> 3)][i & 7] = (TC) (w - (float) hi);
+                pl[2 * n + (i >> 3)][i & 7] = (TC) (w - (float) hi);
                 sum += w;
             }
         l += sum;
@@ -514,7 +516,7 @@ struct AttnWave {
         products<2 * NT * DT>([&](int i) __attribute__((always_inline)) { return __builtin_bit_cast(v8, values(sv, r0 + 16 * (i / DT), i % DT)); },
                               [&](int i, v8 vf) __attribute__((always_inline)) {
                                   o[i % DT] = mfma32<TC>(vf, p[i / DT], o[i % DT]);
-                                  if constexpr (SPLIT) o[i % DT] = mfma32<TC>(vf, pl[i / DT], o[i % DT]);
+                                  o[i % DT] = mfma32<TC>(vf, pl[i / DT], o[i % DT]);
                               }, [](int) {});
     }
 
