@@ -168,3 +168,17 @@ def test_16_bit_results_have_the_outputs_rounding_only(ctx, typ, shape, qscale):
     check(out, ref, tol, typ)
     mine, least = (float((x.double().cpu() - ref).square().mean().sqrt()) for x in (out, ref.to(q.dtype)))
     assert mine <= 1.01 * least                             # (some values on a border between two steps go to the other one)
+
+
+# ---- no groups: both tables NULL
+def test_no_groups_without_tables(ctx):
+    lens, rows = [40, 300, 17], [1, 3, 0]
+    c, row_start, q = case("f16", lens, rows, 8, 2, 64, 16, seed=31)
+    a = Attn(ctx, c, 8, row_start, lens, (), "f16")
+    d = q.to(DEV)
+    out = torch.zeros_like(d)
+    for _ in range(2):
+        a.ctx.paged_plan(c.pages, 8, a.R, a.row_start.data_ptr(), a.kv_len.data_ptr(), 0, 0, 0, a.ws.data_ptr(), a.ws.numel())
+        a.run(d.view(len(d), -1), out.view(len(d), -1), 0.125)
+        torch.cuda.synchronize()
+        check(out, *reference(c, q.double(), row_start, lens, 0.125, q.dtype), "no groups")

@@ -97,6 +97,17 @@ Z2O_HD int page_of(const int32_t * table, int n_seq, int table_len, int n_pages,
 }
 inline int page_shift_of(int page_rows) { int s = 0; while ((1 << s) < page_rows) ++s; return s; }
 
+// The group that sequence `seq` is in (start [n_group + 1] ascending); -1: none. No groups: `start` is not read.
+Z2O_HD int group_of(const int32_t * start, int n_group, int seq) {
+    if (n_group <= 0) return -1;
+    int lo = -1, hi = n_group + 1;                                       // start[lo] <= seq < start[hi]
+    while (hi - lo > 1) {
+        const int m = (lo + hi) >> 1;
+        if (start[m] <= seq) lo = m; else hi = m;
+    }
+    return lo < n_group ? lo : -1;
+}
+
 // ---- attention: how the work is cut
 // A span is a run of query rows over a run of cache rows: a group's rows over its shared prefix, a sequence's rows over the
 // rest. Its rows are cut into tiles of at most TILE_RH row-heads of one key head. A tile of more than NARROW_RH row-heads is

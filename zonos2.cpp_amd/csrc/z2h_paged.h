@@ -50,16 +50,6 @@ struct PlanArgs {
 
 __device__ __forceinline__ int tile_place(int i, bool wide, int max_tiles) { return wide ? i : max_tiles - 1 - i; }
 
-// the last index i of [0, n) with start[i] <= x (start ascending; -1: none)
-__device__ __forceinline__ int last_at_or_before(const int32_t * start, int n, int x) {
-    int lo = -1, hi = n;
-    while (hi - lo > 1) {
-        const int m = (lo + hi) >> 1;
-        if (start[m] <= x) lo = m; else hi = m;
-    }
-    return lo;
-}
-
 constexpr int PLAN_T = 1024;
 // sum of v over the lower threads of the block, and the block's total
 __device__ __forceinline__ int block_scan(int v, int * s_wave, int & total) {
@@ -136,7 +126,7 @@ __global__ void __launch_bounds__(PLAN_T) k_paged_plan(PlanArgs a) {
     if (tid == 0) s_total = 0;
     auto start_of = [&](int s) { return min(max(a.row_start[s], 0), a.n_rows); };
     auto len_of = [&](int s) { return min(max(a.kv_len[s], 0), a.cap); };
-    auto group_of = [&](int g) { return min(max(a.group_start[g], 0), a.n_seq); };
+    auto first_of = [&](int g) { return min(max(a.group_start[g], 0), a.n_seq); };
     // ---- tiles of every span: the groups' prefixes, then the sequences' own keys. A span's tiles have tr rows each but for the last.
     int n_tiles[2] = {0, 0};                                     // narrow, wide
     unsigned long long units = 0;
@@ -145,7 +135,7 @@ __global__ void __launch_bounds__(PLAN_T) k_paged_plan(PlanArgs a) {
         int r0 = 0, r1 = 0, key0 = 0, key1 = 0, seq = 0, len = 0;
         const bool own = x >= a.n_group;
         if (x < a.n_group) {
-            const int s0 = group_of(x), s1 = group_of(x + 1);
+            const int s0 = first_of(x), s1 = first_of(x + 1);
             if (s0 < s1) {
                 r0 = start_of(s0); r1 = start_of(s1); seq = s0;
                 key1 = max(0, min(a.prefix_len[x], len_of(s0)));
@@ -153,8 +143,8 @@ __global__ void __launch_bounds__(PLAN_T) k_paged_plan(PlanArgs a) {
         } else if (x < a.n_group + a.n_seq) {
             seq = x - a.n_group;
             r0 = start_of(seq); r1 = start_of(seq + 1); len = key1 = len_of(seq);
-            const int g = last_at_or_before(a.group_start, a.n_group + 1, seq);
-            if (g >= 0 && g < a.n_group) key0 = max(0, min(a.prefix_len[g], len_of(group_of(g))));
+            const int g = z2o::group_of(a.group_start, a.n_group, seq);
+            if (g >= 0) key0 = max(0, min(a.prefix_len[g], len_of(first_of(g))));
         }
         const bool some = r1 > r0 && (own || key1 > 0);
         const int n = some ? (r1 - r0 + tr - 1) / tr : 0, last = some ? r1 - r0 - (n - 1) * tr : 0;
