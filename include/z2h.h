@@ -315,7 +315,7 @@ int z2h_paged_append(z2h_ctx * ctx, const z2h_pages * pages, const z2h_rope * ro
  * d_group_start[g + 1]) (d_group_start [n_group + 1] ascending), whose first d_prefix_len[g] cache rows hold the same
  * values: they are read through the group's first sequence, and only as many as it has. Sequences outside every group
  * share nothing; n_group may be 0. A page entry outside [0, n_pages) reads as page 0; lengths are clamped to the
- * table.
+ * table. Row or group tables that are not ascending make no plan: z2h_paged_attn then leaves d_out as it was.
  *
  * z2h_paged_attn: d_out = softmax(scale q k^T) v for d_q [n_rows][n_head][head_dim], rows q_stride / out_stride apart,
  * n_head a multiple of n_head_kv, at most 64 query heads per key head; query head h reads key head h / (n_head /

@@ -182,3 +182,25 @@ def test_no_groups_without_tables(ctx):
         a.run(d.view(len(d), -1), out.view(len(d), -1), 0.125)
         torch.cuda.synchronize()
         check(out, *reference(c, q.double(), row_start, lens, 0.125, q.dtype), "no groups")
+
+
+# ---- tables that go back would put a row into several spans: no plan, and the output stays as it was
+def test_tables_that_are_not_ascending_make_no_plan(ctx):
+    lens, rows = [40, 60, 17, 90], [2, 3, 1, 2]
+    c, row_start, q = case("f16", lens, rows, 8, 2, 64, 16, seed=32)
+    d = q.to(DEV)
+    groups = [(0, 2, 32), (2, 4, 16)]
+    for field, bad in (("row_start", [0, 5, 2, 6, 8]), ("row_start", [0, 2, 5, 100, 8]), ("group_start", [0, 3, 2]), ("group_start", [2, 0, 4])):
+        a = Attn(ctx, c, 8, row_start, lens, groups, "f16")
+        good = getattr(a, field).clone()
+        setattr(a, field, torch.tensor(bad, dtype=torch.int32, device=DEV))
+        out = torch.full_like(d, 7.0)
+        a.plan()
+        a.run(d.view(len(d), -1), out.view(len(d), -1), 0.125)
+        torch.cuda.synchronize()
+        assert bool((out == 7).all()), (field, bad)
+        setattr(a, field, good)                             # the same workspace, planned again
+        a.plan()
+        a.run(d.view(len(d), -1), out.view(len(d), -1), 0.125)
+        torch.cuda.synchronize()
+        assert bool(torch.isfinite(out).all()) and not bool((out == 7).any())

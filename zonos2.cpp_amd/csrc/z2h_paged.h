@@ -115,27 +115,31 @@ struct PlanKind {
 };
 
 // One block: a chain of scans and searches, bound by its barriers and dependent loads; 11 us for 64 sequences, 16 us for 256, once
-// for all layers of a step. Everything is clamped to the tables' sizes, so that whatever the lengths say no entry leads outside the buffers.
+// for all layers of a step. Everything is clamped to the tables' sizes, so that whatever the lengths say no entry leads outside the buffers; tables
+// that are not ascending make no plan.
 __global__ void __launch_bounds__(PLAN_T) k_paged_plan(PlanArgs a) {
     __shared__ int s_wave[PLAN_T / 64];
     __shared__ unsigned long long s_total;
+    __shared__ int s_overlap;
     constexpr int LDS_TILES = 8192;
     __shared__ int s_begin[LDS_TILES];
     const int tid = threadIdx.x, group = a.n_head / a.nkv, tr = z2o::tile_rows(group);
     for (int t = tid; t < a.n_rows; t += PLAN_T) a.rows[t] = PlanRow{0, -1, 0, -1, 0, {0, 0, 0}};
-    if (tid == 0) s_total = 0;
+    if (tid == 0) { s_total = 0; s_overlap = 0; }
     auto start_of = [&](int s) { return min(max(a.row_start[s], 0), a.n_rows); };
     auto len_of = [&](int s) { return min(max(a.kv_len[s], 0), a.cap); };
     auto first_of = [&](int g) { return min(max(a.group_start[g], 0), a.n_seq); };
     // ---- tiles of every span: the groups' prefixes, then the sequences' own keys. A span's tiles have tr rows each but for the last.
     int n_tiles[2] = {0, 0};                                     // narrow, wide
     unsigned long long units = 0;
+    bool overlap = false;                                        // a table that goes back: a row could be in several spans of a kind
     for (int base = 0; base < a.n_group + a.n_seq; base += PLAN_T) {
         const int x = base + tid;
         int r0 = 0, r1 = 0, key0 = 0, key1 = 0, seq = 0, len = 0;
         const bool own = x >= a.n_group;
         if (x < a.n_group) {
             const int s0 = first_of(x), s1 = first_of(x + 1);
+            overlap |= a.group_start[x + 1] < a.group_start[x];
             if (s0 < s1) {
                 r0 = start_of(s0); r1 = start_of(s1); seq = s0;
                 key1 = max(0, min(a.prefix_len[x], len_of(s0)));
@@ -143,6 +147,7 @@ __global__ void __launch_bounds__(PLAN_T) k_paged_plan(PlanArgs a) {
         } else if (x < a.n_group + a.n_seq) {
             seq = x - a.n_group;
             r0 = start_of(seq); r1 = start_of(seq + 1); len = key1 = len_of(seq);
+            overlap |= a.row_start[seq + 1] < a.row_start[seq];
             const int g = z2o::group_of(a.group_start, a.n_group, seq);
             if (g >= 0) key0 = max(0, min(a.prefix_len[g], len_of(first_of(g))));
         }
@@ -166,7 +171,12 @@ __global__ void __launch_bounds__(PLAN_T) k_paged_plan(PlanArgs a) {
         }
     }
     atomicAdd(&s_total, units);                                  // integers: the order does not matter
+    if (overlap) s_overlap = 1;
     __syncthreads();
+    if (s_overlap) {                                             // places and sizes below count on a row's two tiles at most
+        if (tid == 0) a.head[PH_MAGIC] = 0;
+        return;
+    }
     int shift = 0, n_parts = 0, n_wide_shares = 0;
     while (s_total >> shift >= 1ull << 28) ++shift;
 #pragma unroll 1
