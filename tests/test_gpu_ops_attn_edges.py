@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 import torch
 
+from ops_cut_cases import CASES
 from ops_helpers import DEV, TYPES, Attn, Cache, check, context, half_step
 from zonos2_amd import z2h
 
@@ -150,7 +151,11 @@ def test_infinities_with_large_queries_and_a_negative_scale(ctx, typ):
 # A weight is carried as two numbers of the cache's type: off by half a step of half a step, 2^-22 of it in f16 and 2^-16 in bf16. In f16 the second
 # part is below the normal range where the weight is below 2^-3, and then off by 2^-25 at most; the largest weight is 2^6 or more, so n keys add
 # n 2^-31 of the largest value.
-TWO = {torch.float16: 2.0 ** -22, torch.bfloat16: 2.0 ** -16}
+TWO = {torch.float32: 2.0 ** -21, torch.float16: 2.0 ** -22, torch.bfloat16: 2.0 ** -16}
+
+
+def below_normal(c, q, lens):
+    return 0.0 if q.dtype == torch.bfloat16 else max(lens) * 2.0 ** -31 * float(torch.nan_to_num(c.buf[1], 0.0).abs().max())
 
 
 @pytest.mark.parametrize("typ", ["f16", "bf16"])
@@ -162,8 +167,7 @@ def test_16_bit_results_have_the_outputs_rounding_only(ctx, typ, shape, qscale):
     print(f"rounding {typ} {shape} {qscale}", flush=True)
     c, row_start, q = case(typ, **p, seed=21, qscale=qscale)
     ref, tol = reference(c, q.double(), row_start, p["lens"], 0.125, q.dtype, up=TWO[q.dtype])
-    if typ == "f16":
-        tol += max(p["lens"]) * 2.0 ** -31 * float(torch.nan_to_num(c.buf[1], 0.0).abs().max())
+    tol += below_normal(c, q, p["lens"])
     out = run(ctx, typ, c, row_start, q, p["lens"], p["groups"])
     check(out, ref, tol, typ)
     mine, least = (float((x.double().cpu() - ref).square().mean().sqrt()) for x in (out, ref.to(q.dtype)))
@@ -204,3 +208,62 @@ def test_tables_that_are_not_ascending_make_no_plan(ctx):
         a.run(d.view(len(d), -1), out.view(len(d), -1), 0.125)
         torch.cuda.synchronize()
         assert bool(torch.isfinite(out).all()) and not bool((out == 7).any())
+
+
+# ---- calls that small ones do not stand for (what each reaches is checked on the CPU)
+def _cut_case(name):
+    p = {k: v for k, v in CASES[name].items() if k not in ("name", "reaches")}
+    print(f"cut: {name}", flush=True)
+    return p, case(**p, seed=41)
+
+
+@pytest.mark.parametrize("name", list(CASES))
+def test_long_and_many(ctx, name):
+    p, (c, row_start, q) = _cut_case(name)
+    scale = float(np.float32(p["hd"] ** -0.5))
+    ref, tol = reference(c, q.double(), row_start, p["lens"], scale, q.dtype, up=TWO[q.dtype])
+    check(run(ctx, p["typ"], c, row_start, q, p["lens"], p["groups"], scale), ref, tol + below_normal(c, q, p["lens"]), name)
+
+
+@pytest.mark.parametrize("name", [n for n in CASES if n.startswith("long walks") or "in a row" in n])
+def test_long_walks_repeat_bit_for_bit(ctx, name):
+    """Keys and values pass through LDS in many steps, which waves that have nothing to multiply help to fill: no answer depends on who
+    came first."""
+    p, (c, row_start, q) = _cut_case(name)
+    a = Attn(ctx, c, p["heads"], row_start, p["lens"], p["groups"], p["typ"])
+    d = q.to(DEV)
+    outs = [torch.empty_like(d) for _ in range(30)]
+    a.plan()
+    for o in outs:
+        a.run(d.view(len(d), -1), o.view(len(d), -1), p["hd"] ** -0.5)
+    torch.cuda.synchronize()
+    assert bool(torch.isfinite(outs[0]).all()) and all(torch.equal(o, outs[0]) for o in outs)
+
+
+def test_a_billion_rows_per_sequence(ctx):
+    """The longest sequences that a table may describe, over two pages again and again: lengths near 2^30, and more steps in the call than are
+    counted one by one. A piece adds up 2^17 steps one after the other, their sums by 2^17 roundings of at most 2^-24 of what has come together (half
+    of it on average), the values by four times as many: 2^-8 and 2^-6 of a result whose values are all positive."""
+    P, hd, S = 4096, 32, 8
+    g = torch.Generator().manual_seed(5)
+    c = Cache([P, P], 1, hd, P, torch.float16, 6)
+    pages = [int(c.table_host[s, 0]) for s in range(2)]
+    for i, page in enumerate(pages):
+        c.buf[1][page] = (torch.rand(P * hd, generator=g) + 1 + 2 * i).half()
+    per = (1 << 30) // P
+    turn = [(s + 1) * per // 10 for s in range(S)]          # the page from which on a sequence has the second one
+    c.table_host = np.where(np.arange(per)[None] < np.array(turn)[:, None], pages[0], pages[1]).astype(np.int32)
+    c.upload()
+    lens = [(1 << 30) - 37 * s for s in range(S)]
+    q = torch.randn((S, 1, hd), generator=g).half()
+    out = run(ctx, "f16", c, np.arange(S + 1), q, lens)
+    k, v = ([b[p].view(P, hd).double() for p in pages] for b in c.buf)
+    for s in range(S):
+        w = [torch.exp(0.125 * (x @ q[s, 0].double())) for x in k]
+        last = lens[s] - (per - 1) * P                      # rows of the last page
+        some = [torch.full((P,), float(turn[s]), dtype=torch.float64), torch.full((P,), float(per - 1 - turn[s]), dtype=torch.float64)]
+        some[1][:last] += 1
+        ref = sum((n * x) @ y for n, x, y in zip(some, w, v)) / sum((n * x).sum() for n, x in zip(some, w))
+        err = ((out[s, 0].double().cpu() - ref).abs() / ref).max()
+        print(f"sequence {s}: off by {float(err):.2e}", flush=True)
+        assert float(err) <= 2.0 ** -8 + 2.0 ** -6 + 2.0 ** -11
