@@ -3,6 +3,7 @@
 #include "../../zonos2.cpp_amd/csrc/z2h_ops_rules.h"
 #include <cstdio>
 #include <cstdlib>
+#include <initializer_list>
 
 #define EXPECT(cond) do { if (!(cond)) { std::printf("line %d: %s\n", __LINE__, #cond); std::exit(1); } } while (0)
 
@@ -15,7 +16,17 @@ static void groups() {
     EXPECT(z2o::group_of(some, 4, 7) == -1);
 }
 
+static void launches() {
+    for (int threads : {64, 256, 1024}) {
+        EXPECT(z2o::launch_blocks(threads) >= 1 << 20 && z2o::launch_blocks(threads) * threads < 1ll << 32);
+        EXPECT(z2o::launch_blocks(threads) <= 0x7fffffff);
+    }
+    // the largest calls' counts: 32-bit numbers of their own
+    EXPECT(4 * (z2o::MAX_ROW_HEADS / 4) <= 0x7fffffff - 4 * 256 && z2o::MAX_VERIFY_BLOCKS <= 0x7fffffff);
+}
+
 int main() {
+    launches();
     groups();
     std::puts("ok");
 }

@@ -38,7 +38,7 @@ int launched(z2h_ctx * ctx) {
 #define ON_DEVICE OnDevice on_(ctx); if (!on_.ok) return z2h_ctx_fail(ctx, Z2H_EDEVICE, "hipSetDevice failed")
 
 template <typename T, typename TC>
-void rope_launch(const RopeArgs & a, int n_rows, bool halves, hipStream_t stream) {
+void rope_launch(RopeArgs & a, int n_rows, bool halves, hipStream_t stream) {
     // 16-byte accesses where every row, head and unit of pairs allows them
     constexpr int N = 16 / (int) sizeof(T);
     const auto al = [](const void * p, int64_t stride) { return !p || ((uintptr_t) p % 16 == 0 && stride * (int64_t) sizeof(T) % 16 == 0); };
@@ -47,14 +47,16 @@ void rope_launch(const RopeArgs & a, int n_rows, bool halves, hipStream_t stream
     // few rows: their heads over several blocks, so that a row is one round of loads
     const int np = !wide ? 1 : halves ? N : N / 2, units = a.n_dims / 2 / np + (a.hd - a.n_dims) / (wide ? N : 1);
     const int rounds = (a.nh + a.nkv + 256 / units - 1) / (256 / units);
-    const dim3 grid(n_rows, std::min(rounds, std::max(1, 1024 / n_rows)));
-    if (halves && wide) hipLaunchKernelGGL((k_rope_append<T, TC, true, true>), grid, dim3(256), 0, stream, a);
-    else if (halves) hipLaunchKernelGGL((k_rope_append<T, TC, true, false>), grid, dim3(256), 0, stream, a);
-    else if (wide) hipLaunchKernelGGL((k_rope_append<T, TC, false, true>), grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((k_rope_append<T, TC, false, false>), grid, dim3(256), 0, stream, a);
+    for (a.row0 = 0; a.row0 < n_rows; a.row0 += z2o::launch_blocks(256)) {
+        const dim3 grid(std::min<int64_t>(n_rows - a.row0, z2o::launch_blocks(256)), std::min(rounds, std::max(1, 1024 / n_rows)));
+        if (halves && wide) hipLaunchKernelGGL((k_rope_append<T, TC, true, true>), grid, dim3(256), 0, stream, a);
+        else if (halves) hipLaunchKernelGGL((k_rope_append<T, TC, true, false>), grid, dim3(256), 0, stream, a);
+        else if (wide) hipLaunchKernelGGL((k_rope_append<T, TC, false, true>), grid, dim3(256), 0, stream, a);
+        else hipLaunchKernelGGL((k_rope_append<T, TC, false, false>), grid, dim3(256), 0, stream, a);
+    }
 }
 template <typename T>
-void rope_launch(const RopeArgs & a, int n_rows, bool halves, int cache, hipStream_t stream) {
+void rope_launch(RopeArgs & a, int n_rows, bool halves, int cache, hipStream_t stream) {
     if (cache == Z2H_BF16) rope_launch<T, __bf16>(a, n_rows, halves, stream);
     else rope_launch<T, _Float16>(a, n_rows, halves, stream);
 }
@@ -86,15 +88,17 @@ int compute_units(int device) {
 int attn_blocks(int n_cu) { return 2 * n_cu; }
 
 template <int HD, typename T, typename TC>
-void attn_launch(const PagedArgs & a, int blocks, hipStream_t stream) {
+void attn_launch(PagedArgs & a, int blocks, hipStream_t stream) {
     hipLaunchKernelGGL((k_paged_attn<HD, T, TC>), dim3(blocks), dim3(256), 0, stream, a);
     // a block per (row, head) while the device holds all of them at once: 1024 of 24 partial results each 7.0 us against 5.3, 8192 of 10
     // each 9.4 against 14.9
     if (a.n_rows * a.n_head <= 4 * blocks) hipLaunchKernelGGL((k_paged_join<HD, T, true>), dim3(a.n_rows * a.n_head), dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((k_paged_join<HD, T, false>), dim3((a.n_rows * a.n_head + 3) / 4), dim3(256), 0, stream, a);
+    else
+        for (int64_t n = ((int64_t) a.n_rows * a.n_head + 3) / 4; a.join0 < n; a.join0 += z2o::launch_blocks(256))
+            hipLaunchKernelGGL((k_paged_join<HD, T, false>), dim3(std::min(n - a.join0, z2o::launch_blocks(256))), dim3(256), 0, stream, a);
 }
 template <int HD>
-void attn_launch(const PagedArgs & a, int type, int blocks, hipStream_t stream) {
+void attn_launch(PagedArgs & a, int type, int blocks, hipStream_t stream) {
     switch (type) {
         case Z2H_F32: attn_launch<HD, float, _Float16>(a, blocks, stream); break;
         case Z2H_F16: attn_launch<HD, _Float16, _Float16>(a, blocks, stream); break;
@@ -251,8 +255,16 @@ int z2h_verify(z2h_ctx * ctx, int n_seq, int n_draft_max, int n_codebooks, int v
     const int draws = n_seq * n_codebooks;
     ON_DEVICE;
     const int rows = n_seq * (n_draft_max + 1) * n_codebooks;
-    if (d_temperature && vocab <= z2o::VERIFY_SHORT) hipLaunchKernelGGL(k_verify_stats<256>, dim3(rows), dim3(256), 0, st, a);
-    else if (d_temperature) hipLaunchKernelGGL(k_verify_stats<1024>, dim3(rows * a.n_chunk), dim3(1024), 0, st, a);
+    if (d_temperature) {
+        const int threads = vocab <= z2o::VERIFY_SHORT ? 256 : 1024;
+        const int64_t blocks = (int64_t) rows * a.n_chunk;       // (a row of at most VERIFY_SHORT logits is one chunk)
+        for (; a.block0 < blocks; a.block0 += z2o::launch_blocks(threads)) {
+            const dim3 grid(std::min(blocks - a.block0, z2o::launch_blocks(threads)));
+            if (threads == 256) hipLaunchKernelGGL(k_verify_stats<256>, grid, dim3(256), 0, st, a);
+            else hipLaunchKernelGGL(k_verify_stats<1024>, grid, dim3(1024), 0, st, a);
+        }
+        if (int rc = launched(ctx)) return rc;                   // (no draws from statistics that nobody formed)
+    }
     if (vocab <= z2o::VERIFY_ONE) hipLaunchKernelGGL(k_verify, dim3(draws), dim3(256), 0, st, a);
     else {
         // shares of 1024 codes (a round of the block's loads) or more, about 512 blocks in all

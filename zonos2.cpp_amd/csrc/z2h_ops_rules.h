@@ -18,6 +18,9 @@ constexpr int64_t MAX_ROW_HEADS = 1ll << 26;       // rows x heads of one attent
 constexpr int MAX_VOCAB = 1 << 20;
 constexpr int MAX_ROPE_DIMS = 128;
 
+// Blocks of `threads` that one launch may have (its threads are counted in 32 bits); calls of more launch several times.
+constexpr int64_t launch_blocks(int threads) { return (1ll << 31) / threads; }
+
 // ---- checks: nullptr, or what is wrong
 inline const char * check_rope(const z2h_rope * r, int head_dim) {
     if (!r) return "null rope";

@@ -292,6 +292,7 @@ struct PagedArgs {
     const PlanStrip * strips;
     const PlanShare * shares;
     int max_tiles, blocks;
+    int64_t join0;                                               // first block of this launch of k_paged_join
     float2 * part_ml;
     float * part_o;
 };
@@ -908,7 +909,7 @@ template <int HD, typename T, bool SHARED>
 __global__ void __launch_bounds__(256) k_paged_join(PagedArgs a) {
     constexpr int STEP = SHARED ? 4 : 1;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
-    const int id = SHARED ? (int) blockIdx.x : 4 * (int) blockIdx.x + wave, from = SHARED ? wave : 0;
+    const int id = SHARED ? (int) blockIdx.x : 4 * (int) (a.join0 + blockIdx.x) + wave, from = SHARED ? wave : 0;
     if (id >= a.n_rows * a.n_head) return;
     const int row = id / a.n_head, head = id % a.n_head, group = a.n_head / a.nkv, g = head / group;
     const PlanRow r = uniform_copy(a.rows + row);

@@ -36,6 +36,7 @@ struct RopeArgs {
     double turn[z2o::MAX_ROPE_DIMS / 2];           // turns per position of each pair
     float mscale;
     int n_dims, hd, nh, nkv;
+    int64_t row0;                                  // of this launch
     const int32_t * seq, * pos;                    // seq NULL: rows of queries only
     const void * q, * k, * v;
     void * q_out, * kc, * vc;
@@ -70,7 +71,8 @@ template <typename T, bool WIDE> struct RopeUnit { static constexpr int N = WIDE
 template <typename T, typename TC, bool HALVES, bool WIDE>
 __global__ void __launch_bounds__(256) k_rope_append(RopeArgs a) {
     constexpr int N = RopeUnit<T, WIDE>::N, NP = HALVES ? N : WIDE ? N / 2 : 1;      // values behind the pairs; pairs per unit
-    const int t = blockIdx.x, tid = threadIdx.x;
+    const int64_t t = a.row0 + blockIdx.x;
+    const int tid = threadIdx.x;
     const int seq = a.seq ? a.seq[t] : 0, pos = a.pos[t];
     if (a.seq && (seq < 0 || seq >= a.n_seq)) return;
     const int half = a.n_dims / 2, up = half / NP, U = up + (a.hd - a.n_dims) / N, HL = 256 / U;

@@ -27,6 +27,7 @@ static_assert(sizeof(VerifyDraw) == z2o::VERIFY_DRAW_BYTES, "workspace layout");
 
 struct VerifyArgs {
     int n_seq, K, C, V, n_chunk, n_share;
+    int64_t block0;                                              // of this launch of k_verify_stats
     const int32_t * draft, * n_draft;
     const float * target, * temperature, * draft_probs;
     const double * u_accept, * u_draw;
@@ -83,8 +84,9 @@ __global__ void __launch_bounds__(NT) k_verify_stats(VerifyArgs a) {
     constexpr int NW = NT / 64, N = z2o::VERIFY_PER_THREAD;
     __shared__ double s_m[NW], s_z[NW];
     __shared__ int s_i[NW];
-    const int64_t row = blockIdx.x / a.n_chunk;
-    const int chunk = blockIdx.x % a.n_chunk;
+    const int id = (int) (a.block0 + blockIdx.x);
+    const int64_t row = id / a.n_chunk;
+    const int chunk = id % a.n_chunk;
     const int s = (int) (row / ((int64_t) (a.K + 1) * a.C)), k = (int) (row / a.C % (a.K + 1));
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c0 = chunk * NT * N;
     if (a.n_draft && k > min(max(a.n_draft[s], 0), a.K)) return;           // behind the last draft's successor
