@@ -2132,8 +2132,8 @@ static int paged_pass(z2h_ctx * ctx, const z2h_pages * pages, int64_t layer_stri
     if (const char * e = check_paged(ctx, pages)) return seterr(ctx, Z2H_EINVAL, e);
     if (n_rows <= 0 || n_rows > ctx->Tmax) return seterr(ctx, Z2H_EINVAL, "n_rows out of range");
     if (n_out < 0 || n_out > ctx->Tmax) return seterr(ctx, Z2H_EINVAL, "n_out out of range");
-    const int64_t ws_need = z2h_paged_ws_bytes(ctx, pages, hp.n_head, n_rows, n_group);        // (checks the pages)
-    if (!ws_need) return Z2H_EINVAL;
+    int64_t ws_need;
+    if (int rc = z2h_paged_ws(ctx, pages, hp.n_head, n_rows, n_group, &ws_need)) return rc;   // (checks the pages)
     const int64_t tables = paged_tables_bytes(*pages, n_group);
     if (!d_ws || (uintptr_t) d_ws % 256 || ws_bytes < ws_need + tables) return seterr(ctx, Z2H_EINVAL, "workspace misaligned or too small");
     if (layer_stride % 8 || layer_stride < pages->n_pages * pages->page_stride || layer_stride > ((int64_t) 1 << 40))

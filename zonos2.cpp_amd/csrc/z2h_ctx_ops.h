@@ -7,6 +7,9 @@
 Z2H_LOCAL int z2h_ctx_fail(z2h_ctx * ctx, int code, const char * what) noexcept;   // sets the error string, returns code
 Z2H_LOCAL int z2h_ctx_device(const z2h_ctx * ctx) noexcept;
 
+// z2h_paged_ws_bytes with the reason of a refusal
+Z2H_LOCAL int z2h_paged_ws(z2h_ctx * ctx, const z2h_pages * pages, int n_head, int n_rows, int n_group, int64_t * bytes);
+
 // One layer's attention of z2h_step_paged on the context's fused projection rows qkvg [n_rows][R] (query heads, key heads, value
 // heads, a gate per query head): norms, append, attention, gates; out is [n_rows][n_head head_dim].
 struct Z2hPagedPass {

@@ -161,11 +161,8 @@ int z2h_paged_append(z2h_ctx * ctx, const z2h_pages * pages, const z2h_rope * ro
 }
 
 int64_t z2h_paged_ws_bytes(z2h_ctx * ctx, const z2h_pages * pages, int n_head, int n_rows, int n_group) {
-    if (!ctx) return 0;
-    if (const char * e = z2o::check_attn(pages, n_head, n_rows, n_group)) { z2h_ctx_fail(ctx, Z2H_EINVAL, e); return 0; }
-    const int n_cu = compute_units(z2h_ctx_device(ctx));
-    if (!n_cu) { z2h_ctx_fail(ctx, Z2H_EDEVICE, "compute-unit count query failed"); return 0; }
-    return z2o::attn_ws(*pages, n_head, n_rows, n_group, attn_blocks(n_cu)).bytes;
+    int64_t bytes;
+    return ctx && z2h_paged_ws(ctx, pages, n_head, n_rows, n_group, &bytes) == Z2H_OK ? bytes : 0;
 }
 
 int z2h_paged_plan(z2h_ctx * ctx, const z2h_pages * pages, int n_head, int n_rows, const int32_t * d_row_start,
@@ -276,6 +273,14 @@ int z2h_verify(z2h_ctx * ctx, int n_seq, int n_draft_max, int n_codebooks, int v
 }
 
 } // extern "C"
+
+int z2h_paged_ws(z2h_ctx * ctx, const z2h_pages * pages, int n_head, int n_rows, int n_group, int64_t * bytes) {
+    CHECK(z2o::check_attn(pages, n_head, n_rows, n_group));
+    const int n_cu = compute_units(z2h_ctx_device(ctx));
+    if (!n_cu) return z2h_ctx_fail(ctx, Z2H_EDEVICE, "compute-unit count query failed");
+    *bytes = z2o::attn_ws(*pages, n_head, n_rows, n_group, attn_blocks(n_cu)).bytes;
+    return Z2H_OK;
+}
 
 int z2h_paged_layer(z2h_ctx * ctx, const Z2hPagedPass & s, int layer, float * qkvg, const float * temp, float * out, void * stream) {
     z2h_pages pages = s.pages;
