@@ -2167,7 +2167,8 @@ static int paged_pass(z2h_ctx * ctx, const z2h_pages * pages, int64_t layer_stri
     }
     for (int i = 0; i < n_out; ++i)
         if (out_rows[i] < 0 || out_rows[i] >= n_rows) return seterr(ctx, Z2H_EINVAL, "out_rows entry out of range");
-    HIPX(hipSetDevice(ctx->device));
+    DeviceScope on(ctx->device);                                     // the caller's current device comes back on return
+    if (!on.ok) return seterr(ctx, Z2H_EDEVICE, "hipSetDevice failed");
     ctx->resident_T = ctx->resident_last = 0;
     const PassInputs h = pass_inputs(ctx->h_pin, n_rows, W), d = pass_inputs(ctx->d_slot, n_rows, W);
     for (int s = 0; s < S; ++s)
