@@ -252,7 +252,8 @@ int z2h_step_resident(z2h_ctx * ctx, int n_active);
  * runs the model's layers over them. The operators take a context for its device and its error string only: no tensor,
  * no weights and no z2h_finalize are needed, nothing is allocated, nothing synchronizes, and every call may be captured
  * into a HIP graph. All tensors are on the context's device. Work is enqueued on `stream` (a hipStream_t, NULL = the null stream); the
- * caller's current device is the same on return. Strides are in elements.
+ * caller's current device is the same on return. Strides are in elements. No rows (no sequences to verify): nothing is done, and
+ * their tensors may be NULL.
  *
  * Tables of lengths, positions and pages are read on the device and are not checked on the host: an entry out of range
  * never leads outside the buffers described to the call (each function says what it does then). */

@@ -25,7 +25,13 @@ static void launches() {
     EXPECT(4 * (z2o::MAX_ROW_HEADS / 4) <= 0x7fffffff - 4 * 256 && z2o::MAX_VERIFY_BLOCKS <= 0x7fffffff);
 }
 
+static void no_rows() {
+    EXPECT(!z2o::check_rows(nullptr, 128, 2, 64, Z2H_F16, 0) && z2o::check_rows(nullptr, 128, 2, 64, Z2H_F16, 1));
+    EXPECT(z2o::check_rows(nullptr, 127, 2, 64, Z2H_F16, 0) && z2o::check_rows(nullptr, 128, 2, 64, Z2H_Q8_0, 0));
+}
+
 int main() {
+    no_rows();
     launches();
     groups();
     std::puts("ok");

@@ -267,3 +267,24 @@ def test_a_billion_rows_per_sequence(ctx):
         err = ((out[s, 0].double().cpu() - ref).abs() / ref).max()
         print(f"sequence {s}: off by {float(err):.2e}", flush=True)
         assert float(err) <= 2.0 ** -8 + 2.0 ** -6 + 2.0 ** -11
+
+
+# ---- no rows: tensors of no elements have no address
+def test_no_rows_without_tensors(ctx):
+    c, row_start, q = case("f16", [20, 30], [0, 0], 4, 2, 64, 16, seed=33)
+    old = [b.clone() for b in c.dev]
+    rope = z2h.Rope(n_dims=64)
+    ctx.rope_rows(rope, 0, 4, 64, z2h.F16, 0, 256, 0, 256, 0)
+    ctx.paged_append(c.pages, rope, 0, 0, 0, z2h.F16, 0, 128, 0, 128, 4, 0, 256, 0, 256)
+    a = Attn(ctx, c, 4, row_start, [20, 30], (), "f16")
+    empty = torch.empty((0, 256), dtype=torch.float16, device=DEV)
+    assert empty.data_ptr() == 0
+    a.plan()
+    a.run(empty, empty, 0.125)
+    ctx.verify(0, 2, 1, 10, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+    torch.cuda.synchronize()
+    assert all(torch.equal(x.view(torch.int16), y.view(torch.int16)) for x, y in zip(old, c.dev))
+    for call in (lambda: ctx.rope_rows(rope, 0, 0, 64, z2h.F16, 0, 256, 0, 256, 0), lambda: ctx.rope_rows(rope, 0, 4, 64, z2h.F16, 0, 255, 0, 256, 0),
+                 lambda: ctx.verify(0, 2, 1, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)):
+        with pytest.raises(z2h.Z2HError):
+            call()

@@ -120,11 +120,11 @@ int z2h_rope_rows(z2h_ctx * ctx, const z2h_rope * rope, int n_rows, int n_head, 
     if (!ctx) return Z2H_EINVAL;
     CHECK(z2o::check_rope(rope, head_dim));
     REQUIRE(n_rows >= 0 && n_head > 0 && n_head <= 65536, "rope: row or head count out of range");
-    CHECK(z2o::check_rows(d_x, x_stride, n_head, head_dim, type));
-    CHECK(z2o::check_rows(d_out, out_stride, n_head, head_dim, type));
+    CHECK(z2o::check_rows(d_x, x_stride, n_head, head_dim, type, n_rows));
+    CHECK(z2o::check_rows(d_out, out_stride, n_head, head_dim, type, n_rows));
+    if (n_rows == 0) return Z2H_OK;
     REQUIRE(d_x != d_out || x_stride == out_stride, "rope: in place with different strides");
     REQUIRE(d_pos, "null positions");
-    if (n_rows == 0) return Z2H_OK;
     RopeArgs a{};
     a.hd = head_dim; a.nh = n_head;
     a.pos = d_pos;
@@ -139,16 +139,16 @@ int z2h_paged_append(z2h_ctx * ctx, const z2h_pages * pages, const z2h_rope * ro
     CHECK(z2o::check_pages(pages));
     CHECK(z2o::check_rope(rope, pages->head_dim));
     REQUIRE(n_rows >= 0, "append: n_rows out of range");
+    CHECK(z2o::check_rows(d_k, k_stride, pages->n_head_kv, pages->head_dim, type, n_rows));
+    CHECK(z2o::check_rows(d_v, v_stride, pages->n_head_kv, pages->head_dim, type, n_rows));
+    if (n_rows == 0) return Z2H_OK;
     REQUIRE(d_seq && d_pos, "append: null sequences or positions");
-    CHECK(z2o::check_rows(d_k, k_stride, pages->n_head_kv, pages->head_dim, type));
-    CHECK(z2o::check_rows(d_v, v_stride, pages->n_head_kv, pages->head_dim, type));
     if (d_q) {
         REQUIRE(n_head > 0 && n_head <= 65536, "append: n_head out of range");
         CHECK(z2o::check_rows(d_q, q_stride, n_head, pages->head_dim, type));
         CHECK(z2o::check_rows(d_q_out, q_out_stride, n_head, pages->head_dim, type));
         REQUIRE(d_q != d_q_out || q_stride == q_out_stride, "append: queries in place with different strides");
     }
-    if (n_rows == 0) return Z2H_OK;
     RopeArgs a{};
     a.hd = pages->head_dim; a.nh = d_q ? n_head : 0; a.nkv = pages->n_head_kv;
     a.seq = d_seq; a.pos = d_pos;
@@ -195,9 +195,9 @@ int z2h_paged_attn(z2h_ctx * ctx, const z2h_pages * pages, int n_head, int n_row
     if (!ctx) return Z2H_EINVAL;
     CHECK(z2o::check_attn(pages, n_head, n_rows, n_group));
     CHECK(z2o::check_attn_type(type, pages->type));
-    CHECK(z2o::check_rows(d_q, q_stride, n_head, pages->head_dim, type));
-    CHECK(z2o::check_rows(d_out, out_stride, n_head, pages->head_dim, type));
-    REQUIRE(d_q != d_out || q_stride == out_stride, "attention: in place with different strides");
+    CHECK(z2o::check_rows(d_q, q_stride, n_head, pages->head_dim, type, n_rows));
+    CHECK(z2o::check_rows(d_out, out_stride, n_head, pages->head_dim, type, n_rows));
+    REQUIRE(n_rows == 0 || d_q != d_out || q_stride == out_stride, "attention: in place with different strides");
     REQUIRE(std::isfinite(scale), "attention: scale must be finite");
     const int n_cu = compute_units(z2h_ctx_device(ctx));
     if (!n_cu) return z2h_ctx_fail(ctx, Z2H_EDEVICE, "compute-unit count query failed");
@@ -236,9 +236,9 @@ int z2h_verify(z2h_ctx * ctx, int n_seq, int n_draft_max, int n_codebooks, int v
                int64_t ws_bytes, void * stream) {
     if (!ctx) return Z2H_EINVAL;
     CHECK(z2o::check_verify(n_seq, n_draft_max, n_codebooks, vocab));
+    if (n_seq == 0) return Z2H_OK;
     REQUIRE(d_target && d_u_draw && d_n_accept && d_codes && (n_draft_max == 0 || (d_draft && d_u_accept)), "verify: null argument");
     CHECK(check_ws(d_ws, ws_bytes, z2o::verify_ws_bytes(n_seq, n_draft_max, n_codebooks, vocab)));
-    if (n_seq == 0) return Z2H_OK;
     VerifyArgs a{};
     a.n_seq = n_seq; a.K = n_draft_max; a.C = n_codebooks; a.V = vocab;
     a.draft = d_draft; a.n_draft = d_n_draft; a.target = d_target; a.temperature = d_temperature; a.draft_probs = d_draft_probs;

@@ -51,10 +51,10 @@ inline const char * check_pages(const z2h_pages * p) {
 
 inline int type_size(int type) { return type == Z2H_F32 ? 4 : type == Z2H_F16 || type == Z2H_BF16 ? 2 : 0; }
 
-// a row tensor of n_head heads: rows `stride` elements apart, elements aligned to their size
-inline const char * check_rows(const void * p, int64_t stride, int n_head, int head_dim, int type) {
-    if (!p) return "null row tensor";
+// a row tensor of n_head heads: rows `stride` elements apart, elements aligned to their size (no rows: it may be null)
+inline const char * check_rows(const void * p, int64_t stride, int n_head, int head_dim, int type, int n_rows = 1) {
     if (!type_size(type)) return "row type must be F32, F16 or BF16";
+    if (!p && n_rows) return "null row tensor";
     if (stride < (int64_t) n_head * head_dim) return "row stride below a row's size";
     if ((uintptr_t) p % type_size(type)) return "row tensor not aligned to its elements";
     return nullptr;
