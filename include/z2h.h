@@ -325,7 +325,7 @@ int z2h_paged_append(z2h_ctx * ctx, const z2h_pages * pages, const z2h_rope * ro
  * values to 2^-16 of them (bf16) or 2^-22. Results do not depend on timing (no atomics). Cache rows that a row does not see
  * do not reach it, whatever they hold. A value that is not finite reaches every row that sees it; a key whose score is minus
  * infinity has no weight, and one whose score is infinity or no number leaves the row without a number. (Rows that see such a
- * cache row take longer: about 2 ms over 16384 keys.)
+ * cache row take longer: about 1.5 ms over 16384 keys.)
  *
  * The workspace (z2h_paged_ws_bytes; 0 = the shapes are refused, see z2h_last_error; 256-byte aligned) holds the plan
  * and the partial results of one call at a time: calls and graphs that may overlap need one each. z2h_paged_attn with

@@ -6,12 +6,13 @@
 // by side in one product), the rest of its keys with its own sequence, and both where shares of equal work end.
 //   k_paged_plan     one block: tiles of query rows, the shares and the places of partial results, from the lengths (z2h_ops_rules.h)
 //   k_paged_attn     a share of the wide strips per block and of the narrow ones per wave
-//   k_paged_join     one wave per (row, head): its pieces' partial results
+//   k_paged_join     a wave per (row, head), or a block of four while the device holds them all: its pieces' partial results, and rows
+//                    that hold NaN once more
 // Single tokens are bound by reading the cache once; groups of many rows and prompt chunks by the products and the exponentials.
-// Measured (attention + join): 64 single rows over 2048 shared and 16 to 2048 own keys, 4 key heads of 128: 22.4 + 5.4 us for
-// 60 MB; 256 rows over 16384 shared keys, 8 key heads of 128, 32 query heads: 134 + 9.5 us for 253 MB and 69 GFLOP (103 with the
-// products of the weights' second parts, at 770 TFLOP/s); 4 prompt chunks of 333 rows behind 1500 shared ones: 50 + 11.7 us; one row over
-// 700 keys: 10.0 + 3.6 us, of dependent loads.
+// Measured (attention + join): 64 single rows over 2048 shared and 16 to 2048 own keys, 4 key heads of 128: 22.1 + 5.4 us for
+// 60 MB; 256 rows over 16384 shared keys, 8 key heads of 128, 32 query heads: 129 + 10 us for 253 MB and 69 GFLOP (103 with the
+// products of the weights' second parts, at 800 TFLOP/s); 4 prompt chunks of 333 rows behind 1500 shared ones: 48.7 + 11.6 us; one row over
+// 700 keys: 10.1 + 3.7 us, of dependent loads. The plan: 20 us for one sequence, 30 for 64, 44 for 256.
 #pragma once
 #include "z2h_common.h"
 #include "z2h_ops_rules.h"
@@ -114,7 +115,7 @@ struct PlanKind {
     }
 };
 
-// One block: a chain of scans and searches, bound by its barriers and dependent loads; 11 us for 64 sequences, 16 us for 256, once
+// One block: a chain of scans and searches, bound by its barriers and dependent loads; 30 us for 64 sequences, 44 us for 256, once
 // for all layers of a step. Everything is clamped to the tables' sizes, so that whatever the lengths say no entry leads outside the buffers; tables
 // that are not ascending make no plan.
 __global__ void __launch_bounds__(PLAN_T) k_paged_plan(PlanArgs a) {
@@ -332,11 +333,12 @@ __device__ __forceinline__ float other_half(float v) {
 // {16 t + 4 h + j, 16 t + 8 + 4 h + j} (h the lane's half, j < 4): P never moves between lanes. V^T's operand for these keys is two
 // transposing LDS reads of 4 keys x 16 dims each from V rows stored as they are. K and V rows lie in LDS with their 16-byte
 // pieces permuted by row, so that both reads take all banks (no conflict counted).
-// A step of 64 keys takes a wave 4.0 thousand cycles beside the other block's wave: K Q with the requests of the next keys 1.2, the softmax
-// 1.0, P V 0.8, the barrier 0.15, the rest masks and addresses. 256 rows over 16384 shared keys: 110 us with operands read just before each
-// product and all requests behind the barrier, 104 so. Products and vector instructions each take 40 % of the cycles. Two waves per
-// SIMD are what the registers leave: 32 of queries, 64 of O, 32 of scores at head size 128. More row-heads per wave would halve the
-// LDS reads per product, but not the exponentials, and leave one wave per SIMD.
+// A step of 64 keys takes a wave 4.6 thousand cycles beside the other block's wave: K Q with the requests of the next keys 1.2, the softmax
+// and the weights' two parts 1.3, P V 1.2, the barrier 0.1, the rest masks and addresses. Operands read just before each product and
+// all requests behind the barrier cost 6 us more over 16384 shared keys. Products take 41 % of the cycles, vector instructions 42 %. Two waves
+// per SIMD are what the registers leave: 32 of queries, 64 of O, 32 of scores at head size 128. More row-heads per wave would halve the
+// LDS reads per product, but not the exponentials, and leave one wave per SIMD. Scalar registers do not hold all sizes, strides and
+// addresses of both walks: 97 (head size 128) to 264 (64) of them lie in lanes of vector registers.
 template <int HD>
 struct Tile {
     static constexpr int NC = HD / 8, RP = 128 / HD;             // 16-byte pieces of a row, rows per 256 bytes
@@ -509,7 +511,7 @@ struct AttnWave {
         // The weights meet the values as two numbers of the cache's type, the second carrying what the first's rounding leaves: off by 2^-22 of
         // them in f16, 2^-16 in bf16. One alone (2^-11, 2^-8) errs as much as the output's own rounding, over any number of keys: with
         // values of mean zero the output shrinks as the error does (1.3 times the rounding's rms in all; with one number 256 rows over 16384
-        // shared keys take 103 us and 4 chunks of 333 rows 40, with two 134 and 50).
+        // shared keys take 103 us and 4 chunks of 333 rows 40, with two 129 and 49).
         v8 p[2 * NT], pl[2 * NT];
         float sum = 0.0f;
 #pragma unroll
@@ -851,7 +853,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_attn(PagedArgs a) {
 }
 
 // A (row, head) in plain fp32, by one wave: 64 keys at a time, a lane each for the scores, then the dims over the lanes. A value that is
-// not finite reaches the row whatever its weight. For rows whose results hold NaN (see AttnWave): 2 ms over 16384 keys, of chains of loads.
+// not finite reaches the row whatever its weight. For rows whose results hold NaN (see AttnWave): 1.5 ms over 16384 keys, of chains of loads.
 template <int HD, typename T, typename TC, int E>
 __device__ __forceinline__ void walk_row(const PagedArgs & a, const PlanRow & r, int row, int head, float * s_q, float (&o)[E], float & l) {
     const int lane = threadIdx.x & 63, g = head / (a.n_head / a.nkv), d = E * lane;

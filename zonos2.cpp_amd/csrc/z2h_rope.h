@@ -67,7 +67,7 @@ template <typename T, bool WIDE> struct RopeUnit { static constexpr int N = WIDE
 // grid (rows, shares of the heads). A thread keeps one unit of a head (pairs, or dims behind them) and walks the heads: rotated
 // query heads, then rotated key heads and copied value heads. WIDE: rows, strides and pairs allow 16-byte accesses. With both kinds of
 // pairs a thread reads and writes whole 16-byte units, so the rows pass once at the rate of a copy: 4099 rows of 32 heads of 128 in
-// bf16 (67 MB) 14.1 us, 2088 rows of queries, keys and values into bf16 pages (51 MB) 12.6 us, 16 fp32 rows 3.8 us (launch).
+// bf16 (67 MB) 13.8 us, 2088 rows of queries, keys and values into bf16 pages (51 MB) 12.2 us, 16 fp32 rows 3.8 us (launch).
 template <typename T, typename TC, bool HALVES, bool WIDE>
 __global__ void __launch_bounds__(256) k_rope_append(RopeArgs a) {
     constexpr int N = RopeUnit<T, WIDE>::N, NP = HALVES ? N : WIDE ? N / 2 : 1;      // values behind the pairs; pairs per unit
