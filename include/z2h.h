@@ -26,8 +26,8 @@
  *   z2h_set_expert_mask   zonos2_set_expert_mask       src/zonos2.cpp:203-239, src/zonos2.h:136
  *   z2h_destroy           zonos2_batch_free            src/zonos2-graph.cpp:692-701 (+ drops the model reference)
  * Without a reference counterpart: the mixed pass, the operators on device tensors around a paged cache (z2h_rope_rows,
- * z2h_paged_append, z2h_paged_plan, z2h_paged_attn, z2h_verify) with the paged pass over them (z2h_step_paged), capture,
- * graph and profiling switches.
+ * z2h_paged_append, z2h_paged_plan, z2h_paged_attn, z2h_verify, z2h_prompt_attn, z2h_moe_rows, z2h_pages_fork, z2h_pages_compact)
+ * with the paged pass over them (z2h_step_paged), capture, graph and profiling switches.
  */
 #ifndef Z2H_H
 #define Z2H_H
@@ -360,6 +360,77 @@ int z2h_verify(z2h_ctx * ctx, int n_seq, int n_draft_max, int n_codebooks, int v
                const int32_t * d_n_draft, const float * d_target, const float * d_temperature, const float * d_draft_probs,
                const double * d_u_accept, const double * d_u_draw, int32_t * d_n_accept, int32_t * d_codes, void * d_ws,
                int64_t ws_bytes, void * stream);
+
+/* Attention of whole prompts that lie packed one behind the other: sequence s is rows [d_row_start[s], d_row_start[s + 1]) of
+ * d_q [n_rows][n_head][head_dim] and of d_k, d_v [n_rows][n_head_kv][head_dim] (d_row_start [n_seq + 1] ascending on the device), and row r of it
+ * attends to its sequence's rows up to r itself: d_out = softmax(scale q k^T) v, [n_rows][n_head][head_dim]. The rows' keys and values are
+ * read as they lie, columns of one fused projection say (rows *_stride apart), before or after z2h_paged_append puts them into pages. All
+ * four are of `type` (Z2H_F32, Z2H_F16 or Z2H_BF16); head_dim is 32, 64 or 128, n_head a multiple of n_head_kv, at most 64 query heads
+ * per key head; query head h reads key head h / (n_head / n_head_kv). d_out may be d_q (with the same stride). A sequence may have no
+ * rows; rows of no sequence are left as they were. Entries of d_row_start are clamped to 0 .. n_rows; rows between entries that descend
+ * get some value or none.
+ * Softmax and sums in fp32; F32 rows are multiplied in fp32, 16-bit rows' weights meet the values to 2^-16 of them (bf16) or 2^-22. Results do
+ * not depend on timing (no atomics). Rows that a row does not see do not reach it, whatever they hold. A value that is not finite reaches
+ * every row that sees it; a key whose score is minus infinity has no weight, and one whose score is infinity or no number leaves the row
+ * without a number. (Rows that see such a value take longer: they are formed a second time, key by key.) */
+int z2h_prompt_attn(z2h_ctx * ctx, int n_seq, const int32_t * d_row_start, int n_rows, int n_head, int n_head_kv, int head_dim,
+                    float scale, int type, const void * d_q, int64_t q_stride, const void * d_k, int64_t k_stride, const void * d_v,
+                    int64_t v_stride, void * d_out, int64_t out_stride, void * stream);
+
+/* The experts of one mixture-of-experts layer: gate and up [n_expert][n_ff][n_embd], down [n_expert][n_embd][n_ff], of Z2H_F16 or
+ * Z2H_BF16, 16-byte aligned; n_embd and n_ff are multiples of 8 (8 .. 65536), n_expert 1 .. 1024. */
+typedef struct z2h_experts {
+    const void * gate, * up, * down;
+    int32_t type, n_expert, n_ff, n_embd;
+} z2h_experts;
+
+/* A mixture-of-experts layer for a few rows (a step's, a request's drafts; 1 .. Z2H_MOE_ROWS_MAX), in two launches:
+ *   p = softmax(d_logits of the row), the top_k experts by p + d_bias (NULL: by p; equal ones: the lower index first), w = p of these,
+ *   divided by their sum if `renorm` is not 0;   out = sum_j w_j down_e(j) (silu(gate_e(j) x) * (up_e(j) x)).
+ * d_logits [n_rows][n_expert] are fp32, d_bias [n_expert]. d_x and d_out are [n_rows][n_embd] of `type`, rows *_stride apart: Z2H_F32 or
+ * Z2H_F16 with F16 experts, Z2H_BF16 with BF16 ones; d_out may be d_x. d_sel and d_weights [n_rows][top_k] (either may be NULL) receive the
+ * experts and their w, the first the one with the largest p + bias. An expert whose logit is minus infinity is never taken: -1 and 0
+ * stand in the places that remain, and a row without any expert gives zeros. A row with a logit or a sum p + bias that is no number, or
+ * with an infinite logit, has no number as its result, and -1 and no number in d_sel and d_weights. top_k is 1 .. min(n_expert, 16).
+ * Sums in fp32; fp32 rows meet the weights as two f16 numbers, off by 2^-22 of the largest of 256 neighbours at most, and so do the products
+ * silu(..) * .. (two bf16 numbers with bf16 experts, 2^-16 each). A row that holds a value that is not finite has results that are not
+ * finite, and no other row's change. Results do not depend on timing.
+ * The workspace (z2h_moe_rows_ws_bytes; 0: the sizes are refused; 256-byte aligned) holds one call at a time: calls and graphs that may
+ * overlap need one each. */
+#define Z2H_MOE_ROWS_MAX 128
+int64_t z2h_moe_rows_ws_bytes(const z2h_experts * experts, int n_rows, int top_k);
+int z2h_moe_rows(z2h_ctx * ctx, const z2h_experts * experts, int n_rows, int top_k, int renorm, const float * d_logits,
+                 const float * d_bias, int type, const void * d_x, int64_t x_stride, void * d_out, int64_t out_stride, int32_t * d_sel,
+                 float * d_weights, void * d_ws, int64_t ws_bytes, void * stream);
+
+/* The pages of a paged cache as sequences come, share, grow and go, without a word from the host: the calls below change the page table
+ * (`pages->table`, written here) and d_refs [n_pages], which says for every page how many table entries name it (0: free), and copy
+ * what has to be copied in all n_layer layers. `pages` describes layer 0; layer L's k and v lie L * layer_stride elements behind (as in
+ * z2h_step_paged). A sequence holds the pages that its table row names before the first entry outside [0, n_pages); entries behind
+ * that one are not looked at, and -1 is written where a sequence has no page. n_pages is at most 2^22. To begin: every entry -1, every
+ * count 0. The workspace (z2h_pages_ws_bytes, n the fork's items; 0: the sizes are refused; 256-byte aligned) holds one call at a time;
+ * calls on the same cache follow each other on one stream.
+ *
+ * z2h_pages_fork: item i makes sequence d_dst[i] the holder of the first d_rows[i] rows of sequence d_src[i], with room for d_room[i] rows.
+ * What the destination held is given up. Whole pages of the rows are shared; the rows in the last, partly filled page are copied into a
+ * page of its own, so that both sequences may go on; pages for the rest of the room are new (nothing is written to them). With
+ * d_src[i] == d_dst[i] the sequence keeps its own rows: it is cut off (0 rows and no room: ended), given room, or both, and its
+ * partly filled page is copied only if another sequence names that page too. Rows are clamped to 0 .. what the source holds, the room to rows ..
+ * the table's. New pages are the free ones, those that the call's destinations gave up among them, lowest first, in the order of
+ * the items and of their entries. d_held[i] (NULL: not told) is the number of rows that the destination now has pages for: the room, or where
+ * no page was left, less: the pages up to there. An item whose source or destination is outside [0, n_seq), whose destination an
+ * item before it has too, or whose source is not its destination but an item's changes nothing: -1. n is at most 4096.
+ *
+ * z2h_pages_compact: the pages in use become pages 0 .. n_used - 1: those from n_used on move, in ascending order, to the free ones before, in
+ * ascending order. The new table goes to d_table_out [n_seq][table_len] and the new counts to d_refs_out [n_pages] (either may be the old
+ * one itself), n_used to d_n_used (NULL: not told). A moved page's old place keeps what it holds. An entry that names a page with a
+ * count of 0 becomes -1 or stays. */
+int64_t z2h_pages_ws_bytes(z2h_ctx * ctx, const z2h_pages * pages, int n);
+int z2h_pages_fork(z2h_ctx * ctx, const z2h_pages * pages, int n_layer, int64_t layer_stride, int32_t * d_refs, int n, const int32_t * d_src,
+                   const int32_t * d_dst, const int32_t * d_rows, const int32_t * d_room, int32_t * d_held, void * d_ws, int64_t ws_bytes,
+                   void * stream);
+int z2h_pages_compact(z2h_ctx * ctx, const z2h_pages * pages, int n_layer, int64_t layer_stride, int32_t * d_refs, int32_t * d_table_out,
+                      int32_t * d_refs_out, int32_t * d_n_used, void * d_ws, int64_t ws_bytes, void * stream);
 
 /* The pass of z2h_step_mixed over a paged cache in place of the context's bands: the model's layers with
  * z2h_paged_append, z2h_paged_plan and z2h_paged_attn in them. A prompt that sequences share is stored once and read

@@ -1,0 +1,52 @@
+// z2h_moe.hip — z2h_moe_rows of include/z2h.h: a mixture-of-experts layer for a few rows on the caller's tensors.
+#include "z2h_ops_common.h"
+#include "z2h_moe.h"
+
+using namespace z2d;
+
+namespace {
+
+template <typename T, typename TW>
+void moe_launch(const MoeArgs & a, hipStream_t st) {
+    hipLaunchKernelGGL((k_moe_gate_up<T, TW>), dim3(1024), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((k_moe_down<T, TW>), dim3(1024), dim3(256), 0, st, a);
+}
+
+} // namespace
+
+extern "C" {
+
+int64_t z2h_moe_rows_ws_bytes(const z2h_experts * experts, int n_rows, int top_k) {
+    return z2o::check_moe(experts, n_rows, top_k) ? 0 : z2o::moe_ws(*experts, n_rows, top_k).bytes;
+}
+
+int z2h_moe_rows(z2h_ctx * ctx, const z2h_experts * experts, int n_rows, int top_k, int renorm, const float * d_logits,
+                 const float * d_bias, int type, const void * d_x, int64_t x_stride, void * d_out, int64_t out_stride, int32_t * d_sel,
+                 float * d_weights, void * d_ws, int64_t ws_bytes, void * stream) {
+    if (!ctx) return Z2H_EINVAL;
+    CHECK(z2o::check_moe(experts, n_rows, top_k));
+    CHECK(z2o::check_moe_type(type, experts->type));
+    CHECK(z2o::check_rows(d_x, x_stride, 1, experts->n_embd, type, n_rows));
+    CHECK(z2o::check_rows(d_out, out_stride, 1, experts->n_embd, type, n_rows));
+    if (n_rows == 0) return Z2H_OK;
+    REQUIRE(d_x != d_out || x_stride == out_stride, "moe: in place with different strides");
+    REQUIRE(d_logits, "moe: null logits");
+    const z2o::MoeWs w = z2o::moe_ws(*experts, n_rows, top_k);
+    CHECK(check_ws(d_ws, ws_bytes, w.bytes));
+    uint8_t * ws = (uint8_t *) d_ws;
+    MoeArgs a{};
+    a.gate = experts->gate; a.up = experts->up; a.down = experts->down;
+    a.E = experts->n_expert; a.F = experts->n_ff; a.D = experts->n_embd; a.n = n_rows; a.k = top_k; a.renorm = renorm;
+    a.logits = d_logits; a.bias = d_bias; a.x = d_x; a.xs = x_stride; a.out = d_out; a.os = out_stride;
+    a.sel = d_sel; a.weights = d_weights;
+    a.routes = (int32_t *) ws; a.w = (float *) (ws + w.w); a.h = (float *) (ws + w.h);
+    ON_DEVICE;
+    switch (type) {
+        case Z2H_F32: moe_launch<float, _Float16>(a, (hipStream_t) stream); break;
+        case Z2H_F16: moe_launch<_Float16, _Float16>(a, (hipStream_t) stream); break;
+        default: moe_launch<__bf16, __bf16>(a, (hipStream_t) stream); break;
+    }
+    return launched(ctx);
+}
+
+} // extern "C"

@@ -1,41 +1,15 @@
 // z2h_ops.hip — the operators on device tensors of include/z2h.h: rotary rows, paged append, attention over shared
 // prefixes, draft verification. A translation unit of their own: z2h.hip's kernels keep their code layout.
 #include "z2h.h"
-#include "z2h_ctx_ops.h"
-#include "z2h_ops_rules.h"
+#include "z2h_ops_common.h"
 #include "z2h_rope.h"
 #include "z2h_paged.h"
 #include "z2h_verify.h"
 #include "z2h_paged_step.h"
 
-#include <algorithm>
-#include <atomic>
-
 using namespace z2d;
 
 namespace {
-
-// makes the context's device current for a scope and restores the caller's on every way out
-struct OnDevice {
-    int prev = -1;
-    bool ok = false, moved = false;
-    explicit OnDevice(const z2h_ctx * ctx) {
-        const int device = z2h_ctx_device(ctx);
-        if (hipGetDevice(&prev) != hipSuccess) return;
-        moved = prev != device;
-        ok = !moved || hipSetDevice(device) == hipSuccess;
-    }
-    ~OnDevice() { if (ok && moved) (void) hipSetDevice(prev); }
-};
-
-int launched(z2h_ctx * ctx) {
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? Z2H_OK : z2h_ctx_fail(ctx, Z2H_EDEVICE, hipGetErrorString(e));
-}
-
-#define CHECK(expr) do { if (const char * e_ = (expr)) return z2h_ctx_fail(ctx, Z2H_EINVAL, e_); } while (0)
-#define REQUIRE(cond, what) do { if (!(cond)) return z2h_ctx_fail(ctx, Z2H_EINVAL, what); } while (0)
-#define ON_DEVICE OnDevice on_(ctx); if (!on_.ok) return z2h_ctx_fail(ctx, Z2H_EDEVICE, "hipSetDevice failed")
 
 template <typename T, typename TC>
 void rope_launch(RopeArgs & a, int n_rows, bool halves, hipStream_t stream) {
@@ -74,16 +48,6 @@ int rope_run(z2h_ctx * ctx, RopeArgs & a, const z2h_rope * rope, int n_rows, int
     return launched(ctx);
 }
 
-int compute_units(int device) {
-    static std::atomic<int> known[64] = {};
-    const bool slot = device >= 0 && device < 64;
-    int n = slot ? known[device].load(std::memory_order_relaxed) : 0;
-    if (n <= 0) {
-        if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || n <= 0) return 0;
-        if (slot) known[device].store(n, std::memory_order_relaxed);
-    }
-    return n;
-}
 // blocks of k_paged_attn: as many as the device holds at once
 int attn_blocks(int n_cu) { return 2 * n_cu; }
 
@@ -104,11 +68,6 @@ void attn_launch(PagedArgs & a, int type, int blocks, hipStream_t stream) {
         case Z2H_F16: attn_launch<HD, _Float16, _Float16>(a, blocks, stream); break;
         default: attn_launch<HD, __bf16, __bf16>(a, blocks, stream); break;
     }
-}
-
-const char * check_ws(const void * ws, int64_t have, int64_t need) {
-    if (!ws || (uintptr_t) ws % 256) return "workspace must be 256-byte aligned";
-    return have < need ? "workspace too small" : nullptr;
 }
 
 } // namespace

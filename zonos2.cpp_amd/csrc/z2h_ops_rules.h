@@ -4,6 +4,7 @@
 #include "z2h.h"
 #include <cmath>
 #include <cstdint>
+#include <initializer_list>
 
 #if defined(__HIPCC__)
 #define Z2O_HD __host__ __device__ inline
@@ -189,6 +190,73 @@ inline AttnWs attn_ws(const z2h_pages & p, int n_head, int n_rows, int n_group, 
     return w;
 }
 
+// ---- attention over packed prompts
+// A sequence's rows are cut into tiles of `rows` rows; tile j of sequence s is slot start[s] / rows + s + j, so that a slot's sequence is found by
+// searching the row table alone. A sequence may have a slot too many.
+Z2O_HD int64_t prompt_slot(int start, int seq, int rows) { return (int64_t) start / rows + seq; }
+inline int64_t prompt_slots(int n_rows, int n_seq, int rows) { return (int64_t) n_rows / rows + n_seq; }
+constexpr int MAX_PROMPTS = 1 << 20;
+inline const char * check_prompt(int n_seq, int n_rows, int n_head, int n_head_kv, int head_dim) {
+    if (head_dim != 32 && head_dim != 64 && head_dim != 128) return "prompt: head_dim must be 32, 64 or 128";
+    if (n_head_kv <= 0 || n_head_kv > 1024) return "prompt: n_head_kv out of range";
+    if (n_head <= 0 || n_head % n_head_kv || n_head / n_head_kv > MAX_GROUP) return "n_head must be 1 .. 64 times n_head_kv";
+    if (n_rows < 0 || (int64_t) n_rows * n_head > MAX_ROW_HEADS) return "n_rows out of range";
+    if (n_seq < 0 || n_seq > MAX_PROMPTS) return "prompt: n_seq out of range";
+    return nullptr;
+}
+
+// ---- mixture of experts for a few rows
+constexpr int MOE_MAX_EXPERTS = 1024, MOE_MAX_TOP = 16, MOE_MAX_DIM = 65536;
+inline const char * check_experts(const z2h_experts * x) {
+    if (!x) return "null experts";
+    if (!x->gate || !x->up || !x->down) return "experts: null weights";
+    if (((uintptr_t) x->gate | (uintptr_t) x->up | (uintptr_t) x->down) % 16) return "experts: weights must be 16-byte aligned";
+    if (x->type != Z2H_F16 && x->type != Z2H_BF16) return "experts: the weights must be F16 or BF16";
+    if (x->n_expert <= 0 || x->n_expert > MOE_MAX_EXPERTS) return "experts: n_expert out of range";
+    for (int32_t d : {x->n_ff, x->n_embd})
+        if (d <= 0 || d % 8 || d > MOE_MAX_DIM) return "experts: n_ff and n_embd must be multiples of 8, at most 65536";
+    return nullptr;
+}
+inline const char * check_moe(const z2h_experts * x, int n_rows, int top_k) {
+    if (const char * e = check_experts(x)) return e;
+    if (n_rows < 0 || n_rows > Z2H_MOE_ROWS_MAX) return "moe: n_rows out of range (0 .. 128)";
+    if (top_k <= 0 || top_k > MOE_MAX_TOP || top_k > x->n_expert) return "moe: top_k must be 1 .. min(n_expert, 16)";
+    return nullptr;
+}
+inline const char * check_moe_type(int type, int experts) {
+    if (type == Z2H_F32 || type == Z2H_F16) return experts == Z2H_F16 ? nullptr : "F32 and F16 rows need F16 experts";
+    if (type == Z2H_BF16) return experts == Z2H_BF16 ? nullptr : "BF16 rows need BF16 experts";
+    return "row type must be F32, F16 or BF16";
+}
+
+// ---- a paged cache's upkeep
+constexpr int MAX_POOL = 1 << 22, MAX_FORKS = 4096, POOL_SEG = 1024;
+inline const char * check_pool(const z2h_pages * p, int n) {
+    if (const char * e = check_pages(p)) return e;
+    if (p->n_pages > MAX_POOL) return "pages: n_pages above 2^22";
+    if (n < 0 || n > MAX_FORKS) return "pages: more than 4096 items";
+    return nullptr;
+}
+inline const char * check_layers(const z2h_pages * p, int n_layer, int64_t layer_stride) {
+    if (n_layer <= 0 || n_layer > 65536) return "pages: n_layer out of range";
+    if (n_layer > 1 && (layer_stride % 8 || layer_stride < p->n_pages * p->page_stride)) return "pages: layer_stride must be a multiple of 8, at least n_pages page_strides";
+    if (n_layer * (int64_t) p->n_head_kv * p->page_rows * p->head_dim > 1ll << 32) return "pages: a page of more than 2^34 bytes in all layers";
+    return nullptr;
+}
+// Rows that a fork keeps and has room for, of what the source holds and the table has; whole pages, pages in all.
+struct ForkSize { int rows, room, whole, pages; };
+Z2O_HD ForkSize fork_size(int rows, int room, int have_pages, int table_len, int page_shift) {
+    const int held = have_pages << page_shift, most = table_len << page_shift;
+    ForkSize f;
+    f.rows = rows < 0 ? 0 : rows < held ? rows : held;
+    f.room = room < f.rows ? f.rows : room < most ? room : most;
+    f.whole = f.rows >> page_shift;
+    f.pages = (int) (((int64_t) f.room + (1 << page_shift) - 1) >> page_shift);
+    return f;
+}
+// Workspace: a bit per page, counts per 1024 pages, and per item 32 bytes (fork) or per page its new number and a move (compact).
+struct PoolWs { int64_t bits = 0, counts = 0, items = 0, map = 0, moves = 0, bytes = 0; int segs = 0; };
+
 // ---- verification
 constexpr int VERIFY_PER_THREAD = 32;              // logits of a row per thread of k_verify_stats
 constexpr int VERIFY_SHORT = 256 * VERIFY_PER_THREAD, VERIFY_CHUNK = 1024 * VERIFY_PER_THREAD;
@@ -212,6 +280,27 @@ inline int64_t verify_ws_bytes(int n_seq, int n_draft_max, int n_codebooks, int 
     const int64_t draws = vocab > VERIFY_ONE ? (int64_t) n_seq * n_codebooks : 0;
     return 256 + verify_stats_bytes(n_seq, n_draft_max, n_codebooks, vocab) + align256(draws * VERIFY_DRAW_BYTES) +
            align256(draws * ((vocab + 255) / 256) * 8);
+}
+
+struct MoeWs { int64_t w = 0, h = 0, bytes = 0; };
+inline MoeWs moe_ws(const z2h_experts & x, int n_rows, int top_k) {
+    MoeWs m;
+    const int64_t routes = (int64_t) n_rows * top_k;
+    m.w = 256 + align256(routes * 4);
+    m.h = m.w + align256(routes * 4);
+    m.bytes = m.h + align256(routes * x.n_ff * 4);
+    return m;
+}
+
+inline PoolWs pool_ws(int n_pages, int n) {
+    PoolWs w;
+    w.segs = (n_pages + POOL_SEG - 1) / POOL_SEG;
+    w.counts = (int64_t) w.segs * (POOL_SEG / 8);
+    w.items = w.counts + align256((int64_t) w.segs * 4);
+    w.map = w.items + align256((int64_t) n * 32);
+    w.moves = w.map + align256((int64_t) n_pages * 4);
+    w.bytes = w.moves + 256 + align256((int64_t) n_pages * 4);           // (a move: two numbers, at most half of the pages)
+    return w;
 }
 
 } // namespace z2o

@@ -1,0 +1,312 @@
+// z2h_pages.h — a paged cache's upkeep on the device: sequences that take over others' rows, room for more, the end of sequences, and moving
+// the pages in use together.
+//
+// All state is the page table and a count per page (how many entries name it). Counts are sums, so that no order of the items matters; free
+// pages are handed out lowest first by rank: a bit per page and a count per 1024 pages say which is the r-th, and every block finds its own.
+//   k_pages_release   a block per item: is it sound, what does it give up and share
+//   k_pages_scan      the bits and counts, and in one more block the items' needs and places among the free pages
+//   k_pages_take      new pages into the table, and the rows of partly filled pages copied in all layers
+//   k_pages_moves     (compact) every page's new number
+//   k_pages_compact   pages moved in all layers, table and counts rewritten
+#pragma once
+#include "z2h_common.h"
+#include "z2h_ops_rules.h"
+
+namespace z2d {
+
+struct PoolArgs {
+    uint8_t * k, * v;
+    int64_t page_bytes, layer_bytes;                             // apart
+    int32_t * table, * refs;
+    int n_pages, n_seq, table_len, page_shift, row_bytes, nkv, n_layer, segs;
+    unsigned long long * bits;
+    int * counts;
+};
+// of an item that is sound; keeps: the partly filled page stays its own
+struct ForkItem { int ok, src, dst, part_page, keeps, need, base, spare; };
+static_assert(sizeof(ForkItem) == 32, "workspace layout");
+struct ForkArgs {
+    PoolArgs p;
+    int n;
+    const int32_t * src, * dst, * rows, * room;
+    int32_t * held;
+    ForkItem * items;
+    int item0;
+};
+
+// leading entries of a sequence that name a page, by the whole block of 256
+__device__ __forceinline__ int held_pages(const PoolArgs & p, int seq, int * s_min) {
+    const int32_t * row = p.table + (int64_t) seq * p.table_len;
+    __syncthreads();
+    if (threadIdx.x == 0) *s_min = p.table_len;
+    __syncthreads();
+    for (int e = threadIdx.x; e < p.table_len; e += 256)
+        if ((unsigned) row[e] >= (unsigned) p.n_pages) { atomicMin(s_min, e); break; }
+    __syncthreads();
+    return *s_min;
+}
+
+__global__ void __launch_bounds__(256) k_pages_release(ForkArgs a) {
+    __shared__ int s_min, s_bad;
+    const int i = a.item0 + blockIdx.x, tid = threadIdx.x;
+    const PoolArgs & p = a.p;
+    const int src = a.src[i], dst = a.dst[i];
+    if (tid == 0) s_bad = src < 0 || src >= p.n_seq || dst < 0 || dst >= p.n_seq;
+    __syncthreads();
+    bool bad = false;
+    for (int j = tid; j < a.n; j += 256) {
+        const int d = a.dst[j];
+        bad |= (d == dst && j < i) || (d == src && src != dst);
+    }
+    if (bad) s_bad = 1;
+    __syncthreads();
+    if (s_bad) {
+        if (tid == 0) a.items[i] = ForkItem{0, 0, 0, -1, 0, 0, 0, 0};
+        return;
+    }
+    const int32_t * from = p.table + (int64_t) src * p.table_len, * own = p.table + (int64_t) dst * p.table_len;
+    const int have = held_pages(p, src, &s_min), given = src == dst ? have : held_pages(p, dst, &s_min);
+    const z2o::ForkSize f = z2o::fork_size(a.rows[i], a.room[i], have, p.table_len, p.page_shift);
+    const int part = f.rows & ((1 << p.page_shift) - 1), stay = src == dst ? f.whole + (part > 0) : 0;
+    for (int e = tid; e < given; e += 256)
+        if (e >= stay) atomicSub(p.refs + own[e], 1);
+    if (src != dst)
+        for (int e = tid; e < f.whole; e += 256) atomicAdd(p.refs + from[e], 1);
+    if (tid == 0) a.items[i] = ForkItem{1 + have, src, dst, part ? from[f.whole] : -1, 0, 0, 0, 0};
+}
+
+// which pages are free (FREE) or in use: a bit each, and counts per 1024. With a fork's items, one more block for these.
+template <bool FREE>
+__global__ void __launch_bounds__(256) k_pages_scan(ForkArgs a) {
+    __shared__ int s_wave[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const PoolArgs & p = a.p;
+    if ((int) blockIdx.x < p.segs) {
+        int count = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int word = 4 * wave + j, page = (int) blockIdx.x * z2o::POOL_SEG + 64 * word + lane;
+            const bool in = page < p.n_pages, used = in && p.refs[page] > 0;
+            const unsigned long long b = __ballot(FREE ? in && !used : used);
+            if (lane == 0) p.bits[(int64_t) blockIdx.x * (z2o::POOL_SEG / 64) + word] = b;
+            count += __popcll(b);
+        }
+        if (lane == 0) s_wave[wave] = count;
+        __syncthreads();
+        if (tid == 0) p.counts[blockIdx.x] = s_wave[0] + s_wave[1] + s_wave[2] + s_wave[3];
+        return;
+    }
+    int total = 0;
+    for (int i0 = 0; i0 < a.n; i0 += 256) {
+        const int i = i0 + tid;
+        ForkItem it{};
+        if (i < a.n) it = a.items[i];
+        if (it.ok) {
+            const z2o::ForkSize f = z2o::fork_size(a.rows[i], a.room[i], it.ok - 1, p.table_len, p.page_shift);
+            it.keeps = it.part_page >= 0 && it.src == it.dst && p.refs[it.part_page] <= 1;
+            it.need = f.pages - f.whole - it.keeps;
+        }
+        int x = it.need;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(x, o);
+            if (lane >= o) x += y;
+        }
+        __syncthreads();
+        if (lane == 63) s_wave[wave] = x;
+        __syncthreads();
+        int below = total;
+        for (int w = 0; w < 4; ++w) {
+            if (w < wave) below += s_wave[w];
+            total += s_wave[w];
+        }
+        it.base = below + x - it.need;
+        if (i < a.n) a.items[i] = it;
+    }
+}
+
+// The bits' counts of all segments before each, in LDS (segs <= 4096), by a block of 256; entry segs: all of them.
+__device__ __forceinline__ void seg_prefix(const PoolArgs & p, int * s_pre, int * s_wave) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int total = 0;
+    for (int i0 = 0; i0 < p.segs; i0 += 256) {
+        const int i = i0 + tid, c = i < p.segs ? p.counts[i] : 0;
+        int x = c;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(x, o);
+            if (lane >= o) x += y;
+        }
+        __syncthreads();
+        if (lane == 63) s_wave[wave] = x;
+        __syncthreads();
+        int below = total;
+        for (int w = 0; w < 4; ++w) {
+            if (w < wave) below += s_wave[w];
+            total += s_wave[w];
+        }
+        if (i < p.segs) s_pre[i] = below + x - c;
+    }
+    if (tid == 0) s_pre[p.segs] = total;
+    __syncthreads();
+}
+// the n-th set bit of w (it has more)
+__device__ __forceinline__ int nth_bit(unsigned long long w, int n) {
+    int at = 0;
+#pragma unroll
+    for (int half = 32; half; half >>= 1) {
+        const int c = __popcll(w & ((1ull << half) - 1));
+        if (n >= c) { n -= c; w >>= half; at += half; }
+    }
+    return at;
+}
+// the page of rank r among the pages whose bit is set (or not set, among the first `n`); r is below their number
+template <bool SET>
+__device__ __forceinline__ int page_of_rank(const PoolArgs & p, const int * s_pre, int r) {
+    auto before = [&](int seg) { return SET ? s_pre[seg] : seg * z2o::POOL_SEG - s_pre[seg]; };
+    int lo = 0, hi = p.segs;
+    while (hi - lo > 1) {
+        const int m = (lo + hi) >> 1;
+        if (before(m) <= r) lo = m; else hi = m;
+    }
+    r -= before(lo);
+    const unsigned long long * w = p.bits + (int64_t) lo * (z2o::POOL_SEG / 64);
+    for (int i = 0; i < z2o::POOL_SEG / 64; ++i) {
+        const unsigned long long x = SET ? w[i] : ~w[i];
+        const int c = __popcll(x);
+        if (r < c) return lo * z2o::POOL_SEG + 64 * i + nth_bit(x, r);
+        r -= c;
+    }
+    return -1;
+}
+// pages below `page` whose bit is set
+__device__ __forceinline__ int set_before(const PoolArgs & p, const int * s_pre, int page) {
+    const int seg = page / z2o::POOL_SEG, word = page / 64 % (z2o::POOL_SEG / 64);
+    if (seg >= p.segs) return s_pre[p.segs];
+    const unsigned long long * w = p.bits + (int64_t) seg * (z2o::POOL_SEG / 64);
+    int n = s_pre[seg];
+    for (int i = 0; i < word; ++i) n += __popcll(w[i]);
+    return n + __popcll(w[word] & ((1ull << (page & 63)) - 1));
+}
+
+typedef unsigned unit_t __attribute__((ext_vector_type(4)));
+
+// `bytes` at the start of every head's run of a page (HEADS), or the whole page, to the same place of another, in all layers; work of thread t of T
+template <bool HEADS>
+__device__ __forceinline__ void copy_page(const PoolArgs & p, int from, int to, int bytes, int t, int T) {
+    const int heads = HEADS ? p.nkv : 1, units = bytes / 16, total = p.n_layer * 2 * heads * units;
+    const int run_bytes = p.row_bytes << p.page_shift;
+    const int64_t src = from * p.page_bytes, dst = to * p.page_bytes;
+    constexpr int U = 8;
+    for (int u0 = t; u0 < total; u0 += U * T) {
+        unit_t x[U];
+        int64_t at[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int u = u0 + i * T, run = u / units, head = run % heads, kv = run / heads;
+            at[i] = (int64_t) (kv >> 1) * p.layer_bytes + (int64_t) head * run_bytes + (u - run * units) * 16;
+            if (u < total) x[i] = *(const unit_t *) ((kv & 1 ? p.v : p.k) + src + at[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int u = u0 + i * T, kv = u / units / heads;
+            if (u < total) *(unit_t *) ((kv & 1 ? p.v : p.k) + dst + at[i]) = x[i];
+        }
+    }
+}
+
+__global__ void __launch_bounds__(256) k_pages_take(ForkArgs a) {
+    __shared__ int s_pre[z2o::MAX_POOL / z2o::POOL_SEG + 1], s_wave[4];
+    const int i = a.item0 + blockIdx.x, tid = threadIdx.x;
+    const PoolArgs & p = a.p;
+    const ForkItem it = a.items[i];
+    if (!it.ok) {
+        if (blockIdx.y == 0 && tid == 0 && a.held) a.held[i] = -1;
+        return;
+    }
+    const z2o::ForkSize f = z2o::fork_size(a.rows[i], a.room[i], it.ok - 1, p.table_len, p.page_shift);
+    const bool copy = it.part_page >= 0 && !it.keeps;
+    if (blockIdx.y && !copy) return;
+    seg_prefix(p, s_pre, s_wave);
+    const int got = max(0, min(it.need, s_pre[p.segs] - it.base)), first = f.whole + it.keeps;
+    if (blockIdx.y == 0) {
+        const int32_t * from = p.table + (int64_t) it.src * p.table_len;
+        int32_t * own = p.table + (int64_t) it.dst * p.table_len;
+        if (it.src != it.dst)
+            for (int e = tid; e < f.whole; e += 256) own[e] = from[e];
+        for (int e = first + tid; e < p.table_len; e += 256) {
+            int page = -1;
+            if (e < first + got) {
+                page = page_of_rank<true>(p, s_pre, it.base + e - first);
+                p.refs[page] = 1;
+            }
+            own[e] = page;
+        }
+        if (tid == 0) {
+            if (copy && it.src == it.dst) atomicSub(p.refs + it.part_page, 1);
+            if (a.held) a.held[i] = min(f.room, (first + got) << p.page_shift);
+        }
+    }
+    if (copy && got > 0)
+        copy_page<true>(p, it.part_page, page_of_rank<true>(p, s_pre, it.base), (f.rows & ((1 << p.page_shift) - 1)) * p.row_bytes,
+                        (int) blockIdx.y * 256 + tid, (int) gridDim.y * 256);
+}
+
+struct CompactArgs {
+    PoolArgs p;
+    int32_t * table_out, * refs_out, * n_used;
+    int32_t * map;                                               // [n_pages] new numbers
+    int32_t * n_moves;
+    int2 * moves;
+    int blocks;                                                  // that copy
+};
+
+__global__ void __launch_bounds__(256) k_pages_moves(CompactArgs a) {
+    __shared__ int s_pre[z2o::MAX_POOL / z2o::POOL_SEG + 1], s_wave[4];
+    const PoolArgs & p = a.p;
+    seg_prefix(p, s_pre, s_wave);
+    const int used = s_pre[p.segs], stay = set_before(p, s_pre, used), moves = used - stay;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        *a.n_moves = moves;
+        if (a.n_used) *a.n_used = used;
+    }
+    const int page = blockIdx.x * 256 + threadIdx.x;
+    if (page >= p.n_pages) return;
+    const bool set = p.bits[page >> 6] >> (page & 63) & 1;
+    if (page < used) {
+        a.map[page] = page;
+        if (set) a.refs_out[page] = p.refs[page];
+        return;
+    }
+    if (!set) {
+        a.map[page] = -1;
+        a.refs_out[page] = 0;
+        return;
+    }
+    const int m = set_before(p, s_pre, page) - stay, to = page_of_rank<false>(p, s_pre, m), refs = p.refs[page];
+    a.map[page] = to;
+    a.moves[m] = make_int2(page, to);
+    a.refs_out[page] = 0;
+    a.refs_out[to] = refs;
+}
+
+__global__ void __launch_bounds__(256) k_pages_compact(CompactArgs a) {
+    const PoolArgs & p = a.p;
+    const int tid = threadIdx.x;
+    if ((int) blockIdx.x >= a.blocks) {
+        const int64_t n = (int64_t) p.n_seq * p.table_len, step = (int64_t) (gridDim.x - a.blocks) * 256;
+        for (int64_t i = (int64_t) (blockIdx.x - a.blocks) * 256 + tid; i < n; i += step) {
+            const int page = p.table[i];
+            a.table_out[i] = (unsigned) page < (unsigned) p.n_pages ? a.map[page] : -1;
+        }
+        return;
+    }
+    const int moves = *a.n_moves, page_bytes = (p.nkv * p.row_bytes) << p.page_shift, units = page_bytes / 16 * 2 * p.n_layer;
+    const int per = max(1, units / (256 * 8));                   // blocks that share a page
+    for (int64_t w = blockIdx.x; w < (int64_t) moves * per; w += a.blocks) {
+        const int2 m = a.moves[w / per];
+        copy_page<false>(p, m.x, m.y, page_bytes, (int) (w % per) * 256 + tid, per * 256);
+    }
+}
+
+} // namespace z2d

@@ -1,0 +1,54 @@
+// z2h_prompt.hip — z2h_prompt_attn of include/z2h.h: causal attention of packed prompts.
+#include "z2h_ops_common.h"
+#include "z2h_prompt.h"
+
+using namespace z2d;
+
+namespace {
+
+template <int HD, typename T>
+void prompt_launch(PromptArgs & a, hipStream_t st) {
+    for (int64_t n = ((int64_t) a.n_rows * a.n_head + 3) / 4; a.block0 < n; a.block0 += z2o::launch_blocks(256))
+        hipLaunchKernelGGL((k_prompt_walk<HD, T>), dim3(std::min(n - a.block0, z2o::launch_blocks(256))), dim3(256), 0, st, a);
+}
+template <int HD>
+void prompt_launch(PromptArgs & a, int type, hipStream_t st) {
+    switch (type) {
+        case Z2H_F32: prompt_launch<HD, float>(a, st); break;
+        case Z2H_F16: prompt_launch<HD, _Float16>(a, st); break;
+        default: prompt_launch<HD, __bf16>(a, st); break;
+    }
+}
+
+} // namespace
+
+extern "C" {
+
+int z2h_prompt_attn(z2h_ctx * ctx, int n_seq, const int32_t * d_row_start, int n_rows, int n_head, int n_head_kv, int head_dim,
+                    float scale, int type, const void * d_q, int64_t q_stride, const void * d_k, int64_t k_stride, const void * d_v,
+                    int64_t v_stride, void * d_out, int64_t out_stride, void * stream) {
+    if (!ctx) return Z2H_EINVAL;
+    CHECK(z2o::check_prompt(n_seq, n_rows, n_head, n_head_kv, head_dim));
+    CHECK(z2o::check_rows(d_q, q_stride, n_head, head_dim, type, n_rows));
+    CHECK(z2o::check_rows(d_k, k_stride, n_head_kv, head_dim, type, n_rows));
+    CHECK(z2o::check_rows(d_v, v_stride, n_head_kv, head_dim, type, n_rows));
+    CHECK(z2o::check_rows(d_out, out_stride, n_head, head_dim, type, n_rows));
+    REQUIRE(std::isfinite(scale), "prompt: scale must be finite");
+    if (n_rows == 0 || n_seq == 0) return Z2H_OK;
+    REQUIRE(d_q != d_out || q_stride == out_stride, "prompt: in place with different strides");
+    REQUIRE(d_row_start, "prompt: null row table");
+    PromptArgs a{};
+    a.start = d_row_start; a.n_seq = n_seq; a.n_rows = n_rows; a.n_head = n_head; a.nkv = n_head_kv;
+    a.q = d_q; a.k = d_k; a.v = d_v; a.out = d_out;
+    a.qs = q_stride; a.ks = k_stride; a.vs = v_stride; a.os = out_stride;
+    a.scale = scale;
+    ON_DEVICE;
+    switch (head_dim) {
+        case 32: prompt_launch<32>(a, type, (hipStream_t) stream); break;
+        case 64: prompt_launch<64>(a, type, (hipStream_t) stream); break;
+        default: prompt_launch<128>(a, type, (hipStream_t) stream); break;
+    }
+    return launched(ctx);
+}
+
+} // extern "C"

@@ -77,6 +77,12 @@ def lib() -> C.CDLL:
         "z2h_paged_attn": (i32, [vp, vp, i32, i32, i32, C.c_float, i32, vp, i64, vp, i64, vp, i64, vp]),
         "z2h_verify_ws_bytes": (i64, [i32, i32, i32, i32]),
         "z2h_verify": (i32, [vp, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, vp]),
+        "z2h_prompt_attn": (i32, [vp, i32, vp, i32, i32, i32, i32, C.c_float, i32, vp, i64, vp, i64, vp, i64, vp, i64, vp]),
+        "z2h_moe_rows_ws_bytes": (i64, [vp, i32, i32]),
+        "z2h_moe_rows": (i32, [vp, vp, i32, i32, i32, vp, vp, i32, vp, i64, vp, i64, vp, vp, vp, i64, vp]),
+        "z2h_pages_ws_bytes": (i64, [vp, vp, i32]),
+        "z2h_pages_fork": (i32, [vp, vp, i32, i64, vp, i32, vp, vp, vp, vp, vp, vp, i64, vp]),
+        "z2h_pages_compact": (i32, [vp, vp, i32, i64, vp, vp, vp, vp, vp, i64, vp]),
         "z2h_step_paged_ws_bytes": (i64, [vp, vp, i32, i32]),
         "z2h_step_paged": (i32, [vp, vp, i64, i32, vp, vp, i32, vp, vp, vp, vp, vp, i32, i32, vp, vp, vp, vp, i64]),
         "z2h_last_error": (C.c_char_p, [vp]),
@@ -97,7 +103,8 @@ EXPORTS = ("z2h_model_create", "z2h_model_upload_tensor", "z2h_model_finalize", 
            "z2h_read_capture", "z2h_device_bytes", "z2h_set_graphs", "z2h_profile_begin", "z2h_profile_end", "z2h_sample", "z2h_set_prefill_chunk",
            "z2h_sample_feed", "z2h_step_resident", "z2h_create_batch_rows", "z2h_step_mixed",
            "z2h_rope_rows", "z2h_paged_append", "z2h_paged_ws_bytes", "z2h_paged_plan", "z2h_paged_attn", "z2h_verify_ws_bytes",
-           "z2h_verify", "z2h_step_paged_ws_bytes", "z2h_step_paged", "z2h_last_error", "z2h_destroy")
+           "z2h_verify", "z2h_prompt_attn", "z2h_moe_rows_ws_bytes", "z2h_moe_rows", "z2h_pages_ws_bytes", "z2h_pages_fork",
+           "z2h_pages_compact", "z2h_step_paged_ws_bytes", "z2h_step_paged", "z2h_last_error", "z2h_destroy")
 KERNEL_FAMILIES = ("resnorm", "gemv_qkv", "qkv_post", "attn", "attn_combine", "gemv_wo", "router_down", "router_tail",
                    "gemv_gateup", "gemv_down", "gemv_dense", "gemv_head", "swiglu")
 
@@ -126,6 +133,12 @@ class Pages(C.Structure):
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_int64), ("type", C.c_int32), ("n_pages", C.c_int32),
                 ("page_rows", C.c_int32), ("n_head_kv", C.c_int32), ("head_dim", C.c_int32), ("n_seq", C.c_int32),
                 ("table_len", C.c_int32), ("table", C.c_void_p)]
+
+
+class Experts(C.Structure):
+    """z2h_experts (include/z2h.h): gate, up and down are device pointers (ints)."""
+    _fields_ = [("gate", C.c_void_p), ("up", C.c_void_p), ("down", C.c_void_p), ("type", C.c_int32), ("n_expert", C.c_int32),
+                ("n_ff", C.c_int32), ("n_embd", C.c_int32)]
 
 
 class Z2HError(RuntimeError):
@@ -395,6 +408,36 @@ class Context:
                d_u_accept, d_u_draw, d_n_accept, d_codes, d_ws, ws_bytes, stream=None):
         self.check(lib().z2h_verify(self.ctx, n_seq, n_draft_max, n_codebooks, vocab, d_draft, d_n_draft, d_target, d_temperature,
                                     d_draft_probs, d_u_accept, d_u_draw, d_n_accept, d_codes, d_ws, ws_bytes, stream))
+
+    def prompt_attn(self, n_seq, d_row_start, n_rows, n_head, n_head_kv, head_dim, scale, type, d_q, q_stride, d_k, k_stride, d_v,
+                    v_stride, d_out, out_stride, stream=None):
+        self.check(lib().z2h_prompt_attn(self.ctx, n_seq, d_row_start, n_rows, n_head, n_head_kv, head_dim, scale, type, d_q, q_stride,
+                                         d_k, k_stride, d_v, v_stride, d_out, out_stride, stream))
+
+    def moe_rows_ws_bytes(self, experts, n_rows, top_k) -> int:
+        n = int(lib().z2h_moe_rows_ws_bytes(C.byref(experts), n_rows, top_k))
+        if n <= 0:
+            raise Z2HError(EINVAL, "z2h_moe_rows: sizes out of range")
+        return n
+
+    def moe_rows(self, experts, n_rows, top_k, renorm, d_logits, d_bias, type, d_x, x_stride, d_out, out_stride, d_sel, d_weights,
+                 d_ws, ws_bytes, stream=None):
+        self.check(lib().z2h_moe_rows(self.ctx, C.byref(experts), n_rows, top_k, 1 if renorm else 0, d_logits, d_bias, type, d_x, x_stride,
+                                      d_out, out_stride, d_sel, d_weights, d_ws, ws_bytes, stream))
+
+    def pages_ws_bytes(self, pages, n=0) -> int:
+        got = int(lib().z2h_pages_ws_bytes(self.ctx, C.byref(pages), n))
+        if got <= 0:
+            raise Z2HError(EINVAL, lib().z2h_last_error(self.ctx).decode())
+        return got
+
+    def pages_fork(self, pages, n_layer, layer_stride, d_refs, n, d_src, d_dst, d_rows, d_room, d_held, d_ws, ws_bytes, stream=None):
+        self.check(lib().z2h_pages_fork(self.ctx, C.byref(pages), n_layer, layer_stride, d_refs, n, d_src, d_dst, d_rows, d_room, d_held,
+                                        d_ws, ws_bytes, stream))
+
+    def pages_compact(self, pages, n_layer, layer_stride, d_refs, d_table_out, d_refs_out, d_n_used, d_ws, ws_bytes, stream=None):
+        self.check(lib().z2h_pages_compact(self.ctx, C.byref(pages), n_layer, layer_stride, d_refs, d_table_out, d_refs_out, d_n_used, d_ws,
+                                           ws_bytes, stream))
 
     def step_paged_ws_bytes(self, pages, n_rows, n_group) -> int:
         n = int(lib().z2h_step_paged_ws_bytes(self.ctx, C.byref(pages), n_rows, n_group))
