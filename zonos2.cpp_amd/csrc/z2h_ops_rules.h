@@ -295,7 +295,7 @@ inline MoeWs moe_ws(const z2h_experts & x, int n_rows, int top_k) {
 inline PoolWs pool_ws(int n_pages, int n) {
     PoolWs w;
     w.segs = (n_pages + POOL_SEG - 1) / POOL_SEG;
-    w.counts = (int64_t) w.segs * (POOL_SEG / 8);
+    w.counts = align256((int64_t) w.segs * (POOL_SEG / 8));
     w.items = w.counts + align256((int64_t) w.segs * 4);
     w.map = w.items + align256((int64_t) n * 32);
     w.moves = w.map + align256((int64_t) n_pages * 4);
