@@ -96,28 +96,367 @@ __device__ __forceinline__ void prompt_walk(const PromptArgs & a, int first, int
     }
 }
 
+// Rows of T in LDS, stored as they are with their 16-byte pieces permuted by row: keys so that 32 rows' pieces of the same dims take all
+// banks, values so that transposing reads (16 bits) or two rows 4 apart (fp32) do.
 template <int HD, typename T>
-__global__ void __launch_bounds__(256) k_prompt_walk(PromptArgs a) {
-    __shared__ float s_q[4][HD];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t id = (a.block0 + blockIdx.x) * 4 + wave;
-    if (id >= (int64_t) a.n_rows * a.n_head) return;
-    const int row = (int) (id / a.n_head), head = (int) (id % a.n_head);
-    // (the sequence by a search over the table, one row at a time)
-    int lo = -1, hi = a.n_seq;
-    while (hi - lo > 1) {
-        const int m = (lo + hi) >> 1;
-        if (prompt_start(a, m) <= row) lo = m; else hi = m;
+struct Rows {
+    static constexpr int N = 16 / (int) sizeof(T), NC = HD / N, RP = NC >= 16 ? 1 : 16 / NC;   // elements and pieces, rows per 256 bytes
+    static __device__ __forceinline__ int k_perm(int row) { return (row / RP) & (NC < 16 ? NC - 1 : 15); }
+    static __device__ __forceinline__ int v_perm(int row) {
+        if constexpr (sizeof(T) == 2) return 4 * ((row / RP) & (NC / 4 - 1));
+        else return NC >= 16 ? 8 * ((row >> 2) & 1) : 0;
     }
-    if (lo < 0 || row >= prompt_start(a, lo + 1)) return;
-    constexpr int E = HD >= 64 ? HD / 64 : 1;
-    float o[E], l;
-    prompt_walk<HD, T>(a, prompt_start(a, lo), row, head, s_q[wave], o, l);
-    T * out = (T *) a.out + row * a.os + (int64_t) head * HD + E * lane;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    if (E * lane < HD)
+    static __device__ __forceinline__ int k_at(int row, int piece) { return row * HD + (piece ^ k_perm(row)) * N; }
+    static __device__ __forceinline__ int v_at(int row, int piece) { return row * HD + (piece ^ v_perm(row)) * N; }
+};
+
+// One wave's 32 row-heads against 32 NT keys. S^T = K Q^T leaves a lane one row-head's scores (16 of 32 keys, the lane 32 away the others) in
+// the order in which they are the right operand of O^T = V^T P^T: weights never move between lanes.
+template <int HD, typename T> struct PromptMath;
+
+// 16 bits: v_mfma_f32_32x32x16; the weights meet the values as two numbers of the type, the second carrying what the first's rounding leaves.
+// One alone (2^-12, 2^-9 on average) would err as much as the output's own rounding over any number of keys.
+template <int HD, typename T>
+struct PromptMath {
+    static constexpr int NT = 2, KS = HD / 16, DT = HD / 32, BIAS = __is_same(T, _Float16) ? 6 : 0;
+    typedef typename Vec8<T>::type v8;
+    typedef Rows<HD, T> R;
+    v8 q[KS], p[2 * NT], pl[2 * NT];
+    int k_place[KS], v_place[DT];
+
+    __device__ __forceinline__ void init(const float (&x)[KS * 8], int lane) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) out[e] = (T) (o[e] * inv);
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) q[ks][j] = (T) x[8 * ks + j];
+        const int i16 = lane & 15, r = 4 * (lane >> 5) + (i16 >> 2);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) k_place[ks] = R::k_at(lane & 31, 2 * ks + (lane >> 5));
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+            const int d = 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
+            v_place[dt] = R::v_at(r, d >> 3) + (d & 7);
+        }
+    }
+    // dims that the lane holds of its query, in the order of init's x
+    static __device__ __forceinline__ int dim(int i, int lane) { return 16 * (i >> 3) + 8 * (lane >> 5) + (i & 7); }
+    static constexpr int QN = KS * 8;
+
+    __device__ __forceinline__ void scores(v16f_t (&s)[NT], const T * sk) const {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[n] = v16f_t{};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) s[n] = mfma32<T>(*(const v8 *) (sk + k_place[ks] + 32 * n * HD), q[ks], s[n]);
+    }
+    __device__ __forceinline__ float weigh(v16f_t (&s)[NT], float c, float mu) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                typedef typename Pair<float>::type f2;
+                typedef typename Pair<T>::type c2;
+                const f2 w = {__builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], c, -mu)), __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i + 1], c, -mu))};
+                const c2 hi = __builtin_convertvector(w, c2);
+                const c2 lo = __builtin_convertvector(two_rest(w, hi), c2);
+                p[2 * n + (i >> 3)][i & 7] = hi[0];
+                p[2 * n + (i >> 3)][(i & 7) + 1] = hi[1];
+                pl[2 * n + (i >> 3)][i & 7] = lo[0];
+                pl[2 * n + (i >> 3)][(i & 7) + 1] = lo[1];
+                sum += w[0];
+                sum += w[1];
+            }
+        return sum;
+    }
+    // V^T operand of 16 keys from LDS row r0 on, dims 32 dt ..: lanes 16 g + i read keys 4 (g / 2) + i / 4, dims 16 (g & 1) + 4 (i & 3)
+    __device__ __forceinline__ v8 values(const T * sv, int r0, int dt) const {
+        const T * at = sv + v_place[dt] + r0 * HD;
+        typedef __attribute__((address_space(3))) s4_t lds4;
+        const s4_t x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *) at);
+        const s4_t x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *) (at + 8 * HD));
+        return __builtin_bit_cast(v8, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+    __device__ __forceinline__ void add(v16f_t (&o)[DT], const T * sv) const {
+#pragma unroll
+        for (int t = 0; t < 2 * NT; ++t)
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const v8 v = values(sv, 16 * t, dt);
+                o[dt] = mfma32<T>(v, p[t], o[dt]);
+                o[dt] = mfma32<T>(v, pl[t], o[dt]);
+            }
+    }
+};
+
+// fp32: v_mfma_f32_32x32x2, products and weights in fp32 (1/16 of the 16-bit rate).
+template <int HD>
+struct PromptMath<HD, float> {
+    static constexpr int NT = 1, DT = HD / 32, BIAS = 0, QN = HD / 2;
+    typedef Rows<HD, float> R;
+    float q[QN];
+    float p[16];
+    int k_row, k_xor, v_at[DT];
+    typedef float v4 __attribute__((ext_vector_type(4)));
+
+    __device__ __forceinline__ void init(const float (&x)[QN], int lane) {
+#pragma unroll
+        for (int i = 0; i < QN; ++i) q[i] = x[i];
+        k_row = (lane & 31) * HD;
+        k_xor = (lane >> 5) ^ R::k_perm(lane & 31);              // (of the pieces 2 j + half, the row's permutation)
+        const int row = 4 * (lane >> 5);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) v_at[dt] = R::v_at(row, 8 * dt + ((lane & 31) >> 2)) + (lane & 3);
+    }
+    static __device__ __forceinline__ int dim(int i, int lane) { return 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3); }
+    __device__ __forceinline__ void scores(v16f_t (&s)[NT], const float * sk) const {
+        s[0] = v16f_t{};
+#pragma unroll
+        for (int j = 0; j < HD / 8; ++j) {
+            const v4 k = *(const v4 *) (sk + k_row + ((2 * j) ^ k_xor) * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], q[4 * j + e], s[0], 0, 0, 0);
+        }
+    }
+    __device__ __forceinline__ float weigh(v16f_t (&s)[NT], float c, float mu) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][i], c, -mu));
+            sum += p[i];
+        }
+        return sum;
+    }
+    // register i of a lane's half h is key 8 (i / 4) + 4 h + i % 4
+    __device__ __forceinline__ void add(v16f_t (&o)[DT], const float * sv) const {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(sv[v_at[dt] + (8 * (i >> 2) + (i & 3)) * HD], p[i], o[dt], 0, 0, 0);
+    }
+};
+
+// A wave's rows and running sums.
+template <int HD, typename T>
+struct PromptWave {
+    typedef PromptMath<HD, T> M;
+    M math;
+    v16f_t o[M::DT];
+    float m, l, c;                                               // m includes -BIAS: f16 weights up to 2^14, kept to 2^-24
+    int vis;                                                     // keys that the lane's row sees
+
+    // row-heads first_rh .. + 31 of rows row0 .. row0 + rows - 1, whose first sees `before` + 1 keys
+    __device__ __forceinline__ void init(const PromptArgs & a, int row0, int rows, int before, int g, int first_rh, int lane) {
+        const int group = a.n_head / a.nkv, rh = first_rh + (lane & 31);
+        const bool live = rh < rows * group;
+        const int r = live ? rh / group : 0, head = g * group + (live ? rh % group : 0);
+        const T * src = (const T *) a.q + (row0 + r) * a.qs + (int64_t) head * HD;
+        vis = live ? before + r + 1 : 0x7fffffff;
+        const bool zero = !live || a.scale == 0.0f;
+        const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
+        c = zero ? 1.0f : fabsf(a.scale) * 1.44269504088896341f;
+        float x[M::QN];
+        constexpr int N = 16 / (int) sizeof(T);
+        if (((uintptr_t) src & 15) == 0) {
+            typedef T tv __attribute__((ext_vector_type(N)));
+#pragma unroll
+            for (int i = 0; i < M::QN; i += N) {
+                const tv y = *(const tv *) (src + M::dim(i, lane));
+#pragma unroll
+                for (int j = 0; j < N; ++j) x[i + j] = (float) y[j];
+            }
+        } else
+#pragma unroll
+            for (int i = 0; i < M::QN; ++i) x[i] = (float) src[M::dim(i, lane)];
+        float up = sign;
+        if constexpr (sizeof(T) == 4) {
+            // a power of two keeps the scores of large queries finite, and those of tiny ones from vanishing
+            float mx = 0.0f;
+#pragma unroll
+            for (int i = 0; i < M::QN; ++i) mx = fmaxf(mx, fabsf(x[i]));
+            mx = fmaxf(mx, other_half(mx));
+            int e = 0;
+            if (mx > 0.0f && mx < __builtin_inff()) (void) frexpf(mx, &e);
+            e = min(-e, 120);
+            up = ldexpf(sign, e);
+            c = zero ? 1.0f : ldexpf(c, -e);
+        }
+        c = fminf(fmaxf(c, 0x1p-126f), 0x1p127f);                 // hidden scores stay -inf whatever the scale
+#pragma unroll
+        for (int i = 0; i < M::QN; ++i) x[i] = zero ? 0.0f : x[i] * up;
+        math.init(x, lane);
+        m = -__builtin_inff();
+        l = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < M::DT; ++dt) o[dt] = v16f_t{};
+    }
+
+    // keys key0 .. key0 + 32 NT (counted from the sequence's first) in LDS; those at or behind `vis` are hidden
+    __device__ __forceinline__ void step(const T * sk, const T * sv, int key0, int lane) {
+        constexpr int NT = M::NT;
+        v16f_t s[NT];
+        math.scores(s, sk);
+        if (__any(key0 + 32 * NT > vis)) {
+            const int h4 = 4 * (lane >> 5);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (key0 + 32 * n + 8 * (i >> 2) + h4 + (i & 3) >= vis) s[n][i] = -__builtin_inff();
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[n][i]);
+        mx = fmaxf(mx, other_half(mx)) * c;
+        // the maximum moves only where a score exceeds it by 2^8: rarely behind the first keys
+        const bool up = mx > m + (8.0f + M::BIAS);
+        if (__any(up)) {
+            const float mn = up ? mx - M::BIAS : m;
+            const float w = mn == m || m == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - mn);   // (nothing to scale yet)
+            m = mn;
+            l *= w;
+#pragma unroll
+            for (int dt = 0; dt < M::DT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[dt][i] *= w;
+        }
+        l += math.weigh(s, c, m == -__builtin_inff() ? 0.0f : m);
+        math.add(o, sv);
+    }
+
+    // What is not finite meets both parts of a weight, and hidden rows' weights of 0: the product is then NaN where the definition has
+    // infinity or leaves it out, never anything else that is wrong. So a row-head that holds NaN is formed once more, in plain fp32.
+    // s_q: HD floats of LDS of the wave's own.
+    __device__ __forceinline__ void store(const PromptArgs & a, int first, int row0, int rows, int g, int first_rh, int lane, float * s_q) {
+        const int group = a.n_head / a.nkv, heads = rows * group, rh = first_rh + (lane & 31);
+        l += other_half(l);
+        float nan = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < M::DT; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) nan = o[dt][i] != o[dt][i] ? 1.0f : nan;
+        nan = fmaxf(nan, other_half(nan));
+        const bool again = rh < heads && (nan != 0.0f || l != l);
+        if (rh < heads && !again) {
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            T * out = (T *) a.out + (row0 + rh / group) * a.os + (int64_t) (g * group + rh % group) * HD;
+#pragma unroll
+            for (int dt = 0; dt < M::DT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4)
+                    store4(out + 32 * dt + 2 * i + 4 * (lane >> 5), o[dt][i] * inv, o[dt][i + 1] * inv, o[dt][i + 2] * inv, o[dt][i + 3] * inv);
+        }
+        for (unsigned long long todo = __ballot(again) & 0xffffffffull; todo; todo &= todo - 1) {
+            constexpr int E = HD >= 64 ? HD / 64 : 1;
+            const int at = first_rh + __builtin_ctzll(todo), row = row0 + at / group, head = g * group + at % group;
+            float x[E], sum;
+            prompt_walk<HD, T>(a, first, row, head, s_q, x, sum);
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            T * out = (T *) a.out + row * a.os + (int64_t) head * HD + E * lane;
+            if (E * lane < HD)
+#pragma unroll
+                for (int e = 0; e < E; ++e) out[e] = (T) (x[e] * inv);
+        }
+    }
+};
+
+// Brings 16 rows of K or V to LDS at a time. ALIGNED: every piece is 16 bytes that may be loaded at once, straight to LDS; else by elements.
+template <int HD, typename T, bool ALIGNED>
+struct PromptLoad {
+    typedef Rows<HD, T> R;
+    static constexpr int ROWS = 64 / R::NC, N = 16 / ROWS;       // rows per instruction, instructions for 16 rows
+    const T * k, * v;                                            // the key head's first row of the sequence
+    int64_t ks, vs;
+    int last, row, piece_k[N], piece_v[N];                       // of the lane: its row, its pieces' first elements
+    __device__ __forceinline__ PromptLoad(const PromptArgs & a, int first, int n_keys, int g, int lane)
+        : k((const T *) a.k + first * a.ks + (int64_t) g * HD), v((const T *) a.v + first * a.vs + (int64_t) g * HD), ks(a.ks), vs(a.vs),
+          last(n_keys - 1), row(lane / R::NC) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            piece_k[i] = ((lane % R::NC) ^ R::k_perm(i * ROWS + row)) * R::N;
+            piece_v[i] = ((lane % R::NC) ^ R::v_perm(i * ROWS + row)) * R::N;
+        }
+    }
+    static __device__ __forceinline__ void move(const T * from, T * to, int lane) {
+        if constexpr (ALIGNED) to_lds(from, to);
+        else {
+            T x[R::N];
+#pragma unroll
+            for (int j = 0; j < R::N; ++j) x[j] = from[j];
+#pragma unroll
+            for (int j = 0; j < R::N; ++j) to[lane * R::N + j] = x[j];
+        }
+    }
+    // rows key .. key + 15 (a multiple of 16) to the rows of LDS at `to`; rows behind the sequence's end are its last one again
+    __device__ __forceinline__ void keys16(int key, T * to, int lane) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) move(k + min(key + i * ROWS + row, last) * ks + piece_k[i], to + i * ROWS * HD, lane);
+    }
+    __device__ __forceinline__ void values16(int key, T * to, int lane) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) move(v + min(key + i * ROWS + row, last) * vs + piece_v[i], to + i * ROWS * HD, lane);
+    }
+};
+
+// What a block has to do: rows row0 .. row0 + rows - 1 of a sequence that begins at row `first`, with key head g. Long tiles come first.
+struct PromptTile { int first, row0, rows, g; };
+__device__ __forceinline__ PromptTile prompt_tile(const PromptArgs & a, int tile_rows, int lane) {
+    const int64_t id = a.block0 + blockIdx.x;
+    const int64_t slot = z2o::prompt_slots(a.n_rows, a.n_seq, tile_rows) - 1 - id / a.nkv;
+    PromptTile t;
+    t.g = (int) (id % a.nkv);
+    const int s = prompt_seq(a, slot, tile_rows, lane), start = prompt_start(a, s), end = prompt_start(a, s + 1);
+    const int64_t at = start + (slot - z2o::prompt_slot(start, s, tile_rows)) * tile_rows;
+    t.first = start;
+    t.row0 = (int) min(max(at, (int64_t) 0), (int64_t) a.n_rows);
+    t.rows = max(0, min(tile_rows, end - t.row0));
+    if (at < start) t.rows = 0;
+    return t;
+}
+
+// Four waves of 32 row-heads each over the same keys, 32 NT at a time in LDS, the next ones on their way into the other buffer.
+template <int HD, typename T, bool ALIGNED>
+__global__ void __launch_bounds__(256, 2) k_prompt(PromptArgs a) {
+    constexpr int KEYS = 32 * PromptMath<HD, T>::NT;
+    __shared__ __attribute__((aligned(1024))) T s_k0[KEYS * HD], s_k1[KEYS * HD], s_v0[KEYS * HD], s_v1[KEYS * HD];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6), group = a.n_head / a.nkv;
+    const PromptTile t = prompt_tile(a, z2o::tile_rows(group), lane);
+    if (t.rows <= 0) return;
+    const int before = t.row0 - t.first, n_keys = before + t.rows;
+    const PromptLoad<HD, T, ALIGNED> load(a, t.first, n_keys, t.g, lane);
+    auto bring = [&](int key, T * sk, T * sv) __attribute__((always_inline)) {
+        constexpr int PARTS = KEYS / 16;                         // 16 rows each of K and of V
+#pragma unroll
+        for (int i = 0; i < 2 * PARTS; i += 4) {
+            const int part = i + wave;
+            if (part < PARTS) load.keys16(key + 16 * part, sk + 16 * part * HD, lane);
+            else load.values16(key + 16 * (part - PARTS), sv + 16 * (part - PARTS) * HD, lane);
+        }
+    };
+    bring(0, s_k0, s_v0);
+    PromptWave<HD, T> w;
+    w.init(a, t.row0, t.rows, before, t.g, 32 * wave, lane);
+    // the wave's rows see keys up to `mine`
+    const int mine = 32 * wave < t.rows * group ? before + min(t.rows, (32 * wave + 31) / group + 1) : 0;
+    int key = 0;
+    auto stage = [&](const T * sk, const T * sv, T * ok, T * ov) __attribute__((always_inline)) {
+        wait_loads_but<0>();
+        __syncthreads();
+        if (key + KEYS < n_keys) bring(key + KEYS, ok, ov);
+        if (key < mine) w.step(sk, sv, key, lane);
+        key += KEYS;
+    };
+    while (key < n_keys) {
+        stage(s_k0, s_v0, s_k1, s_v1);
+        if (key >= n_keys) break;
+        stage(s_k1, s_v1, s_k0, s_v0);
+    }
+    __syncthreads();
+    w.store(a, t.first, t.row0, t.rows, t.g, 32 * wave, lane, (float *) s_k0 + wave * HD);
 }
 
 } // namespace z2d

@@ -8,8 +8,13 @@ namespace {
 
 template <int HD, typename T>
 void prompt_launch(PromptArgs & a, hipStream_t st) {
-    for (int64_t n = ((int64_t) a.n_rows * a.n_head + 3) / 4; a.block0 < n; a.block0 += z2o::launch_blocks(256))
-        hipLaunchKernelGGL((k_prompt_walk<HD, T>), dim3(std::min(n - a.block0, z2o::launch_blocks(256))), dim3(256), 0, st, a);
+    const auto al = [](const void * p, int64_t stride) { return (uintptr_t) p % 16 == 0 && stride * (int64_t) sizeof(T) % 16 == 0; };
+    const bool aligned = al(a.k, a.ks) && al(a.v, a.vs);
+    for (int64_t n = z2o::prompt_slots(a.n_rows, a.n_seq, z2o::tile_rows(a.n_head / a.nkv)) * a.nkv; a.block0 < n; a.block0 += z2o::launch_blocks(256)) {
+        const dim3 grid(std::min(n - a.block0, z2o::launch_blocks(256)));
+        if (aligned) hipLaunchKernelGGL((k_prompt<HD, T, true>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((k_prompt<HD, T, false>), grid, dim3(256), 0, st, a);
+    }
 }
 template <int HD>
 void prompt_launch(PromptArgs & a, int type, hipStream_t st) {
