@@ -6,10 +6,19 @@ using namespace z2d;
 
 namespace {
 
+template <typename T, typename TW, int CT>
+void down_launch(const MoeArgs & a, hipStream_t st) {
+    hipLaunchKernelGGL((k_moe_down<T, TW, CT>), dim3(a.tiles, a.shares), dim3(MOE_T), 0, st, a);
+}
 template <typename T, typename TW>
 void moe_launch(const MoeArgs & a, hipStream_t st) {
-    hipLaunchKernelGGL((k_moe_gate_up<T, TW>), dim3(1024), dim3(256), 0, st, a);
-    hipLaunchKernelGGL((k_moe_down<T, TW>), dim3(1024), dim3(256), 0, st, a);
+    const int blocks = (int) std::min<int64_t>(512, (int64_t) std::min(a.E, a.n * a.k) * (a.F / 8));
+    if (a.n <= 16) hipLaunchKernelGGL((k_moe_gate_up<T, TW, 1>), dim3(blocks), dim3(MOE_T), 0, st, a);
+    else hipLaunchKernelGGL((k_moe_gate_up<T, TW, 2>), dim3(blocks), dim3(MOE_T), 0, st, a);
+    if (a.n <= 16) down_launch<T, TW, 1>(a, st);
+    else if (a.n <= 32) down_launch<T, TW, 2>(a, st);
+    else if (a.n <= 64) down_launch<T, TW, 4>(a, st);
+    else down_launch<T, TW, 8>(a, st);
 }
 
 } // namespace
@@ -39,7 +48,9 @@ int z2h_moe_rows(z2h_ctx * ctx, const z2h_experts * experts, int n_rows, int top
     a.E = experts->n_expert; a.F = experts->n_ff; a.D = experts->n_embd; a.n = n_rows; a.k = top_k; a.renorm = renorm;
     a.logits = d_logits; a.bias = d_bias; a.x = d_x; a.xs = x_stride; a.out = d_out; a.os = out_stride;
     a.sel = d_sel; a.weights = d_weights;
-    a.routes = (int32_t *) ws; a.w = (float *) (ws + w.w); a.h = (float *) (ws + w.h);
+    a.shares = z2o::moe_shares(a.D); a.tiles = (a.D + 15) / 16;
+    a.table = (MoeTable *) ws; a.touched = (MoeTouched *) (ws + w.touched); a.w = (float *) (ws + w.w);
+    a.tickets = (int32_t *) (ws + w.tickets); a.parts = (float *) (ws + w.parts); a.h = (float *) (ws + w.h);
     ON_DEVICE;
     switch (type) {
         case Z2H_F32: moe_launch<float, _Float16>(a, (hipStream_t) stream); break;

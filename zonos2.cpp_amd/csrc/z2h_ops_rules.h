@@ -282,12 +282,21 @@ inline int64_t verify_ws_bytes(int n_seq, int n_draft_max, int n_codebooks, int 
            align256(draws * ((vocab + 255) / 256) * 8);
 }
 
-struct MoeWs { int64_t w = 0, h = 0, bytes = 0; };
+// Blocks that share 16 dims of the output: enough for about 512 blocks.
+inline int moe_shares(int n_embd) {
+    const int tiles = (n_embd + 15) / 16, s = (512 + tiles - 1) / tiles;
+    return s < 1 ? 1 : s > 16 ? 16 : s;
+}
+struct MoeWs { int64_t touched = 0, w = 0, tickets = 0, parts = 0, h = 0, bytes = 0; };
 inline MoeWs moe_ws(const z2h_experts & x, int n_rows, int top_k) {
     MoeWs m;
     const int64_t routes = (int64_t) n_rows * top_k;
-    m.w = 256 + align256(routes * 4);
-    m.h = m.w + align256(routes * 4);
+    const int shares = moe_shares(x.n_embd);
+    m.touched = 256;
+    m.w = m.touched + align256((routes < x.n_expert ? routes : x.n_expert) * 24);
+    m.tickets = m.w + align256(routes * 4);
+    m.parts = m.tickets + align256((int64_t) (x.n_embd + 15) / 16 * 4);
+    m.h = m.parts + (shares > 1 ? align256((int64_t) shares * n_rows * x.n_embd * 4) : 0);
     m.bytes = m.h + align256(routes * x.n_ff * 4);
     return m;
 }
