@@ -182,12 +182,12 @@ __device__ __forceinline__ void route(const MoeArgs & a, MoeRouting & s) {
 // the i-th row that takes an expert (it has more)
 __device__ __forceinline__ int nth_row(const unsigned * rows, int i) {
     int word = 0;
+    unsigned w = rows[0];
 #pragma unroll
-    for (int m = 0; m < MOE_MASKS - 1; ++m) {
-        const int c = __popc(rows[word]);
-        if (i >= c) { i -= c; ++word; }
+    for (int m = 1; m < MOE_MASKS; ++m) {
+        const int c = __popc(w);
+        if (word == m - 1 && i >= c) { i -= c; word = m; w = rows[m]; }
     }
-    unsigned w = rows[word];
     for (; i > 0; --i) w &= w - 1;
     return 32 * word + __builtin_ctz(w);
 }
@@ -261,18 +261,49 @@ struct SplitColumn {
 };
 
 // ---- gate and up
+// Blocks of one compute unit at a time: two where the registers allow it.
+template <typename T, int NT>
+constexpr int moe_per_cu() { return sizeof(T) == 2 && NT == 1 ? 2 : 1; }
 constexpr int MOE_FR = 8;                                        // operands of a wave in a pass: 256 columns of the matrix
-// NT tiles of 16 rows of x. The wave's columns are one of eight slices of up to 2048; tiles of 16 matrix rows (8 of gate, 8 of up) follow each
-// other, the next one's weights on their way while this one is multiplied, and the slices' sums meet in LDS.
+
+// The tiles of 16 matrix rows (8 of gate, 8 of up) that a block has, in the order in which it takes them: for every 16 NT rows of x that take the
+// expert, all its tiles; and a tile's columns in passes of up to 2048.
+struct MoeCursor {
+    int tile, pass, c0, t, e, count, from, to;
+    __device__ __forceinline__ void enter(const MoeRouting & s, int tile_, int per, int end) {
+        tile = from = tile_;
+        pass = c0 = 0;
+        t = tile / per;
+        to = min(end, (t + 1) * per);
+        e = __builtin_amdgcn_readfirstlane((int) s.list[t]);
+        count = 0;
+#pragma unroll
+        for (int i = 0; i < MOE_MASKS; ++i) count += __popc(s.rows[e][i]);
+        count = __builtin_amdgcn_readfirstlane(count);
+    }
+    // false: that was the last
+    __device__ __forceinline__ bool next(const MoeRouting & s, int per, int end, int passes, int rows) {
+        if (++pass < passes) return true;
+        pass = 0;
+        if (++tile < to) return true;
+        if (c0 + rows < count) { tile = from; c0 += rows; return true; }
+        if (to >= end) return false;
+        enter(s, to, per, end);
+        return true;
+    }
+};
+
+// NT tiles of 16 rows of x stay in registers while the expert's tiles pass by, the next tile's weights on their way. A wave has one of eight
+// slices of the columns; the slices' sums meet in LDS.
 template <typename T, typename TW, int NT>
-__global__ void __launch_bounds__(MOE_T, NT == 1 ? 4 : 2) k_moe_gate_up(MoeArgs a) {
+__global__ void __launch_bounds__(MOE_T, (2 * moe_per_cu<T, NT>())) k_moe_gate_up(MoeArgs a) {
     constexpr bool SPLIT = sizeof(T) == 4;
     typedef typename Vec8<TW>::type v8;
     __shared__ MoeRouting s;
     __shared__ float s_sum[2][MOE_WAVES][NT][256];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     route(a, s);
-    if (blockIdx.x == 0) {
+    if (blockIdx.x == gridDim.x - 1) {
         for (int i = tid; i < a.n * a.k; i += MOE_T) {
             if (a.sel) a.sel[i] = s.sel[i];
             if (a.weights) a.weights[i] = s.w[i];
@@ -285,183 +316,237 @@ __global__ void __launch_bounds__(MOE_T, NT == 1 ? 4 : 2) k_moe_gate_up(MoeArgs 
             for (int i = 0; i < MOE_MASKS; ++i) x.rows[i] = s.rows[x.e][i];
             a.touched[t] = x;
         }
-        for (int r = tid; r < a.n; r += MOE_T)
-            for (int j = 0; j < a.k; ++j) {
-                const int e = s.sel[r * a.k + j];
-                if (e < 0) continue;
-                int t = 0;
-                for (int hi = s.n; hi - t > 1;) { const int m = (t + hi) >> 1; if (s.list[m] <= e) t = m; else hi = m; }
-                a.w[s.pos0[t] + rows_before(s.rows[e], r)] = s.w[r * a.k + j];
-            }
+        for (int i = tid; i < a.n * a.k; i += MOE_T) {
+            const int e = s.sel[i];
+            if (e < 0) continue;
+            int t = 0;
+            for (int hi = s.n; hi - t > 1;) { const int m = (t + hi) >> 1; if (s.list[m] <= e) t = m; else hi = m; }
+            a.w[s.pos0[t] + rows_before(s.rows[e], i / a.k)] = s.w[i];
+        }
     }
-    const int per = a.F / 8, n_tiles = s.n * per, frags = (a.D + 31) / 32;
+    const int per = a.F / 8, n_tiles = __builtin_amdgcn_readfirstlane(s.n) * per, frags = (a.D + 31) / 32;
     const int t0 = (int) ((int64_t) n_tiles * blockIdx.x / gridDim.x), t1 = (int) ((int64_t) n_tiles * (blockIdx.x + 1) / gridDim.x);
+    if (t0 >= t1) return;
     const int passes = (frags + MOE_FR * MOE_WAVES - 1) / (MOE_FR * MOE_WAVES), mine = (frags + passes * MOE_WAVES - 1) / (passes * MOE_WAVES);
-    const int k8 = 8 * (lane >> 4), col = lane & 15, r16 = lane & 15;
-    // the lane's matrix row of tile i of an expert: gate for lanes' rows 0 .. 7, up behind them
-    const TW * mat = (const TW *) (r16 < 8 ? a.gate : a.up) + (int64_t) (r16 & 7) * a.D + k8;
-    int buf = 0;
-    for (int from = t0; from < t1;) {
-        const int t = from / per, e = s.list[t], to = min(t1, (t + 1) * per);
-        int count = 0;
+    const int k8 = 8 * (lane >> 4), col = lane & 15;
+    // the lane's matrix row of an expert's first tile: gate for rows 0 .. 7 of the operand, up behind them
+    const TW * mat = (const TW *) (col < 8 ? a.gate : a.up) + (int64_t) (col & 7) * a.D + k8;
+    auto inside = [&](int f0, int i) __attribute__((always_inline)) { return i < mine && 32 * (f0 + i) + k8 < a.D; };
+    auto request = [&](const MoeCursor & c, v8 (&w)[MOE_FR]) __attribute__((always_inline)) {
+        const int f0 = (c.pass * MOE_WAVES + wave) * mine;
+        const TW * p = mat + ((int64_t) c.e * a.F + (c.tile - c.t * per) * 8) * a.D + 32 * f0;
 #pragma unroll
-        for (int i = 0; i < MOE_MASKS; ++i) count += __popc(s.rows[e][i]);
-        const TW * base = mat + ((int64_t) e * a.F - (int64_t) t * per * 8) * a.D;      // + tile * 8 rows
-        for (int c0 = 0; c0 < count; c0 += 16 * NT) {
-            for (int tile = from; tile < to; ++tile) {
-                v4f_t sum[NT];
+        for (int i = 0; i < MOE_FR; ++i) w[i] = inside(f0, i) ? *(const v8 *) (p + 32 * i) : v8{};
+    };
+    SplitColumn<MOE_FR, TW> b[NT];                               // 16-bit rows: hi alone
+    auto columns = [&](const MoeCursor & c) __attribute__((always_inline)) {
+        const int f0 = (c.pass * MOE_WAVES + wave) * mine;
 #pragma unroll
-                for (int c = 0; c < NT; ++c) sum[c] = v4f_t{};
-                for (int pass = 0; pass < passes; ++pass) {
-                    const int f0 = (pass * MOE_WAVES + wave) * mine;
-                    v8 w[MOE_FR];
-                    const TW * p = base + (int64_t) tile * 8 * a.D + 32 * f0;
+        for (int n = 0; n < NT; ++n) {
+            const int at = c.c0 + 16 * n + col;
+            const bool live = at < c.count;
+            const T * x = (const T *) a.x + (live ? nth_row(s.rows[c.e], at) : 0) * a.xs + 32 * f0 + k8;
+            if constexpr (SPLIT) {
+                float y[MOE_FR][8];
 #pragma unroll
-                    for (int i = 0; i < MOE_FR; ++i) w[i] = i < mine && 32 * (f0 + i) + k8 < a.D ? *(const v8 *) (p + 32 * i) : v8{};
+                for (int i = 0; i < MOE_FR; ++i) {
+                    if (live && inside(f0, i)) load8(x + 32 * i, y[i]);
+                    else
 #pragma unroll
-                    for (int c = 0; c < NT; ++c) {
-                        const int at = c0 + 16 * c + col;
-                        const bool live = at < count;
-                        const T * x = (const T *) a.x + (live ? nth_row(s.rows[e], at) : 0) * a.xs + 32 * f0 + k8;
-                        float y[MOE_FR][8];
+                        for (int j = 0; j < 8; ++j) y[i][j] = 0.0f;
+                }
+                b[n].set(y);
+            } else {
+                const bool wide = ((uintptr_t) x & 15) == 0;
 #pragma unroll
-                        for (int i = 0; i < MOE_FR; ++i) {
-                            if (live && i < mine && 32 * (f0 + i) + k8 < a.D) load8(x + 32 * i, y[i]);
-                            else
+                for (int i = 0; i < MOE_FR; ++i) {
+                    b[n].hi[i] = v8{};
+                    if (live && inside(f0, i)) {
+                        if (wide) b[n].hi[i] = *(const v8 *) (x + 32 * i);
+                        else
 #pragma unroll
-                                for (int j = 0; j < 8; ++j) y[i][j] = 0.0f;
-                        }
-                        if constexpr (SPLIT) {
-                            SplitColumn<MOE_FR, TW> b;
-                            b.set(y);
-                            v4f_t part{};
-#pragma unroll
-                            for (int i = 0; i < MOE_FR; ++i) {
-                                part = mfma16<TW>(w[i], b.hi[i], part);
-                                part = mfma16<TW>(w[i], b.lo[i], part);
-                            }
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) sum[c][i] = __builtin_fmaf(part[i], b.back, sum[c][i]);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < MOE_FR; ++i) {
-                                v8 b;
-#pragma unroll
-                                for (int j = 0; j < 8; ++j) b[j] = (TW) y[i][j];
-                                sum[c] = mfma16<TW>(w[i], b, sum[c]);
-                            }
-                        }
+                            for (int j = 0; j < 8; ++j) b[n].hi[i][j] = x[32 * i + j];
                     }
                 }
-#pragma unroll
-                for (int c = 0; c < NT; ++c)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s_sum[buf][wave][c][(4 * (lane >> 4) + i) * 16 + col] = sum[c][i];
-                lds_sync();
-                for (int i = tid; i < NT * 128; i += MOE_T) {
-                    const int c = i >> 7, row = (i >> 3) & 15, f = i & 7;
-                    if (c0 + 16 * c + row < count) {
-                        float g = 0.0f, u = 0.0f;
-#pragma unroll
-                        for (int v = 0; v < MOE_WAVES; ++v) {
-                            g += s_sum[buf][v][c][f * 16 + row];
-                            u += s_sum[buf][v][c][(f + 8) * 16 + row];
-                        }
-                        a.h[(int64_t) (s.pos0[t] + c0 + 16 * c + row) * a.F + (tile - t * per) * 8 + f] = z_silu(g) * u;
-                    }
-                }
-                buf ^= 1;
             }
         }
-        from = to;
+    };
+    v4f_t sum[NT];
+    MoeCursor cur, nxt;
+    int buf = 0;
+    bool fresh = true, more;                                     // the right operands have to be formed anew
+    auto step = [&](const v8 (&w)[MOE_FR], v8 (&ahead)[MOE_FR]) __attribute__((always_inline)) {
+        nxt = cur;
+        more = nxt.next(s, per, t1, passes, 16 * NT);
+        if (more) request(nxt, ahead);
+        if (fresh) columns(cur);
+        if (cur.pass == 0)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) sum[n] = v4f_t{};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            v4f_t part{};
+            if constexpr (!SPLIT) part = sum[n];
+#pragma unroll
+            for (int i = 0; i < MOE_FR; ++i) {
+                part = mfma16<TW>(w[i], b[n].hi[i], part);
+                if constexpr (SPLIT) part = mfma16<TW>(w[i], b[n].lo[i], part);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[n][i] = SPLIT ? __builtin_fmaf(part[i], b[n].back, sum[n][i]) : part[i];
+        }
+        if (cur.pass == passes - 1) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s_sum[buf][wave][n][(4 * (lane >> 4) + i) * 16 + col] = sum[n][i];
+            lds_sync();
+            if (tid < NT * 128) {
+                const int n = tid >> 7, row = (tid >> 3) & 15, f = tid & 7, at = cur.c0 + 16 * n + row;
+                if (at < cur.count) {
+                    float g = 0.0f, u = 0.0f;
+#pragma unroll
+                    for (int v = 0; v < MOE_WAVES; ++v) {
+                        g += s_sum[buf][v][n][f * 16 + row];
+                        u += s_sum[buf][v][n][(f + 8) * 16 + row];
+                    }
+                    a.h[(int64_t) (s.pos0[cur.t] + at) * a.F + (cur.tile - cur.t * per) * 8 + f] = z_silu(g) * u;
+                }
+            }
+            buf ^= 1;                                            // (the next tile's sums go elsewhere: one barrier per tile)
+        }
+        fresh = more && (passes > 1 || nxt.t != cur.t || nxt.c0 != cur.c0);
+        cur = nxt;
+    };
+    v8 w0[MOE_FR], w1[MOE_FR];
+    cur.enter(s, t0, per, t1);
+    request(cur, w0);
+    for (;;) {
+        step(w0, w1);
+        if (!more) break;
+        step(w1, w0);
+        if (!more) break;
     }
 }
 
 // ---- down
-constexpr int MOE_DF = 4;                                        // operands of a unit: 128 hidden dims of an expert
-// 16 dims of out and all rows (CT tiles of 16) per block, over its share of the units (an expert's 128 hidden dims), dealt to the waves in runs.
-// The right operand is w h of the rows that take the expert, 0 for the others, whose sums it does not reach whatever the weights hold.
-template <typename T, typename TW, int CT>
-__global__ void __launch_bounds__(MOE_T, CT <= 2 ? 4 : 2) k_moe_down(MoeArgs a) {
+constexpr int MOE_DF = 4, MOE_DW = 4, MOE_DT = 64 * MOE_DW;      // operands of a unit: 128 hidden dims of an expert; waves of a block
+// 16 dims of out and all rows per block, over its share of the units (128 hidden dims of an expert), dealt to the waves in runs. The right
+// operand is w h of 16 rows that take the expert; its sums go to the rows' places in LDS when the wave turns to other rows. The next unit's
+// weights and h are on their way while this one is multiplied.
+template <typename T, typename TW>
+__global__ void __launch_bounds__(MOE_DT, 3) k_moe_down(MoeArgs a) {
     typedef typename Vec8<TW>::type v8;
-    __shared__ float s_sum[MOE_WAVES][CT][256];
+    extern __shared__ __attribute__((aligned(16))) float s_out[];        // [waves][n][16]
     __shared__ int s_last;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    float * out = s_out + wave * a.n * 16;
+    for (int i = lane; i < a.n * 4; i += 64) ((v4f_t *) out)[i] = v4f_t{};
     const int n = uniform(&a.table->n)[0], chunks = (a.F + 32 * MOE_DF - 1) / (32 * MOE_DF), units = n * chunks;
-    const int share = (int) blockIdx.y * MOE_WAVES + wave, shares = a.shares * MOE_WAVES;
+    const int share = (int) blockIdx.y * MOE_DW + wave, shares = a.shares * MOE_DW;
     const int u0 = (int) ((int64_t) units * share / shares), u1 = (int) ((int64_t) units * (share + 1) / shares);
     const int k8 = 8 * (lane >> 4), col = lane & 15, d = 16 * (int) blockIdx.x + col;
     const TW * mat = (const TW *) a.down + (int64_t) min(d, a.D - 1) * a.F + k8;
-    v4f_t sum[CT];
+    struct Unit { int u, t, from, to, c0, count; MoeTouched x; };
+    auto enter = [&](Unit & c, int u) __attribute__((always_inline)) {
+        c.u = c.from = u;
+        c.t = u / chunks;
+        c.to = min(u1, (c.t + 1) * chunks);
+        c.c0 = c.count = 0;
+        c.x = uniform_copy(a.touched + c.t);
 #pragma unroll
-    for (int c = 0; c < CT; ++c) sum[c] = v4f_t{};
-    for (int u = u0; u < u1; ++u) {
-        const MoeTouched t = uniform_copy(a.touched + u / chunks);
-        const int f0 = u % chunks * 32 * MOE_DF;
-        v8 w[MOE_DF];
-        const TW * p = mat + (int64_t) t.e * a.D * a.F + f0;
+        for (int i = 0; i < MOE_MASKS; ++i) c.count += __popc(c.x.rows[i]);
+    };
+    auto next = [&](Unit & c) __attribute__((always_inline)) {
+        if (++c.u < c.to) return true;
+        if (c.c0 + 16 < c.count) { c.u = c.from; c.c0 += 16; return true; }
+        if (c.to >= u1) return false;
+        enter(c, c.to);
+        return true;
+    };
+    struct Data { v8 w[MOE_DF]; float h[MOE_DF][8], weight; };
+    auto request = [&](const Unit & c, Data & x) __attribute__((always_inline)) {
+        const int f0 = (c.u - c.t * chunks) * 32 * MOE_DF, at = c.c0 + col;
+        const TW * p = mat + (int64_t) c.x.e * a.D * a.F + f0;
+        const int pos = c.x.pos0 + min(at, c.count - 1);
+        const float * h = a.h + (int64_t) pos * a.F + f0 + k8;
 #pragma unroll
-        for (int i = 0; i < MOE_DF; ++i) w[i] = d < a.D && f0 + 32 * i + k8 < a.F ? *(const v8 *) (p + 32 * i) : v8{};
+        for (int i = 0; i < MOE_DF; ++i) {
+            const bool in = f0 + 32 * i + k8 < a.F;
+            x.w[i] = d < a.D && in ? *(const v8 *) (p + 32 * i) : v8{};
+            v4f_t y0{}, y1{};
+            if (at < c.count && in) { y0 = *(const v4f_t *) (h + 32 * i); y1 = *(const v4f_t *) (h + 32 * i + 4); }
 #pragma unroll
-        for (int c = 0; c < CT; ++c) {
-            if (!((t.rows[c >> 1] >> (16 * (c & 1))) & 0xffffu)) continue;
-            const int row = 16 * c + col;
-            const bool live = t.rows[c >> 1] >> (row & 31) & 1;
-            const int pos = live ? t.pos0 + rows_before(t.rows, row) : 0;
-            const float wt = live ? a.w[pos] : 0.0f;
-            const float * h = a.h + (int64_t) pos * a.F + f0 + k8;
-            float y[MOE_DF][8];
+            for (int j = 0; j < 4; ++j) { x.h[i][j] = y0[j]; x.h[i][4 + j] = y1[j]; }
+        }
+        x.weight = a.w[pos];
+    };
+    v4f_t sum{};
+    Unit cur, nxt;
+    bool more = u0 < u1;
+    auto step = [&](const Data & x, Data & ahead) __attribute__((always_inline)) {
+        nxt = cur;
+        more = next(nxt);
+        if (more) request(nxt, ahead);
+        SplitColumn<MOE_DF, TW> b;
+        b.set(x.h);
+        v4f_t part{};
 #pragma unroll
-            for (int i = 0; i < MOE_DF; ++i) {
-                if (live && f0 + 32 * i + k8 < a.F) load8(h + 32 * i, y[i]);
-                else
+        for (int i = 0; i < MOE_DF; ++i) {
+            part = mfma16<TW>(x.w[i], b.hi[i], part);
+            part = mfma16<TW>(x.w[i], b.lo[i], part);
+        }
+        const float back = b.back * x.weight;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) y[i][j] = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) y[i][j] *= wt;
+        for (int i = 0; i < 4; ++i) sum[i] = __builtin_fmaf(part[i], back, sum[i]);
+        if (!more || nxt.t != cur.t || nxt.c0 != cur.c0) {
+            if (cur.c0 + col < cur.count) {
+                v4f_t * to = (v4f_t *) (out + nth_row(cur.x.rows, cur.c0 + col) * 16 + 4 * (lane >> 4));
+                *to += sum;
             }
-            SplitColumn<MOE_DF, TW> b;
-            b.set(y);
-            v4f_t part{};
-#pragma unroll
-            for (int i = 0; i < MOE_DF; ++i) {
-                part = mfma16<TW>(w[i], b.hi[i], part);
-                part = mfma16<TW>(w[i], b.lo[i], part);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sum[c][i] = live ? __builtin_fmaf(part[i], b.back, sum[c][i]) : sum[c][i];
+            sum = v4f_t{};
+        }
+        cur = nxt;
+    };
+    if (more) {
+        Data x0, x1;
+        enter(cur, u0);
+        request(cur, x0);
+        for (;;) {
+            step(x0, x1);
+            if (!more) break;
+            step(x1, x0);
+            if (!more) break;
         }
     }
-#pragma unroll
-    for (int c = 0; c < CT; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s_sum[wave][c][(4 * (lane >> 4) + i) * 16 + col] = sum[c][i];
     __syncthreads();
-    auto store = [&](int row, int d, float v) {
+    auto store = [&](int row, int at, float v) {
         if (a.table->no_number[row >> 5] >> (row & 31) & 1) v = __builtin_nanf("");
-        ((T *) a.out)[row * a.os + d] = (T) v;
+        ((T *) a.out)[row * a.os + at] = (T) v;
     };
-    for (int i = tid; i < CT * 256; i += MOE_T) {
-        const int row = i >> 4, dd = i & 15, at = 16 * (int) blockIdx.x + dd;
-        if (row >= a.n || at >= a.D) continue;
+    for (int i = tid; i < a.n * 16; i += MOE_DT) {
+        const int row = i >> 4, at = 16 * (int) blockIdx.x + (i & 15);
+        if (at >= a.D) continue;
         float v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < MOE_WAVES; ++w) v += s_sum[w][row >> 4][dd * 16 + (row & 15)];
+        for (int w = 0; w < MOE_DW; ++w) v += s_out[w * a.n * 16 + i];
         if (a.shares == 1) store(row, at, v);
-        else a.parts[((int64_t) blockIdx.y * a.n + row) * a.D + at] = v;
+        else __hip_atomic_store(a.parts + ((int64_t) blockIdx.y * a.n + row) * a.D + at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     if (a.shares == 1) return;
-    // the last block of a tile's joins what all have left, in their order
-    __threadfence();
+    // the last block of a tile's joins what all have left, in their order. What it joins is stored and read past the caches of one part of the
+    // chip, and every wave's stores have arrived before its block takes a ticket (a fence of the whole chip here writes its caches back:
+    // 75 us in place of 10 for one row).
+    wait_loads_but<0>();
     __syncthreads();
-    if (tid == 0) s_last = __hip_atomic_fetch_add(a.tickets + blockIdx.x, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == a.shares - 1;
+    if (tid == 0) s_last = __hip_atomic_fetch_add(a.tickets + blockIdx.x, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.shares - 1;
     __syncthreads();
     if (!s_last) return;
-    for (int i = tid; i < CT * 256; i += MOE_T) {
+    for (int i = tid; i < a.n * 16; i += MOE_DT) {
         const int row = i >> 4, at = 16 * (int) blockIdx.x + (i & 15);
-        if (row >= a.n || at >= a.D) continue;
+        if (at >= a.D) continue;
         float v = 0.0f;
-        for (int p = 0; p < a.shares; ++p) v += a.parts[((int64_t) p * a.n + row) * a.D + at];
+        for (int p = 0; p < a.shares; ++p) v += __hip_atomic_load(a.parts + ((int64_t) p * a.n + row) * a.D + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         store(row, at, v);
     }
 }

@@ -6,19 +6,16 @@ using namespace z2d;
 
 namespace {
 
-template <typename T, typename TW, int CT>
-void down_launch(const MoeArgs & a, hipStream_t st) {
-    hipLaunchKernelGGL((k_moe_down<T, TW, CT>), dim3(a.tiles, a.shares), dim3(MOE_T), 0, st, a);
+template <typename T, typename TW, int NT>
+void gate_up_launch(const MoeArgs & a, int n_cu, hipStream_t st) {
+    const int64_t tiles = (int64_t) std::min(a.E, a.n * a.k) * (a.F / 8);
+    hipLaunchKernelGGL((k_moe_gate_up<T, TW, NT>), dim3(std::min<int64_t>(n_cu * moe_per_cu<T, NT>(), tiles)), dim3(MOE_T), 0, st, a);
 }
 template <typename T, typename TW>
-void moe_launch(const MoeArgs & a, hipStream_t st) {
-    const int blocks = (int) std::min<int64_t>(512, (int64_t) std::min(a.E, a.n * a.k) * (a.F / 8));
-    if (a.n <= 16) hipLaunchKernelGGL((k_moe_gate_up<T, TW, 1>), dim3(blocks), dim3(MOE_T), 0, st, a);
-    else hipLaunchKernelGGL((k_moe_gate_up<T, TW, 2>), dim3(blocks), dim3(MOE_T), 0, st, a);
-    if (a.n <= 16) down_launch<T, TW, 1>(a, st);
-    else if (a.n <= 32) down_launch<T, TW, 2>(a, st);
-    else if (a.n <= 64) down_launch<T, TW, 4>(a, st);
-    else down_launch<T, TW, 8>(a, st);
+void moe_launch(const MoeArgs & a, int n_cu, hipStream_t st) {
+    if (a.n <= 16) gate_up_launch<T, TW, 1>(a, n_cu, st);
+    else gate_up_launch<T, TW, 2>(a, n_cu, st);
+    hipLaunchKernelGGL((k_moe_down<T, TW>), dim3(a.tiles, a.shares), dim3(MOE_DT), MOE_DW * a.n * 64, st, a);
 }
 
 } // namespace
@@ -51,11 +48,13 @@ int z2h_moe_rows(z2h_ctx * ctx, const z2h_experts * experts, int n_rows, int top
     a.shares = z2o::moe_shares(a.D); a.tiles = (a.D + 15) / 16;
     a.table = (MoeTable *) ws; a.touched = (MoeTouched *) (ws + w.touched); a.w = (float *) (ws + w.w);
     a.tickets = (int32_t *) (ws + w.tickets); a.parts = (float *) (ws + w.parts); a.h = (float *) (ws + w.h);
+    const int n_cu = compute_units(z2h_ctx_device(ctx));
+    if (!n_cu) return z2h_ctx_fail(ctx, Z2H_EDEVICE, "compute-unit count query failed");
     ON_DEVICE;
     switch (type) {
-        case Z2H_F32: moe_launch<float, _Float16>(a, (hipStream_t) stream); break;
-        case Z2H_F16: moe_launch<_Float16, _Float16>(a, (hipStream_t) stream); break;
-        default: moe_launch<__bf16, __bf16>(a, (hipStream_t) stream); break;
+        case Z2H_F32: moe_launch<float, _Float16>(a, n_cu, (hipStream_t) stream); break;
+        case Z2H_F16: moe_launch<_Float16, _Float16>(a, n_cu, (hipStream_t) stream); break;
+        default: moe_launch<__bf16, __bf16>(a, n_cu, (hipStream_t) stream); break;
     }
     return launched(ctx);
 }

@@ -282,9 +282,9 @@ inline int64_t verify_ws_bytes(int n_seq, int n_draft_max, int n_codebooks, int 
            align256(draws * ((vocab + 255) / 256) * 8);
 }
 
-// Blocks that share 16 dims of the output: enough for about 512 blocks.
+// Blocks that share 16 dims of the output: enough for about 768 blocks, three per compute unit.
 inline int moe_shares(int n_embd) {
-    const int tiles = (n_embd + 15) / 16, s = (512 + tiles - 1) / tiles;
+    const int tiles = (n_embd + 15) / 16, s = (768 + tiles - 1) / tiles;
     return s < 1 ? 1 : s > 16 ? 16 : s;
 }
 struct MoeWs { int64_t touched = 0, w = 0, tickets = 0, parts = 0, h = 0, bytes = 0; };
