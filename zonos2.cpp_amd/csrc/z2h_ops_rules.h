@@ -195,6 +195,8 @@ inline AttnWs attn_ws(const z2h_pages & p, int n_head, int n_rows, int n_group, 
 // searching the row table alone. A sequence may have a slot too many.
 Z2O_HD int64_t prompt_slot(int start, int seq, int rows) { return (int64_t) start / rows + seq; }
 Z2O_HD int64_t prompt_slots(int n_rows, int n_seq, int rows) { return (int64_t) n_rows / rows + n_seq; }
+// Rows of a tile of 16 row-heads (0: a group has more than these).
+Z2O_HD int small_rows(int group) { return 16 / group; }
 constexpr int MAX_PROMPTS = 1 << 20;
 inline const char * check_prompt(int n_seq, int n_rows, int n_head, int n_head_kv, int head_dim) {
     if (head_dim != 32 && head_dim != 64 && head_dim != 128) return "prompt: head_dim must be 32, 64 or 128";

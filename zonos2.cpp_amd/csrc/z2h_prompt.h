@@ -96,6 +96,56 @@ __device__ __forceinline__ void prompt_walk(const PromptArgs & a, int first, int
     }
 }
 
+// The lane's part of a row-head's query, whose sign and (fp32) a power of two of whose size are taken out: scores are `c` times the products, in
+// units of log2. whole: the largest of all lanes that have a part of the row-head.
+template <typename T, int QN, typename D, typename W>
+__device__ __forceinline__ float prompt_query(const PromptArgs & a, const T * src, bool live, D dim, float (&x)[QN], W whole) {
+    const bool zero = !live || a.scale == 0.0f;
+    const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
+    float c = zero ? 1.0f : fabsf(a.scale) * 1.44269504088896341f;
+    constexpr int N = 16 / (int) sizeof(T);
+    if (((uintptr_t) src & 15) == 0) {
+        typedef T tv __attribute__((ext_vector_type(N)));
+#pragma unroll
+        for (int i = 0; i < QN; i += N) {
+            const tv y = *(const tv *) (src + dim(i));
+#pragma unroll
+            for (int j = 0; j < N; ++j) x[i + j] = (float) y[j];
+        }
+    } else
+#pragma unroll
+        for (int i = 0; i < QN; ++i) x[i] = (float) src[dim(i)];
+    float up = sign;
+    if constexpr (sizeof(T) == 4) {
+        // a power of two keeps the scores of large queries finite, and those of tiny ones from vanishing
+        float mx = 0.0f;
+#pragma unroll
+        for (int i = 0; i < QN; ++i) mx = fmaxf(mx, fabsf(x[i]));
+        mx = whole(mx);
+        int e = 0;
+        if (mx > 0.0f && mx < __builtin_inff()) (void) frexpf(mx, &e);
+        e = min(-e, 120);
+        up = ldexpf(sign, e);
+        c = zero ? 1.0f : ldexpf(c, -e);
+    }
+#pragma unroll
+    for (int i = 0; i < QN; ++i) x[i] = zero ? 0.0f : x[i] * up;
+    return fminf(fmaxf(c, 0x1p-126f), 0x1p127f);                  // hidden scores stay -inf whatever the scale
+}
+
+// A row-head formed once more in plain fp32, and stored; by one wave
+template <int HD, typename T>
+__device__ __forceinline__ void prompt_again(const PromptArgs & a, int first, int row, int head, float * s_q, int lane) {
+    constexpr int E = HD >= 64 ? HD / 64 : 1;
+    float x[E], sum;
+    prompt_walk<HD, T>(a, first, row, head, s_q, x, sum);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    T * out = (T *) a.out + row * a.os + (int64_t) head * HD + E * lane;
+    if (E * lane < HD)
+#pragma unroll
+        for (int e = 0; e < E; ++e) out[e] = (T) (x[e] * inv);
+}
+
 // Rows of T in LDS, stored as they are with their 16-byte pieces permuted by row: keys so that 32 rows' pieces of the same dims take all
 // banks, values so that transposing reads (16 bits) or two rows 4 apart (fp32) do.
 template <int HD, typename T>
@@ -254,38 +304,8 @@ struct PromptWave {
         const int r = live ? rh / group : 0, head = g * group + (live ? rh % group : 0);
         const T * src = (const T *) a.q + (row0 + r) * a.qs + (int64_t) head * HD;
         vis = live ? before + r + 1 : 0x7fffffff;
-        const bool zero = !live || a.scale == 0.0f;
-        const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
-        c = zero ? 1.0f : fabsf(a.scale) * 1.44269504088896341f;
         float x[M::QN];
-        constexpr int N = 16 / (int) sizeof(T);
-        if (((uintptr_t) src & 15) == 0) {
-            typedef T tv __attribute__((ext_vector_type(N)));
-#pragma unroll
-            for (int i = 0; i < M::QN; i += N) {
-                const tv y = *(const tv *) (src + M::dim(i, lane));
-#pragma unroll
-                for (int j = 0; j < N; ++j) x[i + j] = (float) y[j];
-            }
-        } else
-#pragma unroll
-            for (int i = 0; i < M::QN; ++i) x[i] = (float) src[M::dim(i, lane)];
-        float up = sign;
-        if constexpr (sizeof(T) == 4) {
-            // a power of two keeps the scores of large queries finite, and those of tiny ones from vanishing
-            float mx = 0.0f;
-#pragma unroll
-            for (int i = 0; i < M::QN; ++i) mx = fmaxf(mx, fabsf(x[i]));
-            mx = fmaxf(mx, other_half(mx));
-            int e = 0;
-            if (mx > 0.0f && mx < __builtin_inff()) (void) frexpf(mx, &e);
-            e = min(-e, 120);
-            up = ldexpf(sign, e);
-            c = zero ? 1.0f : ldexpf(c, -e);
-        }
-        c = fminf(fmaxf(c, 0x1p-126f), 0x1p127f);                 // hidden scores stay -inf whatever the scale
-#pragma unroll
-        for (int i = 0; i < M::QN; ++i) x[i] = zero ? 0.0f : x[i] * up;
+        c = prompt_query<T, M::QN>(a, src, live, [&](int i) { return M::dim(i, lane); }, x, [](float mx) { return fmaxf(mx, other_half(mx)); });
         math.init(x, lane);
         m = -__builtin_inff();
         l = 0.0f;
@@ -328,6 +348,23 @@ struct PromptWave {
         math.add(o, sv);
     }
 
+    // the sums over other keys of the same row-heads
+    template <typename F>
+    __device__ __forceinline__ void join(float m2, float l2, F o2) {
+        const float mn = fmaxf(m, m2);
+        const float w = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - mn), w2 = m2 == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m2 - mn);
+        // (both of a row-head's lanes have the same maxima; without one there is no weight, whatever the values were)
+        m = mn;
+        l = l * w + l2 * w2;
+#pragma unroll
+        for (int dt = 0; dt < M::DT; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float x = o2(dt, i);
+                o[dt][i] = (w != 0.0f ? o[dt][i] * w : 0.0f) + (w2 != 0.0f ? x * w2 : 0.0f);
+            }
+    }
+
     // What is not finite meets both parts of a weight, and hidden rows' weights of 0: the product is then NaN where the definition has
     // infinity or leaves it out, never anything else that is wrong. So a row-head that holds NaN is formed once more, in plain fp32.
     // s_q: HD floats of LDS of the wave's own.
@@ -351,15 +388,8 @@ struct PromptWave {
                     store4(out + 32 * dt + 2 * i + 4 * (lane >> 5), o[dt][i] * inv, o[dt][i + 1] * inv, o[dt][i + 2] * inv, o[dt][i + 3] * inv);
         }
         for (unsigned long long todo = __ballot(again) & 0xffffffffull; todo; todo &= todo - 1) {
-            constexpr int E = HD >= 64 ? HD / 64 : 1;
-            const int at = first_rh + __builtin_ctzll(todo), row = row0 + at / group, head = g * group + at % group;
-            float x[E], sum;
-            prompt_walk<HD, T>(a, first, row, head, s_q, x, sum);
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            T * out = (T *) a.out + row * a.os + (int64_t) head * HD + E * lane;
-            if (E * lane < HD)
-#pragma unroll
-                for (int e = 0; e < E; ++e) out[e] = (T) (x[e] * inv);
+            const int at = first_rh + __builtin_ctzll(todo);
+            prompt_again<HD, T>(a, first, row0 + at / group, g * group + at % group, s_q, lane);
         }
     }
 };
@@ -418,12 +448,277 @@ __device__ __forceinline__ PromptTile prompt_tile(const PromptArgs & a, int tile
     return t;
 }
 
-// Four waves of 32 row-heads each over the same keys, 32 NT at a time in LDS, the next ones on their way into the other buffer.
+// ---- few tiles: 16 row-heads per block, the keys dealt to its four waves
+typedef float v4f_t __attribute__((ext_vector_type(4)));
+// the largest (or the sum) of a column's values, whose four lanes are 16 apart
+template <bool SUM>
+__device__ __forceinline__ float column(float v) {
+    auto both = [](float a, float b) { return SUM ? a + b : fmaxf(a, b); };
+    v = both(v, other_half(v));
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+    const unsigned r0 = r[0], r1 = r[1];
+    return both(__builtin_bit_cast(float, r0), __builtin_bit_cast(float, r1));
+}
+template <typename T, int N, bool ALIGNED>
+__device__ __forceinline__ void load_piece(const T * p, T (&x)[N]) {
+    if constexpr (ALIGNED) {
+        typedef T tv __attribute__((ext_vector_type(N)));
+        const tv y = *(const tv *) p;
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = y[i];
+    } else
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = p[i];
+}
+
+// One wave's 16 row-heads (a lane: row-head lane % 16, group g = lane / 16 of four) against KEYS keys at a time: keys from memory to registers, 16-bit
+// values through LDS (transposed as they are read), fp32 values to registers too.
 template <int HD, typename T, bool ALIGNED>
-__global__ void __launch_bounds__(256, 2) k_prompt(PromptArgs a) {
-    constexpr int KEYS = 32 * PromptMath<HD, T>::NT;
-    __shared__ __attribute__((aligned(1024))) T s_k0[KEYS * HD], s_k1[KEYS * HD], s_v0[KEYS * HD], s_v1[KEYS * HD];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6), group = a.n_head / a.nkv;
+struct SmallMath {
+    static constexpr int KEYS = 32, KS = HD / 32, DT = HD / 16, BIAS = __is_same(T, _Float16) ? 6 : 0, QN = HD / 4;
+    static constexpr int NC = HD / 8, RP = NC >= 16 ? 1 : 16 / NC, ROWS = 64 / NC, LDS = 2 * KEYS * HD;
+    typedef typename Vec8<T>::type v8;
+    v8 q[KS];
+    struct Data { v8 k[2][KS]; };
+    static __device__ __forceinline__ int perm(int row) { return 2 * ((row / RP) & (NC / 2 - 1)); }
+    static __device__ __forceinline__ int dim(int i, int g) { return 32 * (i >> 3) + 8 * g + (i & 7); }
+    // dim of register i of o's tile t
+    static __device__ __forceinline__ int out_dim(int t, int i, int g) { return 16 * t + 4 * g + i; }
+    __device__ __forceinline__ void init(const float (&x)[QN]) {
+#pragma unroll
+        for (int i = 0; i < QN; ++i) q[i >> 3][i & 7] = (T) x[i];
+    }
+    __device__ __forceinline__ void request(Data & d, const T * k, int64_t ks, const T * v, int64_t vs, int key, int last, T * lds, int lane) const {
+        const int l = lane & 15, g = lane >> 4;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                T x[8];
+                load_piece<T, 8, ALIGNED>(k + min(key + 16 * t + l, last) * ks + 32 * i + 8 * g, x);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) d.k[t][i][j] = x[j];
+            }
+        const int row = lane / NC, piece = lane % NC;
+#pragma unroll
+        for (int r = 0; r < KEYS; r += ROWS) {
+            const T * from = v + min(key + r + row, last) * vs + (piece ^ perm(r + row)) * 8;
+            if constexpr (ALIGNED) to_lds(from, lds + r * HD);
+            else {
+                T x[8];
+                load_piece<T, 8, false>(from, x);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) lds[r * HD + lane * 8 + j] = x[j];
+            }
+        }
+    }
+    // register i of s: key key0 + key_of(i, g)
+    static constexpr int SN = 8;
+    static __device__ __forceinline__ int key_of(int i, int g) { return 16 * (i >> 2) + 4 * g + (i & 3); }
+    __device__ __forceinline__ void scores(const Data & d, float (&s)[SN]) const {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            v4f_t x{};
+#pragma unroll
+            for (int i = 0; i < KS; ++i) x = mfma16(d.k[t][i], q[i], x);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[4 * t + i] = x[i];
+        }
+    }
+    static __device__ __forceinline__ v4f_t mfma16(v8 a, v8 b, v4f_t c) {
+        if constexpr (__is_same(T, _Float16)) return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+    __device__ __forceinline__ void add(const Data &, const float (&w)[SN], v4f_t (&o)[DT], const T * lds, int lane) const {
+        v8 hi, lo;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            typedef typename Pair<float>::type f2;
+            typedef typename Pair<T>::type c2;
+            const f2 y = {w[i], w[i + 1]};
+            const c2 h = __builtin_convertvector(y, c2), r = __builtin_convertvector(two_rest(y, h), c2);
+            hi[i] = h[0]; hi[i + 1] = h[1];
+            lo[i] = r[0]; lo[i + 1] = r[1];
+        }
+        const int l = lane & 15, row = 4 * (lane >> 4) + (l >> 2);
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+            const int d = 16 * t + 4 * (l & 3);
+            typedef __attribute__((address_space(3))) s4_t lds4;
+            // (rows 16 apart are permuted alike)
+            const T * at = lds + row * HD + ((d >> 3) ^ perm(row)) * 8 + (d & 7);
+            const s4_t x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *) at);
+            const s4_t x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *) (at + 16 * HD));
+            const v8 v = __builtin_bit_cast(v8, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
+            o[t] = mfma16(v, hi, o[t]);
+            o[t] = mfma16(v, lo, o[t]);
+        }
+    }
+};
+template <int HD, bool ALIGNED>
+struct SmallMath<HD, float, ALIGNED> {
+    static constexpr int KEYS = 16, DT = HD / 16, BIAS = 0, QN = HD / 4, SN = 4, LDS = HD * 16;
+    static constexpr int VE = HD >= 64 ? 4 : 2, VQ = DT / VE;     // values: VQ pieces of VE dims of a row per lane
+    float q[QN];
+    struct Data { float k[QN], v[4][VQ][VE]; };
+    static __device__ __forceinline__ int dim(int i, int g) { return 16 * (i >> 2) + 4 * g + (i & 3); }
+    static __device__ __forceinline__ int out_dim(int t, int i, int g) { return t / VE * 16 * VE + (4 * g + i) * VE + t % VE; }
+    static __device__ __forceinline__ int key_of(int i, int g) { return 4 * g + i; }
+    __device__ __forceinline__ void init(const float (&x)[QN]) {
+#pragma unroll
+        for (int i = 0; i < QN; ++i) q[i] = x[i];
+    }
+    __device__ __forceinline__ void request(Data & d, const float * k, int64_t ks, const float * v, int64_t vs, int key, int last, float *, int lane) const {
+        const int l = lane & 15, g = lane >> 4;
+        const float * row = k + min(key + l, last) * ks + 4 * g;
+#pragma unroll
+        for (int j = 0; j < QN / 4; ++j) {
+            float x[4];
+            load_piece<float, 4, ALIGNED>(row + 16 * j, x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d.k[4 * j + e] = x[e];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < VQ; ++j) load_piece<float, VE, ALIGNED>(v + min(key + 4 * g + i, last) * vs + 16 * VE * j + VE * l, d.v[i][j]);
+    }
+    __device__ __forceinline__ void scores(const Data & d, float (&s)[SN]) const {
+        v4f_t x[4] = {};                                         // (four chains: a product waits for the one before it in its own)
+#pragma unroll
+        for (int i = 0; i < QN; ++i) x[i & 3] = __builtin_amdgcn_mfma_f32_16x16x4f32(d.k[i], q[i], x[i & 3], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] = (x[0][i] + x[1][i]) + (x[2][i] + x[3][i]);
+    }
+    __device__ __forceinline__ void add(const Data & d, const float (&w)[SN], v4f_t (&o)[DT], const float *, int) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int t = 0; t < DT; ++t) o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(d.v[i][t / VE][t % VE], w[i], o[t], 0, 0, 0);
+    }
+};
+
+template <int HD, typename T, bool ALIGNED>
+__global__ void __launch_bounds__(256, 2) k_prompt_small(PromptArgs a) {
+    typedef SmallMath<HD, T, ALIGNED> M;
+    constexpr int DT = M::DT, SN = M::SN;
+    // of every wave: two buffers of values, then its sums [16][HD]
+    constexpr int BYTES = M::LDS * (int) sizeof(T) > 16 * HD * 4 ? M::LDS * (int) sizeof(T) : 16 * HD * 4;
+    __shared__ __attribute__((aligned(1024))) uint8_t s_lds[4][BYTES];
+    __shared__ float s_m[4][16], s_l[4][16];
+    __shared__ int s_again[16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = a.n_head / a.nkv, col = lane & 15, g = lane >> 4;
+    const PromptTile t = prompt_tile(a, z2o::small_rows(group), lane);
+    if (t.rows <= 0) return;
+    const int before = t.row0 - t.first, n_keys = before + t.rows, heads = t.rows * group;
+    const T * k = (const T *) a.k + t.first * a.ks + (int64_t) t.g * HD, * v = (const T *) a.v + t.first * a.vs + (int64_t) t.g * HD;
+    T * lds = (T *) s_lds[wave];
+    typename M::Data d0, d1;
+    M math;
+    int key = M::KEYS * wave;
+    if (key < n_keys) math.request(d0, k, a.ks, v, a.vs, key, n_keys - 1, lds, lane);
+    // the queries
+    const bool live = col < heads;
+    const int r = live ? col / group : 0, head = t.g * group + (live ? col % group : 0), vis = before + r + 1;
+    float c, m = -__builtin_inff(), l = 0.0f;
+    {
+        float x[M::QN];
+        c = prompt_query<T, M::QN>(a, (const T *) a.q + (t.row0 + r) * a.qs + (int64_t) head * HD, live, [&](int i) { return M::dim(i, g); }, x,
+                                   [](float mx) { return column<false>(mx); });
+        math.init(x);
+    }
+    v4f_t o[DT];
+#pragma unroll
+    for (int i = 0; i < DT; ++i) o[i] = v4f_t{};
+    auto step = [&](typename M::Data & d, typename M::Data & ahead, T * here, T * there) __attribute__((always_inline)) {
+        wait_loads_but<0>();                                     // (the values in LDS)
+        const bool more = key + 4 * M::KEYS < n_keys;
+        if (more) math.request(ahead, k, a.ks, v, a.vs, key + 4 * M::KEYS, n_keys - 1, there, lane);
+        float s[SN];
+        math.scores(d, s);
+        float mx = -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < SN; ++i) {
+            if (key + M::key_of(i, g) >= vis) s[i] = -__builtin_inff();
+            mx = fmaxf(mx, s[i]);
+        }
+        mx = column<false>(mx) * c;
+        const bool up = mx > m + (8.0f + M::BIAS);
+        if (__any(up)) {
+            const float mn = up ? mx - M::BIAS : m;
+            const float w = mn == m || m == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= w;
+#pragma unroll
+            for (int i = 0; i < DT; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[i][j] *= w;
+        }
+        const float mu = m == -__builtin_inff() ? 0.0f : m;
+        float w[SN];
+#pragma unroll
+        for (int i = 0; i < SN; ++i) {
+            w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -mu));
+            l += w[i];
+        }
+        math.add(d, w, o, here, lane);
+        key += 4 * M::KEYS;
+    };
+    T * other = lds + M::LDS / 2;
+    while (key < n_keys) {
+        step(d0, d1, lds, other);
+        if (key >= n_keys) break;
+        step(d1, d0, other, lds);
+    }
+    // ---- the waves' sums together, 16 threads per row-head
+    l = column<true>(l);
+    wait_lds();
+    float * mine = (float *) s_lds[wave];
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mine[col * HD + ((M::out_dim(i, j, g) + 4 * col) & (HD - 1))] = o[i][j];
+    if (g == 0) { s_m[wave][col] = m; s_l[wave][col] = l; }
+    if (tid < 16) s_again[tid] = 0;
+    __syncthreads();
+    const int rh = tid >> 4;
+    const float mm = fmaxf(fmaxf(s_m[0][rh], s_m[1][rh]), fmaxf(s_m[2][rh], s_m[3][rh]));
+    float f[4], sum = 0.0f, y[HD / 16];
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i) y[i] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        f[w] = s_m[w][rh] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(s_m[w][rh] - mm);
+        sum = __builtin_fmaf(f[w], s_l[w][rh], sum);
+        if (s_m[w][rh] != -__builtin_inff() || s_l[w][rh] != 0.0f)
+#pragma unroll
+            for (int i = 0; i < HD / 16; ++i) y[i] = __builtin_fmaf(f[w], ((const float *) s_lds[w])[rh * HD + (((tid & 15) * (HD / 16) + i + 4 * rh) & (HD - 1))], y[i]);
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    bool nan = sum != sum;
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i) nan |= y[i] != y[i];
+    if (nan) s_again[rh] = 1;
+    __syncthreads();
+    if (rh < heads && !s_again[rh]) {
+        T * out = (T *) a.out + (t.row0 + rh / group) * a.os + (int64_t) (t.g * group + rh % group) * HD + (tid & 15) * (HD / 16);
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) out[i] = (T) (y[i] * inv);
+    }
+    for (int i = wave; i < heads; i += 4)
+        if (s_again[i]) prompt_again<HD, T>(a, t.first, t.row0 + i / group, t.g * group + i % group, (float *) s_lds[wave], lane);
+}
+
+// ---- many tiles: 128 row-heads per block
+// Four waves of 32 row-heads each over the same keys, 32 NT at a time in LDS, the next ones on their way into the other buffer. HALVES 2: eight
+// waves, the second four over every other 32 NT keys; their sums are joined in LDS.
+template <int HD, typename T, bool ALIGNED, int HALVES>
+__global__ void __launch_bounds__(256 * HALVES, 2) k_prompt(PromptArgs a) {
+    constexpr int KEYS = 32 * PromptMath<HD, T>::NT, DT = PromptMath<HD, T>::DT;
+    __shared__ __attribute__((aligned(1024))) T s_k0[HALVES][KEYS * HD], s_k1[HALVES][KEYS * HD], s_v0[HALVES][KEYS * HD], s_v1[HALVES][KEYS * HD];
+    __shared__ float s_ml[HALVES == 2 ? 4 : 1][2][64];
+    const int lane = threadIdx.x & 63, group = a.n_head / a.nkv;
+    const int wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6) & 3, half = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 8);
     const PromptTile t = prompt_tile(a, z2o::tile_rows(group), lane);
     if (t.rows <= 0) return;
     const int before = t.row0 - t.first, n_keys = before + t.rows;
@@ -437,26 +732,43 @@ __global__ void __launch_bounds__(256, 2) k_prompt(PromptArgs a) {
             else load.values16(key + 16 * (part - PARTS), sv + 16 * (part - PARTS) * HD, lane);
         }
     };
-    bring(0, s_k0, s_v0);
+    int key = half * KEYS;
+    if (key < n_keys) bring(key, s_k0[half], s_v0[half]);
     PromptWave<HD, T> w;
     w.init(a, t.row0, t.rows, before, t.g, 32 * wave, lane);
     // the wave's rows see keys up to `mine`
     const int mine = 32 * wave < t.rows * group ? before + min(t.rows, (32 * wave + 31) / group + 1) : 0;
-    int key = 0;
     auto stage = [&](const T * sk, const T * sv, T * ok, T * ov) __attribute__((always_inline)) {
         wait_loads_but<0>();
         __syncthreads();
-        if (key + KEYS < n_keys) bring(key + KEYS, ok, ov);
+        if (key + HALVES * KEYS < n_keys) bring(key + HALVES * KEYS, ok, ov);
         if (key < mine) w.step(sk, sv, key, lane);
-        key += KEYS;
+        key += HALVES * KEYS;
     };
-    while (key < n_keys) {
-        stage(s_k0, s_v0, s_k1, s_v1);
-        if (key >= n_keys) break;
-        stage(s_k1, s_v1, s_k0, s_v0);
+    // (both halves take the first one's number of steps: they share the barriers)
+    for (int at = 0; at < n_keys;) {
+        stage(s_k0[half], s_v0[half], s_k1[half], s_v1[half]);
+        if ((at += HALVES * KEYS) >= n_keys) break;
+        stage(s_k1[half], s_v1[half], s_k0[half], s_v0[half]);
+        at += HALVES * KEYS;
     }
     __syncthreads();
-    w.store(a, t.first, t.row0, t.rows, t.g, 32 * wave, lane, (float *) s_k0 + wave * HD);
+    if constexpr (HALVES == 2) {
+        float * to = (float *) (wave < 2 ? wave ? s_k1[0] : s_k0[0] : wave == 2 ? s_v0[0] : s_v1[0]);    // 32 HD floats each at least
+        if (half) {
+            s_ml[wave][0][lane] = w.m;
+            s_ml[wave][1][lane] = w.l;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) to[(16 * dt + i) * 64 + lane] = w.o[dt][i];
+        }
+        __syncthreads();
+        if (half) return;
+        w.join(s_ml[wave][0][lane], s_ml[wave][1][lane], [&](int dt, int i) { return to[(16 * dt + i) * 64 + lane]; });
+        wait_lds();
+        w.store(a, t.first, t.row0, t.rows, t.g, 32 * wave, lane, to);
+    } else w.store(a, t.first, t.row0, t.rows, t.g, 32 * wave, lane, (float *) s_k0 + wave * HD);
 }
 
 } // namespace z2d

@@ -6,22 +6,36 @@ using namespace z2d;
 
 namespace {
 
+bool prompt_small(int64_t tiles, int n_cu) {
+    static const int f = getenv("PSMALL") ? atoi(getenv("PSMALL")) : 1;
+    return tiles * 4 < (int64_t) n_cu * f;
+}
+
 template <int HD, typename T>
-void prompt_launch(PromptArgs & a, hipStream_t st) {
+void prompt_launch(PromptArgs & a, int n_cu, hipStream_t st) {
     const auto al = [](const void * p, int64_t stride) { return (uintptr_t) p % 16 == 0 && stride * (int64_t) sizeof(T) % 16 == 0; };
     const bool aligned = al(a.k, a.ks) && al(a.v, a.vs);
-    for (int64_t n = z2o::prompt_slots(a.n_rows, a.n_seq, z2o::tile_rows(a.n_head / a.nkv)) * a.nkv; a.block0 < n; a.block0 += z2o::launch_blocks(256)) {
+    const int group = a.n_head / a.nkv;
+    static const int pf = getenv("PPAIR") ? atoi(getenv("PPAIR")) : 256;
+    const bool pair = (int64_t) a.n_rows * group * a.nkv / 128 <= pf;
+    const bool small = group <= 16 && prompt_small((int64_t) a.n_rows * group * a.nkv / 128, n_cu);
+    for (int64_t n = z2o::prompt_slots(a.n_rows, a.n_seq, small ? z2o::small_rows(group) : z2o::tile_rows(group)) * a.nkv; a.block0 < n;
+         a.block0 += z2o::launch_blocks(256)) {
         const dim3 grid(std::min(n - a.block0, z2o::launch_blocks(256)));
-        if (aligned) hipLaunchKernelGGL((k_prompt<HD, T, true>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((k_prompt<HD, T, false>), grid, dim3(256), 0, st, a);
+        if (small && aligned) hipLaunchKernelGGL((k_prompt_small<HD, T, true>), grid, dim3(256), 0, st, a);
+        else if (small) hipLaunchKernelGGL((k_prompt_small<HD, T, false>), grid, dim3(256), 0, st, a);
+        else if (pair && aligned) hipLaunchKernelGGL((k_prompt<HD, T, true, 2>), grid, dim3(512), 0, st, a);
+        else if (pair) hipLaunchKernelGGL((k_prompt<HD, T, false, 2>), grid, dim3(512), 0, st, a);
+        else if (aligned) hipLaunchKernelGGL((k_prompt<HD, T, true, 1>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((k_prompt<HD, T, false, 1>), grid, dim3(256), 0, st, a);
     }
 }
 template <int HD>
-void prompt_launch(PromptArgs & a, int type, hipStream_t st) {
+void prompt_launch(PromptArgs & a, int type, int n_cu, hipStream_t st) {
     switch (type) {
-        case Z2H_F32: prompt_launch<HD, float>(a, st); break;
-        case Z2H_F16: prompt_launch<HD, _Float16>(a, st); break;
-        default: prompt_launch<HD, __bf16>(a, st); break;
+        case Z2H_F32: prompt_launch<HD, float>(a, n_cu, st); break;
+        case Z2H_F16: prompt_launch<HD, _Float16>(a, n_cu, st); break;
+        default: prompt_launch<HD, __bf16>(a, n_cu, st); break;
     }
 }
 
@@ -47,11 +61,13 @@ int z2h_prompt_attn(z2h_ctx * ctx, int n_seq, const int32_t * d_row_start, int n
     a.q = d_q; a.k = d_k; a.v = d_v; a.out = d_out;
     a.qs = q_stride; a.ks = k_stride; a.vs = v_stride; a.os = out_stride;
     a.scale = scale;
+    const int n_cu = compute_units(z2h_ctx_device(ctx));
+    if (!n_cu) return z2h_ctx_fail(ctx, Z2H_EDEVICE, "compute-unit count query failed");
     ON_DEVICE;
     switch (head_dim) {
-        case 32: prompt_launch<32>(a, type, (hipStream_t) stream); break;
-        case 64: prompt_launch<64>(a, type, (hipStream_t) stream); break;
-        default: prompt_launch<128>(a, type, (hipStream_t) stream); break;
+        case 32: prompt_launch<32>(a, type, n_cu, (hipStream_t) stream); break;
+        case 64: prompt_launch<64>(a, type, n_cu, (hipStream_t) stream); break;
+        default: prompt_launch<128>(a, type, n_cu, (hipStream_t) stream); break;
     }
     return launched(ctx);
 }
