@@ -32,6 +32,19 @@ static void prompts() {
     }
 }
 
+// which way calls are cut: the sizes that tests/test_gpu_ops_prompt.py names, on a card of 256 compute units
+static void cuts() {
+    for (int hd : {32, 64, 128})
+        for (bool fp32 : {false, true}) {
+            EXPECT(z2o::prompt_cut(260, 3, 4, 2, hd, fp32, 256) == z2o::PROMPT_SMALL);
+            EXPECT(z2o::prompt_cut(1331, 8, 60, 20, hd, fp32, 256) == (hd == 32 && fp32 ? z2o::PROMPT_SMALL : z2o::PROMPT_WIDE));
+        }
+    EXPECT(z2o::prompt_cut(1310, 1, 16, 4, 128, false, 256) == z2o::PROMPT_PAIR && z2o::prompt_cut(2100, 2, 16, 8, 128, true, 256) == z2o::PROMPT_PAIR);
+    EXPECT(z2o::prompt_cut(2100, 2, 16, 8, 64, false, 256) == z2o::PROMPT_PAIR && z2o::prompt_cut(2100, 2, 16, 8, 32, false, 256) == z2o::PROMPT_SMALL);
+    EXPECT(z2o::prompt_cut(1, 1, 17, 1, 128, false, 256) == z2o::PROMPT_WIDE && z2o::prompt_cut(1, 1, 64, 1, 32, true, 256) == z2o::PROMPT_WIDE);   // (groups of more than 16)
+    EXPECT(z2o::prompt_cut(1 << 20, 1 << 20, 64, 1, 128, true, 256) == z2o::PROMPT_WIDE);
+}
+
 static void experts() {
     z2h_experts good{(void *) 256, (void *) 512, (void *) 768, Z2H_F16, 32, 1536, 2048};
     EXPECT(!z2o::check_experts(&good) && z2o::check_experts(nullptr));
@@ -82,6 +95,7 @@ static void pool() {
 
 int main() {
     prompts();
+    cuts();
     experts();
     pool();
     std::puts("ok");

@@ -133,6 +133,32 @@ def test_few_heads_long_prompt(ctx, typ):
     c.check(c.run(ctx), typ)
 
 
+# sequences and heads at which a call is cut in each of its ways on this card: 16 row-heads per block, 128 with eight waves, 128 with four
+CUTS = {"small": dict(lens=[90, 130, 40], heads=4, kvh=2), "pair": dict(lens=[1310], heads=16, kvh=4), "pair_f32": dict(lens=[1100, 1000], heads=16, kvh=8),
+        "wide": dict(lens=[300, 1, 250, 77, 90, 33, 400, 180], heads=60, kvh=20)}
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("cut", list(CUTS))
+@pytest.mark.parametrize("hd,pad", [(128, 8), (64, 3), (32, 8)])
+def test_every_cut(ctx, cut, typ, hd, pad):
+    """Plain values, then a value that is not finite in the middle of the longest prompt's last rows."""
+    print(f"prompt {cut} {typ} hd {hd}", flush=True)
+    c = Case(typ, hd=hd, pad=pad, seed=3, **CUTS[cut])
+    ref, tol = c.check(c.run(ctx), f"{cut} {typ}")
+    s = int(np.argmax(CUTS[cut]["lens"]))
+    end = c.bounds[s + 1]
+    c.host[end - 3, (c.heads + c.kvh) * hd + 1] = math.inf
+    c.host[end - 2, c.heads * hd] = math.nan
+    out = c.run(ctx).cpu()
+    rows = torch.ones(c.n, dtype=torch.bool)
+    rows[end - 3:end] = False
+    check(out[rows], ref[rows], tol[rows], f"{cut} {typ} rows that do not see them")
+    grp = c.heads // c.kvh
+    assert bool((out[end - 3, :grp, 1] == math.inf).all()) and bool(torch.isnan(out[end - 2:end, :grp]).all())
+    assert bool(torch.isfinite(out[end - 3:end, grp:]).all())
+
+
 @pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
 def test_peaked(ctx, typ):
     """Scores far apart: softmax near one-hot, the running maximum moving often."""

@@ -197,6 +197,18 @@ Z2O_HD int64_t prompt_slot(int start, int seq, int rows) { return (int64_t) star
 Z2O_HD int64_t prompt_slots(int n_rows, int n_seq, int rows) { return (int64_t) n_rows / rows + n_seq; }
 // Rows of a tile of 16 row-heads (0: a group has more than these).
 Z2O_HD int small_rows(int group) { return 16 / group; }
+// How a call is cut, by its tiles of 128 row-heads. Few: 16 row-heads per block, whose keys four waves share (one prompt of 300 rows, 16 heads of 128
+// in 16 bits, 37 tiles: 9.2 us against 14.7 with 128 row-heads; 600 rows, 75 tiles: 16.0 against 21.1; 8 x 128 rows, 128 tiles: 14.4 against 11.3. Heads
+// of 64 half as much work each; fp32 products are slower, so that more blocks pay longer: 300 rows 17.0 against 48.5, 4 x 300, 150 tiles:
+// 39 against 52, 16 x 256, 512 tiles: 106 against 76). Up to a tile and a quarter per compute unit of long prompts: 128 row-heads and eight waves, each
+// four over half of the keys (2400 rows, 300 tiles: 57.9 against 67.4; 8 x 256: 17.6 against 19.2; heads of 64, 4 x 300: 17.4 against 14.8,
+// 1200: 24.1 against 26.9; 512 tiles of 16 x 256: 32 against 24). Otherwise 128 row-heads and four waves.
+enum PromptCut { PROMPT_WIDE, PROMPT_PAIR, PROMPT_SMALL };
+inline PromptCut prompt_cut(int n_rows, int n_seq, int n_head, int n_head_kv, int head_dim, bool fp32, int n_cu) {
+    const int64_t tiles = (int64_t) n_rows * n_head / TILE_RH;
+    if (n_head / n_head_kv <= 16 && tiles * head_dim <= (fp32 ? 96ll : 42ll) * n_cu) return PROMPT_SMALL;
+    return 4 * tiles <= 5ll * n_cu && (int64_t) n_rows * head_dim >= 32768ll * n_seq ? PROMPT_PAIR : PROMPT_WIDE;
+}
 constexpr int MAX_PROMPTS = 1 << 20;
 inline const char * check_prompt(int n_seq, int n_rows, int n_head, int n_head_kv, int head_dim) {
     if (head_dim != 32 && head_dim != 64 && head_dim != 128) return "prompt: head_dim must be 32, 64 or 128";

@@ -192,13 +192,25 @@ struct PromptMath {
     static __device__ __forceinline__ int dim(int i, int lane) { return 16 * (i >> 3) + 8 * (lane >> 5) + (i & 7); }
     static constexpr int QN = KS * 8;
 
-    __device__ __forceinline__ void scores(v16f_t (&s)[NT], const T * sk) const {
+    // (keys are requested four products ahead: the compiler by itself reads, waits and multiplies in turn)
+    template <typename B>
+    __device__ __forceinline__ void scores(v16f_t (&s)[NT], const T * sk, B beside) const {
+        constexpr int AHEAD = 4 < NT * KS ? 4 : NT * KS;
+        v8 f[AHEAD];
+        auto read = [&](int i) __attribute__((always_inline)) { return *(const v8 *) (sk + k_place[i / NT] + 32 * (i % NT) * HD); };
 #pragma unroll
         for (int n = 0; n < NT; ++n) s[n] = v16f_t{};
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
+        for (int i = 0; i < AHEAD; ++i) f[i] = read(i);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) s[n] = mfma32<T>(*(const v8 *) (sk + k_place[ks] + 32 * n * HD), q[ks], s[n]);
+        for (int i = 0; i < NT * KS; ++i) {
+            s[i % NT] = mfma32<T>(f[i % AHEAD], q[i / NT], s[i % NT]);
+            if (i + AHEAD < NT * KS) f[i % AHEAD] = read(i + AHEAD);
+            beside(i, NT * KS);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
     __device__ __forceinline__ float weigh(v16f_t (&s)[NT], float c, float mu) {
         float sum = 0.0f;
@@ -260,10 +272,12 @@ struct PromptMath<HD, float> {
         for (int dt = 0; dt < DT; ++dt) v_at[dt] = R::v_at(row, 8 * dt + ((lane & 31) >> 2)) + (lane & 3);
     }
     static __device__ __forceinline__ int dim(int i, int lane) { return 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3); }
-    __device__ __forceinline__ void scores(v16f_t (&s)[NT], const float * sk) const {
+    template <typename B>
+    __device__ __forceinline__ void scores(v16f_t (&s)[NT], const float * sk, B beside) const {
         s[0] = v16f_t{};
 #pragma unroll
         for (int j = 0; j < HD / 8; ++j) {
+            beside(j, HD / 8);
             const v4 k = *(const v4 *) (sk + k_row + ((2 * j) ^ k_xor) * 4);
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], q[4 * j + e], s[0], 0, 0, 0);
@@ -314,10 +328,11 @@ struct PromptWave {
     }
 
     // keys key0 .. key0 + 32 NT (counted from the sequence's first) in LDS; those at or behind `vis` are hidden
-    __device__ __forceinline__ void step(const T * sk, const T * sv, int key0, int lane) {
+    template <typename B>
+    __device__ __forceinline__ void step(const T * sk, const T * sv, int key0, int lane, B beside) {
         constexpr int NT = M::NT;
         v16f_t s[NT];
-        math.scores(s, sk);
+        math.scores(s, sk, beside);
         if (__any(key0 + 32 * NT > vis)) {
             const int h4 = 4 * (lane >> 5);
 #pragma unroll
@@ -723,14 +738,16 @@ __global__ void __launch_bounds__(256 * HALVES, 2) k_prompt(PromptArgs a) {
     if (t.rows <= 0) return;
     const int before = t.row0 - t.first, n_keys = before + t.rows;
     const PromptLoad<HD, T, ALIGNED> load(a, t.first, n_keys, t.g, lane);
+    // this wave's part i of 2 KEYS / 64 of the rows to bring: 16 of K or of V
+    constexpr int PARTS = KEYS / 32;
+    auto bring_part = [&](int i, int key, T * sk, T * sv) __attribute__((always_inline)) {
+        const int part = 4 * i + wave;
+        if (part < KEYS / 16) load.keys16(key + 16 * part, sk + 16 * part * HD, lane);
+        else load.values16(key + 16 * (part - KEYS / 16), sv + 16 * (part - KEYS / 16) * HD, lane);
+    };
     auto bring = [&](int key, T * sk, T * sv) __attribute__((always_inline)) {
-        constexpr int PARTS = KEYS / 16;                         // 16 rows each of K and of V
 #pragma unroll
-        for (int i = 0; i < 2 * PARTS; i += 4) {
-            const int part = i + wave;
-            if (part < PARTS) load.keys16(key + 16 * part, sk + 16 * part * HD, lane);
-            else load.values16(key + 16 * (part - PARTS), sv + 16 * (part - PARTS) * HD, lane);
-        }
+        for (int i = 0; i < PARTS; ++i) bring_part(i, key, sk, sv);
     };
     int key = half * KEYS;
     if (key < n_keys) bring(key, s_k0[half], s_v0[half]);
@@ -741,8 +758,12 @@ __global__ void __launch_bounds__(256 * HALVES, 2) k_prompt(PromptArgs a) {
     auto stage = [&](const T * sk, const T * sv, T * ok, T * ov) __attribute__((always_inline)) {
         wait_loads_but<0>();
         __syncthreads();
-        if (key + HALVES * KEYS < n_keys) bring(key + HALVES * KEYS, ok, ov);
-        if (key < mine) w.step(sk, sv, key, lane);
+        const int next = key + HALVES * KEYS;
+        if (key < mine)
+            w.step(sk, sv, key, lane, [&](int i, int n) __attribute__((always_inline)) {
+                if (i % (n / PARTS) == 0 && next < n_keys) bring_part(i / (n / PARTS), next, ok, ov);
+            });
+        else if (next < n_keys) bring(next, ok, ov);
         key += HALVES * KEYS;
     };
     // (both halves take the first one's number of steps: they share the barriers)

@@ -6,19 +6,13 @@ using namespace z2d;
 
 namespace {
 
-bool prompt_small(int64_t tiles, int n_cu) {
-    static const int f = getenv("PSMALL") ? atoi(getenv("PSMALL")) : 1;
-    return tiles * 4 < (int64_t) n_cu * f;
-}
-
 template <int HD, typename T>
 void prompt_launch(PromptArgs & a, int n_cu, hipStream_t st) {
     const auto al = [](const void * p, int64_t stride) { return (uintptr_t) p % 16 == 0 && stride * (int64_t) sizeof(T) % 16 == 0; };
     const bool aligned = al(a.k, a.ks) && al(a.v, a.vs);
     const int group = a.n_head / a.nkv;
-    static const int pf = getenv("PPAIR") ? atoi(getenv("PPAIR")) : 256;
-    const bool pair = (int64_t) a.n_rows * group * a.nkv / 128 <= pf;
-    const bool small = group <= 16 && prompt_small((int64_t) a.n_rows * group * a.nkv / 128, n_cu);
+    const z2o::PromptCut cut = z2o::prompt_cut(a.n_rows, a.n_seq, a.n_head, a.nkv, HD, sizeof(T) == 4, n_cu);
+    const bool small = cut == z2o::PROMPT_SMALL, pair = cut == z2o::PROMPT_PAIR;
     for (int64_t n = z2o::prompt_slots(a.n_rows, a.n_seq, small ? z2o::small_rows(group) : z2o::tile_rows(group)) * a.nkv; a.block0 < n;
          a.block0 += z2o::launch_blocks(256)) {
         const dim3 grid(std::min(n - a.block0, z2o::launch_blocks(256)));
