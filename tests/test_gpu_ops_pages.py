@@ -169,9 +169,10 @@ def test_a_prompt_taken_over(ctx, page, kvh, hd, layers, dtype, gap):
     assert p.refs.sum() == 0
 
 
-def test_copy_on_write_between_sharers(ctx):
+@pytest.mark.parametrize("n_pages", [20, 9000])
+def test_copy_on_write_between_sharers(ctx, n_pages):
     """Two sequences that name the same partly filled page (one cut off inside what the other shares) and both go on."""
-    p = Pool(ctx, 4, 4, 20)
+    p = Pool(ctx, 4, 4, n_pages)
     p.fork([(0, 0, 0, 40)])
     p.fork([(0, 1, 32, 32), (0, 2, 32, 32)])                                     # two whole pages shared
     p.fork([(1, 1, 20, 20), (2, 2, 19, 40)])                                     # both now end inside page 1
@@ -188,8 +189,14 @@ def test_a_destination_gives_up_what_it_had(ctx):
     p.counts_hold()
 
 
-def test_a_pool_runs_dry(ctx):
-    p = Pool(ctx, 6, 8, 9)
+@pytest.mark.parametrize("taken", [0, 8191])
+def test_a_pool_runs_dry(ctx, taken):
+    """(taken: pages in use that no sequence of the table names)"""
+    p = Pool(ctx, 6, 8, 9 + taken, kvh=1)
+    p.refs[:taken] = 1
+    p.put_tables()
+    if taken:
+        p.counts_hold = lambda: None
     p.fork([(0, 0, 0, 70)])                                                      # 5 of 9 pages
     assert p.fork([(0, 1, 70, 80), (0, 2, 70, 128), (0, 3, 70, 100), (4, 4, 0, 16)]) == [80, 112, 64, 0]
     p.counts_hold()
@@ -198,8 +205,9 @@ def test_a_pool_runs_dry(ctx):
     p.counts_hold()
 
 
-def test_bad_items_change_nothing(ctx):
-    p = Pool(ctx, 5, 4, 30)
+@pytest.mark.parametrize("n_pages", [30, 8193])
+def test_bad_items_change_nothing(ctx, n_pages):
+    p = Pool(ctx, 5, 4, n_pages)
     p.fork([(0, 0, 0, 40), (1, 1, 0, 20)])
     big = 2 ** 31 - 1
     got = p.fork([(0, 2, 40, 50), (0, 2, 33, 33), (5, 3, 1, 1), (0, -1, 1, 1), (0, 5, 1, 1), (-3, 3, 1, 1), (2, 4, 10, 10), (big, big, big, big),
@@ -209,7 +217,7 @@ def test_bad_items_change_nothing(ctx):
     p.fork([(1, 3, -5, -7), (1, 4, big, -big)])
     p.counts_hold()
     # entries out of range end what a sequence holds
-    p.table[0, 1] = 30
+    p.table[0, 1] = n_pages
     p.refs[:] = 0
     for s in range(5):
         for q in p.pages_held(p.table, s):
@@ -232,7 +240,7 @@ def test_many_items(ctx, n):
     p.counts_hold()
 
 
-@pytest.mark.parametrize("n_pages", [1, 63, 64, 65, 1023, 1024, 1025, 70000])
+@pytest.mark.parametrize("n_pages", [1, 63, 64, 65, 1023, 1024, 1025, 8191, 8192, 8193, 70000])
 def test_pools_of_any_size(ctx, n_pages):
     """Free pages far up, in several segments of the pool, in whole words and at their ends."""
     print(f"{n_pages} pages", flush=True)
@@ -247,13 +255,16 @@ def test_pools_of_any_size(ctx, n_pages):
     p.compact(apart=True)
 
 
-def test_random_histories(ctx):
+@pytest.mark.parametrize("n_pages,most", [(60, 8), (8300, 8), (400, 50)])
+def test_random_histories(ctx, n_pages, most):
+    """Pools and items that one block takes care of, and ones for which there are several."""
+    print(f"histories: {n_pages} pages, {most} items", flush=True)
     for seed in range(6):
         rng = np.random.default_rng(seed)
-        p = Pool(ctx, 12, 7, 60, page=16, layers=2, seed=seed)
+        p = Pool(ctx, 12, 7, n_pages, page=16, layers=2, kvh=1, seed=seed)
         for step in range(25):
             items = []
-            for _ in range(int(rng.integers(1, 8))):
+            for _ in range(int(rng.integers(1, most))):
                 s = int(rng.integers(0, 12))
                 items.append((s, s if rng.random() < 0.5 else int(rng.integers(0, 12)), int(rng.integers(0, 112)), int(rng.integers(0, 120))))
             p.fork(items)

@@ -245,6 +245,8 @@ inline const char * check_moe_type(int type, int experts) {
 
 // ---- a paged cache's upkeep
 constexpr int MAX_POOL = 1 << 22, MAX_FORKS = 4096, POOL_SEG = 1024;
+// What one block does by itself (k_fork_few, k_moves_few).
+constexpr int FEW_PAGES = 8192, FEW_FORKS = 32;
 inline const char * check_pool(const z2h_pages * p, int n) {
     if (const char * e = check_pages(p)) return e;
     if (p->n_pages > MAX_POOL) return "pages: n_pages above 2^22";

@@ -8,9 +8,11 @@
 //   k_pages_take      new pages into the table, and the rows of partly filled pages copied in all layers
 //   k_pages_moves     (compact) every page's new number
 //   k_pages_compact   pages moved in all layers, table and counts rewritten
+// Few items on a small pool are latency alone: k_fork_few does the first three's work but the copies in one block, k_moves_few scan and moves.
 #pragma once
 #include "z2h_common.h"
 #include "z2h_ops_rules.h"
+#include "z2h_tile.h"
 
 namespace z2d {
 
@@ -150,13 +152,23 @@ __device__ __forceinline__ void seg_prefix(const PoolArgs & p, int * s_pre, int 
     if (tid == 0) s_pre[p.segs] = total;
     __syncthreads();
 }
+// Bits of a word of 64, in 32-bit operations: 64-bit shifts by a lane's own amount went wrong here, in about one call of a hundred, where the
+// amount lay in the last vector register that the kernel has (v_lshrrev_b64 by v31 of 32).
+__device__ __forceinline__ bool bit_of(const unsigned long long * words, int n) { return ((const unsigned *) words)[n >> 5] >> (n & 31) & 1; }
+// set bits below bit n (0 .. 63)
+__device__ __forceinline__ int bits_below(unsigned long long w, int n) {
+    const unsigned lo = (unsigned) w, hi = (unsigned) (w >> 32), below = (1u << (n & 31)) - 1;
+    return n & 32 ? __popc(lo) + __popc(hi & below) : __popc(lo & below);
+}
 // the n-th set bit of w (it has more)
 __device__ __forceinline__ int nth_bit(unsigned long long w, int n) {
-    int at = 0;
+    unsigned x = (unsigned) w;
+    int at = 0, c = __popc(x);
+    if (n >= c) { n -= c; x = (unsigned) (w >> 32); at = 32; }
 #pragma unroll
-    for (int half = 32; half; half >>= 1) {
-        const int c = __popcll(w & ((1ull << half) - 1));
-        if (n >= c) { n -= c; w >>= half; at += half; }
+    for (int half = 16; half; half >>= 1) {
+        c = __popc(x & ((1u << half) - 1));
+        if (n >= c) { n -= c; x >>= half; at += half; }
     }
     return at;
 }
@@ -186,7 +198,7 @@ __device__ __forceinline__ int set_before(const PoolArgs & p, const int * s_pre,
     const unsigned long long * w = p.bits + (int64_t) seg * (z2o::POOL_SEG / 64);
     int n = s_pre[seg];
     for (int i = 0; i < word; ++i) n += __popcll(w[i]);
-    return n + __popcll(w[word] & ((1ull << (page & 63)) - 1));
+    return n + bits_below(w[word], page & 63);
 }
 
 typedef unsigned unit_t __attribute__((ext_vector_type(4)));
@@ -252,6 +264,162 @@ __global__ void __launch_bounds__(256) k_pages_take(ForkArgs a) {
                         (int) blockIdx.y * 256 + tid, (int) gridDim.y * 256);
 }
 
+// ---- few items, a small pool: one block
+constexpr int FEW_T = 1024, FEW_WORDS = z2o::FEW_PAGES / 64;
+struct FewPool {
+    unsigned long long bits[FEW_WORDS];
+    int pre[FEW_WORDS + 1];                                      // set bits of all words before each
+};
+// The bits of the pages that are free (FREE) or in use, and their counts, by the whole block. Counts that this kernel has changed are read past the
+// cache of the compute unit.
+template <bool FREE>
+__device__ __forceinline__ void few_scan(const PoolArgs & p, FewPool & s) {
+    constexpr int PER = FEW_WORDS / (FEW_T / 64);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int refs[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int page = 64 * (wave + FEW_T / 64 * i) + lane;
+        refs[i] = page < p.n_pages ? __hip_atomic_load(p.refs + page, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int word = wave + FEW_T / 64 * i, page = 64 * word + lane;
+        const unsigned long long b = __ballot(page < p.n_pages && (FREE ? refs[i] <= 0 : refs[i] > 0));
+        if (lane == 0) s.bits[word] = b;
+    }
+    __syncthreads();
+    if (wave == 0) {
+        int total = 0;
+        for (int w0 = 0; w0 < FEW_WORDS; w0 += 64) {
+            const int c = __popcll(s.bits[w0 + lane]);
+            int x = c;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int y = __shfl_up(x, o);
+                if (lane >= o) x += y;
+            }
+            s.pre[w0 + lane] = total + x - c;
+            total += __shfl(x, 63);
+        }
+        if (lane == 0) s.pre[FEW_WORDS] = total;
+    }
+    __syncthreads();
+}
+// the page of rank r among those whose bit is set (or not set); r is below their number
+template <bool SET>
+__device__ __forceinline__ int few_page(const FewPool & s, int r) {
+    auto before = [&](int w) { return SET ? s.pre[w] : 64 * w - s.pre[w]; };
+    int lo = 0, hi = FEW_WORDS;
+    while (hi - lo > 1) {
+        const int m = (lo + hi) >> 1;
+        if (before(m) <= r) lo = m; else hi = m;
+    }
+    return 64 * lo + nth_bit(SET ? s.bits[lo] : ~s.bits[lo], r - before(lo));
+}
+// leading entries of a sequence that name a page, by one wave
+__device__ __forceinline__ int few_held(const PoolArgs & p, int seq, int lane) {
+    const int32_t * row = p.table + (int64_t) seq * p.table_len;
+    for (int e0 = 0; e0 < p.table_len; e0 += 64) {
+        const int e = e0 + lane;
+        const unsigned long long end = __ballot(e >= p.table_len || (unsigned) row[min(e, p.table_len - 1)] >= (unsigned) p.n_pages);
+        if (end) return e0 + __builtin_ctzll(end);
+    }
+    return p.table_len;
+}
+
+// A chain of dependent loads (items, table rows, counts, counts again) between barriers: 5 us for four items on 350 pages, where the three
+// kernels of their own took 14 with the copies, this and the copies 9.
+__global__ void __launch_bounds__(FEW_T) k_fork_few(ForkArgs a) {
+    __shared__ FewPool s;
+    struct Item { int src, dst, ok, keeps, need, base, part_page; z2o::ForkSize f; };
+    __shared__ Item s_item[z2o::FEW_FORKS];
+    const PoolArgs & p = a.p;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (tid < a.n) { s_item[tid].src = a.src[tid]; s_item[tid].dst = a.dst[tid]; }
+    __syncthreads();
+    for (int i = wave; i < a.n; i += FEW_T / 64) {
+        Item & it = s_item[i];
+        const int src = it.src, dst = it.dst;
+        bool bad = src < 0 || src >= p.n_seq || dst < 0 || dst >= p.n_seq;
+        if (lane < a.n) {
+            const int d = s_item[lane].dst;
+            bad |= (d == dst && lane < i) || (d == src && src != dst);
+        }
+        if (__any(bad)) {
+            if (lane == 0) { it.ok = 0; it.need = 0; }
+            continue;
+        }
+        const int have = few_held(p, src, lane), given = src == dst ? have : few_held(p, dst, lane);
+        const int32_t * from = p.table + (int64_t) src * p.table_len, * own = p.table + (int64_t) dst * p.table_len;
+        const z2o::ForkSize f = z2o::fork_size(a.rows[i], a.room[i], have, p.table_len, p.page_shift);
+        const int part = f.rows & ((1 << p.page_shift) - 1), stay = src == dst ? f.whole + (part > 0) : 0;
+        for (int e = lane; e < given; e += 64)
+            if (e >= stay) atomicSub(p.refs + own[e], 1);
+        if (src != dst)
+            for (int e = lane; e < f.whole; e += 64) atomicAdd(p.refs + from[e], 1);
+        if (lane == 0) { it.ok = 1; it.f = f; it.part_page = part ? from[f.whole] : -1; }
+    }
+    static_assert(z2o::FEW_FORKS <= 64, "an item per lane");
+    wait_loads_but<0>();                                         // every wave's counts have arrived
+    __syncthreads();
+    if (wave == FEW_T / 64 - 1) {
+        int need = 0;
+        if (lane < a.n && s_item[lane].ok) {
+            Item & it = s_item[lane];
+            it.keeps = it.part_page >= 0 && it.src == it.dst && __hip_atomic_load(p.refs + it.part_page, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) <= 1;
+            it.need = need = it.f.pages - it.f.whole - it.keeps;
+        }
+        int x = need;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane < a.n) s_item[lane].base = x - need;
+    }
+    few_scan<true>(p, s);
+    for (int i = wave; i < a.n; i += FEW_T / 64) {
+        const Item it = s_item[i];
+        if (!it.ok) {
+            if (lane == 0) {
+                a.items[i].ok = 0;
+                if (a.held) a.held[i] = -1;
+            }
+            continue;
+        }
+        const bool copy = it.part_page >= 0 && !it.keeps;
+        const int got = max(0, min(it.need, s.pre[FEW_WORDS] - it.base)), first = it.f.whole + it.keeps;
+        const int32_t * from = p.table + (int64_t) it.src * p.table_len;
+        int32_t * own = p.table + (int64_t) it.dst * p.table_len;
+        if (it.src != it.dst)
+            for (int e = lane; e < it.f.whole; e += 64) own[e] = from[e];
+        for (int e = first + lane; e < p.table_len; e += 64) {
+            int page = -1;
+            if (e < first + got) {
+                page = few_page<true>(s, it.base + e - first);
+                p.refs[page] = 1;
+            }
+            own[e] = page;
+        }
+        if (lane == 0) {
+            if (copy && it.src == it.dst) atomicSub(p.refs + it.part_page, 1);
+            if (a.held) a.held[i] = min(it.f.room, (first + got) << p.page_shift);
+            // (what is left to do: rows of one page to another)
+            ForkItem to{};
+            to.ok = copy && got > 0;
+            to.part_page = it.part_page;
+            to.base = to.ok ? few_page<true>(s, it.base) : 0;
+            to.need = it.f.rows & ((1 << p.page_shift) - 1);
+            a.items[i] = to;
+        }
+    }
+}
+__global__ void __launch_bounds__(256) k_fork_copy(ForkArgs a) {
+    const ForkItem it = uniform_copy(a.items + blockIdx.x);
+    if (it.ok) copy_page<true>(a.p, it.part_page, it.base, it.need * a.p.row_bytes, (int) blockIdx.y * 256 + threadIdx.x, (int) gridDim.y * 256);
+}
+
 struct CompactArgs {
     PoolArgs p;
     int32_t * table_out, * refs_out, * n_used;
@@ -272,7 +440,7 @@ __global__ void __launch_bounds__(256) k_pages_moves(CompactArgs a) {
     }
     const int page = blockIdx.x * 256 + threadIdx.x;
     if (page >= p.n_pages) return;
-    const bool set = p.bits[page >> 6] >> (page & 63) & 1;
+    const bool set = bit_of(p.bits, page);
     if (page < used) {
         a.map[page] = page;
         if (set) a.refs_out[page] = p.refs[page];
@@ -288,6 +456,36 @@ __global__ void __launch_bounds__(256) k_pages_moves(CompactArgs a) {
     a.moves[m] = make_int2(page, to);
     a.refs_out[page] = 0;
     a.refs_out[to] = refs;
+}
+
+__global__ void __launch_bounds__(FEW_T) k_moves_few(CompactArgs a) {
+    __shared__ FewPool s;
+    const PoolArgs & p = a.p;
+    few_scan<false>(p, s);
+    const int used = s.pre[FEW_WORDS], tid = threadIdx.x;
+    auto before = [&](int page) { return s.pre[page >> 6] + (page & 63 ? bits_below(s.bits[page >> 6], page & 63) : 0); };
+    const int stay = before(used);                               // (used <= FEW_PAGES: the last word's end has an entry of its own)
+    if (tid == 0) {
+        *a.n_moves = used - stay;
+        if (a.n_used) *a.n_used = used;
+    }
+    for (int page = tid; page < p.n_pages; page += FEW_T) {
+        const bool set = bit_of(s.bits, page);
+        int to = page;
+        if (page < used) {
+            if (set) a.refs_out[page] = p.refs[page];
+        } else {
+            to = -1;
+            if (set) {
+                const int m = before(page) - stay, refs = p.refs[page];
+                to = few_page<false>(s, m);
+                a.moves[m] = make_int2(page, to);
+                a.refs_out[to] = refs;
+            }
+            a.refs_out[page] = 0;
+        }
+        a.map[page] = to;
+    }
 }
 
 __global__ void __launch_bounds__(256) k_pages_compact(CompactArgs a) {

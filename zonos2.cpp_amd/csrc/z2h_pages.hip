@@ -43,13 +43,19 @@ int z2h_pages_fork(z2h_ctx * ctx, const z2h_pages * pages, int n_layer, int64_t 
     a.items = (ForkItem *) ((uint8_t *) d_ws + w.items);
     const hipStream_t st = (hipStream_t) stream;
     ON_DEVICE;
+    // 8 units of 16 bytes per thread of what a page may have to copy
+    const int64_t units = (int64_t) n_layer * 2 * pages->n_head_kv * pages->page_rows * pages->head_dim / 8;
+    const int share = (int) std::min<int64_t>(std::max<int64_t>(1, units / (256 * 8)), std::max(1, 8192 / n));
+    if (n <= z2o::FEW_FORKS && pages->n_pages <= z2o::FEW_PAGES) {
+        hipLaunchKernelGGL(k_fork_few, dim3(1), dim3(FEW_T), 0, st, a);
+        if (int rc = launched(ctx)) return rc;
+        hipLaunchKernelGGL(k_fork_copy, dim3(n, share), dim3(256), 0, st, a);
+        return launched(ctx);
+    }
     hipLaunchKernelGGL(k_pages_release, dim3(n), dim3(256), 0, st, a);
     if (int rc = launched(ctx)) return rc;
     hipLaunchKernelGGL(k_pages_scan<true>, dim3(w.segs + 1), dim3(256), 0, st, a);
     if (int rc = launched(ctx)) return rc;
-    // 8 units of 16 bytes per thread of what a page may have to copy
-    const int64_t units = (int64_t) n_layer * 2 * pages->n_head_kv * pages->page_rows * pages->head_dim / 8;
-    const int share = (int) std::min<int64_t>(std::max<int64_t>(1, units / (256 * 8)), std::max(1, 8192 / n));
     hipLaunchKernelGGL(k_pages_take, dim3(n, share), dim3(256), 0, st, a);
     return launched(ctx);
 }
@@ -72,9 +78,12 @@ int z2h_pages_compact(z2h_ctx * ctx, const z2h_pages * pages, int n_layer, int64
     const int64_t entries = (int64_t) pages->n_seq * pages->table_len;
     const hipStream_t st = (hipStream_t) stream;
     ON_DEVICE;
-    hipLaunchKernelGGL(k_pages_scan<false>, dim3(w.segs), dim3(256), 0, st, s);
-    if (int rc = launched(ctx)) return rc;
-    hipLaunchKernelGGL(k_pages_moves, dim3((pages->n_pages + 255) / 256), dim3(256), 0, st, a);
+    if (pages->n_pages <= z2o::FEW_PAGES) hipLaunchKernelGGL(k_moves_few, dim3(1), dim3(FEW_T), 0, st, a);
+    else {
+        hipLaunchKernelGGL(k_pages_scan<false>, dim3(w.segs), dim3(256), 0, st, s);
+        if (int rc = launched(ctx)) return rc;
+        hipLaunchKernelGGL(k_pages_moves, dim3((pages->n_pages + 255) / 256), dim3(256), 0, st, a);
+    }
     if (int rc = launched(ctx)) return rc;
     hipLaunchKernelGGL(k_pages_compact, dim3(a.blocks + (int) std::min<int64_t>((entries + 1023) / 1024, 1024)), dim3(256), 0, st, a);
     return launched(ctx);
