@@ -202,28 +202,31 @@ __device__ __forceinline__ int set_before(const PoolArgs & p, const int * s_pre,
 }
 
 typedef unsigned unit_t __attribute__((ext_vector_type(4)));
+constexpr int COPY_UNITS = 8;                                    // units of 16 bytes that a thread has on their way
 
-// `bytes` at the start of every head's run of a page (HEADS), or the whole page, to the same place of another, in all layers; work of thread t of T
+// `bytes` at the start of every head's run of a page (HEADS), or the whole page, to the same place of another, in all layers, by blocks of 256: block
+// `part` of `parts`, 32 KB at a time.
 template <bool HEADS>
-__device__ __forceinline__ void copy_page(const PoolArgs & p, int from, int to, int bytes, int t, int T) {
+__device__ __forceinline__ void copy_page(const PoolArgs & p, int from, int to, int bytes, int part, int parts) {
     const int heads = HEADS ? p.nkv : 1, units = bytes / 16, total = p.n_layer * 2 * heads * units;
     const int run_bytes = p.row_bytes << p.page_shift;
-    const int64_t src = from * p.page_bytes, dst = to * p.page_bytes;
-    constexpr int U = 8;
-    for (int u0 = t; u0 < total; u0 += U * T) {
+    const int64_t src = from * p.page_bytes, ahead = to * p.page_bytes - src;
+    constexpr int U = COPY_UNITS;
+    for (int u0 = part * 256 * U + (int) threadIdx.x; u0 < total; u0 += parts * 256 * U) {
         unit_t x[U];
-        int64_t at[U];
+        uint8_t * at[U];
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            const int u = u0 + i * T, run = u / units, head = run % heads, kv = run / heads;
-            at[i] = (int64_t) (kv >> 1) * p.layer_bytes + (int64_t) head * run_bytes + (u - run * units) * 16;
-            if (u < total) x[i] = *(const unit_t *) ((kv & 1 ? p.v : p.k) + src + at[i]);
+            const int u = u0 + i * 256, run = u / units, head = HEADS ? run % heads : 0, kv = HEADS ? run / heads : run;
+            at[i] = (kv & 1 ? p.v : p.k) + src + (int64_t) (kv >> 1) * p.layer_bytes + (int64_t) head * run_bytes + (int64_t) (u - run * units) * 16;
+            if (u < total) x[i] = HEADS ? *(const unit_t *) at[i] : __builtin_nontemporal_load((const unit_t *) at[i]);
         }
 #pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const int u = u0 + i * T, kv = u / units / heads;
-            if (u < total) *(unit_t *) ((kv & 1 ? p.v : p.k) + dst + at[i]) = x[i];
-        }
+        for (int i = 0; i < U; ++i)
+            if (u0 + i * 256 < total) {
+                if (HEADS) *(unit_t *) (at[i] + ahead) = x[i];
+                else __builtin_nontemporal_store(x[i], (unit_t *) (at[i] + ahead));
+            }
     }
 }
 
@@ -261,7 +264,7 @@ __global__ void __launch_bounds__(256) k_pages_take(ForkArgs a) {
     }
     if (copy && got > 0)
         copy_page<true>(p, it.part_page, page_of_rank<true>(p, s_pre, it.base), (f.rows & ((1 << p.page_shift) - 1)) * p.row_bytes,
-                        (int) blockIdx.y * 256 + tid, (int) gridDim.y * 256);
+                        (int) blockIdx.y, (int) gridDim.y);
 }
 
 // ---- few items, a small pool: one block
@@ -279,8 +282,8 @@ __device__ __forceinline__ void few_scan(const PoolArgs & p, FewPool & s) {
     int refs[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const int page = 64 * (wave + FEW_T / 64 * i) + lane;
-        refs[i] = page < p.n_pages ? __hip_atomic_load(p.refs + page, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+        const int page = min(64 * (wave + FEW_T / 64 * i) + lane, p.n_pages - 1);
+        refs[i] = __hip_atomic_load(p.refs + page, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -317,26 +320,28 @@ __device__ __forceinline__ int few_page(const FewPool & s, int r) {
     }
     return 64 * lo + nth_bit(SET ? s.bits[lo] : ~s.bits[lo], r - before(lo));
 }
-// leading entries of a sequence that name a page, by one wave
-__device__ __forceinline__ int few_held(const PoolArgs & p, int seq, int lane) {
-    const int32_t * row = p.table + (int64_t) seq * p.table_len;
-    for (int e0 = 0; e0 < p.table_len; e0 += 64) {
-        const int e = e0 + lane;
-        const unsigned long long end = __ballot(e >= p.table_len || (unsigned) row[min(e, p.table_len - 1)] >= (unsigned) p.n_pages);
+// leading entries of a sequence that name a page, by one wave, which has the first 64 of its table row in `first`
+__device__ __forceinline__ int few_held(const PoolArgs & p, const int32_t * row, int first, int lane) {
+    for (int e0 = 0;;) {
+        const unsigned long long end = __ballot(e0 + lane >= p.table_len || (unsigned) first >= (unsigned) p.n_pages);
         if (end) return e0 + __builtin_ctzll(end);
+        if ((e0 += 64) >= p.table_len) return p.table_len;
+        first = row[min(e0 + lane, p.table_len - 1)];
     }
-    return p.table_len;
 }
 
 // A chain of dependent loads (items, table rows, counts, counts again) between barriers: 5 us for four items on 350 pages, where the three
 // kernels of their own took 14 with the copies, this and the copies 9.
 __global__ void __launch_bounds__(FEW_T) k_fork_few(ForkArgs a) {
     __shared__ FewPool s;
-    struct Item { int src, dst, ok, keeps, need, base, part_page; z2o::ForkSize f; };
+    struct Item { int src, dst, rows, room, ok, keeps, need, base, part_page; z2o::ForkSize f; };
     __shared__ Item s_item[z2o::FEW_FORKS];
     const PoolArgs & p = a.p;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    if (tid < a.n) { s_item[tid].src = a.src[tid]; s_item[tid].dst = a.dst[tid]; }
+    if (tid < a.n) {
+        const int src = a.src[tid], dst = a.dst[tid], rows = a.rows[tid], room = a.room[tid];
+        s_item[tid].src = src; s_item[tid].dst = dst; s_item[tid].rows = rows; s_item[tid].room = room;
+    }
     __syncthreads();
     for (int i = wave; i < a.n; i += FEW_T / 64) {
         Item & it = s_item[i];
@@ -350,14 +355,15 @@ __global__ void __launch_bounds__(FEW_T) k_fork_few(ForkArgs a) {
             if (lane == 0) { it.ok = 0; it.need = 0; }
             continue;
         }
-        const int have = few_held(p, src, lane), given = src == dst ? have : few_held(p, dst, lane);
         const int32_t * from = p.table + (int64_t) src * p.table_len, * own = p.table + (int64_t) dst * p.table_len;
-        const z2o::ForkSize f = z2o::fork_size(a.rows[i], a.room[i], have, p.table_len, p.page_shift);
+        const int at = min(lane, p.table_len - 1), from0 = from[at], own0 = own[at];
+        const int have = few_held(p, from, from0, lane), given = src == dst ? have : few_held(p, own, own0, lane);
+        const z2o::ForkSize f = z2o::fork_size(it.rows, it.room, have, p.table_len, p.page_shift);
         const int part = f.rows & ((1 << p.page_shift) - 1), stay = src == dst ? f.whole + (part > 0) : 0;
         for (int e = lane; e < given; e += 64)
-            if (e >= stay) atomicSub(p.refs + own[e], 1);
+            if (e >= stay) atomicSub(p.refs + (e < 64 ? own0 : own[e]), 1);
         if (src != dst)
-            for (int e = lane; e < f.whole; e += 64) atomicAdd(p.refs + from[e], 1);
+            for (int e = lane; e < f.whole; e += 64) atomicAdd(p.refs + (e < 64 ? from0 : from[e]), 1);
         if (lane == 0) { it.ok = 1; it.f = f; it.part_page = part ? from[f.whole] : -1; }
     }
     static_assert(z2o::FEW_FORKS <= 64, "an item per lane");
@@ -417,7 +423,7 @@ __global__ void __launch_bounds__(FEW_T) k_fork_few(ForkArgs a) {
 }
 __global__ void __launch_bounds__(256) k_fork_copy(ForkArgs a) {
     const ForkItem it = uniform_copy(a.items + blockIdx.x);
-    if (it.ok) copy_page<true>(a.p, it.part_page, it.base, it.need * a.p.row_bytes, (int) blockIdx.y * 256 + threadIdx.x, (int) gridDim.y * 256);
+    if (it.ok) copy_page<true>(a.p, it.part_page, it.base, it.need * a.p.row_bytes, (int) blockIdx.y, (int) gridDim.y);
 }
 
 struct CompactArgs {
@@ -500,10 +506,10 @@ __global__ void __launch_bounds__(256) k_pages_compact(CompactArgs a) {
         return;
     }
     const int moves = *a.n_moves, page_bytes = (p.nkv * p.row_bytes) << p.page_shift, units = page_bytes / 16 * 2 * p.n_layer;
-    const int per = max(1, units / (256 * 8));                   // blocks that share a page
+    const int per = max(1, units / (256 * COPY_UNITS));                   // blocks that share a page
     for (int64_t w = blockIdx.x; w < (int64_t) moves * per; w += a.blocks) {
         const int2 m = a.moves[w / per];
-        copy_page<false>(p, m.x, m.y, page_bytes, (int) (w % per) * 256 + tid, per * 256);
+        copy_page<false>(p, m.x, m.y, page_bytes, (int) (w % per), per);
     }
 }
 

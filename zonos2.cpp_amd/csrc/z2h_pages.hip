@@ -45,7 +45,7 @@ int z2h_pages_fork(z2h_ctx * ctx, const z2h_pages * pages, int n_layer, int64_t 
     ON_DEVICE;
     // 8 units of 16 bytes per thread of what a page may have to copy
     const int64_t units = (int64_t) n_layer * 2 * pages->n_head_kv * pages->page_rows * pages->head_dim / 8;
-    const int share = (int) std::min<int64_t>(std::max<int64_t>(1, units / (256 * 8)), std::max(1, 8192 / n));
+    const int share = (int) std::min<int64_t>(std::max<int64_t>(1, units / (256 * COPY_UNITS)), std::max(1, 8192 / n));
     if (n <= z2o::FEW_FORKS && pages->n_pages <= z2o::FEW_PAGES) {
         hipLaunchKernelGGL(k_fork_few, dim3(1), dim3(FEW_T), 0, st, a);
         if (int rc = launched(ctx)) return rc;
@@ -74,7 +74,9 @@ int z2h_pages_compact(z2h_ctx * ctx, const z2h_pages * pages, int n_layer, int64
     CompactArgs a{};
     a.p = s.p; a.table_out = d_table_out; a.refs_out = d_refs_out; a.n_used = d_n_used;
     a.map = (int32_t *) (ws + w.map); a.n_moves = (int32_t *) (ws + w.moves); a.moves = (int2 *) (ws + w.moves + 256);
-    a.blocks = 2048;
+    // eight units of 16 bytes per thread of what half of the pages have, 2048 blocks at most
+    const int64_t units = (int64_t) n_layer * 2 * pages->n_head_kv * pages->page_rows * pages->head_dim / 8;
+    a.blocks = (int) std::min<int64_t>(2048, std::max<int64_t>(1, pages->n_pages / 2 * std::max<int64_t>(1, units / (256 * COPY_UNITS))));
     const int64_t entries = (int64_t) pages->n_seq * pages->table_len;
     const hipStream_t st = (hipStream_t) stream;
     ON_DEVICE;
