@@ -384,7 +384,7 @@ typedef struct z2h_experts {
     int32_t type, n_expert, n_ff, n_embd;
 } z2h_experts;
 
-/* A mixture-of-experts layer for a few rows (a step's, a request's drafts; 1 .. Z2H_MOE_ROWS_MAX), in two launches:
+/* A mixture-of-experts layer for a few rows (a step's, a request's drafts; 1 .. Z2H_MOE_ROWS_MAX), in two or three launches:
  *   p = softmax(d_logits of the row), the top_k experts by p + d_bias (NULL: by p; equal ones: the lower index first), w = p of these,
  *   divided by their sum if `renorm` is not 0;   out = sum_j w_j down_e(j) (silu(gate_e(j) x) * (up_e(j) x)).
  * d_logits [n_rows][n_expert] are fp32, d_bias [n_expert]. d_x and d_out are [n_rows][n_embd] of `type`, rows *_stride apart: Z2H_F32 or

@@ -1,12 +1,17 @@
 // z2h_moe.h — a mixture-of-experts layer for a few rows on the caller's tensors: routing, the experts' gated products, their weighted sum.
 //
 //   p = softmax(logits), the top_k of p + bias, w = p (or p / sum), out = sum_j w_j down (silu(gate x) * (up x))
-//   k_moe_gate_up   every block routes all rows for itself (a wave per row), then takes an equal share of the tiles of 8 gate and 8 up rows of
-//                   the experts that a row takes; h = silu(gate x) * (up x) in fp32
+//   k_moe_route     more than eight rows: each row's experts and weights, a wave per row
+//   k_moe_gate_up   every block lists the experts that a row takes (up to eight rows: after routing them all for itself), then takes an equal
+//                   share of the tiles of 8 gate and 8 up rows of those experts; h = silu(gate x) * (up x) in fp32
 //   k_moe_down      16 dims of out per block (and a share of the experts' hidden dims), all rows; shares are joined by the last block of them
-// Both read every weight that they need once and are bound by that: weights go from memory to the left operand of v_mfma_f32_16x16x32, 16 rows of
-// the matrix by 32 of its columns per instruction, and up to 16 rows of x or h are the right operand, so that the products cost the
-// same for 1 to 16 of them.
+// Both products read every weight that they need once and are bound by that: weights go from memory to the left operand of
+// v_mfma_f32_16x16x32, 16 rows of the matrix by 32 of its columns per instruction, and up to 16 rows of x or h are the right operand, so that
+// the products cost the same for 1 to 16 of them. A row of x goes there as it is (fp32: as two fp16 numbers), h always as two numbers of the
+// weights' type, so that neither loses more than the weights' own rounding did.
+// Measured, bf16 weights: 64 rows, 6 of 64 experts of 1024 x 2048: 218 us, 3.7 TB/s of weights (k_moe_route 5, k_moe_gate_up 120 for
+// 537 MB, k_moe_down 76 for 268 MB); fp16, 16 rows, 4 of 32 experts of 1536 x 2048: 118 us, 4.5 TB/s; fp32 rows, one row: 26 us, 2.9 TB/s,
+// of which 12 are two launches, routing and the join (a layer of 8 x 32 takes those too).
 #pragma once
 #include "z2h_common.h"
 #include "z2h_ops_rules.h"
@@ -33,6 +38,8 @@ struct MoeArgs {
     float * weights;
     MoeTable * table;
     MoeTouched * touched;
+    int32_t * row_sel;                                           // [n k] of k_moe_route; null: every block routes for itself
+    float * row_w;
     float * w;                                                   // [n k] weights of the routes, by place
     int32_t * tickets;                                           // [tiles of out]
     float * h;                                                   // [n k][F], by place
@@ -68,10 +75,10 @@ __device__ __forceinline__ long long wave_max_ll(long long v) {
     return ((long long) __builtin_amdgcn_readlane((int) (v >> 32), 0) << 32) | (unsigned) __builtin_amdgcn_readlane((int) v, 0);
 }
 
-// One row's experts and weights by one wave, into sel and w [k]; false: the row has no number. Experts are told apart by p + bias in 64 bits,
+// One row's experts and weights by one wave, into sel and w [k]; a row without a number: -1 and NaN. Experts are told apart by p + bias in 64 bits,
 // without a bias by the logits themselves (the same order, and equal ones are equal). Expert 64 i + lane is entry i of the lane's.
-template <int EPL>
-__device__ __forceinline__ bool route_row(const MoeArgs & a, int row, short * sel, float * w) {
+template <int EPL, typename S>
+__device__ __forceinline__ void route_row(const MoeArgs & a, int row, S * sel, float * w) {
     const int lane = threadIdx.x & 63;
     const float * src = a.logits + (int64_t) row * a.E;
     constexpr long long NONE = -0x7fffffffffffffffll - 1;
@@ -93,7 +100,7 @@ __device__ __forceinline__ bool route_row(const MoeArgs & a, int row, short * se
     const float inv = 1.0f / wave_tree_f(sum);
     if (__any(bad)) {
         if (lane < a.k) { sel[lane] = -1; w[lane] = __builtin_nanf(""); }
-        return false;
+        return;
     }
     long long key[EPL];
 #pragma unroll
@@ -127,8 +134,15 @@ __device__ __forceinline__ bool route_row(const MoeArgs & a, int row, short * se
         sel[lane] = mine_e;
         w[lane] = a.renorm && total > 0.0f ? mine / total : mine;
     }
-    return true;
 }
+template <typename S>
+__device__ __forceinline__ void route_any(const MoeArgs & a, int row, S * sel, float * w) {
+    if (a.E <= 64) route_row<1>(a, row, sel, w);
+    else if (a.E <= 256) route_row<4>(a, row, sel, w);
+    else route_row<16>(a, row, sel, w);
+}
+// Each row once, in a launch of its own: 4 us for 64 rows of 64 experts, 13 when every block of k_moe_gate_up does all.
+__global__ void __launch_bounds__(64) k_moe_route(MoeArgs a) { route_any(a, blockIdx.x, a.row_sel + blockIdx.x * a.k, a.row_w + blockIdx.x * a.k); }
 
 struct MoeRouting {
     short sel[MOE_ROWS * z2o::MOE_MAX_TOP];
@@ -144,12 +158,18 @@ __device__ __forceinline__ void route(const MoeArgs & a, MoeRouting & s) {
     for (int i = tid; i < a.E * MOE_MASKS; i += MOE_T) (&s.rows[0][0])[i] = 0;
     if (tid < MOE_MASKS) s.no_number[tid] = 0;
     __syncthreads();
-    for (int r = wave; r < a.n; r += MOE_WAVES) {
-        short * sel = s.sel + r * a.k;
-        float * w = s.w + r * a.k;
-        const bool ok = a.E <= 64 ? route_row<1>(a, r, sel, w) : a.E <= 256 ? route_row<4>(a, r, sel, w) : route_row<16>(a, r, sel, w);
-        if (!ok && lane == 0) atomicOr(&s.no_number[r >> 5], 1u << (r & 31));
-        if (ok && lane < a.k && sel[lane] >= 0) atomicOr(&s.rows[sel[lane]][r >> 5], 1u << (r & 31));
+    if (a.row_sel)
+        for (int i = tid; i < a.n * a.k; i += MOE_T) {
+            s.sel[i] = (short) a.row_sel[i];
+            s.w[i] = a.row_w[i];
+        }
+    else
+        for (int r = wave; r < a.n; r += MOE_WAVES) route_any(a, r, s.sel + r * a.k, s.w + r * a.k);
+    __syncthreads();
+    for (int i = tid; i < a.n * a.k; i += MOE_T) {
+        const int r = i / a.k, e = s.sel[i];
+        if (e >= 0) atomicOr(&s.rows[e][r >> 5], 1u << (r & 31));
+        else if (s.w[i] != s.w[i]) atomicOr(&s.no_number[r >> 5], 1u << (r & 31));
     }
     __syncthreads();
     int total = 0;                                               // touched experts << 16 | routes
@@ -433,7 +453,8 @@ __global__ void __launch_bounds__(MOE_T, (2 * moe_per_cu<T, NT>())) k_moe_gate_u
 constexpr int MOE_DF = 4, MOE_DW = 4, MOE_DT = 64 * MOE_DW;      // operands of a unit: 128 hidden dims of an expert; waves of a block
 // 16 dims of out and all rows per block, over its share of the units (128 hidden dims of an expert), dealt to the waves in runs. The right
 // operand is w h of 16 rows that take the expert; its sums go to the rows' places in LDS when the wave turns to other rows. The next unit's
-// weights and h are on their way while this one is multiplied.
+// weights and h are on their way while this one is multiplied. (32 dims per block, which halves the reads of h: 80 us in place of 76 for 64 rows
+// and 64 experts of 1024 x 2048, 58 in place of 52 for 32 rows: fewer blocks are in flight.)
 template <typename T, typename TW>
 __global__ void __launch_bounds__(MOE_DT, 3) k_moe_down(MoeArgs a) {
     typedef typename Vec8<TW>::type v8;
@@ -545,8 +566,12 @@ __global__ void __launch_bounds__(MOE_DT, 3) k_moe_down(MoeArgs a) {
     for (int i = tid; i < a.n * 16; i += MOE_DT) {
         const int row = i >> 4, at = 16 * (int) blockIdx.x + (i & 15);
         if (at >= a.D) continue;
-        float v = 0.0f;
-        for (int p = 0; p < a.shares; ++p) v += __hip_atomic_load(a.parts + ((int64_t) p * a.n + row) * a.D + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        float v = 0.0f, x[z2o::MOE_SHARES];                      // (all requested before the first is added)
+#pragma unroll
+        for (int p = 0; p < z2o::MOE_SHARES; ++p)
+            x[p] = p < a.shares ? __hip_atomic_load(a.parts + ((int64_t) p * a.n + row) * a.D + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0f;
+#pragma unroll
+        for (int p = 0; p < z2o::MOE_SHARES; ++p) v += x[p];
         store(row, at, v);
     }
 }

@@ -6,6 +6,10 @@ using namespace z2d;
 
 namespace {
 
+// Rows up to which every block of k_moe_gate_up routes for itself, a wave per row, which saves a launch: 5 rows 56.0 us in place of 57.5, 8 rows
+// 95.7 and 96.6; with 16, two to a wave, it is even at last (133.8 and 132.5; 128 rows of 128 experts: 134 and 53).
+constexpr int MOE_OWN_ROWS = 8;
+
 template <typename T, typename TW, int NT>
 void gate_up_launch(const MoeArgs & a, int n_cu, hipStream_t st) {
     const int64_t tiles = (int64_t) std::min(a.E, a.n * a.k) * (a.F / 8);
@@ -13,6 +17,9 @@ void gate_up_launch(const MoeArgs & a, int n_cu, hipStream_t st) {
 }
 template <typename T, typename TW>
 void moe_launch(const MoeArgs & a, int n_cu, hipStream_t st) {
+    if (a.row_sel) hipLaunchKernelGGL(k_moe_route, dim3(a.n), dim3(64), 0, st, a);
+    // One tile of 16 rows leaves registers for two blocks per compute unit, two read the weights of an expert with more rows once. From 17 rows
+    // on, two: 32 rows, 8 of 64 experts: 145 us in place of 168; 64 rows, 6 of 64, evenly spread: 218 in place of 212.
     if (a.n <= 16) gate_up_launch<T, TW, 1>(a, n_cu, st);
     else gate_up_launch<T, TW, 2>(a, n_cu, st);
     hipLaunchKernelGGL((k_moe_down<T, TW>), dim3(a.tiles, a.shares), dim3(MOE_DT), MOE_DW * a.n * 64, st, a);
@@ -47,6 +54,7 @@ int z2h_moe_rows(z2h_ctx * ctx, const z2h_experts * experts, int n_rows, int top
     a.sel = d_sel; a.weights = d_weights;
     a.shares = z2o::moe_shares(a.D); a.tiles = (a.D + 15) / 16;
     a.table = (MoeTable *) ws; a.touched = (MoeTouched *) (ws + w.touched); a.w = (float *) (ws + w.w);
+    if (n_rows > MOE_OWN_ROWS) { a.row_sel = (int32_t *) (ws + w.row_sel); a.row_w = (float *) (ws + w.row_w); }
     a.tickets = (int32_t *) (ws + w.tickets); a.parts = (float *) (ws + w.parts); a.h = (float *) (ws + w.h);
     const int n_cu = compute_units(z2h_ctx_device(ctx));
     if (!n_cu) return z2h_ctx_fail(ctx, Z2H_EDEVICE, "compute-unit count query failed");
