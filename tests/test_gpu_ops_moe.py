@@ -148,6 +148,17 @@ def test_all_rows_take_one_expert(ctx, typ):
         m.check(ctx, f"{typ} {n}")
 
 
+@pytest.mark.parametrize("typ", ["f32", "bf16"])
+@pytest.mark.parametrize("E,F,D,k,n", [(12, 1032, 264, 4, 100), (200, 264, 520, 8, 128), (300, 40, 72, 16, 90), (6, 2056, 2056, 3, 48), (64, 8, 40, 6, 64)])
+def test_few_experts_take_most_rows(ctx, typ, E, F, D, k, n):
+    """Experts with many rows beside ones with few, in parts of equal work that begin and end inside an expert."""
+    print(f"moe {typ} E {E} F {F} D {D} k {k} rows {n}", flush=True)
+    m = Layer(typ, E, F, D, n, k, seed=E)
+    m.logits[:, 1::5] += 2.5 * torch.arange(1, (E + 3) // 5 + 1).remainder(4)
+    m.logits[:, E - 1] += 6.0
+    m.check(ctx, f"{typ} {E} {F} {D} {k} {n}")
+
+
 def test_ties_go_to_the_lower_index(ctx):
     m = Layer("f32", 70, 16, 32, 6, 4)
     m.logits[0] = 0.0

@@ -22,9 +22,10 @@ namespace z2d {
 constexpr int MOE_WAVES = 8, MOE_T = 64 * MOE_WAVES;
 constexpr int MOE_ROWS = Z2H_MOE_ROWS_MAX, MOE_MASKS = MOE_ROWS / 32;
 
-// an expert that some rows take: their bits, and the place of the first of their routes (in the order of the rows)
-struct MoeTouched { int e, pos0; unsigned rows[MOE_MASKS]; };
-struct MoeTable { int n, spare[3]; unsigned no_number[MOE_MASKS]; };     // touched experts; rows without a number
+// an expert that some rows take: their bits, the place of the first of their routes (in the order of the rows), and the turns of 16 rows that the
+// experts before it take
+struct MoeTouched { short e, pos0; int turn0; unsigned rows[MOE_MASKS]; };
+struct MoeTable { int n, turns, spare[2]; unsigned no_number[MOE_MASKS]; };      // touched experts and their turns; rows without a number
 static_assert(sizeof(MoeTouched) == 24 && sizeof(MoeTable) == 32, "workspace layout");
 
 struct MoeArgs {
@@ -149,10 +150,13 @@ struct MoeRouting {
     float w[MOE_ROWS * z2o::MOE_MAX_TOP];
     unsigned rows[z2o::MOE_MAX_EXPERTS][MOE_MASKS], no_number[MOE_MASKS];
     short list[z2o::MOE_MAX_EXPERTS], pos0[z2o::MOE_MAX_EXPERTS];        // touched experts in order, and their first routes' places
-    int wave[MOE_WAVES], n;
+    short turn0[2][z2o::MOE_MAX_EXPERTS];                                // turns of 16 rows and of the kernel's own of the experts before
+    unsigned long long wave[MOE_WAVES];
+    int n, turns[2];
 };
 
-// All rows' routes, and of every expert the rows that take it; by the whole block.
+// All rows' routes, and of every expert the rows that take it; by the whole block. An expert takes a turn per ROWS rows.
+template <int ROWS>
 __device__ __forceinline__ void route(const MoeArgs & a, MoeRouting & s) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     for (int i = tid; i < a.E * MOE_MASKS; i += MOE_T) (&s.rows[0][0])[i] = 0;
@@ -172,31 +176,38 @@ __device__ __forceinline__ void route(const MoeArgs & a, MoeRouting & s) {
         else if (s.w[i] != s.w[i]) atomicOr(&s.no_number[r >> 5], 1u << (r & 31));
     }
     __syncthreads();
-    int total = 0;                                               // touched experts << 16 | routes
+    unsigned long long total = 0;                                // 16 bits each: touched experts, turns of ROWS rows, of 16 rows, routes
     for (int e0 = 0; e0 < a.E; e0 += MOE_T) {
         const int e = e0 + tid;
         int routes = 0;
         if (e < a.E)
             for (int i = 0; i < MOE_MASKS; ++i) routes += __popc(s.rows[e][i]);
-        const int mine = routes ? 0x10000 | routes : 0;
-        int x = mine;
+        const unsigned long long mine = ((unsigned long long) ((routes ? 0x10000 : 0) | (routes + ROWS - 1) / ROWS) << 32) |
+                                        (unsigned) ((routes + 15) / 16 << 16 | routes);
+        unsigned long long x = mine;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
-            const int y = __shfl_up(x, o);
+            const unsigned long long y = __shfl_up(x, o);
             if (lane >= o) x += y;
         }
         __syncthreads();
         if (lane == 63) s.wave[wave] = x;
         __syncthreads();
-        int below = total;
+        unsigned long long below = total;
         for (int w = 0; w < MOE_WAVES; ++w) {
             if (w < wave) below += s.wave[w];
             total += s.wave[w];
         }
         below += x - mine;
-        if (routes) { s.list[below >> 16] = (short) e; s.pos0[below >> 16] = (short) (below & 0xffff); }
+        if (routes) {
+            const int t = (int) (below >> 48);
+            s.list[t] = (short) e;
+            s.pos0[t] = (short) below;
+            s.turn0[0][t] = (short) (below >> 16);
+            s.turn0[1][t] = (short) (below >> 32);
+        }
     }
-    if (tid == 0) s.n = total >> 16;
+    if (tid == 0) { s.n = (int) (total >> 48); s.turns[0] = (int) (total >> 16 & 0xffff); s.turns[1] = (int) (total >> 32 & 0xffff); }
     __syncthreads();
 }
 // the i-th row that takes an expert (it has more)
@@ -286,30 +297,48 @@ template <typename T, int NT>
 constexpr int moe_per_cu() { return sizeof(T) == 2 && NT == 1 ? 2 : 1; }
 constexpr int MOE_FR = 8;                                        // operands of a wave in a pass: 256 columns of the matrix
 
-// The tiles of 16 matrix rows (8 of gate, 8 of up) that a block has, in the order in which it takes them: for every 16 NT rows of x that take the
+// A block's or wave's part u0 .. u1 of the units, which are every touched expert's pieces (tiles, chunks) times its turns, so that parts take
+// the same time (without the turns: k_moe_gate_up 205 us in place of 126 for 64 rows most of which take the same few of 64 experts). A piece
+// belongs to the part with its first unit.
+struct MoePieces {
+    int from, to;
+    __device__ __forceinline__ MoePieces(int u0, int u1, int base, int pieces, int turns) {
+        from = max(u0 - base, 0);
+        to = u1 - base;
+        if (turns > 1) { from = (from + turns - 1) / turns; to = (to + turns - 1) / turns; }
+        to = min(to, pieces);
+    }
+};
+// The tiles of 16 matrix rows (8 of gate, 8 of up) that a block has, in the order in which it takes them: for every ROWS rows of x that take the
 // expert, all its tiles; and a tile's columns in passes of up to 2048.
+template <int ROWS>
 struct MoeCursor {
-    int tile, pass, c0, t, e, count, from, to;
-    __device__ __forceinline__ void enter(const MoeRouting & s, int tile_, int per, int end) {
-        tile = from = tile_;
+    int t, tile, pass, c0, e, count, from, to;
+    // from expert t_ on; false: the block has nothing there
+    __device__ __forceinline__ bool enter(const MoeRouting & s, int t_, int per, int u0, int u1) {
         pass = c0 = 0;
-        t = tile / per;
-        to = min(end, (t + 1) * per);
-        e = __builtin_amdgcn_readfirstlane((int) s.list[t]);
-        count = 0;
+        for (t = t_; t < s.n; ++t) {
+            const int base = __builtin_amdgcn_readfirstlane((int) s.turn0[1][t]) * per;
+            if (base >= u1) return false;
+            e = __builtin_amdgcn_readfirstlane((int) s.list[t]);
+            count = 0;
 #pragma unroll
-        for (int i = 0; i < MOE_MASKS; ++i) count += __popc(s.rows[e][i]);
-        count = __builtin_amdgcn_readfirstlane(count);
+            for (int i = 0; i < MOE_MASKS; ++i) count += __popc(s.rows[e][i]);
+            count = __builtin_amdgcn_readfirstlane(count);
+            const MoePieces x(u0, u1, base, per, (count + ROWS - 1) / ROWS);
+            tile = from = x.from;
+            to = x.to;
+            if (from < to) return true;
+        }
+        return false;
     }
     // false: that was the last
-    __device__ __forceinline__ bool next(const MoeRouting & s, int per, int end, int passes, int rows) {
+    __device__ __forceinline__ bool next(const MoeRouting & s, int per, int u0, int u1, int passes) {
         if (++pass < passes) return true;
         pass = 0;
         if (++tile < to) return true;
-        if (c0 + rows < count) { tile = from; c0 += rows; return true; }
-        if (to >= end) return false;
-        enter(s, to, per, end);
-        return true;
+        if (c0 + ROWS < count) { tile = from; c0 += ROWS; return true; }
+        return enter(s, t + 1, per, u0, u1);
     }
 };
 
@@ -322,17 +351,17 @@ __global__ void __launch_bounds__(MOE_T, (2 * moe_per_cu<T, NT>())) k_moe_gate_u
     __shared__ MoeRouting s;
     __shared__ float s_sum[2][MOE_WAVES][NT][256];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    route(a, s);
+    route<16 * NT>(a, s);
     if (blockIdx.x == gridDim.x - 1) {
         for (int i = tid; i < a.n * a.k; i += MOE_T) {
             if (a.sel) a.sel[i] = s.sel[i];
             if (a.weights) a.weights[i] = s.w[i];
         }
         for (int i = tid; i < a.tiles; i += MOE_T) a.tickets[i] = 0;
-        if (tid == 0) a.table->n = s.n;
+        if (tid == 0) { a.table->n = s.n; a.table->turns = s.turns[0]; }
         if (tid < MOE_MASKS) a.table->no_number[tid] = s.no_number[tid];
         for (int t = tid; t < s.n; t += MOE_T) {
-            MoeTouched x{s.list[t], s.pos0[t], {}};
+            MoeTouched x{s.list[t], s.pos0[t], s.turn0[0][t], {}};
             for (int i = 0; i < MOE_MASKS; ++i) x.rows[i] = s.rows[x.e][i];
             a.touched[t] = x;
         }
@@ -344,22 +373,30 @@ __global__ void __launch_bounds__(MOE_T, (2 * moe_per_cu<T, NT>())) k_moe_gate_u
             a.w[s.pos0[t] + rows_before(s.rows[e], i / a.k)] = s.w[i];
         }
     }
-    const int per = a.F / 8, n_tiles = __builtin_amdgcn_readfirstlane(s.n) * per, frags = (a.D + 31) / 32;
-    const int t0 = (int) ((int64_t) n_tiles * blockIdx.x / gridDim.x), t1 = (int) ((int64_t) n_tiles * (blockIdx.x + 1) / gridDim.x);
-    if (t0 >= t1) return;
+    const int per = a.F / 8, units = __builtin_amdgcn_readfirstlane(s.turns[1]) * per, frags = (a.D + 31) / 32;
+    const int u0 = (int) ((int64_t) units * blockIdx.x / gridDim.x), u1 = (int) ((int64_t) units * (blockIdx.x + 1) / gridDim.x);
+    if (u0 >= u1) return;
+    int t0 = 0;                                                  // the expert of unit u0
+    for (int hi = __builtin_amdgcn_readfirstlane(s.n); hi - t0 > 1;) {
+        const int m = (t0 + hi) >> 1;
+        if (__builtin_amdgcn_readfirstlane((int) s.turn0[1][m]) * per <= u0) t0 = m;
+        else hi = m;
+    }
+    MoeCursor<16 * NT> cur, nxt;
+    if (!cur.enter(s, t0, per, u0, u1)) return;
     const int passes = (frags + MOE_FR * MOE_WAVES - 1) / (MOE_FR * MOE_WAVES), mine = (frags + passes * MOE_WAVES - 1) / (passes * MOE_WAVES);
     const int k8 = 8 * (lane >> 4), col = lane & 15;
     // the lane's matrix row of an expert's first tile: gate for rows 0 .. 7 of the operand, up behind them
     const TW * mat = (const TW *) (col < 8 ? a.gate : a.up) + (int64_t) (col & 7) * a.D + k8;
     auto inside = [&](int f0, int i) __attribute__((always_inline)) { return i < mine && 32 * (f0 + i) + k8 < a.D; };
-    auto request = [&](const MoeCursor & c, v8 (&w)[MOE_FR]) __attribute__((always_inline)) {
+    auto request = [&](const MoeCursor<16 * NT> & c, v8 (&w)[MOE_FR]) __attribute__((always_inline)) {
         const int f0 = (c.pass * MOE_WAVES + wave) * mine;
-        const TW * p = mat + ((int64_t) c.e * a.F + (c.tile - c.t * per) * 8) * a.D + 32 * f0;
+        const TW * p = mat + ((int64_t) c.e * a.F + c.tile * 8) * a.D + 32 * f0;
 #pragma unroll
         for (int i = 0; i < MOE_FR; ++i) w[i] = inside(f0, i) ? *(const v8 *) (p + 32 * i) : v8{};
     };
     SplitColumn<MOE_FR, TW> b[NT];                               // 16-bit rows: hi alone
-    auto columns = [&](const MoeCursor & c) __attribute__((always_inline)) {
+    auto columns = [&](const MoeCursor<16 * NT> & c) __attribute__((always_inline)) {
         const int f0 = (c.pass * MOE_WAVES + wave) * mine;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -392,12 +429,11 @@ __global__ void __launch_bounds__(MOE_T, (2 * moe_per_cu<T, NT>())) k_moe_gate_u
         }
     };
     v4f_t sum[NT];
-    MoeCursor cur, nxt;
     int buf = 0;
     bool fresh = true, more;                                     // the right operands have to be formed anew
     auto step = [&](const v8 (&w)[MOE_FR], v8 (&ahead)[MOE_FR]) __attribute__((always_inline)) {
         nxt = cur;
-        more = nxt.next(s, per, t1, passes, 16 * NT);
+        more = nxt.next(s, per, u0, u1, passes);
         if (more) request(nxt, ahead);
         if (fresh) columns(cur);
         if (cur.pass == 0)
@@ -430,7 +466,7 @@ __global__ void __launch_bounds__(MOE_T, (2 * moe_per_cu<T, NT>())) k_moe_gate_u
                         g += s_sum[buf][v][n][f * 16 + row];
                         u += s_sum[buf][v][n][(f + 8) * 16 + row];
                     }
-                    a.h[(int64_t) (s.pos0[cur.t] + at) * a.F + (cur.tile - cur.t * per) * 8 + f] = z_silu(g) * u;
+                    a.h[(int64_t) (s.pos0[cur.t] + at) * a.F + cur.tile * 8 + f] = z_silu(g) * u;
                 }
             }
             buf ^= 1;                                            // (the next tile's sums go elsewhere: one barrier per tile)
@@ -439,7 +475,6 @@ __global__ void __launch_bounds__(MOE_T, (2 * moe_per_cu<T, NT>())) k_moe_gate_u
         cur = nxt;
     };
     v8 w0[MOE_FR], w1[MOE_FR];
-    cur.enter(s, t0, per, t1);
     request(cur, w0);
     for (;;) {
         step(w0, w1);
@@ -463,31 +498,38 @@ __global__ void __launch_bounds__(MOE_DT, 3) k_moe_down(MoeArgs a) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     float * out = s_out + wave * a.n * 16;
     for (int i = lane; i < a.n * 4; i += 64) ((v4f_t *) out)[i] = v4f_t{};
-    const int n = uniform(&a.table->n)[0], chunks = (a.F + 32 * MOE_DF - 1) / (32 * MOE_DF), units = n * chunks;
+    const int n_max = min(a.E, a.n * a.k), turn0 = lane < n_max ? a.touched[lane].turn0 : 0;
+    const int n = uniform(&a.table->n)[0], chunks = (a.F + 32 * MOE_DF - 1) / (32 * MOE_DF), units = uniform(&a.table->turns)[0] * chunks;
     const int share = (int) blockIdx.y * MOE_DW + wave, shares = a.shares * MOE_DW;
     const int u0 = (int) ((int64_t) units * share / shares), u1 = (int) ((int64_t) units * (share + 1) / shares);
+    int t0 = __popcll(__ballot(lane < n && turn0 * chunks <= u0)) - 1;   // the expert of unit u0
+    for (int i = 64 + lane; i - lane < n; i += 64) t0 += __popcll(__ballot(i < n && a.touched[i].turn0 * chunks <= u0));
     const int k8 = 8 * (lane >> 4), col = lane & 15, d = 16 * (int) blockIdx.x + col;
     const TW * mat = (const TW *) a.down + (int64_t) min(d, a.D - 1) * a.F + k8;
     struct Unit { int u, t, from, to, c0, count; MoeTouched x; };
-    auto enter = [&](Unit & c, int u) __attribute__((always_inline)) {
-        c.u = c.from = u;
-        c.t = u / chunks;
-        c.to = min(u1, (c.t + 1) * chunks);
-        c.c0 = c.count = 0;
-        c.x = uniform_copy(a.touched + c.t);
+    auto enter = [&](Unit & c, int t) __attribute__((always_inline)) {
+        c.c0 = 0;
+        for (c.t = t; c.t < n; ++c.t) {
+            c.x = uniform_copy(a.touched + c.t);
+            if (c.x.turn0 * chunks >= u1) return false;
+            c.count = 0;
 #pragma unroll
-        for (int i = 0; i < MOE_MASKS; ++i) c.count += __popc(c.x.rows[i]);
+            for (int i = 0; i < MOE_MASKS; ++i) c.count += __popc(c.x.rows[i]);
+            const MoePieces x(u0, u1, c.x.turn0 * chunks, chunks, (c.count + 15) / 16);
+            c.u = c.from = x.from;
+            c.to = x.to;
+            if (c.from < c.to) return true;
+        }
+        return false;
     };
     auto next = [&](Unit & c) __attribute__((always_inline)) {
         if (++c.u < c.to) return true;
         if (c.c0 + 16 < c.count) { c.u = c.from; c.c0 += 16; return true; }
-        if (c.to >= u1) return false;
-        enter(c, c.to);
-        return true;
+        return enter(c, c.t + 1);
     };
     struct Data { v8 w[MOE_DF]; float h[MOE_DF][8], weight; };
     auto request = [&](const Unit & c, Data & x) __attribute__((always_inline)) {
-        const int f0 = (c.u - c.t * chunks) * 32 * MOE_DF, at = c.c0 + col;
+        const int f0 = c.u * 32 * MOE_DF, at = c.c0 + col;
         const TW * p = mat + (int64_t) c.x.e * a.D * a.F + f0;
         const int pos = c.x.pos0 + min(at, c.count - 1);
         const float * h = a.h + (int64_t) pos * a.F + f0 + k8;
@@ -504,7 +546,7 @@ __global__ void __launch_bounds__(MOE_DT, 3) k_moe_down(MoeArgs a) {
     };
     v4f_t sum{};
     Unit cur, nxt;
-    bool more = u0 < u1;
+    bool more = u0 < u1 && enter(cur, t0);
     auto step = [&](const Data & x, Data & ahead) __attribute__((always_inline)) {
         nxt = cur;
         more = next(nxt);
@@ -531,7 +573,6 @@ __global__ void __launch_bounds__(MOE_DT, 3) k_moe_down(MoeArgs a) {
     };
     if (more) {
         Data x0, x1;
-        enter(cur, u0);
         request(cur, x0);
         for (;;) {
             step(x0, x1);
