@@ -205,6 +205,32 @@ def test_a_pool_runs_dry(ctx, taken):
     p.counts_hold()
 
 
+@pytest.mark.parametrize("n", [32, 40])
+def test_needs_beyond_32_bits(ctx, n):
+    """Items that ask for 2^26 pages each of a pool of 100: their sum passes 2^31."""
+    print(f"pages items {n}", flush=True)
+    length, n_pages = 1 << 26, 100
+    table, refs = torch.full((n, length), -1, dtype=torch.int32, device=DEV), torch.zeros(n_pages, dtype=torch.int32, device=DEV)
+    k, v = (torch.zeros(n_pages * 16 * 32, dtype=torch.float16, device=DEV) for _ in range(2))
+    pages = z2h.Pages(k=k.data_ptr(), v=v.data_ptr(), page_stride=16 * 32, type=z2h.F16, n_pages=n_pages, page_rows=16, n_head_kv=1, head_dim=32,
+                      table=table.data_ptr(), n_seq=n, table_len=length)
+    ws = torch.full((ctx.pages_ws_bytes(pages, n),), 255, dtype=torch.uint8, device=DEV)
+    held = torch.full((n,), -9, dtype=torch.int32, device=DEV)
+    seqs, rows = ints(list(range(n - 1, -1, -1))), ints([0] * n)
+
+    def fork(room):
+        ctx.pages_fork(pages, 1, 0, refs.data_ptr(), n, seqs.data_ptr(), seqs.data_ptr(), rows.data_ptr(), room.data_ptr(), held.data_ptr(),
+                       ws.data_ptr(), ws.numel())
+        torch.cuda.synchronize()
+    for _ in range(2):
+        fork(ints([40] + [1 << 30] * (n - 1)))
+        assert held.tolist() == [40, 97 * 16] + [0] * (n - 2)
+        assert table[n - 1, :4].tolist() == [0, 1, 2, -1] and torch.equal(table[n - 2, :98], ints([*range(3, 100), -1]).view(-1))
+        assert refs.tolist() == [1] * n_pages and int((table >= 0).sum()) == n_pages
+    fork(ints([0] * n))
+    assert refs.tolist() == [0] * n_pages and int((table >= 0).sum()) == 0
+
+
 @pytest.mark.parametrize("n_pages", [30, 8193])
 def test_bad_items_change_nothing(ctx, n_pages):
     p = Pool(ctx, 5, 4, n_pages)

@@ -33,7 +33,6 @@ struct ForkArgs {
     const int32_t * src, * dst, * rows, * room;
     int32_t * held;
     ForkItem * items;
-    int item0;
 };
 
 // leading entries of a sequence that name a page, by the whole block of 256
@@ -50,7 +49,7 @@ __device__ __forceinline__ int held_pages(const PoolArgs & p, int seq, int * s_m
 
 __global__ void __launch_bounds__(256) k_pages_release(ForkArgs a) {
     __shared__ int s_min, s_bad;
-    const int i = a.item0 + blockIdx.x, tid = threadIdx.x;
+    const int i = blockIdx.x, tid = threadIdx.x;
     const PoolArgs & p = a.p;
     const int src = a.src[i], dst = a.dst[i];
     if (tid == 0) s_bad = src < 0 || src >= p.n_seq || dst < 0 || dst >= p.n_seq;
@@ -106,7 +105,7 @@ __global__ void __launch_bounds__(256) k_pages_scan(ForkArgs a) {
         if (it.ok) {
             const z2o::ForkSize f = z2o::fork_size(a.rows[i], a.room[i], it.ok - 1, p.table_len, p.page_shift);
             it.keeps = it.part_page >= 0 && it.src == it.dst && p.refs[it.part_page] <= 1;
-            it.need = f.pages - f.whole - it.keeps;
+            it.need = min(f.pages - f.whole - it.keeps, p.n_pages);
         }
         int x = it.need;
 #pragma unroll
@@ -122,6 +121,7 @@ __global__ void __launch_bounds__(256) k_pages_scan(ForkArgs a) {
             if (w < wave) below += s_wave[w];
             total += s_wave[w];
         }
+        total = min(total, p.n_pages);                           // (256 needs and this are below 2^31)
         it.base = below + x - it.need;
         if (i < a.n) a.items[i] = it;
     }
@@ -232,7 +232,7 @@ __device__ __forceinline__ void copy_page(const PoolArgs & p, int from, int to, 
 
 __global__ void __launch_bounds__(256) k_pages_take(ForkArgs a) {
     __shared__ int s_pre[z2o::MAX_POOL / z2o::POOL_SEG + 1], s_wave[4];
-    const int i = a.item0 + blockIdx.x, tid = threadIdx.x;
+    const int i = blockIdx.x, tid = threadIdx.x;
     const PoolArgs & p = a.p;
     const ForkItem it = a.items[i];
     if (!it.ok) {
@@ -330,8 +330,8 @@ __device__ __forceinline__ int few_held(const PoolArgs & p, const int32_t * row,
     }
 }
 
-// A chain of dependent loads (items, table rows, counts, counts again) between barriers: 5 us for four items on 350 pages, where the three
-// kernels of their own took 14 with the copies, this and the copies 9.
+// A chain of dependent loads (items, table rows, counts, counts again) between barriers: 7 us for four items on 350 pages, and the copies 4; all
+// of it 10.7 us one call behind the other, where the three kernels took 13.9.
 __global__ void __launch_bounds__(FEW_T) k_fork_few(ForkArgs a) {
     __shared__ FewPool s;
     struct Item { int src, dst, rows, room, ok, keeps, need, base, part_page; z2o::ForkSize f; };
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(FEW_T) k_fork_few(ForkArgs a) {
         if (lane < a.n && s_item[lane].ok) {
             Item & it = s_item[lane];
             it.keeps = it.part_page >= 0 && it.src == it.dst && __hip_atomic_load(p.refs + it.part_page, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) <= 1;
-            it.need = need = it.f.pages - it.f.whole - it.keeps;
+            it.need = need = min(it.f.pages - it.f.whole - it.keeps, p.n_pages);
         }
         int x = need;
 #pragma unroll
