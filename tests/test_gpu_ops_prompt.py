@@ -250,6 +250,22 @@ def test_infinite_values_reach_the_rows_that_see_them(ctx, typ):
 
 
 @pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("lens", [[40, 300], [1200, 700]])
+@pytest.mark.parametrize("hd", [32, 128])
+def test_values_near_the_types_largest(ctx, typ, lens, hd):
+    """Sums of weights times such values pass the largest number of fp32; their mean does not. (Rows formed key by key: every 64 keys the
+    mean is scaled and its weights divided once more, three roundings of each, 3 sqrt(n / 64) 2^-24 times eight as a random walk, which
+    the sums' 8 sqrt(n) 2^-24 of the tolerance holds beside their own 8 sqrt(64) 2^-24.)"""
+    c = Case(typ, lens, 8, 2, hd, seed=hd)
+    a, w = (c.heads + c.kvh) * hd, c.width
+    big = torch.finfo(c.dtype).max / 2
+    c.host[:, a:w] = (big * (1 + c.host[:, a:w].double().abs().remainder(0.5))).to(c.dtype)
+    c.host[lens[0]:, a:w] *= -1
+    c.host[:, a + 5] = 1.0
+    c.check(c.run(ctx), f"{typ} {lens} {hd}")
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
 def test_scores_that_are_no_numbers(ctx, typ):
     """A key whose score is minus infinity has no weight; infinity or NaN leaves the rows that see it without a number; a row that
     sees only minus infinities gives zeros."""

@@ -34,10 +34,11 @@ __device__ __forceinline__ int prompt_seq(const PromptArgs & a, int64_t slot, in
     return lo;
 }
 
-// A (row, head) in plain fp32, by one wave: 64 keys at a time, a lane each for the scores, then the dims over the lanes. A value that is
-// not finite reaches the row whatever its weight. s_q: HD floats of the wave's own.
+// A (row, head) in plain fp32, by one wave: 64 keys at a time, a lane each for the scores, then the dims over the lanes. o is the mean by weight of
+// the values so far, so that it is finite where they are. A value that is not finite reaches the row whatever its weight. s_q: HD floats of
+// the wave's own.
 template <int HD, typename T, int E>
-__device__ __forceinline__ void prompt_walk(const PromptArgs & a, int first, int row, int head, float * s_q, float (&o)[E], float & l) {
+__device__ __forceinline__ void prompt_walk(const PromptArgs & a, int first, int row, int head, float * s_q, float (&o)[E]) {
     const int lane = threadIdx.x & 63, g = head / (a.n_head / a.nkv), d = E * lane;
     const T * src = (const T *) a.q + row * a.qs + (int64_t) head * HD;
     float mx = 0.0f;
@@ -49,8 +50,7 @@ __device__ __forceinline__ void prompt_walk(const PromptArgs & a, int first, int
     for (int i = lane; i < HD; i += 64) s_q[i] = a.scale == 0.0f ? 0.0f : ldexpf((float) src[i], -up);
     wait_lds();
     const float c = copysignf(fminf(ldexpf(fabsf(a.scale) * 1.44269504088896341f, up), 0x1p127f), a.scale);
-    float m = -__builtin_inff();
-    l = 0.0f;
+    float m = -__builtin_inff(), l = 0.0f;
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.0f;
     const T * kb = (const T *) a.k + (int64_t) g * HD, * vb = (const T *) a.v + (int64_t) g * HD;
@@ -66,16 +66,17 @@ __device__ __forceinline__ void prompt_walk(const PromptArgs & a, int first, int
         if (__any(!(s < __builtin_inff()))) {                    // infinity or no number: nor is any weight a number
 #pragma unroll
             for (int e = 0; e < E; ++e) o[e] = __builtin_nanf("");
-            l = 1.0f;
             return;
         }
         const float mn = fmaxf(m, wave_max_f(s));
         const float w0 = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-        const float w = s == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(s - mn);
+        float w = s == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(s - mn);
         m = mn;
-        l = l * w0 + wave_tree_f(w);
+        const float old = l * w0, sum = old + wave_tree_f(w), inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        l = sum;
+        w *= inv;
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = is_finite(o[e]) ? o[e] * w0 : o[e];
+        for (int e = 0; e < E; ++e) o[e] = is_finite(o[e]) ? o[e] * (old * inv) : o[e];
         const int n = min(64, row + 1 - key0);
         const bool weighs = s > -__builtin_inff();
         const unsigned long long live = __ballot(weighs);
@@ -137,13 +138,12 @@ __device__ __forceinline__ float prompt_query(const PromptArgs & a, const T * sr
 template <int HD, typename T>
 __device__ __forceinline__ void prompt_again(const PromptArgs & a, int first, int row, int head, float * s_q, int lane) {
     constexpr int E = HD >= 64 ? HD / 64 : 1;
-    float x[E], sum;
-    prompt_walk<HD, T>(a, first, row, head, s_q, x, sum);
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    float x[E];
+    prompt_walk<HD, T>(a, first, row, head, s_q, x);
     T * out = (T *) a.out + row * a.os + (int64_t) head * HD + E * lane;
     if (E * lane < HD)
 #pragma unroll
-        for (int e = 0; e < E; ++e) out[e] = (T) (x[e] * inv);
+        for (int e = 0; e < E; ++e) out[e] = (T) x[e];
 }
 
 // Rows of T in LDS, stored as they are with their 16-byte pieces permuted by row: keys so that 32 rows' pieces of the same dims take all
@@ -380,19 +380,20 @@ struct PromptWave {
             }
     }
 
-    // What is not finite meets both parts of a weight, and hidden rows' weights of 0: the product is then NaN where the definition has
-    // infinity or leaves it out, never anything else that is wrong. So a row-head that holds NaN is formed once more, in plain fp32.
+    // What is not finite meets both parts of a weight, and hidden rows' weights of 0: the product is then NaN where the definition has infinity or
+    // leaves it out, and sums of weights up to 2^8 (f16: 2^14) times the largest values may be infinite where their mean is not. So a row-head
+    // that holds either is formed once more, in plain fp32.
     // s_q: HD floats of LDS of the wave's own.
     __device__ __forceinline__ void store(const PromptArgs & a, int first, int row0, int rows, int g, int first_rh, int lane, float * s_q) {
         const int group = a.n_head / a.nkv, heads = rows * group, rh = first_rh + (lane & 31);
         l += other_half(l);
-        float nan = 0.0f;
+        float odd = 0.0f;
 #pragma unroll
         for (int dt = 0; dt < M::DT; ++dt)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) nan = o[dt][i] != o[dt][i] ? 1.0f : nan;
-        nan = fmaxf(nan, other_half(nan));
-        const bool again = rh < heads && (nan != 0.0f || l != l);
+            for (int i = 0; i < 16; ++i) odd = is_finite(o[dt][i]) ? odd : 1.0f;
+        odd = fmaxf(odd, other_half(odd));
+        const bool again = rh < heads && (odd != 0.0f || !is_finite(l));
         if (rh < heads && !again) {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             T * out = (T *) a.out + (row0 + rh / group) * a.os + (int64_t) (g * group + rh % group) * HD;
@@ -710,10 +711,10 @@ __global__ void __launch_bounds__(256, 2) k_prompt_small(PromptArgs a) {
             for (int i = 0; i < HD / 16; ++i) y[i] = __builtin_fmaf(f[w], ((const float *) s_lds[w])[rh * HD + (((tid & 15) * (HD / 16) + i + 4 * rh) & (HD - 1))], y[i]);
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    bool nan = sum != sum;
+    bool odd = !is_finite(sum);
 #pragma unroll
-    for (int i = 0; i < HD / 16; ++i) nan |= y[i] != y[i];
-    if (nan) s_again[rh] = 1;
+    for (int i = 0; i < HD / 16; ++i) odd |= !is_finite(y[i]);
+    if (odd) s_again[rh] = 1;
     __syncthreads();
     if (rh < heads && !s_again[rh]) {
         T * out = (T *) a.out + (t.row0 + rh / group) * a.os + (int64_t) (t.g * group + rh % group) * HD + (tid & 15) * (HD / 16);
