@@ -245,8 +245,11 @@ inline const char * check_moe_type(int type, int experts) {
 
 // ---- a paged cache's upkeep
 constexpr int MAX_POOL = 1 << 22, MAX_FORKS = 4096, POOL_SEG = 1024;
-// What one block does by itself (k_fork_few, k_moves_few).
-constexpr int FEW_PAGES = 8192, FEW_FORKS = 32;
+// What one block does by itself (k_fork_few, an item per wave, and k_moves_few), where a launch less is worth more than many blocks. In us, a row of
+// calls, against the general kernels: 4 items on 110 pages 9.8 and 11.0, on 8000 10.2 and 11.9; 16 items on 180 pages 10.4 and 11.6, on 8000
+// 12.4 and 11.9; 24 items, two to a wave, 13.0 and 12.0. Compaction of 4 layers, 300 pages: 7.7 and 9.2; 7000: 68.6 and 71.7; 14000:
+// 130.1 and 129.5.
+constexpr int FEW_PAGES = 8192, FEW_FORKS = 16;
 inline const char * check_pool(const z2h_pages * p, int n) {
     if (const char * e = check_pages(p)) return e;
     if (p->n_pages > MAX_POOL) return "pages: n_pages above 2^22";
