@@ -9,8 +9,8 @@
 // v_mfma_f32_16x16x32, 16 rows of the matrix by 32 of its columns per instruction, and up to 16 rows of x or h are the right operand, so that
 // the products cost the same for 1 to 16 of them. A row of x goes there as it is (fp32: as two fp16 numbers), h always as two numbers of the
 // weights' type, so that neither loses more than the weights' own rounding did.
-// Measured, bf16 weights: 64 rows, 6 of 64 experts of 1024 x 2048: 218 us, 3.7 TB/s of weights (k_moe_route 5, k_moe_gate_up 120 for
-// 537 MB, k_moe_down 76 for 268 MB); fp16, 16 rows, 4 of 32 experts of 1536 x 2048: 118 us, 4.5 TB/s; fp32 rows, one row: 26 us, 2.9 TB/s,
+// Measured, bf16 weights: 64 rows, 6 of 64 experts of 1024 x 2048: 217 us, 3.7 TB/s of weights (k_moe_route 5, k_moe_gate_up 121 for
+// 537 MB, k_moe_down 77 for 268 MB); fp16, 16 rows, 4 of 32 experts of 1536 x 2048: 118 us, 4.5 TB/s; fp32 rows, one row: 26 us, 2.9 TB/s,
 // of which 12 are two launches, routing and the join (a layer of 8 x 32 takes those too).
 #pragma once
 #include "z2h_common.h"
@@ -488,8 +488,8 @@ __global__ void __launch_bounds__(MOE_T, (2 * moe_per_cu<T, NT>())) k_moe_gate_u
 constexpr int MOE_DF = 4, MOE_DW = 4, MOE_DT = 64 * MOE_DW;      // operands of a unit: 128 hidden dims of an expert; waves of a block
 // 16 dims of out and all rows per block, over its share of the units (128 hidden dims of an expert), dealt to the waves in runs. The right
 // operand is w h of 16 rows that take the expert; its sums go to the rows' places in LDS when the wave turns to other rows. The next unit's
-// weights and h are on their way while this one is multiplied. (32 dims per block, which halves the reads of h: 80 us in place of 76 for 64 rows
-// and 64 experts of 1024 x 2048, 58 in place of 52 for 32 rows: fewer blocks are in flight.)
+// weights and h are on their way while this one is multiplied. (32 dims per block, which halves the reads of h, leave registers for two blocks per
+// compute unit in place of three: 73 us in place of 76 for 64 rows and 64 experts of 1024 x 2048, 34 in place of 25 for small layers.)
 template <typename T, typename TW>
 __global__ void __launch_bounds__(MOE_DT, 3) k_moe_down(MoeArgs a) {
     typedef typename Vec8<TW>::type v8;
