@@ -8,6 +8,8 @@
 
 namespace z2d {
 
+typedef float v4f_t __attribute__((ext_vector_type(4)));
+
 struct PromptArgs {
     const int32_t * start;
     int n_seq, n_rows, n_head, nkv;
@@ -363,49 +365,70 @@ struct PromptWave {
         math.add(o, sv);
     }
 
-    // the sums over other keys of the same row-heads
+    // The sums over other keys of the same row-heads, four at a time. (A part without weights may hold anything: NaN, which is formed once more.)
     template <typename F>
     __device__ __forceinline__ void join(float m2, float l2, F o2) {
         const float mn = fmaxf(m, m2);
         const float w = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - mn), w2 = m2 == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m2 - mn);
-        // (both of a row-head's lanes have the same maxima; without one there is no weight, whatever the values were)
+        // (both of a row-head's lanes have the same maxima)
         m = mn;
         l = l * w + l2 * w2;
 #pragma unroll
         for (int dt = 0; dt < M::DT; ++dt)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float x = o2(dt, i);
-                o[dt][i] = (w != 0.0f ? o[dt][i] * w : 0.0f) + (w2 != 0.0f ? x * w2 : 0.0f);
+            for (int i = 0; i < 16; i += 4) {
+                const v4f_t x = o2(dt, i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[dt][i + j] = __builtin_fmaf(o[dt][i + j], w, x[j] * w2);
             }
     }
 
     // What is not finite meets both parts of a weight, and hidden rows' weights of 0: the product is then NaN where the definition has infinity or
     // leaves it out, and sums of weights up to 2^8 (f16: 2^14) times the largest values may be infinite where their mean is not. So a row-head
     // that holds either is formed once more, in plain fp32.
-    // s_q: HD floats of LDS of the wave's own.
-    __device__ __forceinline__ void store(const PromptArgs & a, int first, int row0, int rows, int g, int first_rh, int lane, float * s_q) {
+    // The others' rows go through LDS, so that 16 bytes per lane make whole rows of the output. s_own: 32 HD T of LDS of the wave's own.
+    // (What runs once per block is as little code as can be: a new instruction line of 64 bytes takes 70 ns.)
+    __device__ __forceinline__ void store(const PromptArgs & a, int first, int row0, int rows, int g, int first_rh, int lane, T * s_own) {
+        typedef Rows<HD, T> R;
         const int group = a.n_head / a.nkv, heads = rows * group, rh = first_rh + (lane & 31);
         l += other_half(l);
-        float odd = 0.0f;
+        float odd[2] = {l * 0.0f, 0.0f};                         // 0, or NaN where any is not finite
 #pragma unroll
         for (int dt = 0; dt < M::DT; ++dt)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) odd = is_finite(o[dt][i]) ? odd : 1.0f;
-        odd = fmaxf(odd, other_half(odd));
-        const bool again = rh < heads && (odd != 0.0f || !is_finite(l));
-        if (rh < heads && !again) {
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            T * out = (T *) a.out + (row0 + rh / group) * a.os + (int64_t) (g * group + rh % group) * HD;
+            for (int i = 0; i < 16; ++i) odd[i & 1] = __builtin_fmaf(o[dt][i], 0.0f, odd[i & 1]);
+        odd[0] += odd[1];
+        odd[0] += other_half(odd[0]);
+        unsigned again = (unsigned) __ballot(rh < heads && odd[0] != 0.0f);
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-            for (int dt = 0; dt < M::DT; ++dt)
+        for (int dt = 0; dt < M::DT; ++dt)
 #pragma unroll
-                for (int i = 0; i < 16; i += 4)
-                    store4(out + 32 * dt + 2 * i + 4 * (lane >> 5), o[dt][i] * inv, o[dt][i + 1] * inv, o[dt][i + 2] * inv, o[dt][i + 3] * inv);
+            for (int i = 0; i < 16; i += 4) {
+                const int d = 32 * dt + 2 * i + 4 * (lane >> 5);
+                typedef T t4 __attribute__((ext_vector_type(4)));
+                *(t4 *) (s_own + R::k_at(lane & 31, d / R::N) + d % R::N) = __builtin_convertvector(
+                    (v4f_t{o[dt][i] * inv, o[dt][i + 1] * inv, o[dt][i + 2] * inv, o[dt][i + 3] * inv}), t4);
+            }
+        wait_lds();
+        const bool wide = (uintptr_t) a.out % 16 == 0 && a.os * (int64_t) sizeof(T) % 16 == 0;
+        const float part = 1.0f / group;
+#pragma unroll 2
+        for (int j = 0; j < R::NC / 2; ++j) {
+            const int row = (64 * j + lane) / R::NC, piece = lane % R::NC, at = first_rh + row;
+            const int r = (int) ((at + 0.5f) * part);            // (at / group: both are below 2^8)
+            typedef T tv __attribute__((ext_vector_type(R::N)));
+            const tv x = *(const tv *) (s_own + R::k_at(row, piece));
+            if (at >= heads || again >> row & 1) continue;
+            T * out = (T *) a.out + (row0 + r) * a.os + (int64_t) (g * group + at - r * group) * HD + piece * R::N;
+            if (wide) *(tv *) out = x;
+            else
+#pragma unroll
+                for (int e = 0; e < R::N; ++e) out[e] = x[e];
         }
-        for (unsigned long long todo = __ballot(again) & 0xffffffffull; todo; todo &= todo - 1) {
-            const int at = first_rh + __builtin_ctzll(todo);
-            prompt_again<HD, T>(a, first, row0 + at / group, g * group + at % group, s_q, lane);
+        for (; again; again &= again - 1) {
+            const int at = first_rh + __builtin_ctz(again);
+            prompt_again<HD, T>(a, first, row0 + at / group, g * group + at % group, (float *) s_own, lane);
         }
     }
 };
@@ -465,7 +488,6 @@ __device__ __forceinline__ PromptTile prompt_tile(const PromptArgs & a, int tile
 }
 
 // ---- few tiles: 16 row-heads per block, the keys dealt to its four waves
-typedef float v4f_t __attribute__((ext_vector_type(4)));
 // the largest (or the sum) of a column's values, whose four lanes are 16 apart
 template <bool SUM>
 __device__ __forceinline__ float column(float v) {
@@ -783,14 +805,18 @@ __global__ void __launch_bounds__(256 * HALVES, 2) k_prompt(PromptArgs a) {
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) to[(16 * dt + i) * 64 + lane] = w.o[dt][i];
+                for (int i = 0; i < 16; i += 4) *(v4f_t *) (to + ((16 * dt + i) * 16 + lane) * 4) = v4f_t{w.o[dt][i], w.o[dt][i + 1], w.o[dt][i + 2], w.o[dt][i + 3]};
         }
         __syncthreads();
         if (half) return;
-        w.join(s_ml[wave][0][lane], s_ml[wave][1][lane], [&](int dt, int i) { return to[(16 * dt + i) * 64 + lane]; });
+        w.join(s_ml[wave][0][lane], s_ml[wave][1][lane], [&](int dt, int i) { return *(const v4f_t *) (to + ((16 * dt + i) * 16 + lane) * 4); });
         wait_lds();
-        w.store(a, t.first, t.row0, t.rows, t.g, 32 * wave, lane, to);
-    } else w.store(a, t.first, t.row0, t.rows, t.g, 32 * wave, lane, (float *) s_k0 + wave * HD);
+        w.store(a, t.first, t.row0, t.rows, t.g, 32 * wave, lane, (T *) to);
+    } else {
+        constexpr int PER = KEYS / 32;                           // waves' rows that a buffer holds
+        T * to = wave / PER == 0 ? s_k0[0] : wave / PER == 1 ? s_k1[0] : wave / PER == 2 ? s_v0[0] : s_v1[0];
+        w.store(a, t.first, t.row0, t.rows, t.g, 32 * wave, lane, to + wave % PER * 32 * HD);
+    }
 }
 
 } // namespace z2d
