@@ -9,8 +9,8 @@
 // v_mfma_f32_16x16x32, 16 rows of the matrix by 32 of its columns per instruction, and up to 16 rows of x or h are the right operand, so that
 // the products cost the same for 1 to 16 of them. A row of x goes there as it is (fp32: as two fp16 numbers), h always as two numbers of the
 // weights' type, so that neither loses more than the weights' own rounding did.
-// Measured, bf16 weights: 64 rows, 6 of 64 experts of 1024 x 2048: 217 us, 3.7 TB/s of weights (k_moe_route 5, k_moe_gate_up 121 for
-// 537 MB, k_moe_down 77 for 268 MB); fp16, 16 rows, 4 of 32 experts of 1536 x 2048: 118 us, 4.5 TB/s; fp32 rows, one row: 26 us, 2.9 TB/s,
+// Measured, bf16 weights: 64 rows, 6 of 64 experts of 1032 x 2048: 209 us, 3.9 TB/s of weights (k_moe_route 5, k_moe_gate_up 125 for
+// 541 MB, k_moe_down 75 for 270 MB); fp16, 16 rows, 4 of 32 experts of 1536 x 2048: 114 us, 4.7 TB/s; fp32 rows, one row: 27 us, 2.8 TB/s,
 // of which 12 are two launches, routing and the join (a layer of 8 x 32 takes those too).
 #pragma once
 #include "z2h_common.h"
@@ -43,7 +43,8 @@ struct MoeArgs {
     float * row_w;
     float * w;                                                   // [n k] weights of the routes, by place
     int32_t * tickets;                                           // [tiles of out]
-    float * h;                                                   // [n k][F], by place
+    int hs;
+    float * h;                                                   // [n k][hs], by place; see k_moe_down for the columns' order
     float * parts;                                               // [shares][n][D]
 };
 
@@ -458,7 +459,9 @@ __global__ void __launch_bounds__(MOE_T, (2 * moe_per_cu<T, NT>())) k_moe_gate_u
                 for (int i = 0; i < 4; ++i) s_sum[buf][wave][n][(4 * (lane >> 4) + i) * 16 + col] = sum[n][i];
             lds_sync();
             if (tid < NT * 128) {
-                const int n = tid >> 7, row = (tid >> 3) & 15, f = tid & 7, at = cur.c0 + 16 * n + row;
+                int id = tid;
+                asm volatile("" : "+v"(id));                     // (formed here anew: kept over the loop, these would not fit its registers)
+                const int n = id >> 7, row = (id >> 3) & 15, f = id & 7, at = cur.c0 + 16 * n + row;
                 if (at < cur.count) {
                     float g = 0.0f, u = 0.0f;
 #pragma unroll
@@ -466,7 +469,7 @@ __global__ void __launch_bounds__(MOE_T, (2 * moe_per_cu<T, NT>())) k_moe_gate_u
                         g += s_sum[buf][v][n][f * 16 + row];
                         u += s_sum[buf][v][n][(f + 8) * 16 + row];
                     }
-                    a.h[(int64_t) (s.pos0[cur.t] + at) * a.F + cur.tile * 8 + f] = z_silu(g) * u;
+                    a.h[(int64_t) (s.pos0[cur.t] + at) * a.hs + ((cur.tile >> 2) * 32 + (cur.tile & 3) * 4) + ((f & 4) * 4 + (f & 3))] = z_silu(g) * u;
                 }
             }
             buf ^= 1;                                            // (the next tile's sums go elsewhere: one barrier per tile)
@@ -486,10 +489,14 @@ __global__ void __launch_bounds__(MOE_T, (2 * moe_per_cu<T, NT>())) k_moe_gate_u
 
 // ---- down
 constexpr int MOE_DF = 4, MOE_DW = 4, MOE_DT = 64 * MOE_DW;      // operands of a unit: 128 hidden dims of an expert; waves of a block
-// 16 dims of out and all rows per block, over its share of the units (128 hidden dims of an expert), dealt to the waves in runs. The right
-// operand is w h of 16 rows that take the expert; its sums go to the rows' places in LDS when the wave turns to other rows. The next unit's
-// weights and h are on their way while this one is multiplied. (32 dims per block, which halves the reads of h, leave registers for two blocks per
-// compute unit in place of three: 73 us in place of 76 for 64 rows and 64 experts of 1024 x 2048, 34 in place of 25 for small layers.)
+// 16 dims of out and all rows per block, over its share of the units (128 hidden dims of an expert), dealt to the waves in turn, so that they read the
+// matrix row by row together (in runs of their own: 86 us in place of 80 where few experts take most rows). The right operand is w h of 16
+// rows that take the expert; its sums go to the rows' places in LDS when the wave turns to other rows. The next unit's weights and h are
+// on their way while this one is multiplied. h comes from the caches as often as there are tiles of out: of 32 of its columns, the first
+// four of every eight lie before the others, so that the four lanes of a row, who have eight columns each, read 64 bytes in a row at a
+// time (64 rows, 64 experts of 1032 x 2048: the layer 208 us in place of 217). Without any reads of h it would take 20 us less. (32 dims per
+// block, which halves them, leave registers for two blocks per compute unit in place of three: 206 us there, 31 in place of 27 for a layer
+// of 8 x 32; 12 waves over 64 dims, for the near cache's sake: 82 us in place of 78 in this kernel.)
 template <typename T, typename TW>
 __global__ void __launch_bounds__(MOE_DT, 3) k_moe_down(MoeArgs a) {
     typedef typename Vec8<TW>::type v8;
@@ -500,8 +507,7 @@ __global__ void __launch_bounds__(MOE_DT, 3) k_moe_down(MoeArgs a) {
     for (int i = lane; i < a.n * 4; i += 64) ((v4f_t *) out)[i] = v4f_t{};
     const int n_max = min(a.E, a.n * a.k), turn0 = lane < n_max ? a.touched[lane].turn0 : 0;
     const int n = uniform(&a.table->n)[0], chunks = (a.F + 32 * MOE_DF - 1) / (32 * MOE_DF), units = uniform(&a.table->turns)[0] * chunks;
-    const int share = (int) blockIdx.y * MOE_DW + wave, shares = a.shares * MOE_DW;
-    const int u0 = (int) ((int64_t) units * share / shares), u1 = (int) ((int64_t) units * (share + 1) / shares);
+    const int u0 = (int) ((int64_t) units * blockIdx.y / a.shares), u1 = (int) ((int64_t) units * (blockIdx.y + 1) / a.shares);
     int t0 = __popcll(__ballot(lane < n && turn0 * chunks <= u0)) - 1;   // the expert of unit u0
     for (int i = 64 + lane; i - lane < n; i += 64) t0 += __popcll(__ballot(i < n && a.touched[i].turn0 * chunks <= u0));
     const int k8 = 8 * (lane >> 4), col = lane & 15, d = 16 * (int) blockIdx.x + col;
@@ -516,14 +522,14 @@ __global__ void __launch_bounds__(MOE_DT, 3) k_moe_down(MoeArgs a) {
 #pragma unroll
             for (int i = 0; i < MOE_MASKS; ++i) c.count += __popc(c.x.rows[i]);
             const MoePieces x(u0, u1, c.x.turn0 * chunks, chunks, (c.count + 15) / 16);
-            c.u = c.from = x.from;
+            c.u = c.from = x.from + ((wave - c.t * chunks - x.from) & (MOE_DW - 1));
             c.to = x.to;
             if (c.from < c.to) return true;
         }
         return false;
     };
     auto next = [&](Unit & c) __attribute__((always_inline)) {
-        if (++c.u < c.to) return true;
+        if ((c.u += MOE_DW) < c.to) return true;
         if (c.c0 + 16 < c.count) { c.u = c.from; c.c0 += 16; return true; }
         return enter(c, c.t + 1);
     };
@@ -532,13 +538,13 @@ __global__ void __launch_bounds__(MOE_DT, 3) k_moe_down(MoeArgs a) {
         const int f0 = c.u * 32 * MOE_DF, at = c.c0 + col;
         const TW * p = mat + (int64_t) c.x.e * a.D * a.F + f0;
         const int pos = c.x.pos0 + min(at, c.count - 1);
-        const float * h = a.h + (int64_t) pos * a.F + f0 + k8;
+        const float * h = a.h + (int64_t) pos * a.hs + f0 + 4 * (lane >> 4);
 #pragma unroll
         for (int i = 0; i < MOE_DF; ++i) {
             const bool in = f0 + 32 * i + k8 < a.F;
             x.w[i] = d < a.D && in ? *(const v8 *) (p + 32 * i) : v8{};
             v4f_t y0{}, y1{};
-            if (at < c.count && in) { y0 = *(const v4f_t *) (h + 32 * i); y1 = *(const v4f_t *) (h + 32 * i + 4); }
+            if (at < c.count && in) { y0 = *(const v4f_t *) (h + 32 * i); y1 = *(const v4f_t *) (h + 32 * i + 16); }
 #pragma unroll
             for (int j = 0; j < 4; ++j) { x.h[i][j] = y0[j]; x.h[i][4 + j] = y1[j]; }
         }

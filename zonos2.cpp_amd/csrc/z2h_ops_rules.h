@@ -307,6 +307,7 @@ inline int moe_shares(int n_embd) {
     const int tiles = (n_embd + 15) / 16, s = (768 + tiles - 1) / tiles;
     return s < 1 ? 1 : s > MOE_SHARES ? MOE_SHARES : s;
 }
+inline int moe_h_stride(int n_ff) { return (n_ff + 31) / 32 * 32; }
 struct MoeWs { int64_t touched = 0, w = 0, row_sel = 0, row_w = 0, tickets = 0, parts = 0, h = 0, bytes = 0; };
 inline MoeWs moe_ws(const z2h_experts & x, int n_rows, int top_k) {
     MoeWs m;
@@ -319,7 +320,7 @@ inline MoeWs moe_ws(const z2h_experts & x, int n_rows, int top_k) {
     m.tickets = m.row_w + align256(routes * 4);
     m.parts = m.tickets + align256((int64_t) (x.n_embd + 15) / 16 * 4);
     m.h = m.parts + (shares > 1 ? align256((int64_t) shares * n_rows * x.n_embd * 4) : 0);
-    m.bytes = m.h + align256(routes * x.n_ff * 4);
+    m.bytes = m.h + align256(routes * 4 * moe_h_stride(x.n_ff));
     return m;
 }
 
