@@ -5,7 +5,7 @@
 // The running maximum m moves only where a score exceeds it by 2^8, so that sums are seldom scaled. 4 hd flops per row-head and key and 2 hd more for
 // the weights' second parts: long prompts are bound by the products (one of 8191 rows, 32 heads of 128, bf16: 730 us, 1.1 PFLOP/s with the
 // second parts, which is what a matrix product of 8192 reaches; 24 of 16 to 2000 rows, 32 heads of 64: 97 us, 0.86), short ones by a
-// chain of loads and by code that runs once (8 of 256 rows, 16 heads of 128, f16: 15.1 us; one of 37, fp32: 7.8, of which 2.7 are the launch).
+// chain of loads and by code that runs once (8 of 256 rows, 16 heads of 128, f16: 14.7 us; one of 37, fp32: 7.8, of which 2.7 are the launch).
 #pragma once
 #include "z2h_common.h"
 #include "z2h_ops_rules.h"
@@ -105,24 +105,24 @@ __device__ __forceinline__ void prompt_walk(const PromptArgs & a, int first, int
 }
 
 // The lane's part of a row-head's query, whose sign and (fp32) a power of two of whose size are taken out: scores are `c` times the products, in
-// units of log2. whole: the largest of all lanes that have a part of the row-head.
-template <typename T, int QN, typename D, typename W>
-__device__ __forceinline__ float prompt_query(const PromptArgs & a, const T * src, bool live, D dim, float (&x)[QN], W whole) {
+// units of log2. whole: the largest of all lanes that have a part of the row-head; beside: requests that go out behind the query's.
+template <typename T, int QN, typename D, typename W, typename B>
+__device__ __forceinline__ float prompt_query(const PromptArgs & a, const T * src, bool live, D dim, float (&x)[QN], W whole, B beside) {
     const bool zero = !live || a.scale == 0.0f;
     const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
     float c = zero ? 1.0f : fabsf(a.scale) * 1.44269504088896341f;
     constexpr int N = 16 / (int) sizeof(T);
+    typedef T tv __attribute__((ext_vector_type(N)));
+    tv y[QN / N];
     if (((uintptr_t) src & 15) == 0) {
-        typedef T tv __attribute__((ext_vector_type(N)));
 #pragma unroll
-        for (int i = 0; i < QN; i += N) {
-            const tv y = *(const tv *) (src + dim(i));
-#pragma unroll
-            for (int j = 0; j < N; ++j) x[i + j] = (float) y[j];
-        }
+        for (int i = 0; i < QN / N; ++i) y[i] = *(const tv *) (src + dim(N * i));
     } else
 #pragma unroll
-        for (int i = 0; i < QN; ++i) x[i] = (float) src[dim(i)];
+        for (int i = 0; i < QN; ++i) y[i / N][i % N] = src[dim(i)];
+    beside();
+#pragma unroll
+    for (int i = 0; i < QN; ++i) x[i] = (float) y[i / N][i % N];
     float up = sign;
     if constexpr (sizeof(T) == 4) {
         // a power of two keeps the scores of large queries finite, and those of tiny ones from vanishing
@@ -319,14 +319,15 @@ struct PromptWave {
     int vis;                                                     // keys that the lane's row sees
 
     // row-heads first_rh .. + 31 of rows row0 .. row0 + rows - 1, whose first sees `before` + 1 keys
-    __device__ __forceinline__ void init(const PromptArgs & a, int row0, int rows, int before, int g, int first_rh, int lane) {
+    template <typename B>
+    __device__ __forceinline__ void init(const PromptArgs & a, int row0, int rows, int before, int g, int first_rh, int lane, B beside) {
         const int group = a.n_head / a.nkv, rh = first_rh + (lane & 31);
         const bool live = rh < rows * group;
         const int r = live ? rh / group : 0, head = g * group + (live ? rh % group : 0);
         const T * src = (const T *) a.q + (row0 + r) * a.qs + (int64_t) head * HD;
         vis = live ? before + r + 1 : 0x7fffffff;
         float x[M::QN];
-        c = prompt_query<T, M::QN>(a, src, live, [&](int i) { return M::dim(i, lane); }, x, [](float mx) { return fmaxf(mx, other_half(mx)); });
+        c = prompt_query<T, M::QN>(a, src, live, [&](int i) { return M::dim(i, lane); }, x, [](float mx) { return fmaxf(mx, other_half(mx)); }, beside);
         math.init(x, lane);
         m = -__builtin_inff();
         l = 0.0f;
@@ -659,7 +660,6 @@ __global__ void __launch_bounds__(256, 2) k_prompt_small(PromptArgs a) {
     typename M::Data d0, d1;
     M math;
     int key = M::KEYS * wave;
-    if (key < n_keys) math.request(d0, k, a.ks, v, a.vs, key, n_keys - 1, lds, lane);
     // the queries
     const bool live = col < heads;
     const int r = live ? col / group : 0, head = t.g * group + (live ? col % group : 0), vis = before + r + 1;
@@ -667,7 +667,8 @@ __global__ void __launch_bounds__(256, 2) k_prompt_small(PromptArgs a) {
     {
         float x[M::QN];
         c = prompt_query<T, M::QN>(a, (const T *) a.q + (t.row0 + r) * a.qs + (int64_t) head * HD, live, [&](int i) { return M::dim(i, g); }, x,
-                                   [](float mx) { return column<false>(mx); });
+                                   [](float mx) { return column<false>(mx); },
+                                   [&]() __attribute__((always_inline)) { if (key < n_keys) math.request(d0, k, a.ks, v, a.vs, key, n_keys - 1, lds, lane); });
         math.init(x);
     }
     v4f_t o[DT];
@@ -778,9 +779,10 @@ __global__ void __launch_bounds__(256 * HALVES, 2) k_prompt(PromptArgs a) {
         for (int i = 0; i < PARTS; ++i) bring_part(i, key, sk, sv);
     };
     int key = half * KEYS;
-    if (key < n_keys) bring(key, s_k0[half], s_v0[half]);
     PromptWave<HD, T> w;
-    w.init(a, t.row0, t.rows, before, t.g, 32 * wave, lane);
+    w.init(a, t.row0, t.rows, before, t.g, 32 * wave, lane, [&]() __attribute__((always_inline)) {
+        if (key < n_keys) bring(key, s_k0[half], s_v0[half]);
+    });
     // the wave's rows see keys up to `mine`
     const int mine = 32 * wave < t.rows * group ? before + min(t.rows, (32 * wave + 31) / group + 1) : 0;
     auto stage = [&](const T * sk, const T * sv, T * ok, T * ov) __attribute__((always_inline)) {
