@@ -47,7 +47,7 @@ def layer(x, gate, up, down, sel, w, dtype):
     division); the output by sum w |down| dh, its own dot product, its weights (their softmax in fp32: 8 * 2^-24 and 2 * 2^-24 E), and its
     type's rounding."""
     n, D = x.shape
-    out, tol = torch.zeros((n, D), dtype=torch.float64), torch.zeros((n, D), dtype=torch.float64)
+    out, tol = (torch.zeros((n, D), dtype=torch.float64, device=x.device) for _ in range(2))
     e24 = 2.0 ** -24
     ux = 2.0 ** -21 if dtype == torch.float32 else 0.0
     uh = 2.0 ** -16 if dtype == torch.bfloat16 else 2.0 ** -21
@@ -157,6 +157,27 @@ def test_few_experts_take_most_rows(ctx, typ, E, F, D, k, n):
     m.logits[:, 1::5] += 2.5 * torch.arange(1, (E + 3) // 5 + 1).remainder(4)
     m.logits[:, E - 1] += 6.0
     m.check(ctx, f"{typ} {E} {F} {D} {k} {n}")
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [1, 17, 40])
+def test_wide_rows_and_many_hidden_dims(ctx, typ, n):
+    """Rows of more than one pass of columns, more tiles of hidden dims per block than take a pass together (4101 tiles; from 17 rows on on
+    256 blocks at most)."""
+    print(f"moe {typ} rows {n}, wide", flush=True)
+    E, F, D, k = 1, 32808, 2064, 1
+    m = Layer(typ, E, 8, 8, n, k, seed=n, renorm=True)
+    g = torch.Generator(device=DEV).manual_seed(n)
+    gate, up = ((torch.randn((E, F, D), generator=g, device=DEV) * D ** -0.5).to(m.wtype) for _ in range(2))
+    down = (torch.randn((E, D, F), generator=g, device=DEV) * F ** -0.5).to(m.wtype)
+    x = torch.randn((n, D), generator=g, device=DEV).to(m.dtype)
+    m.F, m.D, m.x = F, D, x
+    m.ex = z2h.Experts(gate=gate.data_ptr(), up=up.data_ptr(), down=down.data_ptr(), type=m.ex.type, n_expert=E, n_ff=F, n_embd=D)
+    d = m.put(ctx)
+    m.call(ctx, d)
+    torch.cuda.synchronize()
+    ref, tol = layer(x.double(), gate.double(), up.double(), down.double(), np.zeros((n, 1), np.int64), np.ones((n, 1)), m.dtype)
+    check(d["out"], ref.cpu(), tol.cpu(), typ)
 
 
 def test_ties_go_to_the_lower_index(ctx):

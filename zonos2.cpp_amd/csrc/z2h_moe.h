@@ -311,10 +311,13 @@ struct MoePieces {
     }
 };
 // The tiles of 16 matrix rows (8 of gate, 8 of up) that a block has, in the order in which it takes them: for every ROWS rows of x that take the
-// expert, all its tiles; and a tile's columns in passes of up to 2048.
+// expert, all its tiles. Columns go in passes of up to 2048; with more than one, MOE_GROUP tiles take a pass before their next one, so that
+// the right operands are formed once for all of them (64 rows, 4 of 32 experts of 1536 x 4096: 294 us in place of 534 in fp32,
+// 295 in place of 373 in f16).
+constexpr int MOE_GROUP = 16;
 template <int ROWS>
 struct MoeCursor {
-    int t, tile, pass, c0, e, count, from, to;
+    int t, tile, pass, c0, e, count, from, to, g0;
     // from expert t_ on; false: the block has nothing there
     __device__ __forceinline__ bool enter(const MoeRouting & s, int t_, int per, int u0, int u1) {
         pass = c0 = 0;
@@ -327,7 +330,7 @@ struct MoeCursor {
             for (int i = 0; i < MOE_MASKS; ++i) count += __popc(s.rows[e][i]);
             count = __builtin_amdgcn_readfirstlane(count);
             const MoePieces x(u0, u1, base, per, (count + ROWS - 1) / ROWS);
-            tile = from = x.from;
+            tile = g0 = from = x.from;
             to = x.to;
             if (from < to) return true;
         }
@@ -335,10 +338,12 @@ struct MoeCursor {
     }
     // false: that was the last
     __device__ __forceinline__ bool next(const MoeRouting & s, int per, int u0, int u1, int passes) {
-        if (++pass < passes) return true;
+        if (++tile < (passes > 1 ? min(g0 + MOE_GROUP, to) : to)) return true;
+        if (++pass < passes) { tile = g0; return true; }
         pass = 0;
-        if (++tile < to) return true;
-        if (c0 + ROWS < count) { tile = from; c0 += ROWS; return true; }
+        g0 = tile;
+        if (tile < to) return true;
+        if (c0 + ROWS < count) { tile = g0 = from; c0 += ROWS; return true; }
         return enter(s, t + 1, per, u0, u1);
     }
 };
@@ -350,7 +355,7 @@ __global__ void __launch_bounds__(MOE_T, (2 * moe_per_cu<T, NT>())) k_moe_gate_u
     constexpr bool SPLIT = sizeof(T) == 4;
     typedef typename Vec8<TW>::type v8;
     __shared__ MoeRouting s;
-    __shared__ float s_sum[2][MOE_WAVES][NT][256];
+    __shared__ float s_sum[2][MOE_WAVES][NT][256], s_acc[MOE_GROUP][2][128 * NT];       // of a tile's earlier passes
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     route<16 * NT>(a, s);
     if (blockIdx.x == gridDim.x - 1) {
@@ -437,44 +442,41 @@ __global__ void __launch_bounds__(MOE_T, (2 * moe_per_cu<T, NT>())) k_moe_gate_u
         more = nxt.next(s, per, u0, u1, passes);
         if (more) request(nxt, ahead);
         if (fresh) columns(cur);
-        if (cur.pass == 0)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) sum[n] = v4f_t{};
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             v4f_t part{};
-            if constexpr (!SPLIT) part = sum[n];
 #pragma unroll
             for (int i = 0; i < MOE_FR; ++i) {
                 part = mfma16<TW>(w[i], b[n].hi[i], part);
                 if constexpr (SPLIT) part = mfma16<TW>(w[i], b[n].lo[i], part);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sum[n][i] = SPLIT ? __builtin_fmaf(part[i], b[n].back, sum[n][i]) : part[i];
+            for (int i = 0; i < 4; ++i) sum[n][i] = SPLIT ? part[i] * b[n].back : part[i];
         }
-        if (cur.pass == passes - 1) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s_sum[buf][wave][n][(4 * (lane >> 4) + i) * 16 + col] = sum[n][i];
-            lds_sync();
-            if (tid < NT * 128) {
-                int id = tid;
-                asm volatile("" : "+v"(id));                     // (formed here anew: kept over the loop, these would not fit its registers)
-                const int n = id >> 7, row = (id >> 3) & 15, f = id & 7, at = cur.c0 + 16 * n + row;
-                if (at < cur.count) {
-                    float g = 0.0f, u = 0.0f;
+            for (int i = 0; i < 4; ++i) s_sum[buf][wave][n][(4 * (lane >> 4) + i) * 16 + col] = sum[n][i];
+        lds_sync();
+        if (tid < NT * 128) {
+            int id = tid;
+            asm volatile("" : "+v"(id));                         // (formed here anew: kept over the loop, these would not fit its registers)
+            const int n = id >> 7, row = (id >> 3) & 15, f = id & 7, at = cur.c0 + 16 * n + row;
+            if (at < cur.count) {
+                float g = 0.0f, u = 0.0f;
 #pragma unroll
-                    for (int v = 0; v < MOE_WAVES; ++v) {
-                        g += s_sum[buf][v][n][f * 16 + row];
-                        u += s_sum[buf][v][n][(f + 8) * 16 + row];
-                    }
-                    a.h[(int64_t) (s.pos0[cur.t] + at) * a.hs + ((cur.tile >> 2) * 32 + (cur.tile & 3) * 4) + ((f & 4) * 4 + (f & 3))] = z_silu(g) * u;
+                for (int v = 0; v < MOE_WAVES; ++v) {
+                    g += s_sum[buf][v][n][f * 16 + row];
+                    u += s_sum[buf][v][n][(f + 8) * 16 + row];
                 }
+                float (& acc)[2][128 * NT] = s_acc[cur.tile - cur.g0 & (MOE_GROUP - 1)];         // (0 with one pass)
+                if (cur.pass) { g += acc[0][id]; u += acc[1][id]; }
+                if (cur.pass < passes - 1) { acc[0][id] = g; acc[1][id] = u; }
+                else a.h[(int64_t) (s.pos0[cur.t] + at) * a.hs + ((cur.tile >> 2) * 32 + (cur.tile & 3) * 4) + ((f & 4) * 4 + (f & 3))] = z_silu(g) * u;
             }
-            buf ^= 1;                                            // (the next tile's sums go elsewhere: one barrier per tile)
         }
-        fresh = more && (passes > 1 || nxt.t != cur.t || nxt.c0 != cur.c0);
+        buf ^= 1;                                                // (the next tile's sums go elsewhere: one barrier per tile)
+        fresh = more && (nxt.pass != cur.pass || nxt.t != cur.t || nxt.c0 != cur.c0);
         cur = nxt;
     };
     v8 w0[MOE_FR], w1[MOE_FR];
