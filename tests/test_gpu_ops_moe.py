@@ -180,6 +180,31 @@ def test_wide_rows_and_many_hidden_dims(ctx, typ, n):
     check(d["out"], ref.cpu(), tol.cpu(), typ)
 
 
+def test_offsets_beyond_32_bits(ctx):
+    """The last of 33 experts of 8192 x 8192 lies 2^31 elements behind the first, and so do the second row of x and that of the output."""
+    print("moe offsets", flush=True)
+    E, F, D, n, far = 33, 8192, 8192, 2, (1 << 31) + 8
+    m = Layer("f16", E, 8, 8, n, 1, renorm=True)
+    g = torch.Generator(device=DEV).manual_seed(5)
+    w = [torch.zeros((E, F, D), dtype=torch.float16, device=DEV) for _ in range(3)]
+    for t in w:
+        t[E - 1] = (torch.randn((F, D), generator=g, device=DEV) * D ** -0.5).half()
+    x = torch.zeros(far + D, dtype=torch.float16, device=DEV)
+    x[:D], x[far:] = (torch.randn(D, generator=g, device=DEV).half() for _ in range(2))
+    out = torch.full((far + D,), 7.0, dtype=torch.float16, device=DEV)
+    m.logits[:] = -1.0
+    m.logits[:, E - 1] = 5.0
+    m.F, m.D = F, D
+    m.x = torch.stack([x[:D], x[far:]])
+    m.ex = z2h.Experts(gate=w[0].data_ptr(), up=w[1].data_ptr(), down=w[2].data_ptr(), type=m.ex.type, n_expert=E, n_ff=F, n_embd=D)
+    d = m.put(ctx)
+    m.call(ctx, d, xs=far, os=far, x=x.data_ptr(), out=out.data_ptr())
+    torch.cuda.synchronize()
+    ref, tol = layer(m.x.double(), *(t[E - 1:].double() for t in w), np.zeros((n, 1), np.int64), np.ones((n, 1)), m.dtype)
+    check(torch.stack([out[:D], out[far:]]), ref.cpu(), tol.cpu(), "far")
+    assert bool((out[D:far] == 7).all())
+
+
 def test_ties_go_to_the_lower_index(ctx):
     m = Layer("f32", 70, 16, 32, 6, 4)
     m.logits[0] = 0.0

@@ -301,6 +301,43 @@ def test_random_histories(ctx, n_pages, most):
                 p.counts_hold()
 
 
+@pytest.mark.parametrize("items", [1, 20])
+def test_pages_beyond_32_bits(ctx, items):
+    """Pages 2^27 bytes apart: rows copied from, to and between pages that lie more than 2^32 bytes behind the first."""
+    print(f"pages far apart, items {items}", flush=True)
+    n_pages, stride, P, hd = 40, 1 << 26, 16, 32
+    k, v = (torch.zeros(n_pages * stride, dtype=torch.float16, device=DEV) for _ in range(2))
+    table, refs = np.full((items + 1, 4), -1, np.int32), np.zeros(n_pages, np.int32)
+    refs[:36] = 1                                                # (held by nobody here: taken)
+    table[0, :2], refs[34:36] = (35, 34), 1
+    d_table, d_refs = ints(table), ints(refs)
+    rows = [torch.randn((P, hd), generator=torch.Generator().manual_seed(i)).half() for i in range(4)]
+    for t, (a, b) in zip((k, v), (rows[:2], rows[2:])):
+        t[35 * stride:35 * stride + P * hd], t[34 * stride:34 * stride + P * hd] = a.reshape(-1).to(DEV), b.reshape(-1).to(DEV)
+    pages = z2h.Pages(k=k.data_ptr(), v=v.data_ptr(), page_stride=stride, type=z2h.F16, n_pages=n_pages, page_rows=P, n_head_kv=1, head_dim=hd,
+                      table=d_table.data_ptr(), n_seq=items + 1, table_len=4)
+    ws = torch.full((ctx.pages_ws_bytes(pages, items),), 255, dtype=torch.uint8, device=DEV)
+    src, dst, take, room = ints([0] * items), ints(list(range(1, items + 1))), ints([P + 5] * items), ints([P + 5] * items)
+    ctx.pages_fork(pages, 1, 0, d_refs.data_ptr(), items, src.data_ptr(), dst.data_ptr(), take.data_ptr(), room.data_ptr(), 0, ws.data_ptr(), ws.numel())
+    torch.cuda.synchronize()
+    got = d_table.cpu().numpy()
+    at = lambda t, p: t[p * stride:p * stride + P * hd].view(P, hd).cpu()
+    for i in range(min(items, 4)):
+        assert got[i + 1].tolist() == [35, 36 + i, -1, -1]
+        for t, r in ((k, rows[1]), (v, rows[3])):
+            assert torch.equal(at(t, 36 + i)[:5], r[:5]) and not bool(at(t, 36 + i)[5:].any())
+    # the first 33 pages end: 33 .. move to the front
+    refs = d_refs.cpu().numpy()
+    refs[:34] = 0
+    d_refs.copy_(ints(refs))
+    n = torch.zeros(1, dtype=torch.int32, device=DEV)
+    ctx.pages_compact(pages, 1, 0, d_refs.data_ptr(), d_table.data_ptr(), d_refs.data_ptr(), n.data_ptr(), ws.data_ptr(), ws.numel())
+    torch.cuda.synchronize()
+    assert int(n) == int((refs > 0).sum()) and d_table[0].tolist() == [1, 0, -1, -1]
+    for t, (a, b) in zip((k, v), (rows[:2], rows[2:])):
+        assert torch.equal(at(t, 1), a) and torch.equal(at(t, 0), b) and torch.equal(at(t, 2)[:5], b[:5])
+
+
 def test_compact_edges(ctx):
     """Nothing in use, all in use, one page at the very end, entries that name nothing."""
     p = Pool(ctx, 2, 3, 1500, layers=2, kvh=1, hd=32)

@@ -206,6 +206,23 @@ def test_in_place(ctx, typ, lens):
 
 
 @pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("lens", [[200, 3, 64], [1300]])
+def test_in_place_with_values_that_are_not_finite(ctx, typ, lens):
+    """Rows that are formed key by key read their queries while others are stored already."""
+    c = Case(typ, lens, 8, 2, 64)
+    a = (c.heads + c.kvh) * c.hd
+    c.host[5::37, a + 3] = math.inf
+    c.host[9::41, a + c.hd + 60] = -math.inf
+    c.host[100, c.heads * c.hd + 7] = math.nan
+    apart, flat = c.run(ctx), c.upload()
+    c.call(ctx, flat, flat.data_ptr(), c.R)
+    torch.cuda.synchronize()
+    got = flat[:c.n * c.R].view(c.n, c.R)[:, :c.heads * c.hd].reshape(c.n, c.heads, c.hd)
+    assert torch.equal(torch.isnan(got), torch.isnan(apart)) and bool(torch.isinf(apart).any()) and bool(torch.isnan(apart).any())
+    assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(apart))
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
 def test_rows_of_no_sequence(ctx, typ):
     """Rows before the first sequence and behind the last are left as they were, and what they hold reaches nobody."""
     c = Case(typ, [33, 100], 4, 2, 64, first=9, extra=50)
