@@ -60,6 +60,22 @@ static void experts() {
     EXPECT(!z2o::check_moe(&good, 1, 3) && z2o::check_moe(&good, 1, 4));
     EXPECT(!z2o::check_moe_type(Z2H_F32, Z2H_F16) && !z2o::check_moe_type(Z2H_F16, Z2H_F16) && !z2o::check_moe_type(Z2H_BF16, Z2H_BF16));
     EXPECT(z2o::check_moe_type(Z2H_F32, Z2H_BF16) && z2o::check_moe_type(Z2H_BF16, Z2H_F16) && z2o::check_moe_type(Z2H_Q8_0, Z2H_F16));
+    // a workspace's parts follow each other and hold what the kernels put there; shares of an output dim are as many as the join takes
+    for (int n_expert : {1, 8, 60, 1024})
+        for (int dim : {8, 40, 1032, 2048, 65536})
+            for (int n : {0, 1, 8, 17, 128})
+                for (int k : {1, 16}) {
+                    if (k > n_expert) continue;
+                    const z2h_experts x{(void *) 256, (void *) 256, (void *) 256, Z2H_F16, n_expert, dim, dim};
+                    EXPECT(!z2o::check_moe(&x, n, k));
+                    const z2o::MoeWs w = z2o::moe_ws(x, n, k);
+                    const int64_t routes = (int64_t) n * k, touched = routes < n_expert ? routes : n_expert, shares = z2o::moe_shares(dim);
+                    EXPECT(shares >= 1 && shares <= z2o::MOE_SHARES && z2o::moe_h_stride(dim) >= dim && z2o::moe_h_stride(dim) % 32 == 0);
+                    EXPECT(w.touched >= 32 && w.w >= w.touched + 24 * touched && w.row_sel >= w.w + 4 * routes && w.row_w >= w.row_sel + 4 * routes);
+                    EXPECT(w.tickets >= w.row_w + 4 * routes && w.parts >= w.tickets + 4 * ((dim + 15) / 16));
+                    EXPECT(w.h >= w.parts + (shares > 1 ? 4 * shares * n * dim : 0) && w.bytes >= w.h + 4 * routes * z2o::moe_h_stride(dim));
+                    for (int64_t at : {w.touched, w.w, w.row_sel, w.row_w, w.tickets, w.parts, w.h, w.bytes}) EXPECT(at % 256 == 0);
+                }
 }
 
 static void pool() {
