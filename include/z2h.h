@@ -393,7 +393,7 @@ typedef struct z2h_experts {
  * stand in the places that remain, and a row without any expert gives zeros. A row with a logit or a sum p + bias that is no number, or
  * with an infinite logit, has no number as its result, and -1 and no number in d_sel and d_weights. top_k is 1 .. min(n_expert, 16).
  * Sums in fp32; fp32 rows meet the weights as two f16 numbers, off by 2^-22 of the largest of 256 neighbours at most, and so do the products
- * silu(..) * .. (two bf16 numbers with bf16 experts, 2^-16 each). A row that holds a value that is not finite has results that are not
+ * silu(..) * .. (three bf16 numbers with bf16 experts, 2^-24 of each). A row that holds a value that is not finite has results that are not
  * finite, and no other row's change. Results do not depend on timing.
  * The workspace (z2h_moe_rows_ws_bytes; 0: the sizes are refused; 256-byte aligned) holds one call at a time: calls and graphs that may
  * overlap need one each. */

@@ -7,9 +7,8 @@
 //   k_moe_down      16 dims of out per block (and a share of the experts' hidden dims), all rows; shares are joined by the last block of them
 // Both products read every weight that they need once and are bound by that: weights go from memory to the left operand of
 // v_mfma_f32_16x16x32, 16 rows of the matrix by 32 of its columns per instruction, and up to 16 rows of x or h are the right operand, so that
-// the products cost the same for 1 to 16 of them. A row of x goes there as it is (fp32: as two fp16 numbers), h always as two numbers of the
-// weights' type, so that neither loses more than the weights' own rounding did.
-// Measured, bf16 weights: 64 rows, 6 of 64 experts of 1032 x 2048: 209 us, 3.9 TB/s of weights (k_moe_route 5, k_moe_gate_up 125 for
+// the products cost the same for 1 to 16 of them. A row of x goes there as it is (fp32: as two fp16 numbers), h as two fp16 or three bf16 numbers.
+// Measured, bf16 weights: 64 rows, 6 of 64 experts of 1032 x 2048: 210 us, 3.9 TB/s of weights (k_moe_route 5, k_moe_gate_up 125 for
 // 541 MB, k_moe_down 75 for 270 MB); fp16, 16 rows, 4 of 32 experts of 1536 x 2048: 114 us, 4.7 TB/s; fp32 rows, one row: 27 us, 2.8 TB/s,
 // of which 12 are two launches, routing and the join (a layer of 8 x 32 takes those too).
 #pragma once
@@ -255,12 +254,14 @@ __device__ __forceinline__ float column_max(float v) {
     const unsigned r0 = r[0], r1 = r[1];
     return fmaxf(__builtin_bit_cast(float, r0), __builtin_bit_cast(float, r1));
 }
-// fp32 columns as two numbers of the weights' type each. f16: brought to [2^7, 2^8) by a power of two first, so that both parts together keep
-// every value to 2^-22 of the column's largest; `back` undoes it.
+// fp32 columns as numbers of the weights' type. f16: two each, brought to [2^7, 2^8) by a power of two first, so that both parts together keep
+// every value to 2^-22 of the column's largest; `back` undoes it. bf16: three each, which keep every value to 2^-24 of itself (two keep
+// 2^-16: outputs that are differences of nearly equal terms lose as many of their bits; 64 rows 210 us in place of 209, 5 rows 54 in place of 53).
 template <int FR, typename TW>
 struct SplitColumn {
+    static constexpr int PARTS = __is_same(TW, _Float16) ? 2 : 3;
     typedef typename Vec8<TW>::type v8;
-    v8 hi[FR], lo[FR];
+    v8 part[PARTS][FR];
     float back;
     __device__ __forceinline__ void set(const float (&x)[FR][8]) {
         float up = 1.0f;
@@ -284,10 +285,13 @@ struct SplitColumn {
             for (int j = 0; j < 8; j += 2) {
                 typedef typename Pair<float>::type f2;
                 typedef typename Pair<TW>::type c2;
-                const f2 y = {x[i][j] * up, x[i][j + 1] * up};
-                const c2 h = __builtin_convertvector(y, c2), l = __builtin_convertvector(two_rest(y, h), c2);
-                hi[i][j] = h[0]; hi[i][j + 1] = h[1];
-                lo[i][j] = l[0]; lo[i][j + 1] = l[1];
+                f2 y = {x[i][j] * up, x[i][j + 1] * up};
+#pragma unroll
+                for (int q = 0; q < PARTS; ++q) {
+                    const c2 h = __builtin_convertvector(y, c2);
+                    part[q][i][j] = h[0]; part[q][i][j + 1] = h[1];
+                    if (q + 1 < PARTS) y = two_rest(y, h);
+                }
             }
     }
 };
@@ -401,7 +405,7 @@ __global__ void __launch_bounds__(MOE_T, (2 * moe_per_cu<T, NT>())) k_moe_gate_u
 #pragma unroll
         for (int i = 0; i < MOE_FR; ++i) w[i] = inside(f0, i) ? *(const v8 *) (p + 32 * i) : v8{};
     };
-    SplitColumn<MOE_FR, TW> b[NT];                               // 16-bit rows: hi alone
+    SplitColumn<MOE_FR, TW> b[NT];                               // 16-bit rows: the first part alone
     auto columns = [&](const MoeCursor<16 * NT> & c) __attribute__((always_inline)) {
         const int f0 = (c.pass * MOE_WAVES + wave) * mine;
 #pragma unroll
@@ -423,12 +427,12 @@ __global__ void __launch_bounds__(MOE_T, (2 * moe_per_cu<T, NT>())) k_moe_gate_u
                 const bool wide = ((uintptr_t) x & 15) == 0;
 #pragma unroll
                 for (int i = 0; i < MOE_FR; ++i) {
-                    b[n].hi[i] = v8{};
+                    b[n].part[0][i] = v8{};
                     if (live && inside(f0, i)) {
-                        if (wide) b[n].hi[i] = *(const v8 *) (x + 32 * i);
+                        if (wide) b[n].part[0][i] = *(const v8 *) (x + 32 * i);
                         else
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) b[n].hi[i][j] = x[32 * i + j];
+                            for (int j = 0; j < 8; ++j) b[n].part[0][i][j] = x[32 * i + j];
                     }
                 }
             }
@@ -447,8 +451,8 @@ __global__ void __launch_bounds__(MOE_T, (2 * moe_per_cu<T, NT>())) k_moe_gate_u
             v4f_t part{};
 #pragma unroll
             for (int i = 0; i < MOE_FR; ++i) {
-                part = mfma16<TW>(w[i], b[n].hi[i], part);
-                if constexpr (SPLIT) part = mfma16<TW>(w[i], b[n].lo[i], part);
+                part = mfma16<TW>(w[i], b[n].part[0][i], part);
+                if constexpr (SPLIT) part = mfma16<TW>(w[i], b[n].part[1][i], part);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) sum[n][i] = SPLIT ? part[i] * b[n].back : part[i];
@@ -563,10 +567,9 @@ __global__ void __launch_bounds__(MOE_DT, 3) k_moe_down(MoeArgs a) {
         b.set(x.h);
         v4f_t part{};
 #pragma unroll
-        for (int i = 0; i < MOE_DF; ++i) {
-            part = mfma16<TW>(x.w[i], b.hi[i], part);
-            part = mfma16<TW>(x.w[i], b.lo[i], part);
-        }
+        for (int i = 0; i < MOE_DF; ++i)
+#pragma unroll
+            for (int q = 0; q < b.PARTS; ++q) part = mfma16<TW>(x.w[i], b.part[q][i], part);
         const float back = b.back * x.weight;
 #pragma unroll
         for (int i = 0; i < 4; ++i) sum[i] = __builtin_fmaf(part[i], back, sum[i]);
