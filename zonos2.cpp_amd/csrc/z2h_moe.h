@@ -1,8 +1,8 @@
 // z2h_moe.h — a mixture-of-experts layer for a few rows on the caller's tensors: routing, the experts' gated products, their weighted sum.
 //
 //   p = softmax(logits), the top_k of p + bias, w = p (or p / sum), out = sum_j w_j down (silu(gate x) * (up x))
-//   k_moe_route     more than eight rows: each row's experts and weights, a wave per row
-//   k_moe_gate_up   every block lists the experts that a row takes (up to eight rows: after routing them all for itself), then takes an equal
+//   k_moe_route     more than eight rows or 256 experts: each row's experts and weights, a wave per row
+//   k_moe_gate_up   every block lists the experts that a row takes (without k_moe_route: after routing all rows for itself), then takes an equal
 //                   share of the tiles of 8 gate and 8 up rows of those experts; h = silu(gate x) * (up x) in fp32
 //   k_moe_down      16 dims of out per block (and a share of the experts' hidden dims), all rows; shares are joined by the last block of them
 // Both products read every weight that they need once and are bound by that: weights go from memory to the left operand of
@@ -76,15 +76,16 @@ __device__ __forceinline__ long long wave_max_ll(long long v) {
     return ((long long) __builtin_amdgcn_readlane((int) (v >> 32), 0) << 32) | (unsigned) __builtin_amdgcn_readlane((int) v, 0);
 }
 
-// One row's experts and weights by one wave, into sel and w [k]; a row without a number: -1 and NaN. Experts are told apart by p + bias in 64 bits,
-// without a bias by the logits themselves (the same order, and equal ones are equal). Expert 64 i + lane is entry i of the lane's.
+// One row's experts and weights by one wave, into sel and w [k]; a row without a number: -1 and NaN. Probabilities and p + bias are formed in 64 bits
+// (without a bias the logits themselves tell experts apart), and weights are rounded once. Weights that are to sum to one are formed relative
+// to the largest chosen logit: a bias may keep the others out by any distance. Expert 64 i + lane is entry i of the lane's.
 template <int EPL, typename S>
 __device__ __forceinline__ void route_row(const MoeArgs & a, int row, S * sel, float * w) {
     const int lane = threadIdx.x & 63;
     const float * src = a.logits + (int64_t) row * a.E;
     constexpr long long NONE = -0x7fffffffffffffffll - 1;
-    float z[EPL], p[EPL], b[EPL];
-    float mx = -__builtin_inff(), sum = 0.0f;
+    float z[EPL], b[EPL];
+    float mx = -__builtin_inff();
     bool bad = false;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
@@ -94,22 +95,22 @@ __device__ __forceinline__ void route_row(const MoeArgs & a, int row, S * sel, f
         bad |= !(z[i] < __builtin_inff()) || b[i] != b[i];
         mx = fmaxf(mx, z[i]);
     }
-    mx = wave_max_f(mx);
-    const float m0 = mx == -__builtin_inff() ? 0.0f : mx;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) sum += p[i] = z_expf(z[i] - m0);
-    const float inv = 1.0f / wave_tree_f(sum);
     if (__any(bad)) {
         if (lane < a.k) { sel[lane] = -1; w[lane] = __builtin_nanf(""); }
         return;
     }
+    mx = wave_max_f(mx);
+    const double m0 = mx == -__builtin_inff() ? 0.0 : (double) mx;
+    double p[EPL], sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) sum += p[i] = z_exp_d((double) z[i] - m0);
+    sum = wave_tree_d(sum);
+    const double inv = 1.0 / sum;
     long long key[EPL];
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-        p[i] *= inv;
-        key[i] = z[i] == -__builtin_inff() ? NONE : score_key(a.bias ? (double) p[i] + (double) b[i] : (double) z[i]);
-    }
-    float total = 0.0f, mine = 0.0f;
+    for (int i = 0; i < EPL; ++i)
+        key[i] = z[i] == -__builtin_inff() ? NONE : score_key(a.bias ? p[i] * inv + (double) b[i] : (double) z[i]);
+    float mine = -__builtin_inff();
     short mine_e = -1;
     for (int found = 0; found < a.k; ++found) {
         long long best = key[0];
@@ -123,27 +124,34 @@ __device__ __forceinline__ void route_row(const MoeArgs & a, int row, S * sel, f
             const unsigned long long same = __ballot(key[i] == top);
             if (open && same) {
                 const int at = __builtin_ctzll(same);
-                const float pe = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, p[i]), at));
-                total += pe;
-                if (lane == found) { mine = pe; mine_e = (short) (64 * i + at); }
+                const float ze = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, z[i]), at));
+                if (lane == found) { mine = ze; mine_e = (short) (64 * i + at); }
                 if (lane == at) key[i] = NONE;
                 open = false;
             }
         }
     }
+    const double from = a.renorm ? (double) wave_max_f(mine) : m0;
+    const double we = mine_e < 0 ? 0.0 : z_exp_d((double) mine - from);
+    if (a.renorm) sum = wave_tree_d(we);
     if (lane < a.k) {
         sel[lane] = mine_e;
-        w[lane] = a.renorm && total > 0.0f ? mine / total : mine;
+        w[lane] = mine_e < 0 ? 0.0f : (float) (we / sum);
     }
 }
-template <typename S>
+// Up to this many experts a block of k_moe_gate_up may route for itself; 16 to a lane do not fit its registers (bf16, 300 experts: 8 rows 22.7 us with
+// the launch, 24.0 without and 11 registers spilled; 1 row 21.9 and 21.0).
+constexpr int MOE_OWN_EXPERTS = 256;
+template <int MAX, typename S>
 __device__ __forceinline__ void route_any(const MoeArgs & a, int row, S * sel, float * w) {
     if (a.E <= 64) route_row<1>(a, row, sel, w);
-    else if (a.E <= 256) route_row<4>(a, row, sel, w);
+    else if (MAX <= 256 || a.E <= 256) route_row<4>(a, row, sel, w);
     else route_row<16>(a, row, sel, w);
 }
 // Each row once, in a launch of its own: 4 us for 64 rows of 64 experts, 13 when every block of k_moe_gate_up does all.
-__global__ void __launch_bounds__(64) k_moe_route(MoeArgs a) { route_any(a, blockIdx.x, a.row_sel + blockIdx.x * a.k, a.row_w + blockIdx.x * a.k); }
+__global__ void __launch_bounds__(64) k_moe_route(MoeArgs a) {
+    route_any<z2o::MOE_MAX_EXPERTS>(a, blockIdx.x, a.row_sel + blockIdx.x * a.k, a.row_w + blockIdx.x * a.k);
+}
 
 struct MoeRouting {
     short sel[MOE_ROWS * z2o::MOE_MAX_TOP];
@@ -168,7 +176,7 @@ __device__ __forceinline__ void route(const MoeArgs & a, MoeRouting & s) {
             s.w[i] = a.row_w[i];
         }
     else
-        for (int r = wave; r < a.n; r += MOE_WAVES) route_any(a, r, s.sel + r * a.k, s.w + r * a.k);
+        for (int r = wave; r < a.n; r += MOE_WAVES) route_any<MOE_OWN_EXPERTS>(a, r, s.sel + r * a.k, s.w + r * a.k);
     __syncthreads();
     for (int i = tid; i < a.n * a.k; i += MOE_T) {
         const int r = i / a.k, e = s.sel[i];

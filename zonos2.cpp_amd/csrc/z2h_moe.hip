@@ -54,7 +54,7 @@ int z2h_moe_rows(z2h_ctx * ctx, const z2h_experts * experts, int n_rows, int top
     a.sel = d_sel; a.weights = d_weights;
     a.shares = z2o::moe_shares(a.D); a.tiles = (a.D + 15) / 16;
     a.table = (MoeTable *) ws; a.touched = (MoeTouched *) (ws + w.touched); a.w = (float *) (ws + w.w);
-    if (n_rows > MOE_OWN_ROWS) { a.row_sel = (int32_t *) (ws + w.row_sel); a.row_w = (float *) (ws + w.row_w); }
+    if (n_rows > MOE_OWN_ROWS || a.E > MOE_OWN_EXPERTS) { a.row_sel = (int32_t *) (ws + w.row_sel); a.row_w = (float *) (ws + w.row_w); }
     a.tickets = (int32_t *) (ws + w.tickets); a.parts = (float *) (ws + w.parts); a.h = (float *) (ws + w.h); a.hs = z2o::moe_h_stride(a.F);
     const int n_cu = compute_units(z2h_ctx_device(ctx));
     if (!n_cu) return z2h_ctx_fail(ctx, Z2H_EDEVICE, "compute-unit count query failed");
