@@ -15,14 +15,20 @@ void gate_up_launch(const MoeArgs & a, int n_cu, hipStream_t st) {
     const int64_t tiles = (int64_t) std::min(a.E, a.n * a.k) * (a.F / 8);
     hipLaunchKernelGGL((k_moe_gate_up<T, TW, NT>), dim3(std::min<int64_t>(n_cu * moe_per_cu<T, NT>(), tiles)), dim3(MOE_T), 0, st, a);
 }
+// (each kernel takes its bounds and places from what the one before leaves in the workspace: none is launched behind one that could not be)
 template <typename T, typename TW>
-void moe_launch(const MoeArgs & a, int n_cu, hipStream_t st) {
-    if (a.row_sel) hipLaunchKernelGGL(k_moe_route, dim3(a.n), dim3(64), 0, st, a);
+int moe_launch(z2h_ctx * ctx, const MoeArgs & a, int n_cu, hipStream_t st) {
+    if (a.row_sel) {
+        hipLaunchKernelGGL(k_moe_route, dim3(a.n), dim3(64), 0, st, a);
+        if (int rc = launched(ctx)) return rc;
+    }
     // One tile of 16 rows leaves registers for two blocks per compute unit, two read the weights of an expert with more rows once. From 17 rows
     // on, two: 32 rows, 8 of 64 experts: 145 us in place of 168; 64 rows, 6 of 64, evenly spread: 218 in place of 212.
     if (a.n <= 16) gate_up_launch<T, TW, 1>(a, n_cu, st);
     else gate_up_launch<T, TW, 2>(a, n_cu, st);
+    if (int rc = launched(ctx)) return rc;
     hipLaunchKernelGGL((k_moe_down<T, TW>), dim3(a.tiles, a.shares), dim3(MOE_DT), MOE_DW * a.n * 64, st, a);
+    return launched(ctx);
 }
 
 } // namespace
@@ -60,11 +66,10 @@ int z2h_moe_rows(z2h_ctx * ctx, const z2h_experts * experts, int n_rows, int top
     if (!n_cu) return z2h_ctx_fail(ctx, Z2H_EDEVICE, "compute-unit count query failed");
     ON_DEVICE;
     switch (type) {
-        case Z2H_F32: moe_launch<float, _Float16>(a, n_cu, (hipStream_t) stream); break;
-        case Z2H_F16: moe_launch<_Float16, _Float16>(a, n_cu, (hipStream_t) stream); break;
-        default: moe_launch<__bf16, __bf16>(a, n_cu, (hipStream_t) stream); break;
+        case Z2H_F32: return moe_launch<float, _Float16>(ctx, a, n_cu, (hipStream_t) stream);
+        case Z2H_F16: return moe_launch<_Float16, _Float16>(ctx, a, n_cu, (hipStream_t) stream);
+        default: return moe_launch<__bf16, __bf16>(ctx, a, n_cu, (hipStream_t) stream);
     }
-    return launched(ctx);
 }
 
 } // extern "C"
