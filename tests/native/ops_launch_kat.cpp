@@ -73,6 +73,11 @@ int main() {
     }
     const auto prompt = [&](z2h_ctx * c) { return z2h_prompt_attn(c, 2, i, 600, 8, 2, 64, 0.125f, Z2H_F16, p, 512, p, 128, p, 128, p, 512, nullptr); };
     check("prompt", 1, prompt);
+    for (int vocab : {1025, 131072})
+        for (int logits = 0; logits < 2; ++logits)
+            check("verify", logits + (vocab > 100000 ? 2 : 1), [&](z2h_ctx * c) {
+                return z2h_verify(c, 4, 3, 2, vocab, i, i, f, logits ? f : nullptr, nullptr, d, d, i, i, p, 1ll << 40, nullptr);
+            });
     std::puts(bad ? "failed" : "ok");
     return bad != 0;
 }

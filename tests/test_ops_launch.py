@@ -8,7 +8,8 @@ def test_no_launch_behind_one_that_failed(root, tmp_path):
     inc = [f"-I{root / 'include'}", f"-I{csrc}", f"-I{root / 'zonos2.cpp_amd' / 'host'}"]
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     objs = []
-    for src in (csrc / "z2h_moe.hip", csrc / "z2h_pages.hip", csrc / "z2h_prompt.hip", root / "tests" / "native" / "ops_launch_kat.cpp"):
+    for src in (csrc / "z2h_moe.hip", csrc / "z2h_pages.hip", csrc / "z2h_prompt.hip", csrc / "z2h_ops.hip",
+                root / "tests" / "native" / "ops_launch_kat.cpp"):
         objs.append(tmp_path / (src.stem + ".o"))
         subprocess.run([hipcc, "-x", "hip", "--cuda-host-only", "--offload-arch=gfx950", "-O0", "-std=c++17", "-w", *inc, "-c", str(src),
                         "-o", str(objs[-1])], check=True)

@@ -226,6 +226,7 @@ int z2h_verify(z2h_ctx * ctx, int n_seq, int n_draft_max, int n_codebooks, int v
         // shares of 1024 codes (a round of the block's loads) or more, about 512 blocks in all
         a.n_share = std::min((vocab + 1023) / 1024, std::max(1, 512 / draws));
         hipLaunchKernelGGL(k_verify_sums, dim3(draws * a.n_share), dim3(256), 0, st, a);
+        if (int rc = launched(ctx)) return rc;                   // (nor from verdicts that nobody left)
         hipLaunchKernelGGL(k_verify_pick, dim3(draws), dim3(256), 0, st, a);
     }
     return launched(ctx);
