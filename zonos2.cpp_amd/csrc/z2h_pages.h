@@ -154,8 +154,9 @@ __device__ __forceinline__ void seg_prefix(const PoolArgs & p, int * s_pre, int 
     if (tid == 0) s_pre[p.segs] = total;
     __syncthreads();
 }
-// Bits of a word of 64, in 32-bit operations: 64-bit shifts by a lane's own amount went wrong here, in about one call of a hundred, where the
-// amount lay in the last vector register that the kernel has (v_lshrrev_b64 by v31 of 32).
+// Bits of a word of 64, in 32-bit operations: with a 64-bit shift by a lane's own amount, which lay in the last vector register that the kernel
+// had (v_lshrrev_b64 by v31 of 32), about one call of a hundred had a wrong bit; so none after the change. That register is the only cause
+// found, from the outside; no kernel of the library has such a shift, and a test of the built code keeps it so.
 __device__ __forceinline__ bool bit_of(const unsigned long long * words, int n) { return ((const unsigned *) words)[n >> 5] >> (n & 31) & 1; }
 // set bits below bit n (0 .. 63)
 __device__ __forceinline__ int bits_below(unsigned long long w, int n) {
