@@ -372,7 +372,8 @@ int z2h_verify(z2h_ctx * ctx, int n_seq, int n_draft_max, int n_codebooks, int v
  * Softmax and sums in fp32; F32 rows are multiplied in fp32, 16-bit rows' weights meet the values to 2^-16 of them (bf16) or 2^-22. Results do
  * not depend on timing (no atomics). Rows that a row does not see do not reach it, whatever they hold. A value that is not finite reaches
  * every row that sees it; a key whose score is minus infinity has no weight, and one whose score is infinity or no number leaves the row
- * without a number. (Rows that see such a value take longer: they are formed a second time, key by key.) */
+ * without a number; a row none of whose keys has a weight gives zeros. Scores are formed in fp32; one beyond its range may count as infinite. (Rows that
+ * see such a value take longer, since they are formed a second time, key by key: 200 times as long where all of 8191 rows do.) */
 int z2h_prompt_attn(z2h_ctx * ctx, int n_seq, const int32_t * d_row_start, int n_rows, int n_head, int n_head_kv, int head_dim,
                     float scale, int type, const void * d_q, int64_t q_stride, const void * d_k, int64_t k_stride, const void * d_v,
                     int64_t v_stride, void * d_out, int64_t out_stride, void * stream);

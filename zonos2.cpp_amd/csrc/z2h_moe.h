@@ -8,9 +8,10 @@
 // Both products read every weight that they need once and are bound by that: weights go from memory to the left operand of
 // v_mfma_f32_16x16x32, 16 rows of the matrix by 32 of its columns per instruction, and up to 16 rows of x or h are the right operand, so that
 // the products cost the same for 1 to 16 of them. A row of x goes there as it is (fp32: as two fp16 numbers), h as two fp16 or three bf16 numbers.
-// Measured, bf16 weights: 64 rows, 6 of 64 experts of 1032 x 2048: 210 us, 3.9 TB/s of weights (k_moe_route 5, k_moe_gate_up 125 for
-// 541 MB, k_moe_down 75 for 270 MB); fp16, 16 rows, 4 of 32 experts of 1536 x 2048: 114 us, 4.7 TB/s; fp32 rows, one row: 27 us, 2.8 TB/s,
-// of which 12 are two launches, routing and the join (a layer of 8 x 32 takes those too).
+// Measured, bf16 weights: 64 rows, 6 of 64 experts of 1032 x 2048: 210 us, 3.9 TB/s of weights (k_moe_route 5, k_moe_gate_up 126 for
+// 541 MB, k_moe_down 76 for 270 MB); fp16, 16 rows, 4 of 32 experts of 1536 x 2048: 114 to 118 us, 4.6 TB/s; fp32 rows, one row: 26 us, 2.9 TB/s,
+// of which 12 are two launches, routing and the join (a layer of 8 x 32 takes 13 to 14). A copy reaches 5.15 TB/s: both products let memory
+// stand still between their tiles, since they wait for the weights that they have requested ahead (see there).
 #pragma once
 #include "z2h_common.h"
 #include "z2h_ops_rules.h"
@@ -360,8 +361,9 @@ struct MoeCursor {
     }
 };
 
-// NT tiles of 16 rows of x stay in registers while the expert's tiles pass by, the next tile's weights on their way. A wave has one of eight
-// slices of the columns; the slices' sums meet in LDS.
+// NT tiles of 16 rows of x stay in registers while the expert's tiles pass by. The next tile's weights are requested before the present one's
+// products, but arrive before them too: all of these loads are made under conditions, so that the compiler cannot count which may be left
+// on their way, and it waits for every one before it multiplies. A wave has one of eight slices of the columns; the slices' sums meet in LDS.
 template <typename T, typename TW, int NT>
 __global__ void __launch_bounds__(MOE_T, (2 * moe_per_cu<T, NT>())) k_moe_gate_up(MoeArgs a) {
     constexpr bool SPLIT = sizeof(T) == 4;
@@ -506,9 +508,9 @@ constexpr int MOE_DF = 4, MOE_DW = 4, MOE_DT = 64 * MOE_DW;      // operands of 
 // 16 dims of out and all rows per block, over its share of the units (128 hidden dims of an expert), dealt to the waves in turn, so that they read the
 // matrix row by row together (in runs of their own: 81 us in place of 78 for 64 rows and 64 experts of 1032 x 2048). The right operand is w h of 16
 // rows that take the expert; its sums go to the rows' places in LDS when the wave turns to other rows. The next unit's weights and h are
-// on their way while this one is multiplied. h comes from the caches as often as there are tiles of out: of 32 of its columns, the first
-// four of every eight lie before the others, so that the four lanes of a row, who have eight columns each, read 64 bytes in a row at a
-// time (64 rows, 64 experts of 1032 x 2048: the layer 211 us in place of 217). Without any reads of h it would take 20 us less. (32 dims per
+// requested before this one is multiplied; as in k_moe_gate_up they are conditional loads, and all but one or two are waited for first. h
+// comes from the caches as often as there are tiles of out: of 32 of its columns, the first four of every eight lie before the others, so
+// that the four lanes of a row, who have eight columns each, read 64 bytes in a row at a time (64 rows, 64 experts of 1032 x 2048: the layer 211 us in place of 217). Without any reads of h it would take 20 us less. (32 dims per
 // block, which halves them, leave registers for two blocks per compute unit in place of three: 206 us there, 31 in place of 27 for a layer
 // of 8 x 32; 12 waves over 64 dims, for the near cache's sake: 82 us in place of 78 in this kernel.)
 template <typename T, typename TW>

@@ -6,8 +6,9 @@ using namespace z2d;
 
 namespace {
 
-// Rows up to which every block of k_moe_gate_up routes for itself, a wave per row, which saves a launch: 5 rows 56.0 us in place of 57.5, 8 rows
-// 95.7 and 96.6; with 16, two to a wave, it is even at last (133.8 and 132.5; 128 rows of 128 experts: 134 and 53).
+// Rows up to which every block of k_moe_gate_up routes for itself, a wave per row, which saves a launch: 5 rows, 1 of 16 experts of 4096 x 2048, 57.8 us
+// in place of 59.7, 8 rows 73.4 and 75.4; with 16 rows, two to a wave, it is even at last (4 of 32 of 1536 x 2048: 124.3 and 123.3; 128 rows of
+// 128 experts of 8 x 32: 116 and 52).
 constexpr int MOE_OWN_ROWS = 8;
 
 template <typename T, typename TW, int NT>
@@ -23,7 +24,9 @@ int moe_launch(z2h_ctx * ctx, const MoeArgs & a, int n_cu, hipStream_t st) {
         if (int rc = launched(ctx)) return rc;
     }
     // One tile of 16 rows leaves registers for two blocks per compute unit, two read the weights of an expert with more rows once. From 17 rows
-    // on, two: 32 rows, 8 of 64 experts: 145 us in place of 168; 64 rows, 6 of 64, evenly spread: 218 in place of 212.
+    // on, two: 32 rows most of which take the same 8 of 64 experts 61 us in place of 76, 64 rows the same 6 of 64 81 and 110, 128 rows, 2 of 8, 95 and
+    // 111. Spread evenly over many experts, of whom few have more than 16 rows, one would be a little faster (32 rows, 8 of 64: 174 to 188 in
+    // place of 177 to 195; 64 rows, 6 of 64: 200 in place of 207); the host does not know the spread.
     if (a.n <= 16) gate_up_launch<T, TW, 1>(a, n_cu, st);
     else gate_up_launch<T, TW, 2>(a, n_cu, st);
     if (int rc = launched(ctx)) return rc;

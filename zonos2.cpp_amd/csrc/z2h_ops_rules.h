@@ -197,12 +197,17 @@ Z2O_HD int64_t prompt_slot(int start, int seq, int rows) { return (int64_t) star
 Z2O_HD int64_t prompt_slots(int n_rows, int n_seq, int rows) { return (int64_t) n_rows / rows + n_seq; }
 // Rows of a tile of 16 row-heads (0: a group has more than these).
 Z2O_HD int small_rows(int group) { return 16 / group; }
-// How a call is cut, by its tiles of 128 row-heads. Few: 16 row-heads per block, whose keys four waves share (one prompt of 300 rows, 16 heads of 128
-// in 16 bits, 37 tiles: 9.2 us against 14.7 with 128 row-heads; 600 rows, 75 tiles: 16.0 against 21.1; 8 x 128 rows, 128 tiles: 14.4 against 11.3. Heads
-// of 64 half as much work each; fp32 products are slower, so that more blocks pay longer: 300 rows 17.0 against 48.5, 4 x 300, 150 tiles:
-// 39 against 52, 16 x 256, 512 tiles: 106 against 76). Up to a tile and a quarter per compute unit of long prompts: 128 row-heads and eight waves, each
-// four over half of the keys (2400 rows, 300 tiles: 57.9 against 67.4; 8 x 256: 17.6 against 19.2; heads of 64, 4 x 300: 17.4 against 14.8,
-// 1200: 24.1 against 26.9; 512 tiles of 16 x 256: 32 against 24). Otherwise 128 row-heads and four waves.
+// How a call is cut, by its tiles of 128 row-heads. Few: 16 row-heads per block, whose keys four waves share (small). Up to a tile and a quarter per
+// compute unit of long prompts: 128 row-heads and eight waves, each four over half of the keys (pair). Otherwise 128 row-heads and four waves
+// (wide). Measured, small - pair - wide in us, 16 heads of 128 on 4 key heads, f16 and fp32:
+//   1 x 300 rows,  37 tiles   9.0 - 13.9 - 13.5   16.2 - 48.2 - 48.9      8 x 224, 224 tiles   25.9 - 15.6 - 15.0   50.4 - 42.8 - 42.0
+//   1 x 600,       75        15.9 - 19.0 - 20.6   32.5 - 87.1 - 92.2      8 x 256, 256         30.7 - 16.1 - 18.8   59.5 - 47.9 - 72.7
+//   8 x 128,      128        15.4 - 11.9 - 10.7   25.5 - 29.4 - 28.1      4 x 512, 256         38.9 - 20.1 - 21.3   83.5 - 78.2 - 89.4
+//   4 x 300,      150        20.6 - 15.9 - 15.4   40.1 - 52.4 - 53.5      1 x 2400, 300        97.9 - 55.7 - 65.5    284 -  316 -  365
+//   8 x 192,      192        22.8 - 14.2 - 12.9   41.9 - 38.0 - 37.6      16 x 256, 512        54.0 - 27.5 - 21.4    108 - 83.6 - 75.0
+// Heads of 64: 4 x 300 rows 11.1 - 10.5 - 11.0 and 23.0 - 29.7 - 31.8; 1 x 1200 19.0 - 20.9 - 25.4 and 43.1 - 91.3 - 103; 8 x 512, 512 tiles
+// 31.9 - 23.7 - 21.0 and 68.9 - 75.6 - 76.3. Not met by the rule: 8 x 256 rows of heads of 64 (15.2 - 10.9 - 13.2, taken as wide), and long fp32 prompts
+// (2000 rows, 250 tiles: 202 - 266 - 287, taken as pair; 4000, 500 tiles: 749 - 553 - 746, taken as wide).
 enum PromptCut { PROMPT_WIDE, PROMPT_PAIR, PROMPT_SMALL };
 inline PromptCut prompt_cut(int n_rows, int n_seq, int n_head, int n_head_kv, int head_dim, bool fp32, int n_cu) {
     const int64_t tiles = (int64_t) n_rows * n_head / TILE_RH;

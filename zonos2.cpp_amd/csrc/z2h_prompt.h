@@ -5,7 +5,9 @@
 // The running maximum m moves only where a score exceeds it by 2^8, so that sums are seldom scaled. 4 hd flops per row-head and key and 2 hd more for
 // the weights' second parts: long prompts are bound by the products (one of 8191 rows, 32 heads of 128, bf16: 730 us, 1.1 PFLOP/s with the
 // second parts, which is what a matrix product of 8192 reaches; 24 of 16 to 2000 rows, 32 heads of 64: 97 us, 0.86), short ones by a
-// chain of loads and by code that runs once (8 of 256 rows, 16 heads of 128, f16: 14.7 us; one of 37, fp32: 7.8, of which 2.7 are the launch).
+// chain of loads and by code that runs once (8 of 256 rows, 16 heads of 128, f16: 14.7 to 16.3 us; one of 37, fp32: 7.8, of which 2.7 are the launch).
+// fp32 products reach 151 TFLOP/s: 8191 rows, 32 heads of 128 take 4.1 ms of which they need 3.6; 2000 rows, 16 heads 265 us (109), 16 of 256 rows
+// 75 (29), by the cut and by what PromptLoad says.
 #pragma once
 #include "z2h_common.h"
 #include "z2h_ops_rules.h"
@@ -391,7 +393,8 @@ struct PromptWave {
 
     // What is not finite meets both parts of a weight, and hidden rows' weights of 0: the product is then NaN where the definition has infinity or
     // leaves it out, and sums of weights up to 2^8 (f16: 2^14) times the largest values may be infinite where their mean is not. So a row-head
-    // that holds either is formed once more, in plain fp32.
+    // that holds either is formed once more, in plain fp32: a wave's up to 32 one after the other, so that a value that is no number in the
+    // first of 2000 rows (16 heads of 128) costs 14 ms in place of 0.05, in the first of 8191 (32 heads) 148 in place of 0.76.
     // The others' rows go through LDS, so that 16 bytes per lane make whole rows of the output. s_own: 32 HD T of LDS of the wave's own.
     // (What runs once per block is as little code as can be: a new instruction line of 64 bytes takes 70 ns.)
     __device__ __forceinline__ void store(const PromptArgs & a, int first, int row0, int rows, int g, int first_rh, int lane, T * s_own) {
@@ -440,6 +443,8 @@ struct PromptWave {
 };
 
 // Brings 16 rows of K or V to LDS at a time. ALIGNED: every piece is 16 bytes that may be loaded at once, straight to LDS; else by elements.
+// (fp32: whether a wave brings keys or values in a part is not known before it runs, and the compiler keeps the pieces' places in scratch memory, 12
+// bytes per lane, up to 72 where they are not aligned; reading them waits for the loads to LDS before.)
 template <int HD, typename T, bool ALIGNED>
 struct PromptLoad {
     typedef Rows<HD, T> R;
@@ -642,6 +647,9 @@ struct SmallMath<HD, float, ALIGNED> {
     }
 };
 
+// The next keys and values are requested before the present step's products. Those with the keys go on beside them; before those with 16-bit values the
+// compiler waits for the requested ones too, since it takes both buffers, halves of one array, for the same memory. fp32 heads of 128 take all
+// 256 registers and keep 8 more values in scratch memory (36 bytes per lane), read again in each step.
 template <int HD, typename T, bool ALIGNED>
 __global__ void __launch_bounds__(256, 2) k_prompt_small(PromptArgs a) {
     typedef SmallMath<HD, T, ALIGNED> M;
