@@ -388,8 +388,8 @@ typedef struct z2h_experts {
 /* A mixture-of-experts layer for a few rows (a step's, a request's drafts; 1 .. Z2H_MOE_ROWS_MAX), in two or three launches:
  *   p = softmax(d_logits of the row), the top_k experts by p + d_bias (NULL: by the logits; equal ones: the lower index first), w = p of these,
  *   divided by their sum if `renorm` is not 0;   out = sum_j w_j down_e(j) (silu(gate_e(j) x) * (up_e(j) x)).
- * p, p + d_bias and w are formed in 64 bits (a p more than 745 below the row's largest logit counts as 0 in p + d_bias), w is rounded to fp32;
- * with `renorm` it is right however small the chosen experts' p are.
+ * p, p + d_bias and w are formed in 64 bits (a logit more than 745 below the row's largest makes a p of 0), w is rounded to fp32; with
+ * `renorm` w is right however small the chosen experts' p are.
  * d_logits [n_rows][n_expert] are fp32, d_bias [n_expert]. d_x and d_out are [n_rows][n_embd] of `type`, rows *_stride apart: Z2H_F32 or
  * Z2H_F16 with F16 experts, Z2H_BF16 with BF16 ones; d_out may be d_x. d_sel and d_weights [n_rows][top_k] (either may be NULL) receive the
  * experts and their w, the first the one with the largest p + bias. An expert whose logit is minus infinity is never taken: -1 and 0

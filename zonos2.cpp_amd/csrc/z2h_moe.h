@@ -505,14 +505,15 @@ __global__ void __launch_bounds__(MOE_T, (2 * moe_per_cu<T, NT>())) k_moe_gate_u
 
 // ---- down
 constexpr int MOE_DF = 4, MOE_DW = 4, MOE_DT = 64 * MOE_DW;      // operands of a unit: 128 hidden dims of an expert; waves of a block
-// 16 dims of out and all rows per block, over its share of the units (128 hidden dims of an expert), dealt to the waves in turn, so that they read the
-// matrix row by row together (in runs of their own: 81 us in place of 78 for 64 rows and 64 experts of 1032 x 2048). The right operand is w h of 16
-// rows that take the expert; its sums go to the rows' places in LDS when the wave turns to other rows. The next unit's weights and h are
-// requested before this one is multiplied; as in k_moe_gate_up they are conditional loads, and all but one or two are waited for first. h
-// comes from the caches as often as there are tiles of out: of 32 of its columns, the first four of every eight lie before the others, so
-// that the four lanes of a row, who have eight columns each, read 64 bytes in a row at a time (64 rows, 64 experts of 1032 x 2048: the layer 211 us in place of 217). Without any reads of h it would take 20 us less. (32 dims per
-// block, which halves them, leave registers for two blocks per compute unit in place of three: 206 us there, 31 in place of 27 for a layer
-// of 8 x 32; 12 waves over 64 dims, for the near cache's sake: 82 us in place of 78 in this kernel.)
+// 16 dims of out and all rows per block, over its share of the units (128 hidden dims of an expert), dealt to the waves in turn, so that they read
+// the matrix row by row together (in runs of their own: 81 us in place of 78 for 64 rows and 64 experts of 1032 x 2048). The right operand is w h
+// of 16 rows that take the expert; its sums go to the rows' places in LDS when the wave turns to other rows. The next unit's weights and h are
+// requested before this one is multiplied; as in k_moe_gate_up they are conditional loads, and all but one or two are waited for first. h comes
+// from the caches as often as there are tiles of out: of 32 of its columns, the first four of every eight lie before the others, so that the four
+// lanes of a row, who have eight columns each, read 64 bytes in a row at a time (64 rows, 64 experts of 1032 x 2048: the layer 211 us in place of
+// 217). Without any reads of h it would take 20 us less. (32 dims per block, which halves them, leave registers for two blocks per compute unit in
+// place of three: 206 us there, 31 in place of 27 for a layer of 8 x 32; 12 waves over 64 dims, for the near cache's sake: 82 us in place of 78 in
+// this kernel.)
 template <typename T, typename TW>
 __global__ void __launch_bounds__(MOE_DT, 3) k_moe_down(MoeArgs a) {
     typedef typename Vec8<TW>::type v8;
